@@ -341,6 +341,95 @@ int seeai_xent_bwd(seeai_ctx* ctx, const float* d_probs,
 int seeai_adamw_step(seeai_ctx* ctx, float* d_p, const float* d_g,
                      float* d_m, float* d_v, uint64_t n,
                      const seeai_step_params* params, float clip_norm);
+/* --- Training a block's own weights --------------------------------------
+ * No reference counterpart: the reference's steps train low-rank adapters
+ * beside frozen weights.  These run on the context's device and stream.  The
+ * caller owns every buffer, the workspaces too (device memory, 16-byte
+ * aligned, of the size the *_workspace call gives): a call allocates nothing
+ * and keeps nothing, so it may be captured into a graph; calls that may run
+ * at the same time, or graphs that may, take workspaces of their own.  Rows
+ * are packed; an output may not share memory with another operand (status 2).
+ * dtype 0 = f32, 1 = bf16; sums and statistics are f32 in both. */
+
+/* Normalisation of rows [rows, cols]: kind 0 layer, 1 root mean square.
+ * y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps),
+ * the root-mean-square form without mean and bias (both NULL).  x and y in
+ * `dtype`, the vectors f32; d_bias, d_mean and d_rstd may be NULL. */
+int seeai_norm_fwd(seeai_ctx* ctx, int kind, int dtype, const void* d_x, const float* d_weight,
+                   const float* d_bias, void* d_y, float* d_mean, float* d_rstd, uint64_t rows,
+                   uint64_t cols, float eps);
+/* Its backward pass from the saved statistics: dx in `dtype`, dweight =
+ * sum over rows of dy xhat and dbias = sum over rows of dy in f32 (d_dbias may
+ * be NULL; zero rows give zeros).  The same bits every run. */
+uint64_t seeai_norm_bwd_workspace(uint64_t rows, uint64_t cols);
+int seeai_norm_bwd(seeai_ctx* ctx, int kind, int dtype, const void* d_dy, const void* d_x,
+                   const float* d_weight, const float* d_mean, const float* d_rstd, void* d_dx,
+                   float* d_dweight, float* d_dbias, uint64_t rows, uint64_t cols, void* d_ws,
+                   uint64_t ws_bytes);
+
+/* The gated feed-forward block: G = x wg, U = x wu, y = (act(G) * U) wd, with
+ * x, y [M, D], wg, wu [D, F], wd [F, D] in `dtype`; act as in seeai_gemm_f32.
+ * Products accumulate in f32; in bf16 the product act(G) U rounds once before
+ * the down projection.  d_gate and d_up [M, F] receive G and U for the
+ * backward pass, or are both NULL.  D and F up to 1048576. */
+uint64_t seeai_ffn_workspace(int dtype, uint64_t M, uint64_t D, uint64_t F, int backward);
+int seeai_ffn_fwd(seeai_ctx* ctx, int dtype, int act, const void* d_x, const void* d_wg,
+                  const void* d_wu, const void* d_wd, void* d_gate, void* d_up, void* d_y,
+                  uint64_t M, uint64_t D, uint64_t F, void* d_ws, uint64_t ws_bytes);
+/* Its backward pass from the saved G and U: the gradients of x and of all
+ * three weights, in `dtype` (M = 0 gives zero weight gradients). */
+int seeai_ffn_bwd(seeai_ctx* ctx, int dtype, int act, const void* d_x, const void* d_wg,
+                  const void* d_wu, const void* d_wd, const void* d_gate, const void* d_up,
+                  const void* d_dy, void* d_dx, void* d_dwg, void* d_dwu, void* d_dwd, uint64_t M,
+                  uint64_t D, uint64_t F, void* d_ws, uint64_t ws_bytes);
+
+/* One AdamW step (seeai_adamw_step's update, no clip) over a group of tensors
+ * in one launch.  state_bits 32: m and v f32, the bytes seeai_adamw_step
+ * leaves.  state_bits 8: m and v are codes, one byte an element, m_scale and
+ * v_scale one float per 128 elements (the last block may be short); m stands
+ * for code * scale, v for (code * scale)^2, a code being an e4m3 float (bias 7,
+ * no infinities, 0x7F / 0xFF a NaN).  All-zero bytes are zero moments.  The new
+ * moments round stochastically -- m and sqrt(v) right on average, v itself up
+ * to 1/16 above -- by bits drawn from `seed`, the step's number (its low 32
+ * bits) and the element's number (tensors end to end, each from a multiple of
+ * 128): the same group, seed and step give the same bytes.  A NaN
+ * or infinite moment becomes the NaN code of its element alone.  decay
+ * multiplies the step's weight_decay; p_bf16, where given, receives the new
+ * p rounded to bf16. */
+typedef struct seeai_adamw_tensor {
+  float* p;
+  const void* g; /* f32, or bf16 with grad_dtype 1 */
+  void* m;
+  void* v;
+  float* m_scale; /* 8-bit states only */
+  float* v_scale;
+  uint16_t* p_bf16; /* or NULL */
+  uint64_t n;
+  float decay;
+  uint32_t reserved;
+} seeai_adamw_tensor;
+typedef struct seeai_adamw_group seeai_adamw_group;
+/* Checks the tensors (device pointers; no two writing the same memory: status
+ * 2) and keeps their table on the device.  Not while the stream is captured. */
+int seeai_adamw_group_create(seeai_ctx* ctx, const seeai_adamw_tensor* tensors, uint64_t count,
+                             int state_bits, int grad_dtype, uint32_t seed,
+                             seeai_adamw_group** out);
+/* Waits for the device; the context outlives its groups. */
+void seeai_adamw_group_destroy(seeai_adamw_group* group);
+/* One step on the context's stream.  `params` NULL: with the values that
+ * seeai_adamw_group_hold last put on the device, the only form a captured
+ * stream takes (status 2 with params: each replay would repeat one step's
+ * number).  A refusal raised earlier on the stream (a non-finite clipped norm)
+ * leaves everything untouched, as in seeai_adamw_step. */
+int seeai_adamw_group_step(seeai_adamw_group* group, const seeai_step_params* params);
+/* Puts a step's values on the device, stream-ordered, for the steps with NULL
+ * params after it.  Not while the stream is captured. */
+int seeai_adamw_group_hold(seeai_adamw_group* group, const seeai_step_params* params);
+/* The moments that 8-bit codes stand for: which 0 = m, 1 = v; dtype of d_out
+ * 0 = f32, 1 = bf16 (which holds every code's value exactly where its exponent
+ * range does); scales one per 128 elements from the first. */
+int seeai_adamw_state_values(seeai_ctx* ctx, int which, int dtype, const uint8_t* d_codes,
+                             const float* d_scales, uint64_t n, void* d_out);
 /* The eval argmax, first maximum wins (update_engine.cc:537-565). */
 int seeai_argmax_rows(seeai_ctx* ctx, const float* d_probs, uint64_t rows,
                       uint64_t cols, int32_t* d_out);

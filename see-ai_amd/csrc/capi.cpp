@@ -17,12 +17,15 @@
 #include <cstring>
 #include <initializer_list>
 #include <map>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <tuple>
 #include <vector>
 
 #include "../../include/seeai_hip.h"
+#include "block_args.h"
 #include "common.h"
 #include "operands.h"
 
@@ -3115,6 +3118,235 @@ int seeai_adamw_step(seeai_ctx* c, float* p, const float* g, float* m, float* v,
   if (!c || !params) return SEEAI_INVALID;
   return AdamWLaunch(c, p, g, m, v, n, *params, clip_norm);
 }
+
+// --- Training a block's own weights ---------------------------------------------------------------
+
+namespace {
+
+// The context's device, current for the length of a call.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (hipGetDevice(&before_) != hipSuccess) before_ = device;
+    status_ = before_ == device ? hipSuccess : hipSetDevice(device);
+    changed_ = before_ != device && status_ == hipSuccess;
+  }
+  ~OnDevice() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  hipError_t status() const { return status_; }
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+  hipError_t status_;
+};
+
+// Whether the context's stream is being captured.
+int Capturing(seeai_ctx* c, bool* yes) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (c->stream) SEEAI_TRY(c, hipStreamIsCapturing(c->stream, &st), "capture status");
+  *yes = st != hipStreamCaptureStatusNone;
+  return SEEAI_OK;
+}
+
+}  // namespace
+
+uint64_t seeai_norm_bwd_workspace(uint64_t rows, uint64_t cols) {
+  if (CheckNormShape(0, 0, rows, cols)) return 0;
+  return NormBwdWorkspaceBytes(rows, cols);
+}
+int seeai_norm_fwd(seeai_ctx* c, int kind, int dtype, const void* x, const float* w, const float* b,
+                   void* y, float* mean, float* rstd, uint64_t rows, uint64_t cols, float eps) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckNormFwd(kind, dtype, x, w, b, y, mean, rstd, rows, cols, eps))
+    return Fail(c, SEEAI_INVALID, "norm_fwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "norm_fwd");
+  SEEAI_TRY(c, LaunchNormFwd(kind, dtype, x, w, b, y, mean, rstd, rows, cols, eps, c->stream), "norm_fwd");
+  return SEEAI_OK;
+}
+int seeai_norm_bwd(seeai_ctx* c, int kind, int dtype, const void* dy, const void* x, const float* w,
+                   const float* mean, const float* rstd, void* dx, float* dw, float* db,
+                   uint64_t rows, uint64_t cols, void* ws, uint64_t ws_bytes) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckNormBwd(kind, dtype, dy, x, w, mean, rstd, dx, dw, db, rows, cols, ws,
+                                   ws_bytes, seeai_norm_bwd_workspace(rows, cols)))
+    return Fail(c, SEEAI_INVALID, "norm_bwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "norm_bwd");
+  SEEAI_TRY(c, LaunchNormBwd(kind, dtype, dy, x, w, mean, rstd, dx, dw, db, rows, cols, ws, c->stream),
+            "norm_bwd");
+  return SEEAI_OK;
+}
+
+uint64_t seeai_ffn_workspace(int dtype, uint64_t M, uint64_t D, uint64_t F, int backward) {
+  if (CheckFfnShape(dtype, 0, M, D, F)) return 0;
+  return FfnWorkspaceBytes(dtype, M, D, F, backward);
+}
+int seeai_ffn_fwd(seeai_ctx* c, int dtype, int act, const void* x, const void* wg, const void* wu,
+                  const void* wd, void* gate, void* up, void* y, uint64_t M, uint64_t D, uint64_t F,
+                  void* ws, uint64_t ws_bytes) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckFfnFwd(dtype, act, x, wg, wu, wd, gate, up, y, M, D, F, ws, ws_bytes,
+                                  seeai_ffn_workspace(dtype, M, D, F, 0)))
+    return Fail(c, SEEAI_INVALID, "ffn_fwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "ffn_fwd");
+  FfnArgs a{};
+  a.bf16 = dtype, a.act = act;
+  a.x = x, a.wg = wg, a.wu = wu, a.wd = wd, a.gate = gate, a.up = up, a.y = y;
+  a.M = M, a.D = D, a.F = F, a.ws = ws;
+  SEEAI_TRY(c, LaunchFfnFwd(a, c->stream), "ffn_fwd");
+  return SEEAI_OK;
+}
+int seeai_ffn_bwd(seeai_ctx* c, int dtype, int act, const void* x, const void* wg, const void* wu,
+                  const void* wd, const void* gate, const void* up, const void* dy, void* dx,
+                  void* dwg, void* dwu, void* dwd, uint64_t M, uint64_t D, uint64_t F, void* ws,
+                  uint64_t ws_bytes) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckFfnBwd(dtype, act, x, wg, wu, wd, gate, up, dy, dx, dwg, dwu, dwd, M, D, F,
+                                  ws, ws_bytes, seeai_ffn_workspace(dtype, M, D, F, 1)))
+    return Fail(c, SEEAI_INVALID, "ffn_bwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "ffn_bwd");
+  FfnArgs a{};
+  a.bf16 = dtype, a.act = act;
+  a.x = x, a.wg = wg, a.wu = wu, a.wd = wd, a.gate = const_cast<void*>(gate), a.up = const_cast<void*>(up);
+  a.dy = dy, a.dx = dx, a.dwg = dwg, a.dwu = dwu, a.dwd = dwd;
+  a.M = M, a.D = D, a.F = F, a.ws = ws;
+  SEEAI_TRY(c, LaunchFfnBwd(a, c->stream), "ffn_bwd");
+  return SEEAI_OK;
+}
+
+}  // extern "C" (the group's definition)
+
+struct seeai_adamw_group {
+  seeai_ctx* ctx = nullptr;
+  AdamWGroupTensor* table = nullptr;  // device, the held step's values behind it
+  AdamWGroupStep* held = nullptr;
+  int count = 0, bits = 32, grads_bf16 = 0;
+  uint64_t chunks = 0;
+  uint32_t seed = 0;
+  bool holds = false;
+};
+
+namespace {
+
+AdamWGroupStep GroupStep(const seeai_adamw_group* g, const seeai_step_params& P) {
+  float hy[3];
+  StepHyper(P, hy);
+  return {P.lr, P.beta1, P.beta2, P.eps, P.weight_decay, hy[1], hy[2], AdamWGroupKey(g->seed, P.step)};
+}
+
+}  // namespace
+
+extern "C" {
+
+int seeai_adamw_group_create(seeai_ctx* c, const seeai_adamw_tensor* t, uint64_t count,
+                             int state_bits, int grad_dtype, uint32_t seed,
+                             seeai_adamw_group** out) try {
+  if (!c || !out) return Fail(c, SEEAI_INVALID, "adamw_group_create: null argument");
+  *out = nullptr;
+  if (const char* e = CheckAdamWGroup(t, count, state_bits, grad_dtype))
+    return Fail(c, SEEAI_INVALID, "adamw_group_create: %s", e);
+  bool capturing;
+  if (int rc = Capturing(c, &capturing)) return rc;
+  if (capturing) return Fail(c, SEEAI_INVALID, "adamw_group_create: the stream is being captured");
+  std::vector<AdamWGroupTensor> rows;
+  uint64_t chunks = 0, blocks = 0;
+  for (uint64_t i = 0; i < count; ++i) {
+    const seeai_adamw_tensor& x = t[i];
+    if (x.n == 0) continue;
+    const bool small = state_bits == 8;
+    const uintptr_t by16 = reinterpret_cast<uintptr_t>(x.p) | reinterpret_cast<uintptr_t>(x.g) |
+                           reinterpret_cast<uintptr_t>(x.p_bf16);
+    const uintptr_t states = reinterpret_cast<uintptr_t>(x.m) | reinterpret_cast<uintptr_t>(x.v);
+    rows.push_back({x.p, x.g, x.m, x.v, small ? x.m_scale : nullptr, small ? x.v_scale : nullptr,
+                    x.p_bf16, x.n, chunks, blocks, x.decay,
+                    (by16 & 15) == 0 && (states & (small ? 7 : 15)) == 0});
+    chunks += (x.n + kAdamWChunk - 1) / kAdamWChunk;
+    blocks += (x.n + kAdamWBlock - 1) / kAdamWBlock;
+  }
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "adamw_group_create");
+  const size_t bytes = rows.size() * sizeof(AdamWGroupTensor);
+  auto g = std::make_unique<seeai_adamw_group>();
+  void* mem = nullptr;
+  SEEAI_TRY(c, hipMalloc(&mem, bytes + sizeof(AdamWGroupStep)), "adamw_group table");
+  if (bytes)
+    if (hipError_t e = hipMemcpy(mem, rows.data(), bytes, hipMemcpyHostToDevice); e != hipSuccess) {
+      (void)hipFree(mem);
+      return Hip(c, e, "adamw_group table copy");
+    }
+  g->ctx = c;
+  g->table = static_cast<AdamWGroupTensor*>(mem);
+  g->held = reinterpret_cast<AdamWGroupStep*>(static_cast<uint8_t*>(mem) + bytes);
+  g->count = static_cast<int>(rows.size());
+  g->bits = state_bits;
+  g->grads_bf16 = grad_dtype;
+  g->chunks = chunks;
+  g->seed = seed;
+  *out = g.release();
+  return SEEAI_OK;
+} catch (const std::bad_alloc&) {
+  return Fail(c, SEEAI_INVALID, "adamw_group_create: out of host memory");
+}
+
+void seeai_adamw_group_destroy(seeai_adamw_group* g) {
+  if (!g) return;
+  OnDevice on(g->ctx->device);
+  if (g->table) (void)hipFree(g->table);  // waits for the device
+  delete g;
+}
+
+int seeai_adamw_group_step(seeai_adamw_group* g, const seeai_step_params* params) {
+  if (!g) return SEEAI_INVALID;
+  seeai_ctx* c = g->ctx;
+  if (!params && !g->holds)
+    return Fail(c, SEEAI_INVALID, "adamw_group_step: no params, and none held (seeai_adamw_group_hold)");
+  if (params && params->step == 0) return Fail(c, SEEAI_INVALID, "adamw_group_step: steps count from 1");
+  bool capturing;
+  if (int rc = Capturing(c, &capturing)) return rc;
+  if (capturing && params)
+    return Fail(c, SEEAI_INVALID, "adamw_group_step: a captured step takes held params (NULL)");
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "adamw_group_step");
+  SEEAI_TRY(c, LaunchAdamWGroup(g->table, g->count, g->chunks, g->bits, g->grads_bf16,
+                                params ? GroupStep(g, *params) : AdamWGroupStep{},
+                                params ? nullptr : g->held, c->flag(), c->stream),
+            "adamw_group_step");
+  return SEEAI_OK;
+}
+
+int seeai_adamw_group_hold(seeai_adamw_group* g, const seeai_step_params* params) {
+  if (!g || !params) return Fail(g ? g->ctx : nullptr, SEEAI_INVALID, "adamw_group_hold: null argument");
+  seeai_ctx* c = g->ctx;
+  if (params->step == 0) return Fail(c, SEEAI_INVALID, "adamw_group_hold: steps count from 1");
+  bool capturing;
+  if (int rc = Capturing(c, &capturing)) return rc;
+  if (capturing) return Fail(c, SEEAI_INVALID, "adamw_group_hold: the stream is being captured");
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "adamw_group_hold");
+  SEEAI_TRY(c, LaunchAdamWGroupHold(g->held, GroupStep(g, *params), c->stream), "adamw_group_hold");
+  g->holds = true;
+  return SEEAI_OK;
+}
+
+int seeai_adamw_state_values(seeai_ctx* c, int which, int dtype, const uint8_t* codes,
+                             const float* scales, uint64_t n, void* out) {
+  if (!c) return SEEAI_INVALID;
+  if (which < 0 || which > 1 || dtype < 0 || dtype > 1 || n >> 35)
+    return Fail(c, SEEAI_INVALID, "adamw_state_values: bad which, dtype or size");
+  if (const char* e = CheckOperands({{codes, n, 1, false}, {scales, (n + 127) / 128, 4, false},
+                                     {out, n, TypeSize(dtype), true}}))
+    return Fail(c, SEEAI_INVALID, "adamw_state_values: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "adamw_state_values");
+  SEEAI_TRY(c, LaunchAdamWValues(which, dtype, codes, scales, n, out, c->stream), "adamw_state_values");
+  return SEEAI_OK;
+}
+
 int seeai_argmax_rows(seeai_ctx* c, const float* probs, uint64_t rows, uint64_t cols, int32_t* out) {
   if (!c) return SEEAI_INVALID;
   SEEAI_TRY(c, LaunchArgmaxRows(probs, rows, cols, out, c->stream), "argmax");

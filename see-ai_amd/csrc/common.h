@@ -299,6 +299,64 @@ bool XEntRowResident(size_t C);
 // Whether the backward's row kernel can feed a sink (float4 rows).
 bool XEntBwdSinkFits(const float* probs, const float* dlogits, size_t C);
 
+// Trained norms (k_norm.hip): x, y, dy, dx f32 or bf16, the vectors f32.
+// rms: no mean, no bias (mean, b, db null).  The backward's ws:
+// NormBwdWorkspaceBytes.
+size_t NormBwdWorkspaceBytes(size_t rows, size_t cols);
+hipError_t LaunchNormFwd(int rms, int bf16, const void* x, const float* w, const float* b, void* y,
+                         float* mean, float* rstd, size_t rows, size_t cols, float eps,
+                         hipStream_t s);
+hipError_t LaunchNormBwd(int rms, int bf16, const void* dy, const void* x, const float* w,
+                         const float* mean, const float* rstd, void* dx, float* dw, float* db,
+                         size_t rows, size_t cols, void* ws, hipStream_t s);
+
+// The gated feed-forward block (k_ffn.hip): x, y, dy, dx [M, D], wg, wu and
+// their gradients [D, F], wd and its gradient [F, D], gate, up [M, F], all f32
+// or all bf16.  ws: FfnWorkspaceBytes.
+struct FfnArgs {
+  int bf16, act;
+  const void *x, *wg, *wu, *wd;
+  void *gate, *up;  // the forward's outputs (null: not kept), the backward's inputs
+  void* y;
+  const void* dy;
+  void *dx, *dwg, *dwu, *dwd;
+  size_t M, D, F;
+  void* ws;
+};
+size_t FfnWorkspaceBytes(int bf16, size_t M, size_t D, size_t F, int backward);
+hipError_t LaunchFfnFwd(const FfnArgs& a, hipStream_t s);
+hipError_t LaunchFfnBwd(const FfnArgs& a, hipStream_t s);
+
+// AdamW over a group of tensors (k_adamw_group.hip): the device table's rows
+// and a step's values.  A tensor's chunks of kAdamWChunk elements are
+// workgroups first_chunk on; its blocks of kAdamWBlock elements (one scale)
+// are numbered through the group from first_block.
+constexpr int kAdamWBlock = 128, kAdamWChunk = 2048;
+struct AdamWGroupTensor {
+  float* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  uint16_t* p_bf16;
+  uint64_t n, first_chunk, first_block;
+  float decay;
+  int vec;  // every pointer takes 16-byte accesses of eight neighbours
+};
+struct AdamWGroupStep {
+  float lr, beta1, beta2, eps, weight_decay, inv_bc1, inv_bc2;
+  uint32_t key;  // AdamWGroupKey of the step
+};
+uint32_t AdamWGroupKey(uint32_t seed, uint64_t step);
+// held: null, or device memory whose step takes the place of args.
+hipError_t LaunchAdamWGroup(const AdamWGroupTensor* tab, int count, uint64_t chunks, int bits,
+                            int grads_bf16, const AdamWGroupStep& args, const AdamWGroupStep* held,
+                            const int* flag, hipStream_t s);
+hipError_t LaunchAdamWGroupHold(AdamWGroupStep* held, const AdamWGroupStep& args, hipStream_t s);
+hipError_t LaunchAdamWValues(int second, int bf16, const uint8_t* codes, const float* scales,
+                             uint64_t n, void* out, hipStream_t s);
+
 // Optimizer family (k_optim.hip).  `flag` is the device refusal word that
 // every parameter-writing kernel honours; `scale` a device float slot.
 // ws for the norm: 8 * 1024 bytes.

@@ -70,6 +70,13 @@ class TilePolicy(C.Structure):
                 ("exact_longk_first", C.c_uint32), ("relaxed_tile_192", C.c_uint32)]
 
 
+class AdamWTensor(C.Structure):
+    """seeai_adamw_tensor: one tensor of an AdamW group (device pointers)."""
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("p_bf16", C.c_void_p),
+                ("n", C.c_uint64), ("decay", C.c_float), ("reserved", C.c_uint32)]
+
+
 # Every exported symbol with its ctypes signature: the header, one to one.
 EXPORTS = {
     "seeai_create": (_I, [_I, C.POINTER(_P)]),
@@ -126,6 +133,19 @@ EXPORTS = {
     "seeai_xent_fwd_noalloc": (_I, [_P, _P, _P, _P, _P, _U64, _U64, _I]),
     "seeai_xent_bwd": (_I, [_P, _P, _P, _P, _P, _U64, _U64, _I]),
     "seeai_adamw_step": (_I, [_P, _P, _P, _P, _P, _U64, C.POINTER(StepParams), _F]),
+    "seeai_norm_fwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _U64, _U64, _F]),
+    "seeai_norm_bwd_workspace": (_U64, [_U64, _U64]),
+    "seeai_norm_bwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _U64, _P, _U64]),
+    "seeai_ffn_workspace": (_U64, [_I, _U64, _U64, _U64, _I]),
+    "seeai_ffn_fwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _U64]),
+    "seeai_ffn_bwd": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _U64, _U64,
+                           _P, _U64]),
+    "seeai_adamw_group_create": (_I, [_P, C.POINTER(AdamWTensor), _U64, _I, _I, C.c_uint32,
+                                      C.POINTER(_P)]),
+    "seeai_adamw_group_destroy": (None, [_P]),
+    "seeai_adamw_group_step": (_I, [_P, C.POINTER(StepParams)]),
+    "seeai_adamw_group_hold": (_I, [_P, C.POINTER(StepParams)]),
+    "seeai_adamw_state_values": (_I, [_P, _I, _I, _P, _P, _U64, _P]),
     "seeai_argmax_rows": (_I, [_P, _P, _U64, _U64, _P]),
     "seeai_argmax_tally": (_I, [_P, _P, _P, _U64, _U64, C.POINTER(_U64), C.POINTER(_U64)]),
 }
@@ -253,6 +273,47 @@ class Context:
         import torch
         handle = torch.cuda.current_stream().cuda_stream
         self.check(_lib.seeai_set_stream(self.h, _P(handle) if handle else None))
+
+
+class AdamWGroup:
+    """A group of tensors stepped together (seeai_adamw_group_*).
+
+    ``tensors``: dicts of device tensors -- ``p`` (f32), ``g``, ``m``, ``v``,
+    with 8-bit states ``m_scale`` and ``v_scale``, optionally ``p_bf16`` --
+    with ``n`` (default: p's elements) and ``decay`` (default 1).  The group
+    keeps the tensors alive; the context outlives it."""
+
+    def __init__(self, ctx: Context, tensors, state_bits: int = 32, grads: str = "f32",
+                 seed: int = 0):
+        table = (AdamWTensor * max(len(tensors), 1))()
+        for row, t in zip(table, tensors):
+            for name in ("p", "g", "m", "v", "m_scale", "v_scale", "p_bf16"):
+                setattr(row, name, ptr(t.get(name)))
+            row.n = t["n"] if "n" in t else t["p"].numel()
+            row.decay = t.get("decay", 1.0)
+        h = _P()
+        self.h, self.ctx, self.tensors = None, ctx, list(tensors)
+        ctx.call("seeai_adamw_group_create", table, len(tensors), state_bits,
+                 {"f32": 0, "bf16": 1}[grads], seed, C.byref(h))
+        self.h = h
+
+    def step(self, params: StepParams | None = None):
+        self.ctx.check(_lib.seeai_adamw_group_step(
+            self.h, C.byref(params) if params is not None else None))
+
+    def hold(self, params: StepParams):
+        self.ctx.check(_lib.seeai_adamw_group_hold(self.h, C.byref(params)))
+
+    def close(self):
+        if self.h and self.ctx.h:
+            _lib.seeai_adamw_group_destroy(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 -- interpreter shutdown
+            pass
 
 
 class HipBackend:
