@@ -18,6 +18,7 @@
 // not finite but may be a NaN where f32 arithmetic has an infinity.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 
@@ -26,23 +27,43 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef __attribute__((address_space(3))) uint8_t* LdsPtr;
+typedef __attribute__((address_space(3))) s16x4* LdsTr;
 
-constexpr int kStageK = 32;            // K of one stage
 constexpr int kRsrcWord3 = 0x00020000;  // raw buffer, out-of-range reads give 0
 constexpr int kFar = 0x7FFFFFFF;        // an offset past every range
 
-// s_waitcnt vmcnt(n), other counters untouched (gfx9 encoding).
+// Until at most n of this wave's loads are in flight.
 template <int n>
 __device__ __forceinline__ void WaitVm() {
   static_assert(n >= 0 && n < 64, "vmcnt range");
-  __builtin_amdgcn_s_waitcnt((n & 15) | (7 << 4) | (15 << 8) | ((n >> 4) << 14));
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
 }
 
-// 16 bytes a lane, lane after lane, straight into LDS.
-__device__ __forceinline__ void LoadLds(__amdgpu_buffer_rsrc_t rs, uint8_t* lds, int voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LdsPtr)lds, 16, voff, soff, 0, 0);
+// A raw buffer over [base, base + bytes): reads past it give 0.
+typedef int v4i_ __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4i_ Buffer(const uint16_t* base, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return v4i_{Uniform(static_cast<int>(a)), Uniform(static_cast<int>(a >> 32)), Uniform(bytes), kRsrcWord3};
 }
+// 16 bytes a lane, lane after lane, straight into LDS at `lds`.  Written out
+// because the compiler lets no transposing read of LDS pass a load into LDS it
+// knows of: with its own builtin every half-stage's reads would wait for every
+// stage in flight.  It has no output register; WaitVm and a barrier stand
+// between it and the reads of what it brings.  (The wait states are those
+// between a scalar register's write, m0's included, and this use of it.)
+__device__ __forceinline__ void LoadLds(v4i_ rs, uint32_t lds, int voff, int soff) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(Uniform(lds)), "v"(voff), "s"(rs), "s"(Uniform(soff))
+      : "memory", "m0");
+}
+
+// Until this wave's LDS reads have returned.
+__device__ __forceinline__ void WaitLds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // The workgroup's barrier, which no access may be moved across.
 __device__ __forceinline__ void Barrier() {
@@ -51,67 +72,87 @@ __device__ __forceinline__ void Barrier() {
   asm volatile("" ::: "memory");
 }
 
-// The activation's derivative.
-__device__ __forceinline__ float ActGrad(int act, float x) {
-  switch (act) {
-    case 1: return x > 0.0f ? 1.0f : 0.0f;
-    case 2: {
-      const float kC = 0.7978845608028654f, kA = 0.044715f;
-      const float t = tanhf(kC * (x + kA * x * x * x));
-      return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * (kC * (1.0f + 3.0f * kA * x * x));
-    }
-    case 3: {
-      const float s = SigmoidExpr(x);
-      return s * (1.0f + x * (1.0f - s));
-    }
-    default: return 1.0f;
+// The activation (ActExpr's functions) and its derivative.  GELU's 1 + tanh(t)
+// is 2 sigmoid(2 t), so both smooth ones are x s(.) with one exponential.
+// kFast: the hardware's exponential and reciprocal, a few f32 steps off, for
+// results that leave in bf16.
+template <bool kFast>
+__device__ __forceinline__ float Sigmoid(float x) {
+  if constexpr (kFast)
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+  else
+    return SigmoidExpr(x);
+}
+template <bool kFast>
+__device__ __forceinline__ void Activate(int act, float x, float& a, float& da) {
+  const float kC = 0.7978845608028654f, kA = 0.044715f;
+  if (act == 3) {
+    const float s = Sigmoid<kFast>(x);
+    a = x * s;
+    da = s * (1.0f + x * (1.0f - s));
+  } else if (act == 2) {
+    const float s = Sigmoid<kFast>(2.0f * (kC * (x + kA * x * x * x)));
+    a = x * s;
+    da = s + x * s * (1.0f - s) * (2.0f * kC * (1.0f + 3.0f * kA * x * x));
+  } else {
+    const bool on = act == 0 || x > 0.0f;
+    a = on ? x : 0.0f;
+    da = on ? 1.0f : 0.0f;
   }
 }
 
-template <class T> __device__ __forceinline__ float Get(const T* p);
-template <> __device__ __forceinline__ float Get<float>(const float* p) { return *p; }
-template <> __device__ __forceinline__ float Get<uint16_t>(const uint16_t* p) { return Bf16ToF32(*p); }
-template <class T> __device__ __forceinline__ void Put(T* p, float v);
-template <> __device__ __forceinline__ void Put<float>(float* p, float v) { *p = v; }
-template <> __device__ __forceinline__ void Put<uint16_t>(uint16_t* p, float v) { *p = F32ToBf16(v); }
-
-__device__ __forceinline__ void Get4(const float* p, bool vec, int cnt, float (&v)[4]) {
-  if (vec) {
+// Up to eight neighbours of a row, 16 bytes at a time where they may be.
+__device__ __forceinline__ void Load8(const float* p, bool vec, int cnt, float (&v)[8]) {
+  if (vec && cnt >= 8) {
     const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    const float4 b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = e < cnt ? p[e] : 0.0f;
+    for (int e = 0; e < 8; ++e) v[e] = e < cnt ? p[e] : 0.0f;
   }
 }
-__device__ __forceinline__ void Get4(const uint16_t* p, bool vec, int cnt, float (&v)[4]) {
-  if (vec) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(a.x << 16), v[1] = __uint_as_float(a.x & 0xFFFF0000u);
-    v[2] = __uint_as_float(a.y << 16), v[3] = __uint_as_float(a.y & 0xFFFF0000u);
+__device__ __forceinline__ void Load8(const uint16_t* p, bool vec, int cnt, float (&v)[8]) {
+  if (vec && cnt >= 8) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = e < cnt ? Bf16ToF32(p[e]) : 0.0f;
+    for (int e = 0; e < 8; ++e) v[e] = e < cnt ? Bf16ToF32(p[e]) : 0.0f;
   }
 }
-__device__ __forceinline__ void Put4(float* p, bool vec, int cnt, const float (&v)[4]) {
-  if (vec) {
+__device__ __forceinline__ void Store8(float* p, bool vec, int cnt, const float (&v)[8]) {
+  if (vec && cnt >= 8) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
       if (e < cnt) p[e] = v[e];
   }
 }
-__device__ __forceinline__ void Put4(uint16_t* p, bool vec, int cnt, const float (&v)[4]) {
-  if (vec) {
-    StoreBf16x4(p, v);
+__device__ __forceinline__ bf16x8 Bf16x8(const float (&v)[8]) {
+  bf16x8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = static_cast<__bf16>(v[e]);
+  return o;
+}
+__device__ __forceinline__ void Store8(uint16_t* p, bool vec, int cnt, const float (&v)[8]) {
+  if (vec && cnt >= 8) {
+    *reinterpret_cast<bf16x8*>(p) = Bf16x8(v);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
       if (e < cnt) p[e] = F32ToBf16(v[e]);
   }
 }
+__device__ __forceinline__ void Put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void Put(uint16_t* p, float v) { *p = F32ToBf16(v); }
 
 // The next bf16 plane of a value: its top eight bits, taken off it.
 __device__ __forceinline__ uint32_t TakePlane(float& x) {
@@ -126,17 +167,22 @@ struct Planes {
   size_t plane = 0;  // elements of one plane
   int ld = 0;        // a multiple of 8, zeros past the row's own width
 };
-// Four neighbours into the planes (8-byte aligned: ld and the column are
-// multiples of four).
+// Eight neighbours into the planes (16-byte aligned: the column is a multiple
+// of eight).
 template <class T>
-__device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&v)[4]) {
+__device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&v)[8]) {
   if constexpr (sizeof(T) == 2) {
-    StoreBf16x4(out.p + at, v);
+    *reinterpret_cast<bf16x8*>(out.p + at) = Bf16x8(v);
   } else {
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      const uint32_t a = TakePlane(v[0]), b = TakePlane(v[1]), c = TakePlane(v[2]), d = TakePlane(v[3]);
-      *reinterpret_cast<uint2*>(out.p + k * out.plane + at) = make_uint2(a | b << 16, c | d << 16);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = TakePlane(v[2 * i]);
+        w[i] = lo | TakePlane(v[2 * i + 1]) << 16;
+      }
+      *reinterpret_cast<uint4*>(out.p + k * out.plane + at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -146,13 +192,13 @@ __device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&
 template <class T>
 __global__ void __launch_bounds__(256)
 FfnPackKernel(const T* __restrict__ in, size_t rows, int cols, bool vec, Planes out) {
-  const int quads = out.ld / 4;
-  const size_t n = rows * quads, step = static_cast<size_t>(gridDim.x) * 256;
+  const int octs = out.ld / 8;
+  const size_t n = rows * octs, step = static_cast<size_t>(gridDim.x) * 256;
   for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
-    const size_t r = i / quads;
-    const int c = static_cast<int>(i % quads) * 4;
-    float v[4];
-    Get4(in + r * cols + c, vec && c + 4 <= cols, cols - c, v);
+    const size_t r = i / octs;
+    const int c = static_cast<int>(i % octs) * 8;
+    float v[8];
+    Load8(in + r * cols + c, vec, cols - c, v);
     PutPlanes<T>(out, r * out.ld + c, v);
   }
 }
@@ -163,6 +209,17 @@ __global__ void __launch_bounds__(256) FfnZeroKernel(T* __restrict__ out, size_t
   for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) out[i] = 0;
 }
 
+// f(0), f(1), ... f(n - 1) with the index a constant: accumulators stay in
+// registers where a loop too large to unroll would index them in memory.
+template <class F, int... kI>
+__device__ __forceinline__ void EachOf(F&& f, std::integer_sequence<int, kI...>) {
+  (f(std::integral_constant<int, kI>{}), ...);
+}
+template <int kN, class F>
+__device__ __forceinline__ void Each(F&& f) {
+  EachOf(f, std::make_integer_sequence<int, kN>{});
+}
+
 // The products of one launch.  Operand element (i, k) lies at i ld + k, or,
 // "strided", at k ld + i.  Segments are products of the same shape added up.
 constexpr int kMaxSeg = 12;
@@ -171,12 +228,13 @@ struct MmaArgs {
   int nseg, lda, ldb;
   int M, N, K;
   int act;
-  bool vec;           // outputs (and G, U) take four neighbours at once
+  bool vec;           // outputs (and G, U) take eight neighbours at once
   void *o1, *o2;      // plain: o1 (and o2 of B2); gate: G and U or null
   const void *g, *u;  // gradient: G and U
   Planes h, dg, du;
 };
 
+constexpr int kBigN = 4;
 enum Epilogue {
   kPlain,  // o1 = sum A B
   kTwo,    // o1 = sum A B, o2 = sum A B2
@@ -198,148 +256,23 @@ __device__ __forceinline__ void TileOf(int b, int tiles_m, int tiles_n, int& tm,
   tn = off / rows;
 }
 
-// Transposing reads of `n` fragments, each two reads four K rows apart.  The
-// compiler's own read waits for every load into LDS still in flight, so the
-// reads are written out; each block waits for them itself.  Fragments are at
-// LDS addresses a[] plus kA (plus kB from the fourth on).
-template <int kOff, int kRow>
-__device__ __forceinline__ void ReadTr(const uint32_t (&a)[1], bf16x8 (&f)[1]) {
-  s16x4 r[2];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %2 offset:%3\n\t"
-      "ds_read_b64_tr_b16 %1, %2 offset:%4\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1])
-      : "v"(a[0]), "n"(kOff), "n"(kOff + 4 * kRow)
-      : "memory");
-  f[0] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-}
-template <int kOff, int kRow>
-__device__ __forceinline__ void ReadTr(const uint32_t (&a)[2], bf16x8 (&f)[2]) {
-  s16x4 r[4];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-      "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-      : "v"(a[0]), "v"(a[1]), "n"(kOff), "n"(kOff + 4 * kRow)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    f[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-}
-// Two operands' fragments in one block.
-template <int kOffA, int kRowA, int kOffB, int kRowB>
-__device__ __forceinline__ void ReadTr2(const uint32_t (&a)[1], bf16x8 (&fa)[1], const uint32_t (&b)[1],
-                                        bf16x8 (&fb)[1]) {
-  s16x4 r[4];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-      "ds_read_b64_tr_b16 %2, %5 offset:%8\n\t"
-      "ds_read_b64_tr_b16 %3, %5 offset:%9\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-      : "v"(a[0]), "v"(b[0]), "n"(kOffA), "n"(kOffA + 4 * kRowA), "n"(kOffB), "n"(kOffB + 4 * kRowB)
-      : "memory");
-  fa[0] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-  fb[0] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[2], r[3], 0, 1, 2, 3, 4, 5, 6, 7));
-}
-template <int kOffA, int kRowA, int kOffB, int kRowB>
-__device__ __forceinline__ void ReadTr2(const uint32_t (&a)[1], bf16x8 (&fa)[1], const uint32_t (&b)[2],
-                                        bf16x8 (&fb)[2]) {
-  s16x4 r[6];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %6 offset:%9\n\t"
-      "ds_read_b64_tr_b16 %1, %6 offset:%10\n\t"
-      "ds_read_b64_tr_b16 %2, %7 offset:%11\n\t"
-      "ds_read_b64_tr_b16 %3, %7 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %8 offset:%11\n\t"
-      "ds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5])
-      : "v"(a[0]), "v"(b[0]), "v"(b[1]), "n"(kOffA), "n"(kOffA + 4 * kRowA), "n"(kOffB),
-        "n"(kOffB + 4 * kRowB)
-      : "memory");
-  fa[0] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    fb[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[2 + 2 * i], r[3 + 2 * i], 0, 1, 2, 3, 4, 5, 6, 7));
-}
-template <int kOffA, int kRowA, int kOffB, int kRowB>
-__device__ __forceinline__ void ReadTr2(const uint32_t (&a)[2], bf16x8 (&fa)[2], const uint32_t (&b)[2],
-                                        bf16x8 (&fb)[2]) {
-  s16x4 r[8];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %4, %10 offset:%14\n\t"
-      "ds_read_b64_tr_b16 %5, %10 offset:%15\n\t"
-      "ds_read_b64_tr_b16 %6, %11 offset:%14\n\t"
-      "ds_read_b64_tr_b16 %7, %11 offset:%15\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]),
-        "=&v"(r[7])
-      : "v"(a[0]), "v"(a[1]), "v"(b[0]), "v"(b[1]), "n"(kOffA), "n"(kOffA + 4 * kRowA), "n"(kOffB),
-        "n"(kOffB + 4 * kRowB)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    fa[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-    fb[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[4 + 2 * i], r[5 + 2 * i], 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-}
-template <int kOffA, int kRowA, int kOffB, int kRowB>
-__device__ __forceinline__ void ReadTr2(const uint32_t (&a)[4], bf16x8 (&fa)[4], const uint32_t (&b)[2],
-                                        bf16x8 (&fb)[2]) {
-  s16x4 r[12];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %12 offset:%18\n\t"
-      "ds_read_b64_tr_b16 %1, %12 offset:%19\n\t"
-      "ds_read_b64_tr_b16 %8, %16 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %9, %16 offset:%21\n\t"
-      "ds_read_b64_tr_b16 %10, %17 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %11, %17 offset:%21\n\t"
-      "ds_read_b64_tr_b16 %2, %13 offset:%18\n\t"
-      "ds_read_b64_tr_b16 %3, %13 offset:%19\n\t"
-      "ds_read_b64_tr_b16 %4, %14 offset:%18\n\t"
-      "ds_read_b64_tr_b16 %5, %14 offset:%19\n\t"
-      "ds_read_b64_tr_b16 %6, %15 offset:%18\n\t"
-      "ds_read_b64_tr_b16 %7, %15 offset:%19\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]),
-        "=&v"(r[7]), "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "n"(kOffA),
-        "n"(kOffA + 4 * kRowA), "n"(kOffB), "n"(kOffB + 4 * kRowB)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    fa[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    fb[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[8 + 2 * i], r[9 + 2 * i], 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// One operand's tile of kW rows (or strided columns): how its 64 kW bytes of a
-// stage come into LDS and leave as fragments.
+// One operand's tile of kW rows (or strided columns): how the kW kBK elements of
+// a stage come into LDS and leave as fragments.
 //
-// Contiguous in K: LDS rows of 64 bytes, four 16-byte chunks, chunk c of row r
-// at physical (c + r / 4) % 4: the 32 rows of a fragment read are free of bank
-// conflicts.
+// Contiguous in K: LDS rows of 2 kBK bytes, kBK / 8 chunks of 16.  A fragment
+// read takes one chunk of 32 rows; a row's chunks are rotated by the rows
+// already in its 256 bytes, so sixteen lanes meet all the banks.
 // Strided: LDS rows are K, kW elements long; a fragment is two transposing
 // reads, each of four K rows by 64 bytes a half-wave, so the 64-byte slots of
 // four neighbouring rows are rotated against each other onto different banks.
-template <bool kStrided, int kW, int kWaves>
+template <bool kStrided, int kW, int kBK, int kWaves>
 struct Tile {
-  static constexpr int kLoads = kW / 16 / kWaves;  // wave-loads of a stage, per wave
-  static_assert(kLoads * 16 * kWaves == kW, "loads cover the tile");
-  static constexpr int kBytes = kW * 64;
-  static constexpr int kChunks = kStrided ? kW / 8 : 4;  // 16-byte chunks of an LDS row
-  static constexpr int kRow = kW * 2;                    // bytes of a strided LDS row
+  static constexpr int kBytes = kW * kBK * 2;
+  static constexpr int kLoads = kBytes / 1024 / kWaves;  // wave-loads of a stage, per wave
+  static_assert(kLoads * 1024 * kWaves == kBytes, "loads cover the tile");
+  static constexpr int kRow = kStrided ? kW * 2 : kBK * 2;  // bytes of an LDS row
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kPer256 = 256 / kRow;  // contiguous rows in 256 bytes
   // Where 64-byte slot s of strided row k lies: rotated among the slots of
   // 256 bytes (64 columns: the rows 128 bytes apart rotate by pairs).
   static __device__ __forceinline__ int Slot(int s, int k) {
@@ -363,30 +296,22 @@ struct Tile {
         voff[j] = row * ld * 2 + (SlotAt(p / 4, row) * 4 + p % 4) * 16;
         kc[j] = 0;
       } else {
-        const int c = (p - row / 4) & 3;
+        const int c = (p - row / kPer256) & (kChunks - 1);
         voff[j] = row * ld * 2 + c * 16;
         kc[j] = c * 8;
       }
     }
   }
-  // Stage [k0, k0 + 32) of the operand at `at` (its tile's corner) into LDS.
-  __device__ __forceinline__ void Issue(const uint16_t* at, int k0, int K, uint8_t* lds, int wave) {
+  // Wave-load j of stage [k0, k0 + kBK) of the operand at `at` (its tile's
+  // corner) into LDS.
+  __device__ __forceinline__ void Load(const uint16_t* at, int k0, int K, uint32_t lds, int wave, int j) {
+    const uint32_t to = lds + (j * kWaves + wave) * 1024;
     if constexpr (kStrided) {
-      const int rows = min(K - k0, kStageK);
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint16_t*>(at) + static_cast<size_t>(k0) * ld, 0,
-          Uniform(((rows - 1) * ld + extent) * 2), kRsrcWord3);
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j)
-        LoadLds(rs, lds + Uniform((j * kWaves + wave) * 1024), voff[j], 0);
+      const int rows = min(K - k0, kBK);
+      LoadLds(Buffer(at + static_cast<size_t>(k0) * ld, ((rows - 1) * ld + extent) * 2), to, voff[j], 0);
     } else {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint16_t*>(at), 0, Uniform(extent * ld * 2), kRsrcWord3);
-      const bool tail = k0 + kStageK > k8;
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j)
-        LoadLds(rs, lds + Uniform((j * kWaves + wave) * 1024),
-                tail && k0 + kc[j] >= k8 ? kFar : voff[j], k0 * 2);
+      const bool tail = k0 + kBK > k8;
+      LoadLds(Buffer(at, extent * ld * 2), to, tail && k0 + kc[j] >= k8 ? kFar : voff[j], k0 * 2);
     }
   }
   // Byte offset in the tile of lane l's part of the fragment of rows (columns)
@@ -396,15 +321,25 @@ struct Tile {
       const int i = lane % 16, k = 8 * (lane / 32) + i / 4;
       return k * kRow + Slot(first / 32, k) * 64 + ((lane / 16) & 1) * 32 + (i % 4) * 8;
     } else {
-      const int r = lane % 32;
-      return (first + r) * 64 + ((lane / 32 + r / 4) & 3) * 16;
+      return (first + lane % 32) * kRow + ((lane / 32 + lane % 32 / kPer256) & (kChunks - 1)) * 16;
     }
   }
-  // The same 16 K later (contiguous: two chunks on).
-  static constexpr int kNext = kStrided ? 16 * kRow : 32;
+  // The fragment 16 ks further in K.
+  static __device__ __forceinline__ bf16x8 Read(const uint8_t* stage, uint32_t off, int ks) {
+    if constexpr (kStrided) {
+      const uint8_t* a = stage + off + ks * 16 * kRow;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)a);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(a + 4 * kRow));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {  // two chunks on, round the row's chunks
+      const uint32_t row = off & ~static_cast<uint32_t>(kRow - 1);
+      return *reinterpret_cast<const bf16x8*>(stage + row + ((off + ks * 32) & (kRow - 1)));
+    }
+  }
+  static constexpr int kReads = kStrided ? 2 : 1;  // LDS reads of a fragment
 };
 
-template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int WGM, int WGN, int kStages>
+template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
 __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   constexpr int kWaves = WGM * WGN;
   constexpr bool kDual = kEpi == kTwo || kEpi == kGate;
@@ -412,13 +347,14 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   constexpr int WM = BM / WGM, WN = BNs / WGN;
   constexpr int TM = WM / 32, TN = WN / 32, TB = kDual ? 2 * TN : TN;
   static_assert(TM * 32 * WGM == BM && TN * 32 * WGN == BNs, "waves cover the tile");
-  using TA = Tile<kAS, BM, kWaves>;
-  using TBt = Tile<kBS, BNs, kWaves>;
+  using TA = Tile<kAS, BM, BK, kWaves>;
+  using TBt = Tile<kBS, BNs, BK, kWaves>;
+  constexpr int kSub = BK / 16;  // half-waves of K in a stage
   constexpr int kStage = TA::kBytes + (kDual ? 2 : 1) * TBt::kBytes;
   constexpr int kPerStage = TA::kLoads + (kDual ? 2 : 1) * TBt::kLoads;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kStages * kStage];
 
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int wave = Uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   int tm, tn;
   TileOf(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BNs - 1) / BNs, tm, tn);
   const int m0 = tm * BM, n0 = tn * BNs;
@@ -429,20 +365,32 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   tb.Init(p.ldb, kBS ? p.ldb - n0 : min(p.N - n0, BNs), p.K, wave, lane);
   const size_t a_at = kAS ? static_cast<size_t>(m0) : static_cast<size_t>(m0) * p.lda;
   const size_t b_at = kBS ? static_cast<size_t>(n0) : static_cast<size_t>(n0) * p.ldb;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPtr)smem));
 
-  const int per_seg = (p.K + kStageK - 1) / kStageK, last = p.nseg * per_seg - 1;
-  int seg = 0, k0 = 0;  // the next stage to load
-  auto issue = [&](int buf) {
-    uint8_t* s = smem + buf * kStage;
-    ta.Issue(p.A[seg] + a_at, k0, p.K, s, wave);
-    tb.Issue(p.B[seg] + b_at, k0, p.K, s + TA::kBytes, wave);
-    if constexpr (kDual) tb.Issue(p.B2[seg] + b_at, k0, p.K, s + TA::kBytes + TBt::kBytes, wave);
-    // Past the last stage the loads repeat it, into a buffer nothing reads.
-    if (k0 + kStageK < p.K) {
-      k0 += kStageK;
+  const int per_seg = (p.K + BK - 1) / BK, last = p.nseg * per_seg - 1;
+  // The next stage to load, and its segment's operands.
+  int seg = 0, k0 = 0;
+  const uint16_t *pa = p.A[0] + a_at, *pb = p.B[0] + b_at, *pb2 = kDual ? p.B2[0] + b_at : nullptr;
+  // Part `part` of kSub of the next stage's loads into buffer `buf`.
+  auto issue = [&](int buf, auto part_tag) __attribute__((always_inline)) {
+    constexpr int part = decltype(part_tag)::value;
+    const uint32_t s = lds0 + buf * kStage;
+#pragma unroll
+    for (int l = part * kPerStage / kSub; l < (part + 1) * kPerStage / kSub; ++l) {
+      if (l < TA::kLoads) ta.Load(pa, k0, p.K, s, wave, l);
+      else if (l < TA::kLoads + TBt::kLoads) tb.Load(pb, k0, p.K, s + TA::kBytes, wave, l - TA::kLoads);
+      else tb.Load(pb2, k0, p.K, s + TA::kBytes + TBt::kBytes, wave, l - TA::kLoads - TBt::kLoads);
+    }
+  };
+  // Past the last stage the loads repeat it, into buffers nothing reads.
+  auto advance = [&]() __attribute__((always_inline)) {
+    if (k0 + BK < p.K) {
+      k0 += BK;
     } else if (seg + 1 < p.nseg) {
       ++seg;
       k0 = 0;
+      pa = p.A[seg] + a_at, pb = p.B[seg] + b_at;
+      if constexpr (kDual) pb2 = p.B2[seg] + b_at;
     }
   };
 
@@ -459,140 +407,163 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
 #pragma unroll
   for (int j = 0; j < TB; ++j)
     ob[j] = TA::kBytes + (j / TN) * TBt::kBytes + TBt::Frag(wn + (j % TN) * 32, lane);
-  const uint32_t lds0 = static_cast<uint32_t>(
-      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem));
 
+  // K in steps of 16: the step's fragments are read while the one before is
+  // multiplied, into the other half of fa and fb.
   bf16x8 fa[2][TM], fb[2][TB];
-  // Contiguous operands' fragments come by the compiler's own reads, ahead of
-  // the products of the half-stage before; strided ones behind them, while the
-  // SIMD's other wave multiplies.
-  auto read_ahead = [&](int buf, auto ks_tag) {
+  auto read = [&](int buf, auto ks_tag) __attribute__((always_inline)) {
     constexpr int ks = decltype(ks_tag)::value;
     const uint8_t* s = smem + buf * kStage;
-    // (chunk c + 2 ks of four, so the second half-stage is the other pair)
-    if constexpr (!kAS) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fa[ks][i] = *reinterpret_cast<const bf16x8*>(s + (oa[i] ^ (ks * 32)));
-    }
-    if constexpr (!kBS) {
+    for (int i = 0; i < TM; ++i) fa[ks % 2][i] = TA::Read(s, oa[i], ks);
 #pragma unroll
-      for (int j = 0; j < TB; ++j) fb[ks][j] = *reinterpret_cast<const bf16x8*>(s + (ob[j] ^ (ks * 32)));
-    }
+    for (int j = 0; j < TB; ++j) fb[ks % 2][j] = TBt::Read(s, ob[j], ks);
   };
-  auto read_behind = [&](int buf, auto ks_tag) {
-    constexpr int ks = decltype(ks_tag)::value;
-    const uint32_t s = lds0 + buf * kStage;
-    uint32_t a[TM], b[TB];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) a[i] = s + oa[i];
-#pragma unroll
-    for (int j = 0; j < TB; ++j) b[j] = s + ob[j];
-    if constexpr (kAS && kBS)
-      ReadTr2<ks * TA::kNext, TA::kRow, ks * TBt::kNext, TBt::kRow>(a, fa[ks], b, fb[ks]);
-    else if constexpr (kBS)
-      ReadTr<ks * TBt::kNext, TBt::kRow>(b, fb[ks]);
-  };
-  auto mfmas = [&](auto ks_tag) {
-    constexpr int ks = decltype(ks_tag)::value;
+  auto mfmas = [&](int half) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TB; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[ks][j], fa[ks][i], acc[i][j], 0, 0, 0);
-    if constexpr (kAS || kBS) __builtin_amdgcn_sched_barrier(0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[half][j], fa[half][i], acc[i][j], 0, 0, 0);
   };
-  constexpr std::integral_constant<int, 0> k0_{};
-  constexpr std::integral_constant<int, 1> k1_{};
-
+  // The next step's reads spread over the products of this one.
+  constexpr int kMfmas = TM * TB, kReads = TM * TA::kReads + TB * TBt::kReads;
+  constexpr int kPerSlot = (kReads + kMfmas - 1) / kMfmas;
+  auto interleave = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
+    for (int s = 0; s < kMfmas; ++s) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (s * kPerSlot < kReads) __builtin_amdgcn_sched_group_barrier(0x100, kPerSlot, 0);
+    }
+  };
+  // A stage's steps but the last, each behind the next one's reads.  The loads
+  // of the stage that takes the buffer freed last (`to`) go out a few a step:
+  // all at once they would hold up the products behind them.
+  auto steps = [&](int buf, int to, auto load) __attribute__((always_inline)) {
+    Each<kSub - 1>([&](auto ks) __attribute__((always_inline)) {
+      if constexpr (decltype(load)::value) issue(to, ks);
+      read(buf, std::integral_constant<int, decltype(ks)::value + 1>{});
+      mfmas(decltype(ks)::value % 2);
+      interleave();
+    });
+    if constexpr (decltype(load)::value) issue(to, std::integral_constant<int, kSub - 1>{});
+  };
+
+  // kStages buffers: one multiplied, one taking loads, the others in flight or
+  // landed.  Before the last step of stage `it` every wave has its fragments of
+  // it and stage it + 1 has landed.
+  for (int s = 0; s < kStages - 1; ++s) {
+    Each<kSub>([&](auto part) __attribute__((always_inline)) { issue(s, part); });
+    advance();
+  }
   WaitVm<(kStages - 2) * kPerStage>();
   Barrier();
-  read_ahead(0, k0_);
-  read_behind(0, k0_);
+  read(0, std::integral_constant<int, 0>{});
   for (int it = 0; it < last; ++it) {
-    const int buf = it % kStages;
-    read_ahead(buf, k1_);
-    mfmas(k0_);
-    read_behind(buf, k1_);
-    WaitVm<(kStages - 3) * kPerStage>();
+    steps(it % kStages, (it + kStages - 1) % kStages, std::true_type{});
+    WaitVm<(kStages - 2) * kPerStage>();
+    WaitLds();
     Barrier();
-    issue((it + kStages - 1) % kStages);
-    read_ahead((it + 1) % kStages, k0_);
-    mfmas(k1_);
-    read_behind((it + 1) % kStages, k0_);
+    advance();
+    read((it + 1) % kStages, std::integral_constant<int, 0>{});
+    mfmas((kSub - 1) % 2);
+    interleave();
   }
-  read_ahead(last % kStages, k1_);
-  mfmas(k0_);
-  read_behind(last % kStages, k1_);
-  mfmas(k1_);
+  steps(last % kStages, 0, std::false_type{});
+  mfmas((kSub - 1) % 2);
   WaitVm<0>();  // the repeated loads have landed
 
-  // Accumulator element 4 q + e of block (i, j) is row lane % 32, column
-  // 8 q + 4 (lane / 32) + e: four neighbours of one row at a time.
+  // The epilogue: kW columns of 32 rows at a time through this wave's slice of
+  // LDS.  Accumulator element 4 q + e of block (i, j) is row lane % 32, column
+  // 8 q + 4 (lane / 32) + e; a lane takes eight neighbours of a row away.
+  Barrier();  // every wave is done with the stages
+  constexpr int kW = WN >= 64 ? 64 : 32, kPad = kW + 4, kBoth = kDual ? 2 : 1;
+  static_assert(kWaves * kBoth * 32 * kPad * 4 <= kStages * kStage, "staging fits");
+  constexpr int kPerRow = kW / 8, kRows = kWave / kPerRow;
+  float* st = reinterpret_cast<float*>(smem) + wave * kBoth * 32 * kPad;
   const int h = lane / 32;
+  Each<TM * (WN / kW)>([&](auto part) __attribute__((always_inline)) {
+      constexpr int i = decltype(part)::value / (WN / kW), jb = decltype(part)::value % (WN / kW);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m0 + wm + i * 32 + lane % 32;
+      for (int b = 0; b < kBoth; ++b)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+        for (int jj = 0; jj < kW / 32; ++jj)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn + j * 32 + 8 * q + 4 * h;
-        const int cnt = p.N - n;  // columns left
-        if (m >= p.M) continue;
-        const size_t o = static_cast<size_t>(m) * p.N + n;
-        const bool vec = p.vec && cnt >= 4;
-        float c[4], d[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          c[e] = acc[i][j][4 * q + e];
-          if constexpr (kDual) d[e] = acc[i][TN + j][4 * q + e];
-        }
-        if constexpr (kEpi == kPlain || kEpi == kTwo) {
-          Put4(static_cast<T*>(p.o1) + o, vec, cnt, c);
-          if constexpr (kEpi == kTwo) Put4(static_cast<T*>(p.o2) + o, vec, cnt, d);
-        }
-        if constexpr (kEpi == kGate) {
-          if (n >= p.h.ld) continue;
-          if (p.o1) {
-            Put4(static_cast<T*>(p.o1) + o, vec, cnt, c);
-            Put4(static_cast<T*>(p.o2) + o, vec, cnt, d);
+          for (int q = 0; q < 4; ++q) {
+            const v16f& c = acc[i][b * TN + jb * (kW / 32) + jj];
+            *reinterpret_cast<float4*>(st + (b * 32 + lane % 32) * kPad + jj * 32 + 8 * q + 4 * h) =
+                make_float4(c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = e < cnt ? ActExpr(p.act, c[e]) * d[e] : 0.0f;
-          PutPlanes<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
-        }
-        if constexpr (kEpi == kGrad) {
-          if (n >= p.h.ld) continue;
-          float g[4], u[4];
-          Get4(static_cast<const T*>(p.g) + o, vec, cnt, g);
-          Get4(static_cast<const T*>(p.u) + o, vec, cnt, u);
-          float x[4], y[4], z[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = ActExpr(p.act, g[e]);
-            const bool in = e < cnt;
-            x[e] = in ? c[e] * u[e] * ActGrad(p.act, g[e]) : 0.0f;
-            y[e] = in ? c[e] * a : 0.0f;
-            z[e] = in ? a * u[e] : 0.0f;
+      __builtin_amdgcn_wave_barrier();
+      const int mb = m0 + wm + i * 32, nb = n0 + wn + jb * kW;
+      if ((kEpi == kPlain || kEpi == kTwo) && !p.vec) {
+        // Rows off 16 bytes: a lane a column.
+        const int n = nb + lane % kW;
+        for (int r = lane / kW; r < 32; r += kWave / kW) {
+          if (mb + r < p.M && n < p.N) {
+            const size_t o = static_cast<size_t>(mb + r) * p.N + n;
+            Put(static_cast<T*>(p.o1) + o, st[r * kPad + lane % kW]);
+            if constexpr (kEpi == kTwo) Put(static_cast<T*>(p.o2) + o, st[(32 + r) * kPad + lane % kW]);
           }
-          const size_t w = static_cast<size_t>(m) * p.h.ld + n;
-          PutPlanes<T>(p.dg, w, x);
-          PutPlanes<T>(p.du, w, y);
-          PutPlanes<T>(p.h, w, z);
+        }
+      } else {
+        const int n = nb + (lane % kPerRow) * 8, cnt = p.N - n;
+#pragma unroll
+        for (int t = 0; t < 32 / kRows; ++t) {
+          const int r = lane / kPerRow + t * kRows, m = mb + r;
+          if (m >= p.M || cnt <= 0) continue;
+          const size_t o = static_cast<size_t>(m) * p.N + n;
+          float c[8], d[8];
+          Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
+          if constexpr (kDual) Load8(st + (32 + r) * kPad + (lane % kPerRow) * 8, true, 8, d);
+          if constexpr (kEpi == kPlain || kEpi == kTwo) {
+            Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
+            if constexpr (kEpi == kTwo) Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
+          }
+          if constexpr (kEpi == kGate) {
+            if (p.o1) {
+              Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
+              Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float a, da;
+              Activate<sizeof(T) == 2>(p.act, c[e], a, da);
+              c[e] = e < cnt ? a * d[e] : 0.0f;
+            }
+            PutPlanes<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
+          }
+          if constexpr (kEpi == kGrad) {
+            float g[8], u[8], y[8];
+            Load8(static_cast<const T*>(p.g) + o, p.vec, cnt, g);
+            Load8(static_cast<const T*>(p.u) + o, p.vec, cnt, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float a, da;
+              Activate<sizeof(T) == 2>(p.act, g[e], a, da);
+              const bool in = e < cnt;
+              g[e] = in ? c[e] * u[e] * da : 0.0f;
+              y[e] = in ? c[e] * a : 0.0f;
+              u[e] = in ? a * u[e] : 0.0f;
+            }
+            const size_t w = static_cast<size_t>(m) * p.h.ld + n;
+            PutPlanes<T>(p.dg, w, g);
+            PutPlanes<T>(p.du, w, y);
+            PutPlanes<T>(p.h, w, u);
+          }
         }
       }
-  }
+      __builtin_amdgcn_wave_barrier();
+  });
 }
 
 // --- host ---------------------------------------------------------------------------------------
 
-template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int WGM, int WGN, int kStages>
+template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
 hipError_t LaunchTile(const MmaArgs& a, hipStream_t s) {
   constexpr int BNs = kEpi == kTwo || kEpi == kGate ? BN / 2 : BN;
   const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BNs - 1) / BNs);
-  auto* kernel = &FfnMma<T, kEpi, kAS, kBS, BM, BN, WGM, WGN, kStages>;
+  auto* kernel = &FfnMma<T, kEpi, kAS, kBS, BM, BN, BK, WGM, WGN, kStages>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(WGM * WGN * kWave), 0, s, a);
   return hipGetLastError();
 }
@@ -605,10 +576,10 @@ hipError_t Mma(const MmaArgs& a, hipStream_t s) {
   };
   // (f32's gradient epilogue, nine planes a quad, is past the registers beside 256 x 256.)
   if constexpr (!(kEpi == kGrad && sizeof(T) == 4))
-    if (tiles(256, 256) >= 192) return LaunchTile<T, kEpi, kAS, kBS, 256, 256, 2, 4, 4>(a, s);
-  if (tiles(128, 128) >= 192) return LaunchTile<T, kEpi, kAS, kBS, 128, 128, 2, 2, 4>(a, s);
-  if constexpr (dual) return LaunchTile<T, kEpi, kAS, kBS, 64, 128, 2, 2, 4>(a, s);
-  else return LaunchTile<T, kEpi, kAS, kBS, 64, 64, 2, 2, 4>(a, s);
+    if (tiles(256, 256) >= 192) return LaunchTile<T, kEpi, kAS, kBS, 256, 256, 32, 2, kBigN, 4>(a, s);
+  if (tiles(128, 128) >= 192) return LaunchTile<T, kEpi, kAS, kBS, 128, 128, 32, 2, 2, 4>(a, s);
+  if constexpr (dual) return LaunchTile<T, kEpi, kAS, kBS, 64, 128, 32, 2, 2, 4>(a, s);
+  else return LaunchTile<T, kEpi, kAS, kBS, 64, 64, 32, 2, 2, 4>(a, s);
 }
 
 int Up8(size_t n) { return static_cast<int>((n + 7) / 8 * 8); }
@@ -661,8 +632,8 @@ hipError_t Pack(const void* in, size_t rows, size_t cols, Planes& out, hipStream
     out.p = static_cast<uint16_t*>(const_cast<void*>(in));
     return hipSuccess;
   }
-  const size_t n = rows * (out.ld / 4);
-  const bool vec = cols % 4 == 0 && at % (4 * sizeof(T)) == 0;
+  const size_t n = rows * (out.ld / 8);
+  const bool vec = cols % (16 / sizeof(T)) == 0 && (at & 15) == 0;
   hipLaunchKernelGGL((FfnPackKernel<T>), dim3(GridFor(n, 256, 4096)), dim3(256), 0, s,
                      static_cast<const T*>(in), rows, static_cast<int>(cols), vec, out);
   return hipGetLastError();
@@ -681,11 +652,12 @@ void AddProduct(MmaArgs& a, const Planes& A, const Planes& B, const Planes* B2 =
   }
 }
 
+// Rows that begin on 16 bytes.
 template <class T>
-bool Quads(size_t N, std::initializer_list<const void*> ptrs) {
+bool Octs(size_t N, std::initializer_list<const void*> ptrs) {
   uintptr_t at = 0;
   for (const void* p : ptrs) at |= reinterpret_cast<uintptr_t>(p);
-  return N % 4 == 0 && at % (4 * sizeof(T)) == 0;
+  return N % (16 / sizeof(T)) == 0 && (at & 15) == 0;
 }
 
 MmaArgs Shape(size_t M, size_t N, size_t K) {
@@ -709,11 +681,11 @@ hipError_t Fwd(const FfnArgs& f, hipStream_t s) {
   FFN_TRY(Pack<T>(f.wd, f.F, f.D, l.wd, s));
   MmaArgs a = Shape(f.M, f.F, f.D);
   AddProduct<T>(a, l.x, l.wg, &l.wu);
-  a.act = f.act, a.o1 = f.gate, a.o2 = f.up, a.h = l.h, a.vec = Quads<T>(f.F, {f.gate, f.up});
+  a.act = f.act, a.o1 = f.gate, a.o2 = f.up, a.h = l.h, a.vec = Octs<T>(f.F, {f.gate, f.up});
   FFN_TRY((Mma<T, kGate, false, true>(a, s)));
   a = Shape(f.M, f.D, f.F);
   AddProduct<T>(a, l.h, l.wd);
-  a.o1 = f.y, a.vec = Quads<T>(f.D, {f.y});
+  a.o1 = f.y, a.vec = Octs<T>(f.D, {f.y});
   return Mma<T, kPlain, false, true>(a, s);
 }
 
@@ -737,20 +709,20 @@ hipError_t Bwd(const FfnArgs& f, hipStream_t s) {
   MmaArgs a = Shape(f.M, f.F, f.D);
   AddProduct<T>(a, l.dy, l.wd);
   a.act = f.act, a.g = f.gate, a.u = f.up, a.h = l.h, a.dg = l.dg, a.du = l.du;
-  a.vec = Quads<T>(f.F, {f.gate, f.up});
+  a.vec = Octs<T>(f.F, {f.gate, f.up});
   FFN_TRY((Mma<T, kGrad, false, false>(a, s)));
   a = Shape(f.M, f.D, f.F);
   AddProduct<T>(a, l.dg, l.wg);
   AddProduct<T>(a, l.du, l.wu);
-  a.o1 = f.dx, a.vec = Quads<T>(f.D, {f.dx});
+  a.o1 = f.dx, a.vec = Octs<T>(f.D, {f.dx});
   FFN_TRY((Mma<T, kPlain, false, false>(a, s)));
   a = Shape(f.D, f.F, f.M);
   AddProduct<T>(a, l.x, l.dg, &l.du);
-  a.o1 = f.dwg, a.o2 = f.dwu, a.vec = Quads<T>(f.F, {f.dwg, f.dwu});
+  a.o1 = f.dwg, a.o2 = f.dwu, a.vec = Octs<T>(f.F, {f.dwg, f.dwu});
   FFN_TRY((Mma<T, kTwo, true, true>(a, s)));
   a = Shape(f.F, f.D, f.M);
   AddProduct<T>(a, l.h, l.dy);
-  a.o1 = f.dwd, a.vec = Quads<T>(f.D, {f.dwd});
+  a.o1 = f.dwd, a.vec = Octs<T>(f.D, {f.dwd});
   return Mma<T, kPlain, true, true>(a, s);
 }
 
