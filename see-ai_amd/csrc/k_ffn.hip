@@ -17,6 +17,7 @@
 // MFMA's.  An infinity's remainder is a NaN, so what an infinity reaches is
 // not finite but may be a NaN where f32 arithmetic has an infinity.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -46,20 +47,56 @@ __device__ __forceinline__ v4i_ Buffer(const uint16_t* base, int bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   return v4i_{Uniform(static_cast<int>(a)), Uniform(static_cast<int>(a >> 32)), Uniform(bytes), kRsrcWord3};
 }
-// 16 bytes a lane, lane after lane, straight into LDS at `lds`.  Written out
-// because the compiler lets no transposing read of LDS pass a load into LDS it
-// knows of: with its own builtin every half-stage's reads would wait for every
-// stage in flight.  It has no output register; WaitVm and a barrier stand
-// between it and the reads of what it brings.  (The wait states are those
-// between a scalar register's write, m0's included, and this use of it.)
-__device__ __forceinline__ void LoadLds(v4i_ rs, uint32_t lds, int voff, int soff) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 4\n\t"
-      "buffer_load_dwordx4 %1, %2, %3 offen lds"
-      :
-      : "s"(Uniform(lds)), "v"(voff), "s"(rs), "s"(Uniform(soff))
-      : "memory", "m0");
+// kN loads of 16 bytes a lane, lane after lane, straight into LDS at `lds` and
+// every kStep bytes on.  Written out because the compiler lets no transposing
+// read of LDS pass a load into LDS it knows of: with its own builtin every
+// step's reads would wait for every stage in flight.  They have no output
+// register; WaitVm and a barrier stand between them and the reads of what they
+// bring.  (The wait states are those between a scalar register's write, m0's
+// included, and this use of it.)
+template <int kN, int kStep>
+__device__ __forceinline__ void LoadLds(v4i_ rs, uint32_t lds, const int* voff, int soff) {
+  if constexpr (kN == 1) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %2, %3 offen lds"
+        :
+        : "s"(Uniform(lds)), "v"(voff[0]), "s"(rs), "s"(Uniform(soff))
+        : "memory", "m0");
+  } else if constexpr (kN == 2) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %3, %4 offen lds\n\t"
+        "s_add_u32 m0, m0, %5\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %2, %3, %4 offen lds"
+        :
+        : "s"(Uniform(lds)), "v"(voff[0]), "v"(voff[1]), "s"(rs), "s"(Uniform(soff)), "n"(kStep)
+        : "memory", "m0", "scc");
+  } else if constexpr (kN != 4) {
+    LoadLds<2, kStep>(rs, lds, voff, soff);
+    LoadLds<kN - 2, kStep>(rs, lds + 2 * kStep, voff + 2, soff);
+  } else {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %5, %6 offen lds\n\t"
+        "s_add_u32 m0, m0, %7\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %2, %5, %6 offen lds\n\t"
+        "s_add_u32 m0, m0, %7\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %3, %5, %6 offen lds\n\t"
+        "s_add_u32 m0, m0, %7\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %4, %5, %6 offen lds"
+        :
+        : "s"(Uniform(lds)), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(rs),
+          "s"(Uniform(soff)), "n"(kStep)
+        : "memory", "m0", "scc");
+  }
 }
 
 // Until this wave's LDS reads have returned.
@@ -229,12 +266,15 @@ struct MmaArgs {
   int M, N, K;
   int act;
   bool vec;           // outputs (and G, U) take eight neighbours at once
+  // Where K is shared out over blockIdx.y, `per_split` stages each: the f32
+  // sums [split][M][tiles' operands][N up to 8s] that FfnJoin adds and finishes.
+  float* part;
+  int per_split;
   void *o1, *o2;      // plain: o1 (and o2 of B2); gate: G and U or null
   const void *g, *u;  // gradient: G and U
   Planes h, dg, du;
 };
 
-constexpr int kBigN = 4;
 enum Epilogue {
   kPlain,  // o1 = sum A B
   kTwo,    // o1 = sum A B, o2 = sum A B2
@@ -302,16 +342,20 @@ struct Tile {
       }
     }
   }
-  // Wave-load j of stage [k0, k0 + kBK) of the operand at `at` (its tile's
-  // corner) into LDS.
+  // Wave-loads [j, j + kN) of stage [k0, k0 + kBK) of the operand at `at` (its
+  // tile's corner) into LDS.
+  template <int kN>
   __device__ __forceinline__ void Load(const uint16_t* at, int k0, int K, uint32_t lds, int wave, int j) {
     const uint32_t to = lds + (j * kWaves + wave) * 1024;
     if constexpr (kStrided) {
       const int rows = min(K - k0, kBK);
-      LoadLds(Buffer(at + static_cast<size_t>(k0) * ld, ((rows - 1) * ld + extent) * 2), to, voff[j], 0);
+      LoadLds<kN, kWaves * 1024>(
+          Buffer(at + static_cast<size_t>(k0) * ld, ((rows - 1) * ld + extent) * 2), to, voff + j, 0);
     } else {
-      const bool tail = k0 + kBK > k8;
-      LoadLds(Buffer(at, extent * ld * 2), to, tail && k0 + kc[j] >= k8 ? kFar : voff[j], k0 * 2);
+      int v[kN];
+#pragma unroll
+      for (int l = 0; l < kN; ++l) v[l] = k0 + kc[j + l] >= k8 ? kFar : voff[j + l];
+      LoadLds<kN, kWaves * 1024>(Buffer(at, extent * ld * 2), to, v, k0 * 2);
     }
   }
   // Byte offset in the tile of lane l's part of the fragment of rows (columns)
@@ -338,6 +382,77 @@ struct Tile {
   }
   static constexpr int kReads = kStrided ? 2 : 1;  // LDS reads of a fragment
 };
+
+// Eight neighbours of an output row from their sums: c of A B, d of A B2.
+template <class T, int kEpi>
+__device__ __forceinline__ void Finish(const MmaArgs& p, int m, int n, float (&c)[8], float (&d)[8]) {
+  const int cnt = p.N - n;
+  const size_t o = static_cast<size_t>(m) * p.N + n;
+  if constexpr (kEpi == kPlain || kEpi == kTwo) {
+    Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
+    if constexpr (kEpi == kTwo) Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
+  }
+  if constexpr (kEpi == kGate) {
+    if (p.o1) {
+      Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
+      Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float a, da;
+      Activate<sizeof(T) == 2>(p.act, c[e], a, da);
+      c[e] = e < cnt ? a * d[e] : 0.0f;
+    }
+    PutPlanes<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
+  }
+  if constexpr (kEpi == kGrad) {
+    float g[8], u[8], y[8];
+    Load8(static_cast<const T*>(p.g) + o, p.vec, cnt, g);
+    Load8(static_cast<const T*>(p.u) + o, p.vec, cnt, u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float a, da;
+      Activate<sizeof(T) == 2>(p.act, g[e], a, da);
+      const bool in = e < cnt;
+      g[e] = in ? c[e] * u[e] * da : 0.0f;
+      y[e] = in ? c[e] * a : 0.0f;
+      u[e] = in ? a * u[e] : 0.0f;
+    }
+    const size_t w = static_cast<size_t>(m) * p.h.ld + n;
+    PutPlanes<T>(p.dg, w, g);
+    PutPlanes<T>(p.du, w, y);
+    PutPlanes<T>(p.h, w, u);
+  }
+}
+
+// The workgroups' sums of a product whose K was shared out, added in order and
+// finished.
+template <class T, int kEpi>
+__global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int splits) {
+  constexpr int kBoth = kEpi == kTwo || kEpi == kGate ? 2 : 1;
+  const int np = (p.N + 7) & ~7, octs = np / 8;
+  const size_t n = static_cast<size_t>(p.M) * octs, step = static_cast<size_t>(gridDim.x) * 256;
+  for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
+    const int m = static_cast<int>(i / octs), col = static_cast<int>(i % octs) * 8;
+    float s[2][8] = {};
+    for (int k0 = 0; k0 < splits; k0 += 4) {  // four sums' loads in flight
+      float v[4][kBoth][8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b)
+          Load8(p.part + ((static_cast<size_t>(min(k0 + k, splits - 1)) * p.M + m) * kBoth + b) * np + col,
+                true, 8, v[k][b]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < splits ? v[k][b][e] : 0.0f;
+    }
+    Finish<T, kEpi>(p, m, col, s[0], s[1]);
+  }
+}
 
 template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
 __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
@@ -367,22 +482,32 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   const size_t b_at = kBS ? static_cast<size_t>(n0) : static_cast<size_t>(n0) * p.ldb;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPtr)smem));
 
-  const int per_seg = (p.K + BK - 1) / BK, last = p.nseg * per_seg - 1;
+  const int per_seg = (p.K + BK - 1) / BK, first = blockIdx.y * p.per_split;
+  const int last = min(p.nseg * per_seg - first, p.per_split) - 1;
   // The next stage to load, and its segment's operands.
-  int seg = 0, k0 = 0;
-  const uint16_t *pa = p.A[0] + a_at, *pb = p.B[0] + b_at, *pb2 = kDual ? p.B2[0] + b_at : nullptr;
-  // Part `part` of kSub of the next stage's loads into buffer `buf`.
+  int seg = first / per_seg, k0 = (first - seg * per_seg) * BK;
+  const uint16_t *pa = p.A[seg] + a_at, *pb = p.B[seg] + b_at;
+  const uint16_t* pb2 = kDual ? p.B2[seg] + b_at : nullptr;
+  // Part `part` of kParts of the next stage's loads into buffer `buf`.  With
+  // two buffers the stage is wanted at this one's end: its first half's steps.
+  constexpr int kParts = kStages == 2 ? kSub / 2 : kSub;
   auto issue = [&](int buf, auto part_tag) __attribute__((always_inline)) {
     constexpr int part = decltype(part_tag)::value;
     const uint32_t s = lds0 + buf * kStage;
-#pragma unroll
-    for (int l = part * kPerStage / kSub; l < (part + 1) * kPerStage / kSub; ++l) {
-      if (l < TA::kLoads) ta.Load(pa, k0, p.K, s, wave, l);
-      else if (l < TA::kLoads + TBt::kLoads) tb.Load(pb, k0, p.K, s + TA::kBytes, wave, l - TA::kLoads);
-      else tb.Load(pb2, k0, p.K, s + TA::kBytes + TBt::kBytes, wave, l - TA::kLoads - TBt::kLoads);
-    }
+    // The stage's loads are A's, B's and B2's in turn; a part is a run of them
+    // from one operand or a whole number of operands.
+    constexpr int kLo = part * kPerStage / kParts, kHi = (part + 1) * kPerStage / kParts;
+    constexpr int kB = TA::kLoads, kB2 = TA::kLoads + TBt::kLoads;
+    constexpr int a0 = kLo, an = std::min(kHi, kB) - a0;
+    constexpr int b0 = std::max(kLo, kB), bn = std::min(kHi, kB2) - b0;
+    constexpr int c0 = std::max(kLo, kB2), cn = kHi - c0;
+    if constexpr (an > 0) ta.template Load<an>(pa, k0, p.K, s, wave, a0);
+    if constexpr (bn > 0) tb.template Load<bn>(pb, k0, p.K, s + TA::kBytes, wave, b0 - kB);
+    if constexpr (cn > 0)
+      tb.template Load<cn>(pb2, k0, p.K, s + TA::kBytes + TBt::kBytes, wave, c0 - kB2);
   };
-  // Past the last stage the loads repeat it, into buffers nothing reads.
+  // Past this workgroup's last stage the loads go on, past the product's they
+  // repeat, into buffers nothing reads.
   auto advance = [&]() __attribute__((always_inline)) {
     if (k0 + BK < p.K) {
       k0 += BK;
@@ -441,19 +566,20 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   // all at once they would hold up the products behind them.
   auto steps = [&](int buf, int to, auto load) __attribute__((always_inline)) {
     Each<kSub - 1>([&](auto ks) __attribute__((always_inline)) {
-      if constexpr (decltype(load)::value) issue(to, ks);
+      if constexpr (decltype(load)::value && decltype(ks)::value < kParts) issue(to, ks);
       read(buf, std::integral_constant<int, decltype(ks)::value + 1>{});
       mfmas(decltype(ks)::value % 2);
       interleave();
     });
-    if constexpr (decltype(load)::value) issue(to, std::integral_constant<int, kSub - 1>{});
+    if constexpr (decltype(load)::value && kParts == kSub)
+      issue(to, std::integral_constant<int, kSub - 1>{});
   };
 
   // kStages buffers: one multiplied, one taking loads, the others in flight or
   // landed.  Before the last step of stage `it` every wave has its fragments of
   // it and stage it + 1 has landed.
   for (int s = 0; s < kStages - 1; ++s) {
-    Each<kSub>([&](auto part) __attribute__((always_inline)) { issue(s, part); });
+    Each<kParts>([&](auto part) __attribute__((always_inline)) { issue(s, part); });
     advance();
   }
   WaitVm<(kStages - 2) * kPerStage>();
@@ -496,7 +622,7 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
           }
       __builtin_amdgcn_wave_barrier();
       const int mb = m0 + wm + i * 32, nb = n0 + wn + jb * kW;
-      if ((kEpi == kPlain || kEpi == kTwo) && !p.vec) {
+      if ((kEpi == kPlain || kEpi == kTwo) && !p.vec && !p.part) {
         // Rows off 16 bytes: a lane a column.
         const int n = nb + lane % kW;
         for (int r = lane / kW; r < 32; r += kWave / kW) {
@@ -507,49 +633,21 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
           }
         }
       } else {
-        const int n = nb + (lane % kPerRow) * 8, cnt = p.N - n;
+        const int n = nb + (lane % kPerRow) * 8;
 #pragma unroll
         for (int t = 0; t < 32 / kRows; ++t) {
           const int r = lane / kPerRow + t * kRows, m = mb + r;
-          if (m >= p.M || cnt <= 0) continue;
-          const size_t o = static_cast<size_t>(m) * p.N + n;
+          if (m >= p.M || n >= p.N) continue;
           float c[8], d[8];
           Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
           if constexpr (kDual) Load8(st + (32 + r) * kPad + (lane % kPerRow) * 8, true, 8, d);
-          if constexpr (kEpi == kPlain || kEpi == kTwo) {
-            Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
-            if constexpr (kEpi == kTwo) Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
-          }
-          if constexpr (kEpi == kGate) {
-            if (p.o1) {
-              Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
-              Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float a, da;
-              Activate<sizeof(T) == 2>(p.act, c[e], a, da);
-              c[e] = e < cnt ? a * d[e] : 0.0f;
-            }
-            PutPlanes<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
-          }
-          if constexpr (kEpi == kGrad) {
-            float g[8], u[8], y[8];
-            Load8(static_cast<const T*>(p.g) + o, p.vec, cnt, g);
-            Load8(static_cast<const T*>(p.u) + o, p.vec, cnt, u);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float a, da;
-              Activate<sizeof(T) == 2>(p.act, g[e], a, da);
-              const bool in = e < cnt;
-              g[e] = in ? c[e] * u[e] * da : 0.0f;
-              y[e] = in ? c[e] * a : 0.0f;
-              u[e] = in ? a * u[e] : 0.0f;
-            }
-            const size_t w = static_cast<size_t>(m) * p.h.ld + n;
-            PutPlanes<T>(p.dg, w, g);
-            PutPlanes<T>(p.du, w, y);
-            PutPlanes<T>(p.h, w, u);
+          if (p.part) {
+            const int np = (p.N + 7) & ~7;
+            float* out = p.part + (static_cast<size_t>(blockIdx.y) * p.M + m) * kBoth * np + n;
+            Store8(out, true, 8, c);
+            if constexpr (kDual) Store8(out + np, true, 8, d);
+          } else {
+            Finish<T, kEpi>(p, m, n, c, d);
           }
         }
       }
@@ -559,27 +657,80 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
 
 // --- host ---------------------------------------------------------------------------------------
 
+// How a product runs: its tile, and over how many workgroups a tile's K is
+// shared out.
+struct Plan {
+  int tile = 0;  // of kTiles
+  int splits = 1, per_split = 0;
+};
+struct TileShape {
+  int bm, bn, per_cu;  // rows, columns over all operands, workgroups a CU holds
+  double alone, shared;  // us of a 64-deep stage: on an idle chip, and more per workgroup a CU
+};
+constexpr TileShape kTiles[3] = {{256, 256, 1, 1.0, 0.9}, {128, 128, 2, 0.4, 0.45}, {64, 64, 2, 0.2, 0.2}};
+constexpr int kDeep = 64;
+constexpr size_t kMostPart = size_t{64} << 20;  // bytes of shared-out sums
+Plan Choose(bool dual, size_t M, size_t N, size_t K, int nseg) {
+  const int both = dual ? 2 : 1;
+  const double stages = static_cast<double>((K + kDeep - 1) / kDeep) * nseg;
+  const double np = static_cast<double>((N + 7) / 8 * 8);
+  Plan best;
+  double least = 1e30;
+  for (int t = 0; t < 3; ++t) {
+    const TileShape& s = kTiles[t];
+    const int bn = dual ? (t == 2 ? 64 : s.bn / 2) : s.bn;  // output columns of a tile
+    const double tiles = std::ceil(static_cast<double>(M) / s.bm) * std::ceil(static_cast<double>(N) / bn);
+    const double more = t == 2 && dual ? 2.0 : 1.0;  // its 64 x 128 of both operands
+    for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (k > 1 && (k * 2 > stages || k * M * both * np * 4 > kMostPart)) break;
+      const double per = std::ceil(stages / k), wgs = tiles * std::ceil(stages / per);
+      const double rounds = std::ceil(wgs / (256.0 * s.per_cu));
+      const double held = std::min<double>(s.per_cu, wgs / 256.0);
+      double us = rounds * per * (s.alone + more * held * s.shared) + 5;
+      if (k > 1) us += 4 + 0.2 * k + k * M * both * np * 8 / 3.5e6;
+      if (us < least) {
+        least = us;
+        best = {t, static_cast<int>(std::ceil(stages / per)), static_cast<int>(per)};
+      }
+    }
+  }
+  return best;
+}
+size_t PartBytes(const Plan& plan, bool dual, size_t M, size_t N) {
+  return plan.splits == 1 ? 0 : plan.splits * M * (dual ? 2 : 1) * ((N + 7) / 8 * 8) * 4;
+}
+
 template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
-hipError_t LaunchTile(const MmaArgs& a, hipStream_t s) {
+hipError_t LaunchTile(const MmaArgs& a, int splits, hipStream_t s) {
+  static_assert(BK == kDeep, "per_split counts such stages");
   constexpr int BNs = kEpi == kTwo || kEpi == kGate ? BN / 2 : BN;
   const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BNs - 1) / BNs);
   auto* kernel = &FfnMma<T, kEpi, kAS, kBS, BM, BN, BK, WGM, WGN, kStages>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(WGM * WGN * kWave), 0, s, a);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles), splits), dim3(WGM * WGN * kWave), 0, s, a);
   return hipGetLastError();
 }
 
+// `part`: where a shared-out product's sums go (PartBytes).
 template <class T, int kEpi, bool kAS, bool kBS>
-hipError_t Mma(const MmaArgs& a, hipStream_t s) {
+hipError_t Mma(MmaArgs a, float* part, hipStream_t s) {
   constexpr bool dual = kEpi == kTwo || kEpi == kGate;
-  auto tiles = [&](int bm, int bn) {
-    return static_cast<int64_t>((a.M + bm - 1) / bm) * ((a.N + (dual ? bn / 2 : bn) - 1) / (dual ? bn / 2 : bn));
-  };
+  const Plan plan = Choose(dual, a.M, a.N, a.K, a.nseg);
+  a.per_split = plan.per_split;
+  a.part = plan.splits > 1 ? part : nullptr;
+  hipError_t e;
   // (f32's gradient epilogue, nine planes a quad, is past the registers beside 256 x 256.)
-  if constexpr (!(kEpi == kGrad && sizeof(T) == 4))
-    if (tiles(256, 256) >= 192) return LaunchTile<T, kEpi, kAS, kBS, 256, 256, 32, 2, kBigN, 4>(a, s);
-  if (tiles(128, 128) >= 192) return LaunchTile<T, kEpi, kAS, kBS, 128, 128, 32, 2, 2, 4>(a, s);
-  if constexpr (dual) return LaunchTile<T, kEpi, kAS, kBS, 64, 128, 32, 2, 2, 4>(a, s);
-  else return LaunchTile<T, kEpi, kAS, kBS, 64, 64, 32, 2, 2, 4>(a, s);
+  constexpr bool big = !(kEpi == kGrad && sizeof(T) == 4);
+  if constexpr (big) {
+    if (plan.tile == 0) e = LaunchTile<T, kEpi, kAS, kBS, 256, 256, 64, 2, 4, 2>(a, plan.splits, s);
+  }
+  if (plan.tile == 1 || (!big && plan.tile == 0))
+    e = LaunchTile<T, kEpi, kAS, kBS, 128, 128, 64, 2, 2, 2>(a, plan.splits, s);
+  if (plan.tile == 2) e = LaunchTile<T, kEpi, kAS, kBS, 64, dual ? 128 : 64, 64, 2, 2, dual ? 3 : 4>(a, plan.splits, s);
+  if (e != hipSuccess || plan.splits == 1) return e;
+  const size_t n = static_cast<size_t>(a.M) * ((a.N + 7) / 8);
+  auto* kernel = &FfnJoin<T, kEpi>;
+  hipLaunchKernelGGL(kernel, dim3(GridFor(n, 256, 4096)), dim3(256), 0, s, a, plan.splits);
+  return hipGetLastError();
 }
 
 int Up8(size_t n) { return static_cast<int>((n + 7) / 8 * 8); }
@@ -596,6 +747,11 @@ class Space {
     used_ += (p.plane * planes * 2 + 255) / 256 * 256;
     return p;
   }
+  float* Floats(size_t bytes) {
+    float* p = reinterpret_cast<float*>(base_ + used_);
+    used_ += (bytes + 255) / 256 * 256;
+    return p;
+  }
   size_t used() const { return used_; }
 
  private:
@@ -605,6 +761,7 @@ class Space {
 
 struct Layout {
   Planes x, wg, wu, wd, dy, h, dg, du;
+  float* part;
   size_t bytes;
 };
 Layout Lay(void* ws, int planes, size_t M, size_t D, size_t F, bool backward) {
@@ -620,6 +777,13 @@ Layout Lay(void* ws, int planes, size_t M, size_t D, size_t F, bool backward) {
     l.dg = s.Take(M, F, planes);
     l.du = s.Take(M, F, planes);
   }
+  const int nseg = planes == 1 ? 1 : 6;
+  auto part = [&](bool dual, size_t m, size_t n, size_t k, int segs) {
+    return PartBytes(Choose(dual, m, n, k, segs), dual, m, n);
+  };
+  l.part = s.Floats(backward ? std::max({part(false, M, F, D, nseg), part(false, M, D, F, 2 * nseg),
+                                         part(true, D, F, M, nseg), part(false, F, D, M, nseg)})
+                             : std::max(part(true, M, F, D, nseg), part(false, M, D, F, nseg)));
   l.bytes = s.used();
   return l;
 }
@@ -682,11 +846,11 @@ hipError_t Fwd(const FfnArgs& f, hipStream_t s) {
   MmaArgs a = Shape(f.M, f.F, f.D);
   AddProduct<T>(a, l.x, l.wg, &l.wu);
   a.act = f.act, a.o1 = f.gate, a.o2 = f.up, a.h = l.h, a.vec = Octs<T>(f.F, {f.gate, f.up});
-  FFN_TRY((Mma<T, kGate, false, true>(a, s)));
+  FFN_TRY((Mma<T, kGate, false, true>(a, l.part, s)));
   a = Shape(f.M, f.D, f.F);
   AddProduct<T>(a, l.h, l.wd);
   a.o1 = f.y, a.vec = Octs<T>(f.D, {f.y});
-  return Mma<T, kPlain, false, true>(a, s);
+  return Mma<T, kPlain, false, true>(a, l.part, s);
 }
 
 template <class T>
@@ -710,20 +874,20 @@ hipError_t Bwd(const FfnArgs& f, hipStream_t s) {
   AddProduct<T>(a, l.dy, l.wd);
   a.act = f.act, a.g = f.gate, a.u = f.up, a.h = l.h, a.dg = l.dg, a.du = l.du;
   a.vec = Octs<T>(f.F, {f.gate, f.up});
-  FFN_TRY((Mma<T, kGrad, false, false>(a, s)));
+  FFN_TRY((Mma<T, kGrad, false, false>(a, l.part, s)));
   a = Shape(f.M, f.D, f.F);
   AddProduct<T>(a, l.dg, l.wg);
   AddProduct<T>(a, l.du, l.wu);
   a.o1 = f.dx, a.vec = Octs<T>(f.D, {f.dx});
-  FFN_TRY((Mma<T, kPlain, false, false>(a, s)));
+  FFN_TRY((Mma<T, kPlain, false, false>(a, l.part, s)));
   a = Shape(f.D, f.F, f.M);
   AddProduct<T>(a, l.x, l.dg, &l.du);
   a.o1 = f.dwg, a.o2 = f.dwu, a.vec = Octs<T>(f.F, {f.dwg, f.dwu});
-  FFN_TRY((Mma<T, kTwo, true, true>(a, s)));
+  FFN_TRY((Mma<T, kTwo, true, true>(a, l.part, s)));
   a = Shape(f.F, f.D, f.M);
   AddProduct<T>(a, l.h, l.dy);
   a.o1 = f.dwd, a.vec = Octs<T>(f.D, {f.dwd});
-  return Mma<T, kPlain, true, true>(a, s);
+  return Mma<T, kPlain, true, true>(a, l.part, s);
 }
 
 }  // namespace
