@@ -667,7 +667,7 @@ struct TileShape {
   int bm, bn, per_cu;  // rows, columns over all operands, workgroups a CU holds
   double alone, shared;  // us of a 64-deep stage: on an idle chip, and more per workgroup a CU
 };
-constexpr TileShape kTiles[3] = {{256, 256, 1, 1.0, 0.9}, {128, 128, 2, 0.4, 0.45}, {64, 64, 2, 0.2, 0.2}};
+constexpr TileShape kTiles[3] = {{256, 256, 1, 1.0, 0.9}, {128, 128, 2, 0.4, 0.45}, {64, 64, 2, 0.3, 0.2}};
 constexpr int kDeep = 64;
 constexpr size_t kMostPart = size_t{64} << 20;  // bytes of shared-out sums
 Plan Choose(bool dual, size_t M, size_t N, size_t K, int nseg) {

@@ -128,15 +128,15 @@ __device__ __forceinline__ void LoadVec(const float* w, int t, int cols, float (
   }
 }
 
-// Sums over the kTPR threads of a row: within the wave, then over its waves
-// through LDS (kTPR > 64: the whole workgroup is one row).
+// Sums over the kTPR threads of each row of a workgroup: within the wave, then
+// over a row's waves through LDS (two floats a wave).
 template <int kTPR, int kN>
 __device__ __forceinline__ void RowSum(float (&s)[kN], float* lds) {
 #pragma unroll
   for (int i = 0; i < kN; ++i) s[i] = WaveSumF(s[i]);
   if constexpr (kTPR > kWave) {
     constexpr int kWaves = kTPR / kWave;
-    const int w = threadIdx.x / kWave;
+    const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
     __syncthreads();  // the sums before these have been read
     if (threadIdx.x % kWave == 0)
 #pragma unroll
@@ -146,12 +146,16 @@ __device__ __forceinline__ void RowSum(float (&s)[kN], float* lds) {
     for (int i = 0; i < kN; ++i) {
       s[i] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) s[i] += lds[k * kN + i];
+      for (int k = 0; k < kWaves; ++k) s[i] += lds[(first + k) * kN + i];
     }
   }
 }
 
 constexpr int Threads(int tpr) { return tpr > 256 ? tpr : 256; }
+// The backward's workgroup: eight waves, so that few workgroups fill the chip
+// and few partial rows are left.
+constexpr int kBwdPerSimd = 4;
+constexpr int BwdThreads(int tpr) { return tpr > 512 ? tpr : 512; }
 
 template <class T, int kTPR, int kE, bool kVec>
 __global__ void __launch_bounds__(Threads(kTPR))
@@ -161,11 +165,13 @@ NormFwdKernel(int rms, const T* __restrict__ x, const float* __restrict__ w,
   __shared__ float lds[16];
   constexpr int kRows = Threads(kTPR) / kTPR;
   const int t = threadIdx.x % kTPR;
-  // (the loop is uniform over a row's threads, its barriers too)
-  for (size_t r = static_cast<size_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; r < rows;
-       r += static_cast<size_t>(gridDim.x) * kRows) {
+  // (the loop is uniform over the workgroup, its barriers too)
+  for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < rows;
+       base += static_cast<size_t>(gridDim.x) * kRows) {
+    const size_t r = base + threadIdx.x / kTPR;
+    const bool in = r < rows;
     float v[kE];
-    LoadRow<T, kTPR, kE, kVec>(x + r * cols, t, cols, v);
+    LoadRow<T, kTPR, kE, kVec>(x + r * cols, t, in ? cols : 0, v);
     float mu[1] = {0.0f};
     if (!rms) {
 #pragma unroll
@@ -190,6 +196,7 @@ NormFwdKernel(int rms, const T* __restrict__ x, const float* __restrict__ w,
 #pragma unroll
       for (int e = 0; e < kE; ++e) v[e] += ww[e];
     }
+    if (!in) continue;
     StoreRow<T, kTPR, kE, kVec>(y + r * cols, t, cols, v);
     if (t == 0) {
       if (mean) mean[r] = mu[0];
@@ -198,44 +205,106 @@ NormFwdKernel(int rms, const T* __restrict__ x, const float* __restrict__ w,
   }
 }
 
-// Workgroup g takes rows g kRows + i, stepping the grid; out: [gridDim][2][cols]
-// partials (db behind dw), or dw and db themselves when the grid is one.
+// A row as it lies in memory, for loads that run ahead of their use.
 template <class T, int kTPR, int kE, bool kVec>
-__global__ void __launch_bounds__(Threads(kTPR))
+struct RawRow {
+  static constexpr int kV = Io<T>::kV;
+  uint4 q[kVec ? kE / kV : 1];
+  T e[kVec ? 1 : kE];
+  __device__ __forceinline__ void Load(const T* row, int t, int cols) {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < kE / kV; ++i) {
+        const int c = ColOf<T, kTPR, true>(t, i * kV);
+        q[i] = c < cols ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        const int c = ColOf<T, kTPR, false>(t, i);
+        e[i] = c < cols ? row[c] : T(0);
+      }
+    }
+  }
+  __device__ __forceinline__ void Get(float (&v)[kE]) const {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < kE / kV; ++i) Io<T>::Load(reinterpret_cast<const T*>(&q[i]), v + i * kV);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) v[i] = Io<T>::Get(&e[i]);
+    }
+  }
+};
+
+// Workgroup g takes rows g kRows + i, stepping the grid; out: [gridDim][2][cols]
+// partials (db behind dw), or dw and db themselves when the grid is one.  A
+// row's loads go out while the row before it is reduced: with a wave a row
+// there is nothing else to cover their latency (8192 x 2048 bf16 on MI355X: 30
+// us with, 41 without; the copy rate would be 20).  The weight sits in LDS, a lane's own columns together, to
+// leave the registers to that row.
+template <class T, int kTPR, int kE, bool kVec>
+__global__ void __launch_bounds__(BwdThreads(kTPR), kBwdPerSimd)
 NormBwdKernel(int rms, const T* __restrict__ dy, const T* __restrict__ x,
               const float* __restrict__ w, const float* __restrict__ mean,
               const float* __restrict__ rstd, T* __restrict__ dx, float* __restrict__ dw,
               float* __restrict__ db, float* __restrict__ part, size_t rows, int cols) {
-  constexpr int kRows = Threads(kTPR) / kTPR;
+  constexpr int kRows = BwdThreads(kTPR) / kTPR;
   __shared__ float lds[32];
-  __shared__ float fold[kRows > 1 ? kTPR * kE : 1];
+  __shared__ float own[kTPR * kE];  // element e of thread t at ((e / 4) kTPR + t) 4 + e % 4
   const int t = threadIdx.x % kTPR, sub = threadIdx.x / kTPR;
+  auto at = [&](int e) { return (e / 4 * kTPR + t) * 4 + e % 4; };
   const float inv = 1.0f / static_cast<float>(cols);
-  float ww[kE], sw[kE], sb[kE];
-  LoadVec<T, kTPR, kE, kVec>(w, t, cols, ww);
+  float sw[kE], sb[kE];
+  if (sub == 0) {
+    LoadVec<T, kTPR, kE, kVec>(w, t, cols, sw);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) own[at(e)] = sw[e];
+  }
+  __syncthreads();
 #pragma unroll
   for (int e = 0; e < kE; ++e) sw[e] = sb[e] = 0.0f;
-  for (size_t r = static_cast<size_t>(blockIdx.x) * kRows + sub; r < rows;
-       r += static_cast<size_t>(gridDim.x) * kRows) {
+  const size_t step = static_cast<size_t>(gridDim.x) * kRows;
+  size_t base = static_cast<size_t>(blockIdx.x) * kRows;  // of the workgroup's next rows
+  RawRow<T, kTPR, kE, kVec> rx, rd;
+  float mu = 0.0f, rs = 0.0f;
+  auto fetch = [&]() {  // past the last row: dy = 0 adds nothing
+    const size_t r = base + sub;
+    const int in = r < rows ? cols : 0;
+    rx.Load(x + r * cols, t, in);
+    rd.Load(dy + r * cols, t, in);
+    mu = rms || !in ? 0.0f : mean[r], rs = in ? rstd[r] : 0.0f;
+  };
+  fetch();
+  while (base < rows) {  // (uniform over the workgroup, its barriers too)
     float v[kE], d[kE];
-    LoadRow<T, kTPR, kE, kVec>(x + r * cols, t, cols, v);
-    LoadRow<T, kTPR, kE, kVec>(dy + r * cols, t, cols, d);
-    const float mu = rms ? 0.0f : mean[r], rs = rstd[r];
+    rx.Get(v);
+    rd.Get(d);
+    const float m = mu, q = rs;
+    const bool in = base + sub < rows;
+    T* out = dx + (base + sub) * cols;
+    base += step;
+    fetch();
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {  // (columns past the row: d = 0, so no term)
-      v[e] = (v[e] - mu) * rs;
-      sw[e] += d[e] * v[e];
-      sb[e] += d[e];
-      d[e] *= ww[e];
-      s[0] += d[e];
-      s[1] += d[e] * v[e];
+    for (int e = 0; e < kE; e += 4) {  // (columns past the row: d = 0, so no term)
+      const float4 w4 = *reinterpret_cast<const float4*>(own + at(e));
+      const float ww[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[e + i] = (v[e + i] - m) * q;
+        sw[e + i] += d[e + i] * v[e + i];
+        sb[e + i] += d[e + i];
+        d[e + i] *= ww[i];
+        s[0] += d[e + i];
+        s[1] += d[e + i] * v[e + i];
+      }
     }
     RowSum<kTPR>(s, lds);
     const float c1 = rms ? 0.0f : s[0] * inv, c2 = s[1] * inv;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) d[e] = rs * (d[e] - c1 - v[e] * c2);
-    StoreRow<T, kTPR, kE, kVec>(dx + r * cols, t, cols, d);
+    for (int e = 0; e < kE; ++e) d[e] = q * (d[e] - c1 - v[e] * c2);
+    if (in) StoreRow<T, kTPR, kE, kVec>(out, t, cols, d);
   }
   // The workgroup's row groups add up in order; the last holds the sum.
   if constexpr (kRows > 1) {
@@ -246,8 +315,8 @@ NormBwdKernel(int rms, const T* __restrict__ dy, const T* __restrict__ x,
         if (sub == g) {
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            if (g > 0) s[e] = fold[e * kTPR + t] + s[e];
-            fold[e * kTPR + t] = s[e];
+            if (g > 0) s[e] = own[at(e)] + s[e];
+            own[at(e)] = s[e];
           }
         }
       }
@@ -390,17 +459,19 @@ struct NormCall {
 
 template <class T, int kTPR, int kE, bool kVec>
 hipError_t Run(const NormCall& a, bool bwd, hipStream_t s) {
-  constexpr int kRows = Threads(kTPR) / kTPR;
-  const size_t groups = (a.rows + kRows - 1) / kRows;
   const int cols = static_cast<int>(a.cols);
   if (!bwd) {
+    constexpr int kRows = Threads(kTPR) / kTPR;
+    const size_t groups = (a.rows + kRows - 1) / kRows;
     hipLaunchKernelGGL((NormFwdKernel<T, kTPR, kE, kVec>), Grid(groups), dim3(Threads(kTPR)), 0, s, a.rms,
                        static_cast<const T*>(a.x), a.w, a.b,
                        static_cast<T*>(a.out), a.o1, a.o2, a.rows, cols, a.eps);
     return hipGetLastError();
   }
+  constexpr int kThreads = BwdThreads(kTPR), kRows = kThreads / kTPR;
+  const size_t groups = (a.rows + kRows - 1) / kRows;
   const unsigned grid = static_cast<unsigned>(groups < kBwdGroups ? (groups ? groups : 1) : kBwdGroups);
-  hipLaunchKernelGGL((NormBwdKernel<T, kTPR, kE, kVec>), dim3(grid), dim3(Threads(kTPR)), 0, s,
+  hipLaunchKernelGGL((NormBwdKernel<T, kTPR, kE, kVec>), dim3(grid), dim3(kThreads), 0, s,
                      a.rms, static_cast<const T*>(a.dy), static_cast<const T*>(a.x), a.w, a.mean,
                      a.rstd, static_cast<T*>(a.out), a.o1, a.o2, a.part, a.rows, cols);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || grid == 1) return e;
@@ -413,11 +484,14 @@ hipError_t Run(const NormCall& a, bool bwd, hipStream_t s) {
 
 template <class T, bool kVec>
 hipError_t Pick(const NormCall& a, bool bwd, hipStream_t s) {
+  // Eight elements a lane: four waves a SIMD.  With sixteen the backward's sums
+  // and the row in flight leave it two (8192 x 2048 bf16: 30 us either way;
+  // 3001 x 1023 f32, single elements: 17 us against 16).
   if (a.cols <= 512) return Run<T, 64, 8, kVec>(a, bwd, s);
-  if (a.cols <= 1024) return Run<T, 64, 16, kVec>(a, bwd, s);
-  if (a.cols <= 2048) return Run<T, 64, 32, kVec>(a, bwd, s);
-  if (a.cols <= 4096) return Run<T, 256, 16, kVec>(a, bwd, s);
-  if (a.cols <= 8192) return Run<T, 256, 32, kVec>(a, bwd, s);
+  if (a.cols <= 1024) return Run<T, 128, 8, kVec>(a, bwd, s);
+  if (a.cols <= 2048) return Run<T, 256, 8, kVec>(a, bwd, s);
+  if (a.cols <= 4096) return Run<T, 512, 8, kVec>(a, bwd, s);
+  if (a.cols <= 8192) return Run<T, 1024, 8, kVec>(a, bwd, s);
   return Run<T, 1024, 16, kVec>(a, bwd, s);
 }
 
