@@ -664,10 +664,20 @@ struct Plan {
   int splits = 1, per_split = 0;
 };
 struct TileShape {
-  int bm, bn, per_cu;  // rows, columns over all operands, workgroups a CU holds
-  double alone, shared;  // us of a 64-deep stage: on an idle chip, and more per workgroup a CU
+  int bm, bn, bn_dual, per_cu;  // rows, output columns, workgroups a CU holds
+  // us of a stage of one product and of two side by side: on an idle chip, and
+  // more for every workgroup a CU holds.
+  double alone, shared, alone_dual, shared_dual;
 };
-constexpr TileShape kTiles[3] = {{256, 256, 1, 1.0, 0.9}, {128, 128, 2, 0.4, 0.45}, {64, 64, 2, 0.3, 0.2}};
+// Fitted to some 600 timings (three tiles, K shared out over 1 to 32, 39
+// products from 1 x 5632 x 2048 to 8192 x 2048 x 5632, both types), mean error
+// 12 %; the tile and sharing it picks were within 6 % of the best on average
+// (16 % the worst that was no outlier).  Few tokens take the 64-row tile with
+// K shared out -- 24 x 2048 x 5632: 10 us over 8, 25 us over 1, 95 us on 256 x
+// 256 -- many the 256 x 256: 8192 x 2048 x 11264 333 us against 443 on 128 x 128.
+constexpr TileShape kTiles[3] = {{256, 256, 128, 1, 1.07, 0.37, 1.11, 0.43},
+                                 {128, 128, 64, 2, 0.47, 0.21, 0.58, 0.24},
+                                 {64, 64, 64, 2, 0.18, 0.10, 0.27, 0.29}};
 constexpr int kDeep = 64;
 constexpr size_t kMostPart = size_t{64} << 20;  // bytes of shared-out sums
 Plan Choose(bool dual, size_t M, size_t N, size_t K, int nseg) {
@@ -678,16 +688,16 @@ Plan Choose(bool dual, size_t M, size_t N, size_t K, int nseg) {
   double least = 1e30;
   for (int t = 0; t < 3; ++t) {
     const TileShape& s = kTiles[t];
-    const int bn = dual ? (t == 2 ? 64 : s.bn / 2) : s.bn;  // output columns of a tile
+    const int bn = dual ? s.bn_dual : s.bn;
+    const double alone = dual ? s.alone_dual : s.alone, shared = dual ? s.shared_dual : s.shared;
     const double tiles = std::ceil(static_cast<double>(M) / s.bm) * std::ceil(static_cast<double>(N) / bn);
-    const double more = t == 2 && dual ? 2.0 : 1.0;  // its 64 x 128 of both operands
     for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
       if (k > 1 && (k * 2 > stages || k * M * both * np * 4 > kMostPart)) break;
       const double per = std::ceil(stages / k), wgs = tiles * std::ceil(stages / per);
       const double rounds = std::ceil(wgs / (256.0 * s.per_cu));
       const double held = std::min<double>(s.per_cu, wgs / 256.0);
-      double us = rounds * per * (s.alone + more * held * s.shared) + 5;
-      if (k > 1) us += 4 + 0.2 * k + k * M * both * np * 8 / 3.5e6;
+      double us = rounds * per * (alone + held * shared) + 7;
+      if (k > 1) us += 1 + 0.1 * k + k * M * both * np * 8 / 5.5e6;
       if (us < least) {
         least = us;
         best = {t, static_cast<int>(std::ceil(stages / per)), static_cast<int>(per)};
