@@ -8,7 +8,7 @@
 // rest: the forward's first launch holds a gate tile and the up tile of the
 // same columns side by side and stores act(G) U; the backward's first forms
 // dG, dU and H from its dH accumulators, so dH is never stored.  Two launches
-// forward (G and U; Y), four backward (dH; dX; dWg and dWu; dWd).
+// forward (G and U; Y), three backward (dH; dX; the three weights' gradients).
 //
 // bf16: the operands as they are.  f32: each operand is split into three bf16
 // planes (x = hi + mid + lo, eight bits each, truncated, so exactly x), and a
@@ -188,6 +188,8 @@ __device__ __forceinline__ void Store8(uint16_t* p, bool vec, int cnt, const flo
       if (e < cnt) p[e] = F32ToBf16(v[e]);
   }
 }
+__device__ __forceinline__ float One(const float* p) { return *p; }
+__device__ __forceinline__ float One(const uint16_t* p) { return Bf16ToF32(*p); }
 __device__ __forceinline__ void Put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void Put(uint16_t* p, float v) { *p = F32ToBf16(v); }
 
@@ -224,20 +226,45 @@ __device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&
   }
 }
 
-// rows x cols (packed) into padded planes: operands whose rows or base are off
-// 16 bytes, and every f32 operand.
+// One element into the planes.
 template <class T>
-__global__ void __launch_bounds__(256)
-FfnPackKernel(const T* __restrict__ in, size_t rows, int cols, bool vec, Planes out) {
-  const int octs = out.ld / 8;
-  const size_t n = rows * octs, step = static_cast<size_t>(gridDim.x) * 256;
-  for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
-    const size_t r = i / octs;
-    const int c = static_cast<int>(i % octs) * 8;
-    float v[8];
-    Load8(in + r * cols + c, vec, cols - c, v);
-    PutPlanes<T>(out, r * out.ld + c, v);
+__device__ __forceinline__ void PutPlane(const Planes& out, size_t at, float v) {
+  if constexpr (sizeof(T) == 2) {
+    out.p[at] = F32ToBf16(v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) out.p[k * out.plane + at] = static_cast<uint16_t>(TakePlane(v));
   }
+}
+
+// rows x cols (packed) into padded planes: operands whose rows or base are off
+// 16 bytes, and every f32 operand; all of a call's in one launch.
+struct Piece {
+  const void* in;
+  size_t rows;
+  int cols;
+  bool vec;
+  Planes out;
+  unsigned first;  // its first workgroup
+};
+struct Pieces {
+  Piece q[5];
+  int count;
+  unsigned blocks;
+};
+template <class T>
+__global__ void __launch_bounds__(256) FfnPackKernel(Pieces p) {
+  int k = 0;
+  while (k + 1 < p.count && blockIdx.x >= p.q[k + 1].first) ++k;
+  const Piece& q = p.q[k];
+  const int octs = q.out.ld / 8;
+  const size_t i = static_cast<size_t>(blockIdx.x - q.first) * 256 + threadIdx.x;
+  if (i >= q.rows * octs) return;
+  const size_t r = i / octs;
+  const int c = static_cast<int>(i % octs) * 8;
+  float v[8];
+  Load8(static_cast<const T*>(q.in) + r * q.cols + c, q.vec, q.cols - c, v);
+  PutPlanes<T>(q.out, r * q.out.ld + c, v);
 }
 
 template <class T>
@@ -257,43 +284,57 @@ __device__ __forceinline__ void Each(F&& f) {
   EachOf(f, std::make_integer_sequence<int, kN>{});
 }
 
-// The products of one launch.  Operand element (i, k) lies at i ld + k, or,
+// One product of a launch.  Operand element (i, k) lies at i ld + k, or,
 // "strided", at k ld + i.  Segments are products of the same shape added up.
 constexpr int kMaxSeg = 12;
-struct MmaArgs {
+struct Product {
   const uint16_t *A[kMaxSeg], *B[kMaxSeg], *B2[kMaxSeg];
-  int nseg, lda, ldb;
-  int M, N, K;
-  int act;
-  bool vec;           // outputs (and G, U) take eight neighbours at once
-  // Where K is shared out over blockIdx.y, `per_split` stages each: the f32
-  // sums [split][M][tiles' operands][N up to 8s] that FfnJoin adds and finishes.
+  int lda, ldb, M, N;
+  bool vec;       // outputs (and G, U) take eight neighbours at once
+  void *o1, *o2;  // plain: o1; gate: G and U or null
+  int first;      // its first tile in the launch
+};
+// A launch's products share K, segments and kind.  Tiles [0, whole) are a
+// workgroup each; the rest share K out over `splits` workgroups, `per_split`
+// stages each, whose f32 sums [tile][split][rows][columns, of both operands]
+// FfnJoin adds and finishes.
+struct MmaArgs {
+  Product q[3];
+  int count, nseg, K, act;
+  int tiles, whole, splits, per_split;
   float* part;
-  int per_split;
-  void *o1, *o2;      // plain: o1 (and o2 of B2); gate: G and U or null
   const void *g, *u;  // gradient: G and U
   Planes h, dg, du;
 };
 
 enum Epilogue {
   kPlain,  // o1 = sum A B
-  kTwo,    // o1 = sum A B, o2 = sum A B2
   kGate,   // G = sum A B, U = sum A B2: o1, o2 where kept, h = act(G) U
   kGrad    // d = sum A B: dg = d U act'(G), du = d act(G), h = act(G) U
 };
 
-// Tile -> workgroup order: the 8 XCDs each take a contiguous run of tiles
-// (workgroup b runs on XCD b % 8) walked in bands of row tiles, so concurrent
+// Workgroup -> tile order: the 8 XCDs each take a contiguous run of the n tiles
+// (workgroup b runs on XCD b % 8), walked in bands of row tiles, so concurrent
 // tiles of one XCD share operand panels in its L2.
 constexpr int kBand = 4;
-__device__ __forceinline__ void TileOf(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int n = tiles_m * tiles_n;
-  int t = b;
-  if (n % 8 == 0) t = (b % 8) * (n / 8) + b / 8;
+__device__ __forceinline__ int XcdRun(int b, int n) {
+  const int x = b % 8;
+  return x * (n / 8) + min(x, n % 8) + b / 8;
+}
+__device__ __forceinline__ void TileOf(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int per = kBand * tiles_n, first = t / per * kBand;
   const int rows = min(tiles_m - first, kBand), off = t % per;
   tm = first + off % rows;
   tn = off / rows;
+}
+// The product tile t belongs to, and its corner.
+__device__ __forceinline__ int ProductOf(const MmaArgs& p, int t, int bm, int bn, int& m0, int& n0) {
+  int i = 0;
+  while (i + 1 < p.count && t >= p.q[i + 1].first) ++i;
+  TileOf(t - p.q[i].first, (p.q[i].M + bm - 1) / bm, (p.q[i].N + bn - 1) / bn, m0, n0);
+  m0 *= bm;
+  n0 *= bn;
+  return i;
 }
 
 // One operand's tile of kW rows (or strided columns): how the kW kBK elements of
@@ -385,17 +426,15 @@ struct Tile {
 
 // Eight neighbours of an output row from their sums: c of A B, d of A B2.
 template <class T, int kEpi>
-__device__ __forceinline__ void Finish(const MmaArgs& p, int m, int n, float (&c)[8], float (&d)[8]) {
-  const int cnt = p.N - n;
-  const size_t o = static_cast<size_t>(m) * p.N + n;
-  if constexpr (kEpi == kPlain || kEpi == kTwo) {
-    Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
-    if constexpr (kEpi == kTwo) Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
-  }
+__device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m, int n, float (&c)[8],
+                                       float (&d)[8]) {
+  const int cnt = q.N - n;
+  const size_t o = static_cast<size_t>(m) * q.N + n;
+  if constexpr (kEpi == kPlain) Store8(static_cast<T*>(q.o1) + o, q.vec, cnt, c);
   if constexpr (kEpi == kGate) {
-    if (p.o1) {
-      Store8(static_cast<T*>(p.o1) + o, p.vec, cnt, c);
-      Store8(static_cast<T*>(p.o2) + o, p.vec, cnt, d);
+    if (q.o1) {
+      Store8(static_cast<T*>(q.o1) + o, q.vec, cnt, c);
+      Store8(static_cast<T*>(q.o2) + o, q.vec, cnt, d);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -407,8 +446,8 @@ __device__ __forceinline__ void Finish(const MmaArgs& p, int m, int n, float (&c
   }
   if constexpr (kEpi == kGrad) {
     float g[8], u[8], y[8];
-    Load8(static_cast<const T*>(p.g) + o, p.vec, cnt, g);
-    Load8(static_cast<const T*>(p.u) + o, p.vec, cnt, u);
+    Load8(static_cast<const T*>(p.g) + o, q.vec, cnt, g);
+    Load8(static_cast<const T*>(p.u) + o, q.vec, cnt, u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float a, da;
@@ -424,40 +463,86 @@ __device__ __forceinline__ void Finish(const MmaArgs& p, int m, int n, float (&c
     PutPlanes<T>(p.h, w, u);
   }
 }
-
-// The workgroups' sums of a product whose K was shared out, added in order and
-// finished.
+// The same of one element, for rows off 16 bytes (a lane a column: a lane of
+// eight would touch a line of its own with every access).
 template <class T, int kEpi>
-__global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int splits) {
-  constexpr int kBoth = kEpi == kTwo || kEpi == kGate ? 2 : 1;
-  const int np = (p.N + 7) & ~7, octs = np / 8;
-  const size_t n = static_cast<size_t>(p.M) * octs, step = static_cast<size_t>(gridDim.x) * 256;
-  for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
-    const int m = static_cast<int>(i / octs), col = static_cast<int>(i % octs) * 8;
+__device__ __forceinline__ void Finish1(const MmaArgs& p, const Product& q, int m, int n, float c, float d) {
+  const bool in = n < q.N;
+  const size_t o = static_cast<size_t>(m) * q.N + n;
+  float a = 0.0f, da = 0.0f;
+  if constexpr (kEpi == kPlain) {
+    if (in) Put(static_cast<T*>(q.o1) + o, c);
+  }
+  if constexpr (kEpi == kGate) {
+    if (in && q.o1) {
+      Put(static_cast<T*>(q.o1) + o, c);
+      Put(static_cast<T*>(q.o2) + o, d);
+    }
+    Activate<sizeof(T) == 2>(p.act, c, a, da);
+    if (n < p.h.ld) PutPlane<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, in ? a * d : 0.0f);
+  }
+  if constexpr (kEpi == kGrad) {
+    if (n >= p.h.ld) return;
+    const float g = in ? One(static_cast<const T*>(p.g) + o) : 0.0f;
+    const float u = in ? One(static_cast<const T*>(p.u) + o) : 0.0f;
+    Activate<sizeof(T) == 2>(p.act, g, a, da);
+    const size_t w = static_cast<size_t>(m) * p.h.ld + n;
+    PutPlane<T>(p.dg, w, in ? c * u * da : 0.0f);
+    PutPlane<T>(p.du, w, in ? c * a : 0.0f);
+    PutPlane<T>(p.h, w, in ? a * u : 0.0f);
+  }
+}
+
+// The sums of the tiles whose K was shared out, added in order and finished:
+// workgroup (x, y) takes 2048 elements of the x-th of them, bm x bn large.
+template <class T, int kEpi>
+__global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
+  constexpr int kBoth = kEpi == kGate ? 2 : 1;
+  int m0, n0;
+  const Product& q = p.q[ProductOf(p, p.whole + blockIdx.x, bm, bn, m0, n0)];
+  const size_t row = static_cast<size_t>(kBoth) * bn, split = bm * row;
+  const float* at = p.part + blockIdx.x * p.splits * split;
+  if (q.vec) {
+    const int i = (blockIdx.y * 256 + threadIdx.x) * 8, r = i / bn, col = i % bn;
+    if (m0 + r >= q.M || n0 + col >= q.N) return;
     float s[2][8] = {};
-    for (int k0 = 0; k0 < splits; k0 += 4) {  // four sums' loads in flight
+    for (int k0 = 0; k0 < p.splits; k0 += 4) {  // four sums' loads in flight
       float v[4][kBoth][8];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int b = 0; b < kBoth; ++b)
-          Load8(p.part + ((static_cast<size_t>(min(k0 + k, splits - 1)) * p.M + m) * kBoth + b) * np + col,
-                true, 8, v[k][b]);
+          Load8(at + min(k0 + k, p.splits - 1) * split + r * row + b * bn + col, true, 8, v[k][b]);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int b = 0; b < kBoth; ++b)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < splits ? v[k][b][e] : 0.0f;
+          for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < p.splits ? v[k][b][e] : 0.0f;
     }
-    Finish<T, kEpi>(p, m, col, s[0], s[1]);
+    Finish<T, kEpi>(p, q, m0 + r, n0 + col, s[0], s[1]);
+  } else {
+    float s[8][2] = {};
+    for (int k = 0; k < p.splits; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b) {
+          const int i = (blockIdx.y * 8 + e) * 256 + threadIdx.x;
+          s[e][b] += at[k * split + i / bn * row + b * bn + i % bn];
+        }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = (blockIdx.y * 8 + e) * 256 + threadIdx.x;
+      if (m0 + i / bn < q.M) Finish1<T, kEpi>(p, q, m0 + i / bn, n0 + i % bn, s[e][0], s[e][1]);
+    }
   }
 }
 
 template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
 __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   constexpr int kWaves = WGM * WGN;
-  constexpr bool kDual = kEpi == kTwo || kEpi == kGate;
+  constexpr bool kDual = kEpi == kGate;
   constexpr int BNs = kDual ? BN / 2 : BN;  // columns of the output
   constexpr int WM = BM / WGM, WN = BNs / WGN;
   constexpr int TM = WM / 32, TN = WN / 32, TB = kDual ? 2 * TN : TN;
@@ -470,24 +555,36 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kStages * kStage];
 
   const int wave = Uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
-  int tm, tn;
-  TileOf(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BNs - 1) / BNs, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BNs;
+  // This workgroup's tile, and of its K the stages from `first` on.
+  const int per_seg = (p.K + BK - 1) / BK, total = p.nseg * per_seg;
+  int b = blockIdx.x, tile, first = 0, stages = total, split = 0;
+  const bool shared = b >= p.whole;
+  if (!shared) {
+    tile = XcdRun(b, p.whole);
+  } else {
+    b -= p.whole;
+    const int rest = p.tiles - p.whole;
+    split = b / rest;
+    tile = p.whole + XcdRun(b - split * rest, rest);
+    first = split * p.per_split;
+    stages = min(total - first, p.per_split);
+  }
+  int m0, n0;
+  const Product& q = p.q[ProductOf(p, tile, BM, BNs, m0, n0)];
   TA ta;
   TBt tb;
   // A strided operand's last row ends where its columns do.
-  ta.Init(p.lda, kAS ? p.lda - m0 : min(p.M - m0, BM), p.K, wave, lane);
-  tb.Init(p.ldb, kBS ? p.ldb - n0 : min(p.N - n0, BNs), p.K, wave, lane);
-  const size_t a_at = kAS ? static_cast<size_t>(m0) : static_cast<size_t>(m0) * p.lda;
-  const size_t b_at = kBS ? static_cast<size_t>(n0) : static_cast<size_t>(n0) * p.ldb;
+  ta.Init(q.lda, kAS ? q.lda - m0 : min(q.M - m0, BM), p.K, wave, lane);
+  tb.Init(q.ldb, kBS ? q.ldb - n0 : min(q.N - n0, BNs), p.K, wave, lane);
+  const size_t a_at = kAS ? static_cast<size_t>(m0) : static_cast<size_t>(m0) * q.lda;
+  const size_t b_at = kBS ? static_cast<size_t>(n0) : static_cast<size_t>(n0) * q.ldb;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPtr)smem));
 
-  const int per_seg = (p.K + BK - 1) / BK, first = blockIdx.y * p.per_split;
-  const int last = min(p.nseg * per_seg - first, p.per_split) - 1;
+  const int last = stages - 1;
   // The next stage to load, and its segment's operands.
   int seg = first / per_seg, k0 = (first - seg * per_seg) * BK;
-  const uint16_t *pa = p.A[seg] + a_at, *pb = p.B[seg] + b_at;
-  const uint16_t* pb2 = kDual ? p.B2[seg] + b_at : nullptr;
+  const uint16_t *pa = q.A[seg] + a_at, *pb = q.B[seg] + b_at;
+  const uint16_t* pb2 = kDual ? q.B2[seg] + b_at : nullptr;
   // Part `part` of kParts of the next stage's loads into buffer `buf`.  With
   // two buffers the stage is wanted at this one's end: its first half's steps.
   constexpr int kParts = kStages == 2 ? kSub / 2 : kSub;
@@ -514,8 +611,8 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
     } else if (seg + 1 < p.nseg) {
       ++seg;
       k0 = 0;
-      pa = p.A[seg] + a_at, pb = p.B[seg] + b_at;
-      if constexpr (kDual) pb2 = p.B2[seg] + b_at;
+      pa = q.A[seg] + a_at, pb = q.B[seg] + b_at;
+      if constexpr (kDual) pb2 = q.B2[seg] + b_at;
     }
   };
 
@@ -622,32 +719,28 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
           }
       __builtin_amdgcn_wave_barrier();
       const int mb = m0 + wm + i * 32, nb = n0 + wn + jb * kW;
-      if ((kEpi == kPlain || kEpi == kTwo) && !p.vec && !p.part) {
-        // Rows off 16 bytes: a lane a column.
+      if (!q.vec && !shared) {
         const int n = nb + lane % kW;
-        for (int r = lane / kW; r < 32; r += kWave / kW) {
-          if (mb + r < p.M && n < p.N) {
-            const size_t o = static_cast<size_t>(mb + r) * p.N + n;
-            Put(static_cast<T*>(p.o1) + o, st[r * kPad + lane % kW]);
-            if constexpr (kEpi == kTwo) Put(static_cast<T*>(p.o2) + o, st[(32 + r) * kPad + lane % kW]);
-          }
-        }
+        for (int r = lane / kW; r < 32; r += kWave / kW)
+          if (mb + r < q.M)
+            Finish1<T, kEpi>(p, q, mb + r, n, st[r * kPad + lane % kW],
+                             kDual ? st[(32 + r) * kPad + lane % kW] : 0.0f);
       } else {
         const int n = nb + (lane % kPerRow) * 8;
 #pragma unroll
         for (int t = 0; t < 32 / kRows; ++t) {
           const int r = lane / kPerRow + t * kRows, m = mb + r;
-          if (m >= p.M || n >= p.N) continue;
+          if (m >= q.M || n >= q.N) continue;
           float c[8], d[8];
           Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
           if constexpr (kDual) Load8(st + (32 + r) * kPad + (lane % kPerRow) * 8, true, 8, d);
-          if (p.part) {
-            const int np = (p.N + 7) & ~7;
-            float* out = p.part + (static_cast<size_t>(blockIdx.y) * p.M + m) * kBoth * np + n;
+          if (shared) {
+            float* out = p.part + ((static_cast<size_t>(tile - p.whole) * p.splits + split) * BM + (m - m0)) *
+                                      (kBoth * BNs) + (n - n0);
             Store8(out, true, 8, c);
-            if constexpr (kDual) Store8(out + np, true, 8, d);
+            if constexpr (kDual) Store8(out + BNs, true, 8, d);
           } else {
-            Finish<T, kEpi>(p, m, n, c, d);
+            Finish<T, kEpi>(p, q, m, n, c, d);
           }
         }
       }
@@ -657,11 +750,11 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
 
 // --- host ---------------------------------------------------------------------------------------
 
-// How a product runs: its tile, and over how many workgroups a tile's K is
-// shared out.
+// How a launch runs: its tile, and over how many workgroups the K of the tiles
+// past `whole` is shared out.
 struct Plan {
   int tile = 0;  // of kTiles
-  int splits = 1, per_split = 0;
+  int tiles = 0, whole = 0, splits = 1, per_split = 0;
 };
 struct TileShape {
   int bm, bn, bn_dual, per_cu;  // rows, output columns, workgroups a CU holds
@@ -680,66 +773,91 @@ constexpr TileShape kTiles[3] = {{256, 256, 128, 1, 1.07, 0.37, 1.11, 0.43},
                                  {64, 64, 64, 2, 0.18, 0.10, 0.27, 0.29}};
 constexpr int kDeep = 64;
 constexpr size_t kMostPart = size_t{64} << 20;  // bytes of shared-out sums
-Plan Choose(bool dual, size_t M, size_t N, size_t K, int nseg) {
-  const int both = dual ? 2 : 1;
+struct Shape {
+  size_t M, N;
+};
+// Either every tile's K is shared out, or, with more tiles than the chip holds
+// at once, that of the tiles left over after whole rounds: 528 tiles of the
+// weights' gradients run as two rounds and a sixteenth instead of three.
+Plan Choose(bool dual, std::initializer_list<Shape> products, size_t K, int nseg) {
   const double stages = static_cast<double>((K + kDeep - 1) / kDeep) * nseg;
-  const double np = static_cast<double>((N + 7) / 8 * 8);
   Plan best;
   double least = 1e30;
   for (int t = 0; t < 3; ++t) {
     const TileShape& s = kTiles[t];
     const int bn = dual ? s.bn_dual : s.bn;
     const double alone = dual ? s.alone_dual : s.alone, shared = dual ? s.shared_dual : s.shared;
-    const double tiles = std::ceil(static_cast<double>(M) / s.bm) * std::ceil(static_cast<double>(N) / bn);
-    for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (k > 1 && (k * 2 > stages || k * M * both * np * 4 > kMostPart)) break;
-      const double per = std::ceil(stages / k), wgs = tiles * std::ceil(stages / per);
-      const double rounds = std::ceil(wgs / (256.0 * s.per_cu));
-      const double held = std::min<double>(s.per_cu, wgs / 256.0);
-      double us = rounds * per * (alone + held * shared) + 7;
-      if (k > 1) us += 1 + 0.1 * k + k * M * both * np * 8 / 5.5e6;
-      if (us < least) {
-        least = us;
-        best = {t, static_cast<int>(std::ceil(stages / per)), static_cast<int>(per)};
+    const double tile_bytes = s.bm * bn * (dual ? 2 : 1) * 4.0, chip = 256.0 * s.per_cu;
+    double tiles = 0;
+    for (const Shape& q : products)
+      tiles += std::ceil(static_cast<double>(q.M) / s.bm) * std::ceil(static_cast<double>(q.N) / bn);
+    // us of `wgs` workgroups of `per` stages.
+    auto run = [&](double wgs, double per) {
+      return std::ceil(wgs / chip) * per * (alone + std::min<double>(s.per_cu, wgs / 256.0) * shared);
+    };
+    const double full = std::floor(tiles / chip) * chip;
+    for (double whole : {0.0, full}) {
+      const double rest = tiles - whole;
+      if (whole > 0 && rest == 0) continue;
+      for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (whole > 0 && k == 1) continue;  // the same as sharing nothing out
+        if (k > 1 && (k * 2 > stages || k * rest * tile_bytes > kMostPart)) break;
+        const double per = std::ceil(stages / k), n = std::ceil(stages / per);
+        double us = (whole > 0 ? run(whole, stages) : 0) + run(rest * n, per) + 7;
+        if (k > 1) us += 1 + 0.1 * k + k * rest * tile_bytes * 2 / 5.5e6;
+        if (us < least) {
+          least = us;
+          best = {t, static_cast<int>(tiles), static_cast<int>(k == 1 ? tiles : whole),
+                  static_cast<int>(n), static_cast<int>(per)};
+        }
       }
+      if (full == 0) break;
     }
   }
   return best;
 }
-size_t PartBytes(const Plan& plan, bool dual, size_t M, size_t N) {
-  return plan.splits == 1 ? 0 : plan.splits * M * (dual ? 2 : 1) * ((N + 7) / 8 * 8) * 4;
+size_t PartBytes(const Plan& plan, bool dual) {
+  const TileShape& s = kTiles[plan.tile];
+  return static_cast<size_t>(plan.tiles - plan.whole) * plan.splits * s.bm * (dual ? 2 * s.bn_dual : s.bn) * 4;
 }
 
 template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
-hipError_t LaunchTile(const MmaArgs& a, int splits, hipStream_t s) {
+hipError_t LaunchTile(const MmaArgs& a, hipStream_t s) {
   static_assert(BK == kDeep, "per_split counts such stages");
-  constexpr int BNs = kEpi == kTwo || kEpi == kGate ? BN / 2 : BN;
-  const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BNs - 1) / BNs);
+  const unsigned grid = a.whole + static_cast<unsigned>(a.tiles - a.whole) * a.splits;
   auto* kernel = &FfnMma<T, kEpi, kAS, kBS, BM, BN, BK, WGM, WGN, kStages>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles), splits), dim3(WGM * WGN * kWave), 0, s, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(WGM * WGN * kWave), 0, s, a);
   return hipGetLastError();
 }
 
-// `part`: where a shared-out product's sums go (PartBytes).
+// `part`: where the shared-out sums go (PartBytes).
 template <class T, int kEpi, bool kAS, bool kBS>
 hipError_t Mma(MmaArgs a, float* part, hipStream_t s) {
-  constexpr bool dual = kEpi == kTwo || kEpi == kGate;
-  const Plan plan = Choose(dual, a.M, a.N, a.K, a.nseg);
-  a.per_split = plan.per_split;
-  a.part = plan.splits > 1 ? part : nullptr;
-  hipError_t e;
-  // (f32's gradient epilogue, nine planes a quad, is past the registers beside 256 x 256.)
+  constexpr bool dual = kEpi == kGate;
+  const Shape shape[3] = {{static_cast<size_t>(a.q[0].M), static_cast<size_t>(a.q[0].N)},
+                          {static_cast<size_t>(a.q[1].M), static_cast<size_t>(a.q[1].N)},
+                          {static_cast<size_t>(a.q[2].M), static_cast<size_t>(a.q[2].N)}};
+  const Plan plan = a.count == 1 ? Choose(dual, {shape[0]}, a.K, a.nseg)
+                                 : Choose(dual, {shape[0], shape[1], shape[2]}, a.K, a.nseg);
+  const TileShape& t = kTiles[plan.tile];
+  const int bn = dual ? t.bn_dual : t.bn;
+  for (int i = 0, first = 0; i < a.count; ++i) {
+    a.q[i].first = first;
+    first += ((a.q[i].M + t.bm - 1) / t.bm) * ((a.q[i].N + bn - 1) / bn);
+  }
+  a.tiles = plan.tiles, a.whole = plan.whole, a.splits = plan.splits, a.per_split = plan.per_split;
+  a.part = part;
+  hipError_t e = hipErrorInvalidValue;
+  // (f32's gradient epilogue, nine planes an eight, is past the registers beside 256 x 256.)
   constexpr bool big = !(kEpi == kGrad && sizeof(T) == 4);
   if constexpr (big) {
-    if (plan.tile == 0) e = LaunchTile<T, kEpi, kAS, kBS, 256, 256, 64, 2, 4, 2>(a, plan.splits, s);
+    if (plan.tile == 0) e = LaunchTile<T, kEpi, kAS, kBS, 256, 256, 64, 2, 4, 2>(a, s);
   }
-  if (plan.tile == 1 || (!big && plan.tile == 0))
-    e = LaunchTile<T, kEpi, kAS, kBS, 128, 128, 64, 2, 2, 2>(a, plan.splits, s);
-  if (plan.tile == 2) e = LaunchTile<T, kEpi, kAS, kBS, 64, dual ? 128 : 64, 64, 2, 2, dual ? 3 : 4>(a, plan.splits, s);
-  if (e != hipSuccess || plan.splits == 1) return e;
-  const size_t n = static_cast<size_t>(a.M) * ((a.N + 7) / 8);
+  if (plan.tile == 1) e = LaunchTile<T, kEpi, kAS, kBS, 128, 128, 64, 2, 2, 2>(a, s);
+  if (plan.tile == 2) e = LaunchTile<T, kEpi, kAS, kBS, 64, dual ? 128 : 64, 64, 2, 2, dual ? 3 : 4>(a, s);
+  if (e != hipSuccess || plan.whole == plan.tiles) return e;
   auto* kernel = &FfnJoin<T, kEpi>;
-  hipLaunchKernelGGL(kernel, dim3(GridFor(n, 256, 4096)), dim3(256), 0, s, a, plan.splits);
+  hipLaunchKernelGGL(kernel, dim3(plan.tiles - plan.whole, t.bm * bn / 2048), dim3(256), 0, s, a, t.bm, bn);
   return hipGetLastError();
 }
 
@@ -788,42 +906,35 @@ Layout Lay(void* ws, int planes, size_t M, size_t D, size_t F, bool backward) {
     l.du = s.Take(M, F, planes);
   }
   const int nseg = planes == 1 ? 1 : 6;
-  auto part = [&](bool dual, size_t m, size_t n, size_t k, int segs) {
-    return PartBytes(Choose(dual, m, n, k, segs), dual, m, n);
+  auto part = [&](bool dual, std::initializer_list<Shape> q, size_t k, int segs) {
+    return PartBytes(Choose(dual, q, k, segs), dual);
   };
-  l.part = s.Floats(backward ? std::max({part(false, M, F, D, nseg), part(false, M, D, F, 2 * nseg),
-                                         part(true, D, F, M, nseg), part(false, F, D, M, nseg)})
-                             : std::max(part(true, M, F, D, nseg), part(false, M, D, F, nseg)));
+  l.part = s.Floats(backward ? std::max({part(false, {{M, F}}, D, nseg), part(false, {{M, D}}, F, 2 * nseg),
+                                         part(false, {{D, F}, {D, F}, {F, D}}, M, nseg)})
+                             : std::max(part(true, {{M, F}}, D, nseg), part(false, {{M, D}}, F, nseg)));
   l.bytes = s.used();
   return l;
 }
 
-// An operand as planes: itself where its rows begin on 16 bytes, else packed.
+// An operand as planes: itself where its rows begin on 16 bytes, else to be
+// packed.
 template <class T>
-hipError_t Pack(const void* in, size_t rows, size_t cols, Planes& out, hipStream_t s) {
+void Take(const void* in, size_t rows, size_t cols, Planes& out, Pieces& pieces) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(in);
   if (sizeof(T) == 2 && cols % 8 == 0 && (at & 15) == 0) {
     out.p = static_cast<uint16_t*>(const_cast<void*>(in));
-    return hipSuccess;
+    return;
   }
-  const size_t n = rows * (out.ld / 8);
-  const bool vec = cols % (16 / sizeof(T)) == 0 && (at & 15) == 0;
-  hipLaunchKernelGGL((FfnPackKernel<T>), dim3(GridFor(n, 256, 4096)), dim3(256), 0, s,
-                     static_cast<const T*>(in), rows, static_cast<int>(cols), vec, out);
-  return hipGetLastError();
+  pieces.q[pieces.count++] = {in, rows, static_cast<int>(cols),
+                              cols % (16 / sizeof(T)) == 0 && (at & 15) == 0, out, pieces.blocks};
+  pieces.blocks += static_cast<unsigned>((rows * (out.ld / 8) + 255) / 256);
 }
-
-// The plane products of A B (and A B2), smallest first.
 template <class T>
-void AddProduct(MmaArgs& a, const Planes& A, const Planes& B, const Planes* B2 = nullptr) {
-  constexpr int pairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-  a.lda = A.ld, a.ldb = B.ld;
-  for (int i = sizeof(T) == 2 ? 5 : 0; i < 6; ++i) {
-    a.A[a.nseg] = A.p + pairs[i][0] * A.plane;
-    a.B[a.nseg] = B.p + pairs[i][1] * B.plane;
-    if (B2) a.B2[a.nseg] = B2->p + pairs[i][1] * B2->plane;
-    ++a.nseg;
-  }
+hipError_t Pack(const Pieces& pieces, hipStream_t s) {
+  if (pieces.count == 0) return hipSuccess;
+  auto* kernel = &FfnPackKernel<T>;
+  hipLaunchKernelGGL(kernel, dim3(pieces.blocks), dim3(256), 0, s, pieces);
+  return hipGetLastError();
 }
 
 // Rows that begin on 16 bytes.
@@ -831,12 +942,37 @@ template <class T>
 bool Octs(size_t N, std::initializer_list<const void*> ptrs) {
   uintptr_t at = 0;
   for (const void* p : ptrs) at |= reinterpret_cast<uintptr_t>(p);
-  return N % (16 / sizeof(T)) == 0 && (at & 15) == 0;
+  return N % 8 == 0 && (at & 15) == 0;
 }
 
-MmaArgs Shape(size_t M, size_t N, size_t K) {
+// The plane products of A B (and A B2), smallest first, as segments.
+template <class T>
+Product& AddSegments(MmaArgs& a, Product& q, const Planes& A, const Planes& B, const Planes* B2 = nullptr) {
+  constexpr int pairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+  for (int i = sizeof(T) == 2 ? 5 : 0; i < 6; ++i) {
+    q.A[a.nseg] = A.p + pairs[i][0] * A.plane;
+    q.B[a.nseg] = B.p + pairs[i][1] * B.plane;
+    if (B2) q.B2[a.nseg] = B2->p + pairs[i][1] * B2->plane;
+    ++a.nseg;
+  }
+  return q;
+}
+
+// A launch's next product, its segments the plane products of A B (and A B2),
+// smallest first.
+template <class T>
+Product& AddProduct(MmaArgs& a, size_t M, size_t N, const Planes& A, const Planes& B,
+                    const Planes* B2 = nullptr) {
+  Product& q = a.q[a.count++];
+  q.M = static_cast<int>(M), q.N = static_cast<int>(N);
+  q.lda = A.ld, q.ldb = B.ld;
+  a.nseg = 0;
+  return AddSegments<T>(a, q, A, B, B2);
+}
+
+MmaArgs Launch(size_t K) {
   MmaArgs a{};
-  a.M = static_cast<int>(M), a.N = static_cast<int>(N), a.K = static_cast<int>(K);
+  a.K = static_cast<int>(K);
   return a;
 }
 
@@ -849,17 +985,20 @@ template <class T>
 hipError_t Fwd(const FfnArgs& f, hipStream_t s) {
   if (f.M == 0) return hipSuccess;
   Layout l = Lay(f.ws, sizeof(T) == 2 ? 1 : 3, f.M, f.D, f.F, false);
-  FFN_TRY(Pack<T>(f.x, f.M, f.D, l.x, s));
-  FFN_TRY(Pack<T>(f.wg, f.D, f.F, l.wg, s));
-  FFN_TRY(Pack<T>(f.wu, f.D, f.F, l.wu, s));
-  FFN_TRY(Pack<T>(f.wd, f.F, f.D, l.wd, s));
-  MmaArgs a = Shape(f.M, f.F, f.D);
-  AddProduct<T>(a, l.x, l.wg, &l.wu);
-  a.act = f.act, a.o1 = f.gate, a.o2 = f.up, a.h = l.h, a.vec = Octs<T>(f.F, {f.gate, f.up});
+  Pieces pieces{};
+  Take<T>(f.x, f.M, f.D, l.x, pieces);
+  Take<T>(f.wg, f.D, f.F, l.wg, pieces);
+  Take<T>(f.wu, f.D, f.F, l.wu, pieces);
+  Take<T>(f.wd, f.F, f.D, l.wd, pieces);
+  FFN_TRY(Pack<T>(pieces, s));
+  MmaArgs a = Launch(f.D);
+  Product& gate = AddProduct<T>(a, f.M, f.F, l.x, l.wg, &l.wu);
+  gate.o1 = f.gate, gate.o2 = f.up, gate.vec = Octs<T>(f.F, {f.gate, f.up});
+  a.act = f.act, a.h = l.h;
   FFN_TRY((Mma<T, kGate, false, true>(a, l.part, s)));
-  a = Shape(f.M, f.D, f.F);
-  AddProduct<T>(a, l.h, l.wd);
-  a.o1 = f.y, a.vec = Octs<T>(f.D, {f.y});
+  a = Launch(f.F);
+  Product& down = AddProduct<T>(a, f.M, f.D, l.h, l.wd);
+  down.o1 = f.y, down.vec = Octs<T>(f.D, {f.y});
   return Mma<T, kPlain, false, true>(a, l.part, s);
 }
 
@@ -875,28 +1014,31 @@ hipError_t Bwd(const FfnArgs& f, hipStream_t s) {
     return hipSuccess;
   }
   Layout l = Lay(f.ws, sizeof(T) == 2 ? 1 : 3, f.M, f.D, f.F, true);
-  FFN_TRY(Pack<T>(f.x, f.M, f.D, l.x, s));
-  FFN_TRY(Pack<T>(f.wg, f.D, f.F, l.wg, s));
-  FFN_TRY(Pack<T>(f.wu, f.D, f.F, l.wu, s));
-  FFN_TRY(Pack<T>(f.wd, f.F, f.D, l.wd, s));
-  FFN_TRY(Pack<T>(f.dy, f.M, f.D, l.dy, s));
-  MmaArgs a = Shape(f.M, f.F, f.D);
-  AddProduct<T>(a, l.dy, l.wd);
+  Pieces pieces{};
+  Take<T>(f.x, f.M, f.D, l.x, pieces);
+  Take<T>(f.wg, f.D, f.F, l.wg, pieces);
+  Take<T>(f.wu, f.D, f.F, l.wu, pieces);
+  Take<T>(f.wd, f.F, f.D, l.wd, pieces);
+  Take<T>(f.dy, f.M, f.D, l.dy, pieces);
+  FFN_TRY(Pack<T>(pieces, s));
+  MmaArgs a = Launch(f.D);
+  AddProduct<T>(a, f.M, f.F, l.dy, l.wd).vec = Octs<T>(f.F, {f.gate, f.up});
   a.act = f.act, a.g = f.gate, a.u = f.up, a.h = l.h, a.dg = l.dg, a.du = l.du;
-  a.vec = Octs<T>(f.F, {f.gate, f.up});
   FFN_TRY((Mma<T, kGrad, false, false>(a, l.part, s)));
-  a = Shape(f.M, f.D, f.F);
-  AddProduct<T>(a, l.dg, l.wg);
-  AddProduct<T>(a, l.du, l.wu);
-  a.o1 = f.dx, a.vec = Octs<T>(f.D, {f.dx});
+  a = Launch(f.F);
+  Product& dx = AddProduct<T>(a, f.M, f.D, l.dg, l.wg);
+  AddSegments<T>(a, dx, l.du, l.wu);
+  dx.o1 = f.dx, dx.vec = Octs<T>(f.D, {f.dx});
   FFN_TRY((Mma<T, kPlain, false, false>(a, l.part, s)));
-  a = Shape(f.D, f.F, f.M);
-  AddProduct<T>(a, l.x, l.dg, &l.du);
-  a.o1 = f.dwg, a.o2 = f.dwu, a.vec = Octs<T>(f.F, {f.dwg, f.dwu});
-  FFN_TRY((Mma<T, kTwo, true, true>(a, l.part, s)));
-  a = Shape(f.F, f.D, f.M);
-  AddProduct<T>(a, l.h, l.dy);
-  a.o1 = f.dwd, a.vec = Octs<T>(f.D, {f.dwd});
+  a = Launch(f.M);
+  const Planes* left[3] = {&l.x, &l.x, &l.h};
+  const Planes* right[3] = {&l.dg, &l.du, &l.dy};
+  void* out[3] = {f.dwg, f.dwu, f.dwd};
+  for (int i = 0; i < 3; ++i) {
+    const size_t M = i == 2 ? f.F : f.D, N = i == 2 ? f.D : f.F;
+    Product& q = AddProduct<T>(a, M, N, *left[i], *right[i]);
+    q.o1 = out[i], q.vec = Octs<T>(N, {out[i]});
+  }
   return Mma<T, kPlain, true, true>(a, l.part, s);
 }
 
