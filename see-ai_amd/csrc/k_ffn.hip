@@ -200,7 +200,8 @@ __device__ __forceinline__ uint32_t TakePlane(float& x) {
   return hi >> 16;
 }
 
-// A [rows, ld] operand in bf16 planes: one for bf16, three for f32.
+// A [rows, ld] operand in bf16 planes: one for bf16, three for f32; with kWhole
+// (FfnRows32's) in f32 itself.
 struct Planes {
   uint16_t* p = nullptr;
   size_t plane = 0;  // elements of one plane
@@ -208,9 +209,11 @@ struct Planes {
 };
 // Eight neighbours into the planes (16-byte aligned: the column is a multiple
 // of eight).
-template <class T>
+template <class T, bool kWhole = false>
 __device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (kWhole) {
+    Store8(reinterpret_cast<float*>(out.p) + at, true, 8, v);
+  } else if constexpr (sizeof(T) == 2) {
     *reinterpret_cast<bf16x8*>(out.p + at) = Bf16x8(v);
   } else {
 #pragma unroll
@@ -227,9 +230,11 @@ __device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&
 }
 
 // One element into the planes.
-template <class T>
+template <class T, bool kWhole = false>
 __device__ __forceinline__ void PutPlane(const Planes& out, size_t at, float v) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (kWhole) {
+    reinterpret_cast<float*>(out.p)[at] = v;
+  } else if constexpr (sizeof(T) == 2) {
     out.p[at] = F32ToBf16(v);
   } else {
 #pragma unroll
@@ -291,13 +296,14 @@ struct Product {
   const uint16_t *A[kMaxSeg], *B[kMaxSeg], *B2[kMaxSeg];
   int lda, ldb, M, N;
   bool vec;       // outputs (and G, U) take eight neighbours at once
+  bool vec_a;     // FfnOuter32: A takes four, and `vec` is of four too
   void *o1, *o2;  // plain: o1; gate: G and U or null
   int first;      // its first tile in the launch
 };
 // A launch's products share K, segments and kind.  Tiles [0, whole) are a
 // workgroup each; the rest share K out over `splits` workgroups, `per_split`
 // stages each, whose f32 sums [tile][split][rows][columns, of both operands]
-// FfnJoin adds and finishes.
+// FfnJoin adds and finishes.  (FfnRows32's tiles all share K out.)
 struct MmaArgs {
   Product q[3];
   int count, nseg, K, act;
@@ -425,7 +431,7 @@ struct Tile {
 };
 
 // Eight neighbours of an output row from their sums: c of A B, d of A B2.
-template <class T, int kEpi>
+template <class T, int kEpi, bool kWhole = false>
 __device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m, int n, float (&c)[8],
                                        float (&d)[8]) {
   const int cnt = q.N - n;
@@ -442,7 +448,7 @@ __device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m
       Activate<sizeof(T) == 2>(p.act, c[e], a, da);
       c[e] = e < cnt ? a * d[e] : 0.0f;
     }
-    PutPlanes<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
+    PutPlanes<T, kWhole>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
   }
   if constexpr (kEpi == kGrad) {
     float g[8], u[8], y[8];
@@ -458,14 +464,14 @@ __device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m
       u[e] = in ? a * u[e] : 0.0f;
     }
     const size_t w = static_cast<size_t>(m) * p.h.ld + n;
-    PutPlanes<T>(p.dg, w, g);
-    PutPlanes<T>(p.du, w, y);
-    PutPlanes<T>(p.h, w, u);
+    PutPlanes<T, kWhole>(p.dg, w, g);
+    PutPlanes<T, kWhole>(p.du, w, y);
+    PutPlanes<T, kWhole>(p.h, w, u);
   }
 }
 // The same of one element, for rows off 16 bytes (a lane a column: a lane of
 // eight would touch a line of its own with every access).
-template <class T, int kEpi>
+template <class T, int kEpi, bool kWhole = false>
 __device__ __forceinline__ void Finish1(const MmaArgs& p, const Product& q, int m, int n, float c, float d) {
   const bool in = n < q.N;
   const size_t o = static_cast<size_t>(m) * q.N + n;
@@ -479,7 +485,7 @@ __device__ __forceinline__ void Finish1(const MmaArgs& p, const Product& q, int 
       Put(static_cast<T*>(q.o2) + o, d);
     }
     Activate<sizeof(T) == 2>(p.act, c, a, da);
-    if (n < p.h.ld) PutPlane<T>(p.h, static_cast<size_t>(m) * p.h.ld + n, in ? a * d : 0.0f);
+    if (n < p.h.ld) PutPlane<T, kWhole>(p.h, static_cast<size_t>(m) * p.h.ld + n, in ? a * d : 0.0f);
   }
   if constexpr (kEpi == kGrad) {
     if (n >= p.h.ld) return;
@@ -487,15 +493,15 @@ __device__ __forceinline__ void Finish1(const MmaArgs& p, const Product& q, int 
     const float u = in ? One(static_cast<const T*>(p.u) + o) : 0.0f;
     Activate<sizeof(T) == 2>(p.act, g, a, da);
     const size_t w = static_cast<size_t>(m) * p.h.ld + n;
-    PutPlane<T>(p.dg, w, in ? c * u * da : 0.0f);
-    PutPlane<T>(p.du, w, in ? c * a : 0.0f);
-    PutPlane<T>(p.h, w, in ? a * u : 0.0f);
+    PutPlane<T, kWhole>(p.dg, w, in ? c * u * da : 0.0f);
+    PutPlane<T, kWhole>(p.du, w, in ? c * a : 0.0f);
+    PutPlane<T, kWhole>(p.h, w, in ? a * u : 0.0f);
   }
 }
 
 // The sums of the tiles whose K was shared out, added in order and finished:
 // workgroup (x, y) takes 2048 elements of the x-th of them, bm x bn large.
-template <class T, int kEpi>
+template <class T, int kEpi, bool kWhole = false>
 __global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
   constexpr int kBoth = kEpi == kGate ? 2 : 1;
   int m0, n0;
@@ -504,7 +510,7 @@ __global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
   const float* at = p.part + blockIdx.x * p.splits * split;
   if (q.vec) {
     const int i = (blockIdx.y * 256 + threadIdx.x) * 8, r = i / bn, col = i % bn;
-    if (m0 + r >= q.M || n0 + col >= q.N) return;
+    if (r >= bm || m0 + r >= q.M || n0 + col >= q.N) return;
     float s[2][8] = {};
     for (int k0 = 0; k0 < p.splits; k0 += 4) {  // four sums' loads in flight
       float v[4][kBoth][8];
@@ -520,7 +526,7 @@ __global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < p.splits ? v[k][b][e] : 0.0f;
     }
-    Finish<T, kEpi>(p, q, m0 + r, n0 + col, s[0], s[1]);
+    Finish<T, kEpi, kWhole>(p, q, m0 + r, n0 + col, s[0], s[1]);
   } else {
     float s[8][2] = {};
     for (int k = 0; k < p.splits; ++k)
@@ -529,12 +535,12 @@ __global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
 #pragma unroll
         for (int b = 0; b < kBoth; ++b) {
           const int i = (blockIdx.y * 8 + e) * 256 + threadIdx.x;
-          s[e][b] += at[k * split + i / bn * row + b * bn + i % bn];
+          if (i < bm * bn) s[e][b] += at[k * split + i / bn * row + b * bn + i % bn];
         }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = (blockIdx.y * 8 + e) * 256 + threadIdx.x;
-      if (m0 + i / bn < q.M) Finish1<T, kEpi>(p, q, m0 + i / bn, n0 + i % bn, s[e][0], s[e][1]);
+      if (i < bm * bn && m0 + i / bn < q.M) Finish1<T, kEpi, kWhole>(p, q, m0 + i / bn, n0 + i % bn, s[e][0], s[e][1]);
     }
   }
 }
@@ -748,6 +754,210 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   });
 }
 
+// Few f32 tokens: splitting the weights into planes would move three times
+// their bytes, so the products run on the f32 MFMA (32 x 32 x 2) straight from
+// memory, and H, dG and dU stay f32.  FfnRows32 runs those with the weights: a
+// workgroup takes 32 kR rows by 32 kC columns, its waves K in turns of 32; K's
+// order within eight is the lanes': half-wave h of product j takes k = 4 h + j,
+// so a lane's four values of a row are one load.  Weights contiguous in K have
+// a lane's columns 32 apart; strided ones have kC neighbours a lane, one load.
+// The waves' sums are added in LDS in wave order.  Bound by the weights' bytes up
+// to 32 tokens (8 x 2048 x 5632: the gate's 92 MB in 27 us, 3.4 TB/s; through
+// planes the forward took 135 us, now 48, the backward 214, now 80) and by the
+// f32 MFMA's rate and its operands' loads past them (64: 53 us, floor 21).
+constexpr int kRowsWaves = 8, kRowsK = 32;
+template <bool kGuard>
+__device__ __forceinline__ void Row4(const float* p, bool vec, int left, float (&v)[4]) {
+  if (vec && (!kGuard || left >= 4)) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = !kGuard || e < left ? p[e] : 0.0f;
+  }
+}
+template <bool kGuard, bool kVec, int kC>
+__device__ __forceinline__ void Cols(const float* p, const size_t (&col)[kC], bool in, float (&v)[kC]) {
+#pragma unroll
+  for (int c = 0; c < kC; ++c) v[c] = 0.0f;
+  if (kGuard && !in) return;
+  if constexpr (kVec && kC == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p + col[0]);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  } else if constexpr (kVec && kC == 2) {
+    const float2 a = *reinterpret_cast<const float2*>(p + col[0]);
+    v[0] = a.x, v[1] = a.y;
+  } else {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) v[c] = p[col[c]];
+  }
+}
+template <int kEpi, bool kBS, bool kVec, int kR, int kC>
+__global__ void __launch_bounds__(kRowsWaves * kWave) FfnRows32(MmaArgs p) {
+  constexpr int kBoth = kEpi == kGate ? 2 : 1, BM = 32 * kR, BN = 32 * kC;
+  __shared__ float sums[kRowsWaves][32][32 + 4];
+  const int wave = Uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int i = lane % 32, h = lane / 32;
+  const int per_seg = (p.K + kRowsK - 1) / kRowsK, total = p.nseg * per_seg;
+  const int split = blockIdx.x / p.tiles, tile = blockIdx.x - split * p.tiles;
+  const int first = split * p.per_split, end = min(total, first + p.per_split);
+  int m0, n0;
+  const Product& q = p.q[ProductOf(p, tile, BM, BN, m0, n0)];
+  // Rows and columns past the end repeat the last: nothing of theirs is stored.
+  size_t row[kR], col[kC];
+#pragma unroll
+  for (int r = 0; r < kR; ++r) row[r] = static_cast<size_t>(min(m0 + 32 * r + i, q.M - 1)) * q.lda;
+#pragma unroll
+  for (int c = 0; c < kC; ++c)
+    col[c] = kBS ? (kVec ? min(n0 + kC * i, q.N - kC) + c : min(n0 + kC * i + c, q.N - 1))
+                 : min(n0 + 32 * c + i, q.N - 1) * static_cast<size_t>(q.ldb);
+  v16f acc[kBoth][kR][kC];
+#pragma unroll
+  for (int b = 0; b < kBoth; ++b)
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+      for (int c = 0; c < kC; ++c) acc[b][r][c] = v16f{};
+  for (int s = first + wave; s < end; s += kRowsWaves) {
+    const int seg = s / per_seg, k0 = (s - seg * per_seg) * kRowsK;
+    auto step = [&](auto guard) __attribute__((always_inline)) {
+      constexpr bool kGuard = decltype(guard)::value;
+      float a[kR][kRowsK / 8][4], w[kBoth][kRowsK / 8][4][kC];
+#pragma unroll
+      for (int u = 0; u < kRowsK / 8; ++u) {
+        const int k = k0 + 8 * u + 4 * h, left = p.K - k;
+#pragma unroll
+        for (int r = 0; r < kR; ++r)
+          Row4<kGuard>(reinterpret_cast<const float*>(q.A[seg]) + row[r] + k, kVec, left, a[r][u]);
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b) {
+          const float* B = reinterpret_cast<const float*>(b ? q.B2[seg] : q.B[seg]);
+          if constexpr (kBS) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Cols<kGuard, kVec>(B + static_cast<size_t>(k + j) * q.ldb, col, j < left, w[b][u][j]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+              float v[4];
+              Row4<kGuard>(B + col[c] + k, kVec, left, v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[b][u][j][c] = v[j];
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kRowsK / 8; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int b = 0; b < kBoth; ++b)
+#pragma unroll
+            for (int r = 0; r < kR; ++r)
+#pragma unroll
+              for (int c = 0; c < kC; ++c)
+                acc[b][r][c] =
+                    __builtin_amdgcn_mfma_f32_32x32x2f32(w[b][u][j][c], a[r][u][j], acc[b][r][c], 0, 0, 0);
+    };
+    if (k0 + kRowsK <= p.K) step(std::false_type{});
+    else step(std::true_type{});
+  }
+  // The waves' sums of 32 x 32 after 32 x 32, two elements a thread.
+  constexpr int kEach = 1024 / (kRowsWaves * kWave);
+  Each<kR * kC>([&](auto t) __attribute__((always_inline)) {
+    constexpr int r = decltype(t)::value / kC, c = decltype(t)::value % kC;
+    float v[kBoth][kEach];
+#pragma unroll
+    for (int b = 0; b < kBoth; ++b) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<float4*>(&sums[wave][i][8 * e + 4 * h]) =
+            make_float4(acc[b][r][c][4 * e], acc[b][r][c][4 * e + 1], acc[b][r][c][4 * e + 2], acc[b][r][c][4 * e + 3]);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int x = e * kRowsWaves * kWave + threadIdx.x;
+        v[b][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRowsWaves; ++k) v[b][e] += sums[k][x / 32][x % 32];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int x = e * kRowsWaves * kWave + threadIdx.x;
+      const int m = 32 * r + x / 32, n = kBS ? x % 32 * kC + c : 32 * c + x % 32;
+      if (m0 + m >= q.M) continue;
+      if (p.splits > 1) {
+        float* out = p.part + ((static_cast<size_t>(tile) * p.splits + split) * BM + m) * (kBoth * BN) + n;
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b) out[b * BN] = v[b][e];
+      } else {
+        Finish1<float, kEpi, true>(p, q, m0 + m, n0 + n, v[0][e], v[kBoth - 1][e]);
+      }
+    }
+  });
+}
+
+// The weights' gradients of few f32 tokens: K is the tokens, so what there is to
+// move is the stores.  A workgroup takes 128 x 128, a wave 32 rows of it and four
+// neighbouring columns a lane: stores of 512 bytes.  The operands' 128 columns
+// of up to 32 tokens are staged in LDS (64 tokens of 2048 x 5632: 69 us, with
+// operands straight from memory 90).  8 tokens: 26 us for 138 MB stored, 5.3 TB/s.
+constexpr int kOuterWaves = 4, kOuterK = 32;
+// Tokens [k0, k0 + rows) of operand columns [c0, c0 + 128), zeros past K and
+// past `cols`.
+__device__ __forceinline__ void StageOuter(float (*to)[128], const float* p, int ld, int c0, int cols, bool vec,
+                                           int k0, int K) {
+  constexpr int kThreads = kOuterWaves * kWave;
+#pragma unroll
+  for (int j = 0; j < kOuterK * 32 / kThreads; ++j) {
+    const int x = j * kThreads + threadIdx.x, k = k0 + x / 32, c = c0 + x % 32 * 4;
+    const int left = k < K ? cols - c : 0;
+    float v[4] = {};
+    if (left > 0) Row4<true>(p + static_cast<size_t>(k) * ld + c, vec, left, v);
+    *reinterpret_cast<float4*>(&to[x / 32][x % 32 * 4]) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+__global__ void __launch_bounds__(kOuterWaves * kWave, 4) FfnOuter32(MmaArgs p) {
+  __shared__ float A[kOuterK][128], B[kOuterK][128];
+  const int wave = Uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int i = lane % 32, h = lane / 32;
+  int m0, n0;
+  const Product& q = p.q[ProductOf(p, XcdRun(blockIdx.x, p.tiles), 128, 128, m0, n0)];
+  v16f acc[4] = {};
+  for (int k0 = 0; k0 < p.K; k0 += kOuterK) {
+    if (k0) __syncthreads();
+    StageOuter(A, reinterpret_cast<const float*>(q.A[0]), q.lda, m0, q.M, q.vec_a, k0, p.K);
+    StageOuter(B, reinterpret_cast<const float*>(q.B[0]), q.ldb, n0, q.N, q.vec, k0, p.K);
+    __syncthreads();
+    const int turns = (min(p.K - k0, kOuterK) + 1) / 2;
+#pragma unroll 4
+    for (int u = 0; u < turns; ++u) {
+      const float a = A[2 * u + h][32 * wave + i];
+      const float4 b = *reinterpret_cast<const float4*>(&B[2 * u + h][4 * i]);
+      acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b.x, acc[0], 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b.y, acc[1], 0, 0, 0);
+      acc[2] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b.z, acc[2], 0, 0, 0);
+      acc[3] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b.w, acc[3], 0, 0, 0);
+    }
+  }
+  const int n = n0 + 4 * i;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int m = m0 + 32 * wave + 8 * (e / 4) + 4 * h + e % 4;
+    if (m >= q.M) continue;
+    float* out = static_cast<float*>(q.o1) + static_cast<size_t>(m) * q.N + n;
+    if (q.vec) {
+      if (n < q.N) *reinterpret_cast<float4*>(out) = make_float4(acc[0][e], acc[1][e], acc[2][e], acc[3][e]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (n + c < q.N) out[c] = acc[c][e];
+    }
+  }
+}
+
 // --- host ---------------------------------------------------------------------------------------
 
 // How a launch runs: its tile, and over how many workgroups the K of the tiles
@@ -776,14 +986,17 @@ constexpr size_t kMostPart = size_t{64} << 20;  // bytes of shared-out sums
 struct Shape {
   size_t M, N;
 };
+// (f32's gradient epilogue, nine planes an eight, is past the registers beside 256 x 256.)
+constexpr int FirstTile(Epilogue epi, bool bf16) { return epi == kGrad && !bf16 ? 1 : 0; }
 // Either every tile's K is shared out, or, with more tiles than the chip holds
 // at once, that of the tiles left over after whole rounds: 528 tiles of the
 // weights' gradients run as two rounds and a sixteenth instead of three.
-Plan Choose(bool dual, std::initializer_list<Shape> products, size_t K, int nseg) {
+// (`from`: the first tile of kTiles the kernel comes in.)
+Plan Choose(int from, bool dual, std::initializer_list<Shape> products, size_t K, int nseg) {
   const double stages = static_cast<double>((K + kDeep - 1) / kDeep) * nseg;
   Plan best;
   double least = 1e30;
-  for (int t = 0; t < 3; ++t) {
+  for (int t = from; t < 3; ++t) {
     const TileShape& s = kTiles[t];
     const int bn = dual ? s.bn_dual : s.bn;
     const double alone = dual ? s.alone_dual : s.alone, shared = dual ? s.shared_dual : s.shared;
@@ -837,8 +1050,9 @@ hipError_t Mma(MmaArgs a, float* part, hipStream_t s) {
   const Shape shape[3] = {{static_cast<size_t>(a.q[0].M), static_cast<size_t>(a.q[0].N)},
                           {static_cast<size_t>(a.q[1].M), static_cast<size_t>(a.q[1].N)},
                           {static_cast<size_t>(a.q[2].M), static_cast<size_t>(a.q[2].N)}};
-  const Plan plan = a.count == 1 ? Choose(dual, {shape[0]}, a.K, a.nseg)
-                                 : Choose(dual, {shape[0], shape[1], shape[2]}, a.K, a.nseg);
+  constexpr int from = FirstTile(static_cast<Epilogue>(kEpi), sizeof(T) == 2);
+  const Plan plan = a.count == 1 ? Choose(from, dual, {shape[0]}, a.K, a.nseg)
+                                 : Choose(from, dual, {shape[0], shape[1], shape[2]}, a.K, a.nseg);
   const TileShape& t = kTiles[plan.tile];
   const int bn = dual ? t.bn_dual : t.bn;
   for (int i = 0, first = 0; i < a.count; ++i) {
@@ -848,9 +1062,7 @@ hipError_t Mma(MmaArgs a, float* part, hipStream_t s) {
   a.tiles = plan.tiles, a.whole = plan.whole, a.splits = plan.splits, a.per_split = plan.per_split;
   a.part = part;
   hipError_t e = hipErrorInvalidValue;
-  // (f32's gradient epilogue, nine planes an eight, is past the registers beside 256 x 256.)
-  constexpr bool big = !(kEpi == kGrad && sizeof(T) == 4);
-  if constexpr (big) {
+  if constexpr (from == 0) {
     if (plan.tile == 0) e = LaunchTile<T, kEpi, kAS, kBS, 256, 256, 64, 2, 4, 2>(a, s);
   }
   if (plan.tile == 1) e = LaunchTile<T, kEpi, kAS, kBS, 128, 128, 64, 2, 2, 2>(a, s);
@@ -858,6 +1070,59 @@ hipError_t Mma(MmaArgs a, float* part, hipStream_t s) {
   if (e != hipSuccess || plan.whole == plan.tiles) return e;
   auto* kernel = &FfnJoin<T, kEpi>;
   hipLaunchKernelGGL(kernel, dim3(plan.tiles - plan.whole, t.bm * bn / 2048), dim3(256), 0, s, a, t.bm, bn);
+  return hipGetLastError();
+}
+
+// f32 tokens up to which FfnRows32 and FfnOuter32 run the products.  Forward and
+// backward at 2048 x 5632, us, against the planes: 16 tokens 48, 83 (138, 214);
+// 64 tokens 82, 152 (155, 241); 128 tokens 133, 247 (170, 282); 192 tokens 250,
+// 443 (206, 345).  Smaller weights turn at 192 or later.
+constexpr size_t kRowsMost = 128;
+bool FewRows(int planes, size_t M) { return planes == 3 && M <= kRowsMost; }
+// FfnRows32's tile, and how it shares K out: over workgroups enough for the
+// chip, with a turn for every wave.  Measured on 4 and 64 tokens of 2048 x 5632
+// (forward, whole): gate tiles 32 wide over 768 workgroups 53 and 106 us, over
+// 256 56 and 108, 64 wide 56 and 161; plain ones 64 wide over 256 53 and 100,
+// 32 wide over 512 59 and 116.  Where that leaves the chip short of workgroups
+// the 32 x 32 tile is better: 64 tokens of 333 x 1111 26 us against 43.
+struct RowsPlan {
+  int rows, cols, tiles, splits, per_split;
+};
+RowsPlan ChooseRows(Epilogue epi, const Shape& q, size_t K, int nseg) {
+  const int steps = static_cast<int>((K + kRowsK - 1) / kRowsK) * nseg;
+  const int groups = epi == kPlain ? 256 : 768;
+  RowsPlan plan;
+  const int most = std::max(1, steps / kRowsWaves);
+  const bool small = (q.M + 31) / 32 * ((q.N + 31) / 32) * most < 512;
+  plan.rows = q.M > 32 && !small ? 64 : 32;
+  plan.cols = epi == kPlain && !small ? 64 : 32;
+  plan.tiles = static_cast<int>(((q.M + plan.rows - 1) / plan.rows) * ((q.N + plan.cols - 1) / plan.cols));
+  const int splits = std::min(most, std::max(1, (groups + plan.tiles / 2) / plan.tiles));
+  plan.per_split = (steps + splits - 1) / splits;
+  plan.splits = (steps + plan.per_split - 1) / plan.per_split;
+  return plan;
+}
+size_t RowsPartBytes(const RowsPlan& plan, bool dual) {
+  return plan.splits == 1 ? 0 : static_cast<size_t>(plan.tiles) * plan.splits * plan.rows * plan.cols * (dual ? 8 : 4);
+}
+template <int kEpi, bool kBS>
+hipError_t Rows32(MmaArgs a, bool vec, float* part, hipStream_t s) {
+  const Shape shape{static_cast<size_t>(a.q[0].M), static_cast<size_t>(a.q[0].N)};
+  const RowsPlan plan = ChooseRows(static_cast<Epilogue>(kEpi), shape, a.K, a.nseg);
+  a.tiles = plan.tiles, a.splits = plan.splits, a.per_split = plan.per_split;
+  a.part = part;
+  constexpr int kC = kEpi == kPlain ? 2 : 1;
+  using Kernel = void (*)(MmaArgs);
+  Kernel kernel = vec ? &FfnRows32<kEpi, kBS, true, 1, 1> : &FfnRows32<kEpi, kBS, false, 1, 1>;
+  if (plan.rows == 32 && plan.cols == 32 * kC)
+    kernel = vec ? &FfnRows32<kEpi, kBS, true, 1, kC> : &FfnRows32<kEpi, kBS, false, 1, kC>;
+  if (plan.rows == 64)
+    kernel = vec ? &FfnRows32<kEpi, kBS, true, 2, kC> : &FfnRows32<kEpi, kBS, false, 2, kC>;
+  hipLaunchKernelGGL(kernel, dim3(plan.tiles * plan.splits), dim3(kRowsWaves * kWave), 0, s, a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || plan.splits == 1) return e;
+  auto* join = &FfnJoin<float, kEpi, true>;
+  const unsigned parts = (plan.rows * plan.cols + 2047) / 2048;
+  hipLaunchKernelGGL(join, dim3(plan.tiles, parts), dim3(256), 0, s, a, plan.rows, plan.cols);
   return hipGetLastError();
 }
 
@@ -895,6 +1160,20 @@ struct Layout {
 Layout Lay(void* ws, int planes, size_t M, size_t D, size_t F, bool backward) {
   Space s(ws);
   Layout l;
+  if (FewRows(planes, M)) {
+    l.h = s.Take(M, F, 2);  // (two planes' bytes are f32's)
+    if (backward) {
+      l.dg = s.Take(M, F, 2);
+      l.du = s.Take(M, F, 2);
+    }
+    auto rows = [&](Epilogue epi, size_t n, size_t k, int segs) {
+      return RowsPartBytes(ChooseRows(epi, {M, n}, k, segs), epi == kGate);
+    };
+    l.part = s.Floats(backward ? std::max(rows(kGrad, F, D, 1), rows(kPlain, D, F, 2))
+                               : std::max(rows(kGate, F, D, 1), rows(kPlain, D, F, 1)));
+    l.bytes = s.used();
+    return l;
+  }
   l.x = s.Take(M, D, planes);
   l.wg = s.Take(D, F, planes);
   l.wu = s.Take(D, F, planes);
@@ -906,12 +1185,13 @@ Layout Lay(void* ws, int planes, size_t M, size_t D, size_t F, bool backward) {
     l.du = s.Take(M, F, planes);
   }
   const int nseg = planes == 1 ? 1 : 6;
-  auto part = [&](bool dual, std::initializer_list<Shape> q, size_t k, int segs) {
-    return PartBytes(Choose(dual, q, k, segs), dual);
+  auto part = [&](Epilogue epi, std::initializer_list<Shape> q, size_t k, int segs) {
+    const bool dual = epi == kGate;
+    return PartBytes(Choose(FirstTile(epi, planes == 1), dual, q, k, segs), dual);
   };
-  l.part = s.Floats(backward ? std::max({part(false, {{M, F}}, D, nseg), part(false, {{M, D}}, F, 2 * nseg),
-                                         part(false, {{D, F}, {D, F}, {F, D}}, M, nseg)})
-                             : std::max(part(true, {{M, F}}, D, nseg), part(false, {{M, D}}, F, nseg)));
+  l.part = s.Floats(backward ? std::max({part(kGrad, {{M, F}}, D, nseg), part(kPlain, {{M, D}}, F, 2 * nseg),
+                                         part(kPlain, {{D, F}, {D, F}, {F, D}}, M, nseg)})
+                             : std::max(part(kGate, {{M, F}}, D, nseg), part(kPlain, {{M, D}}, F, nseg)));
   l.bytes = s.used();
   return l;
 }
@@ -981,10 +1261,64 @@ MmaArgs Launch(size_t K) {
     if (hipError_t e_ = (expr); e_ != hipSuccess) return e_; \
   } while (0)
 
+// A product of f32 operands as they are, rows of A by B (and B2).
+Product& AddRaw(MmaArgs& a, size_t M, size_t N, const void* A, size_t lda, const void* B, size_t ldb,
+                const void* B2 = nullptr) {
+  Product& q = a.q[a.count++];
+  q.M = static_cast<int>(M), q.N = static_cast<int>(N);
+  q.lda = static_cast<int>(lda), q.ldb = static_cast<int>(ldb);
+  q.A[0] = static_cast<const uint16_t*>(A);
+  q.B[0] = static_cast<const uint16_t*>(B);
+  q.B2[0] = static_cast<const uint16_t*>(B2);
+  a.nseg = 1;
+  return q;
+}
+bool Fours(size_t n, std::initializer_list<const void*> ptrs) {
+  uintptr_t at = 0;
+  for (const void* p : ptrs) at |= reinterpret_cast<uintptr_t>(p);
+  return n % 4 == 0 && (at & 15) == 0;
+}
+
+hipError_t FwdRows(const FfnArgs& f, const Layout& l, hipStream_t s) {
+  MmaArgs a = Launch(f.D);
+  Product& gate = AddRaw(a, f.M, f.F, f.x, f.D, f.wg, f.F, f.wu);
+  gate.o1 = f.gate, gate.o2 = f.up, gate.vec = Octs<float>(f.F, {f.gate, f.up});
+  a.act = f.act, a.h = l.h;
+  FFN_TRY((Rows32<kGate, true>(a, Fours(f.D, {f.x}) && Fours(f.F, {f.wg, f.wu}), l.part, s)));
+  a = Launch(f.F);
+  Product& down = AddRaw(a, f.M, f.D, l.h.p, l.h.ld, f.wd, f.D);
+  down.o1 = f.y, down.vec = Octs<float>(f.D, {f.y});
+  return Rows32<kPlain, true>(a, Fours(f.D, {f.wd}), l.part, s);
+}
+hipError_t BwdRows(const FfnArgs& f, const Layout& l, hipStream_t s) {
+  MmaArgs a = Launch(f.D);
+  AddRaw(a, f.M, f.F, f.dy, f.D, f.wd, f.D).vec = Octs<float>(f.F, {f.gate, f.up});
+  a.act = f.act, a.g = f.gate, a.u = f.up, a.h = l.h, a.dg = l.dg, a.du = l.du;
+  FFN_TRY((Rows32<kGrad, false>(a, Fours(f.D, {f.dy, f.wd}), l.part, s)));
+  a = Launch(f.F);
+  Product& dx = AddRaw(a, f.M, f.D, l.dg.p, l.dg.ld, f.wg, f.F);
+  dx.A[1] = l.du.p, dx.B[1] = static_cast<const uint16_t*>(f.wu), a.nseg = 2;
+  dx.o1 = f.dx, dx.vec = Octs<float>(f.D, {f.dx});
+  FFN_TRY((Rows32<kPlain, false>(a, Fours(f.F, {f.wg, f.wu}), l.part, s)));
+  a = Launch(f.M);
+  const void* left[3] = {f.x, f.x, l.h.p};
+  const void* right[3] = {l.dg.p, l.du.p, f.dy};
+  void* out[3] = {f.dwg, f.dwu, f.dwd};
+  for (int i = 0; i < 3; ++i) {
+    const size_t M = i == 2 ? f.F : f.D, N = i == 2 ? f.D : f.F;
+    Product& q = AddRaw(a, M, N, left[i], i == 2 ? l.h.ld : f.D, right[i], i == 2 ? f.D : l.dg.ld);
+    q.o1 = out[i], q.vec = Fours(N, {out[i], right[i]}), q.vec_a = Fours(M, {left[i]}), q.first = a.tiles;
+    a.tiles += static_cast<int>((M + 127) / 128 * ((N + 127) / 128));
+  }
+  hipLaunchKernelGGL(FfnOuter32, dim3(a.tiles), dim3(kOuterWaves * kWave), 0, s, a);
+  return hipGetLastError();
+}
+
 template <class T>
 hipError_t Fwd(const FfnArgs& f, hipStream_t s) {
   if (f.M == 0) return hipSuccess;
   Layout l = Lay(f.ws, sizeof(T) == 2 ? 1 : 3, f.M, f.D, f.F, false);
+  if (sizeof(T) == 4 && FewRows(3, f.M)) return FwdRows(f, l, s);
   Pieces pieces{};
   Take<T>(f.x, f.M, f.D, l.x, pieces);
   Take<T>(f.wg, f.D, f.F, l.wg, pieces);
@@ -1014,6 +1348,7 @@ hipError_t Bwd(const FfnArgs& f, hipStream_t s) {
     return hipSuccess;
   }
   Layout l = Lay(f.ws, sizeof(T) == 2 ? 1 : 3, f.M, f.D, f.F, true);
+  if (sizeof(T) == 4 && FewRows(3, f.M)) return BwdRows(f, l, s);
   Pieces pieces{};
   Take<T>(f.x, f.M, f.D, l.x, pieces);
   Take<T>(f.wg, f.D, f.F, l.wg, pieces);

@@ -318,6 +318,23 @@ def test_ffn(hip, ctx, torch_cuda, bf16, act, off):
             assert torch.equal(a, b), "a gradient differs run to run"
 
 
+@pytest.mark.parametrize("bf16,M,D,F", [
+    # the largest tile on every side of an f32 backward; few f32 rows (they take the weights as
+    # they are) about where that ends, K long enough to be shared out, rows on and off 16 bytes
+    (0, 4096, 64, 4096), (1, 4096, 64, 4096), (0, 1, 2048, 640), (0, 33, 1001, 1538),
+    (0, 64, 700, 2052), (0, 65, 700, 2052), (0, 128, 700, 2052), (0, 129, 700, 2052),
+    (0, 64, 4100, 36), (0, 7, 36, 9000)])
+def test_ffn_sizes_a_rule_turns_at(hip, ctx, torch_cuda, bf16, M, D, F):
+    torch = torch_cuda
+    t, step = types(torch, bf16)
+    ins = ffn_inputs(torch, M, D, F, t, 0, M + D + F)
+    gate, up, y = ffn_fwd(hip, ctx, torch, bf16, 3, *ins, True)
+    check_ffn_fwd(torch, 3, step, *ins, gate, up, y)
+    dy = put(torch, gen(torch, 5)(M, D), t, 0)
+    grads = ffn_bwd(hip, ctx, torch, bf16, 3, *ins, gate, up, dy)
+    check_ffn_bwd(torch, 3, step, *ins, gate, up, dy, *grads)
+
+
 def test_ffn_gradients_against_differences(hip, ctx, torch_cuda):
     """Central differences of the block's own forward, f32: the loss sum(y c) along random
     directions of x and of each weight.  A difference at h is off by h^2 of the third
