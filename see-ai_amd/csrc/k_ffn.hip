@@ -262,14 +262,27 @@ __global__ void __launch_bounds__(256) FfnPackKernel(Pieces p) {
   int k = 0;
   while (k + 1 < p.count && blockIdx.x >= p.q[k + 1].first) ++k;
   const Piece& q = p.q[k];
-  const int octs = q.out.ld / 8;
-  const size_t i = static_cast<size_t>(blockIdx.x - q.first) * 256 + threadIdx.x;
-  if (i >= q.rows * octs) return;
-  const size_t r = i / octs;
-  const int c = static_cast<int>(i % octs) * 8;
+  // 2048 elements of the padded rows a workgroup, eight a thread; rows off 16
+  // bytes come a lane an element through LDS.
+  __shared__ float st[256 * 8];
+  const size_t base = static_cast<size_t>(blockIdx.x - q.first) * 2048, r0 = base / q.out.ld;
+  const uint32_t ld = q.out.ld, c0 = static_cast<uint32_t>(base - r0 * ld);
+  if (!q.vec) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t x = e * 256 + threadIdx.x, rr = (c0 + x) / ld, cc = c0 + x - rr * ld;
+      const bool in = r0 + rr < q.rows && cc < static_cast<uint32_t>(q.cols);
+      st[x] = in ? One(static_cast<const T*>(q.in) + (r0 + rr) * q.cols + cc) : 0.0f;
+    }
+    __syncthreads();
+  }
+  const uint32_t at = c0 + threadIdx.x * 8, rr = at / ld, c = at - rr * ld;
+  const size_t r = r0 + rr;
+  if (r >= q.rows) return;
   float v[8];
-  Load8(static_cast<const T*>(q.in) + r * q.cols + c, q.vec, q.cols - c, v);
-  PutPlanes<T>(q.out, r * q.out.ld + c, v);
+  if (q.vec) Load8(static_cast<const T*>(q.in) + r * q.cols + c, true, q.cols - static_cast<int>(c), v);
+  else Load8(st + threadIdx.x * 8, true, 8, v);
+  PutPlanes<T>(q.out, r * ld + c, v);
 }
 
 template <class T>
@@ -508,40 +521,36 @@ __global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
   const Product& q = p.q[ProductOf(p, p.whole + blockIdx.x, bm, bn, m0, n0)];
   const size_t row = static_cast<size_t>(kBoth) * bn, split = bm * row;
   const float* at = p.part + blockIdx.x * p.splits * split;
+  __shared__ float st[kBoth][256 * 8];
+  const int i = (blockIdx.y * 256 + threadIdx.x) * 8, r = i / bn, col = i % bn;
+  const bool in = r < bm && m0 + r < q.M && n0 + col < q.N;
+  float s[2][8] = {};
+  for (int k0 = 0; in && k0 < p.splits; k0 += 4) {  // four sums' loads in flight
+    float v[4][kBoth][8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < kBoth; ++b)
+        Load8(at + min(k0 + k, p.splits - 1) * split + r * row + b * bn + col, true, 8, v[k][b]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < kBoth; ++b)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < p.splits ? v[k][b][e] : 0.0f;
+  }
   if (q.vec) {
-    const int i = (blockIdx.y * 256 + threadIdx.x) * 8, r = i / bn, col = i % bn;
-    if (r >= bm || m0 + r >= q.M || n0 + col >= q.N) return;
-    float s[2][8] = {};
-    for (int k0 = 0; k0 < p.splits; k0 += 4) {  // four sums' loads in flight
-      float v[4][kBoth][8];
+    if (in) Finish<T, kEpi, kWhole>(p, q, m0 + r, n0 + col, s[0], s[1]);
+    return;
+  }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+  for (int b = 0; b < kBoth; ++b) Store8(&st[b][threadIdx.x * 8], true, 8, s[b]);
+  __syncthreads();
 #pragma unroll
-        for (int b = 0; b < kBoth; ++b)
-          Load8(at + min(k0 + k, p.splits - 1) * split + r * row + b * bn + col, true, 8, v[k][b]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int b = 0; b < kBoth; ++b)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < p.splits ? v[k][b][e] : 0.0f;
-    }
-    Finish<T, kEpi, kWhole>(p, q, m0 + r, n0 + col, s[0], s[1]);
-  } else {
-    float s[8][2] = {};
-    for (int k = 0; k < p.splits; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int b = 0; b < kBoth; ++b) {
-          const int i = (blockIdx.y * 8 + e) * 256 + threadIdx.x;
-          if (i < bm * bn) s[e][b] += at[k * split + i / bn * row + b * bn + i % bn];
-        }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = (blockIdx.y * 8 + e) * 256 + threadIdx.x;
-      if (i < bm * bn && m0 + i / bn < q.M) Finish1<T, kEpi, kWhole>(p, q, m0 + i / bn, n0 + i % bn, s[e][0], s[e][1]);
-    }
+  for (int e = 0; e < 8; ++e) {
+    const int x = e * 256 + threadIdx.x, j = blockIdx.y * 2048 + x;
+    if (j < bm * bn && m0 + j / bn < q.M)
+      Finish1<T, kEpi, kWhole>(p, q, m0 + j / bn, n0 + j % bn, st[0][x], st[kBoth - 1][x]);
   }
 }
 
