@@ -241,8 +241,8 @@ struct RawRow {
 // partials (db behind dw), or dw and db themselves when the grid is one.  A
 // row's loads go out while the row before it is reduced: with a wave a row
 // there is nothing else to cover their latency (8192 x 2048 bf16 on MI355X: 30
-// us with, 41 without; the copy rate would be 20).  The weight sits in LDS, a lane's own columns together, to
-// leave the registers to that row.
+// us with, 41 without; the copy rate would be 20).  The weight sits in LDS, a
+// lane's own columns together, to leave the registers to that row.
 template <class T, int kTPR, int kE, bool kVec>
 __global__ void __launch_bounds__(BwdThreads(kTPR), kBwdPerSimd)
 NormBwdKernel(int rms, const T* __restrict__ dy, const T* __restrict__ x,
@@ -437,8 +437,17 @@ NormFoldKernel(const float* __restrict__ part, int n, size_t cols, float* __rest
   }
 }
 
-// Workgroups of the backward pass: two a CU, and no more than the rows fill.
+// Workgroups of the backward pass: two a CU where two of them fit and each has
+// rows to walk (four turns), else one; each leaves a partial row to be written
+// and added.  us over 256 and 512 (layer, bf16): 8192 x 2048 30.6 and 29.0,
+// 32000 x 2048 108 and 80, but 3001 x 1023 13.8 and 15.2, 600 x 2048 12.8 and
+// 15.7, and with 1024 threads a workgroup 2000 x 8192 35 and 48, 16000 x 8192
+// 180 and 194.
 constexpr size_t kBwdGroups = 512;
+size_t BwdGroups(int threads, size_t groups) {
+  const size_t most = threads > 512 || groups < 4 * kBwdGroups ? kBwdGroups / 2 : kBwdGroups;
+  return groups < most ? groups : most;
+}
 constexpr size_t kRegCols = 16384;  // the longest row held in registers
 
 // A launch's workgroups (the kernels walk the rows past them).
@@ -470,7 +479,7 @@ hipError_t Run(const NormCall& a, bool bwd, hipStream_t s) {
   }
   constexpr int kThreads = BwdThreads(kTPR), kRows = kThreads / kTPR;
   const size_t groups = (a.rows + kRows - 1) / kRows;
-  const unsigned grid = static_cast<unsigned>(groups < kBwdGroups ? (groups ? groups : 1) : kBwdGroups);
+  const unsigned grid = groups ? static_cast<unsigned>(BwdGroups(kThreads, groups)) : 1;
   hipLaunchKernelGGL((NormBwdKernel<T, kTPR, kE, kVec>), dim3(grid), dim3(kThreads), 0, s,
                      a.rms, static_cast<const T*>(a.dy), static_cast<const T*>(a.x), a.w, a.mean,
                      a.rstd, static_cast<T*>(a.out), a.o1, a.o2, a.part, a.rows, cols);
