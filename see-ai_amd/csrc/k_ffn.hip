@@ -304,9 +304,10 @@ __device__ __forceinline__ void Each(F&& f) {
 
 // One product of a launch.  Operand element (i, k) lies at i ld + k, or,
 // "strided", at k ld + i.  Segments are products of the same shape added up.
-constexpr int kMaxSeg = 12;
+constexpr int kMaxSeg = 2;
 struct Product {
   const uint16_t *A[kMaxSeg], *B[kMaxSeg], *B2[kMaxSeg];
+  size_t a_plane, b_plane;  // elements between an operand's planes
   int lda, ldb, M, N;
   bool vec;       // outputs (and G, U) take eight neighbours at once
   bool vec_a;     // FfnOuter32: A takes four, and `vec` is of four too
@@ -565,8 +566,10 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   using TA = Tile<kAS, BM, BK, kWaves>;
   using TBt = Tile<kBS, BNs, BK, kWaves>;
   constexpr int kSub = BK / 16;  // half-waves of K in a stage
-  constexpr int kStage = TA::kBytes + (kDual ? 2 : 1) * TBt::kBytes;
-  constexpr int kPerStage = TA::kLoads + (kDual ? 2 : 1) * TBt::kLoads;
+  // A stage holds A's planes, B's and B2's.
+  constexpr int kPl = sizeof(T) == 4 ? 3 : 1, kA = kPl * TA::kBytes, kB = kPl * TBt::kBytes;
+  constexpr int kStage = kA + (kDual ? 2 : 1) * kB;
+  constexpr int kPerStage = kPl * (TA::kLoads + (kDual ? 2 : 1) * TBt::kLoads);
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kStages * kStage];
 
   const int wave = Uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
@@ -602,21 +605,30 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   const uint16_t* pb2 = kDual ? q.B2[seg] + b_at : nullptr;
   // Part `part` of kParts of the next stage's loads into buffer `buf`.  With
   // two buffers the stage is wanted at this one's end: its first half's steps.
-  constexpr int kParts = kStages == 2 ? kSub / 2 : kSub;
+  constexpr int kParts = kPl == 3 ? 1 : kStages == 2 ? kSub / 2 : kSub;
   auto issue = [&](int buf, auto part_tag) __attribute__((always_inline)) {
     constexpr int part = decltype(part_tag)::value;
     const uint32_t s = lds0 + buf * kStage;
+    if constexpr (kPl == 3) {
+#pragma unroll
+      for (int k = 0; k < kPl; ++k) {
+        ta.template Load<TA::kLoads>(pa + k * q.a_plane, k0, p.K, s + k * TA::kBytes, wave, 0);
+        tb.template Load<TBt::kLoads>(pb + k * q.b_plane, k0, p.K, s + kA + k * TBt::kBytes, wave, 0);
+        if constexpr (kDual)
+          tb.template Load<TBt::kLoads>(pb2 + k * q.b_plane, k0, p.K, s + kA + kB + k * TBt::kBytes, wave, 0);
+      }
+      return;
+    }
     // The stage's loads are A's, B's and B2's in turn; a part is a run of them
     // from one operand or a whole number of operands.
     constexpr int kLo = part * kPerStage / kParts, kHi = (part + 1) * kPerStage / kParts;
-    constexpr int kB = TA::kLoads, kB2 = TA::kLoads + TBt::kLoads;
-    constexpr int a0 = kLo, an = std::min(kHi, kB) - a0;
-    constexpr int b0 = std::max(kLo, kB), bn = std::min(kHi, kB2) - b0;
-    constexpr int c0 = std::max(kLo, kB2), cn = kHi - c0;
-    if constexpr (an > 0) ta.template Load<an>(pa, k0, p.K, s, wave, a0);
-    if constexpr (bn > 0) tb.template Load<bn>(pb, k0, p.K, s + TA::kBytes, wave, b0 - kB);
-    if constexpr (cn > 0)
-      tb.template Load<cn>(pb2, k0, p.K, s + TA::kBytes + TBt::kBytes, wave, c0 - kB2);
+    constexpr int kToB = TA::kLoads, kToB2 = TA::kLoads + TBt::kLoads;
+    constexpr int a0 = kLo, an = std::min(kHi, kToB) - a0;
+    constexpr int b0 = std::max(kLo, kToB), bn = std::min(kHi, kToB2) - b0;
+    constexpr int c0 = std::max(kLo, kToB2), cn = kHi - c0;
+    if constexpr (kPl == 1 && an > 0) ta.template Load<an>(pa, k0, p.K, s, wave, a0);
+    if constexpr (kPl == 1 && bn > 0) tb.template Load<bn>(pb, k0, p.K, s + kA, wave, b0 - kToB);
+    if constexpr (kPl == 1 && cn > 0) tb.template Load<cn>(pb2, k0, p.K, s + kA + kB, wave, c0 - kToB2);
   };
   // Past this workgroup's last stage the loads go on, past the product's they
   // repeat, into buffers nothing reads.
@@ -643,28 +655,37 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   for (int i = 0; i < TM; ++i) oa[i] = TA::Frag(wm + i * 32, lane);
 #pragma unroll
   for (int j = 0; j < TB; ++j)
-    ob[j] = TA::kBytes + (j / TN) * TBt::kBytes + TBt::Frag(wn + (j % TN) * 32, lane);
+    ob[j] = kA + (j / TN) * kB + TBt::Frag(wn + (j % TN) * 32, lane);
 
   // K in steps of 16: the step's fragments are read while the one before is
   // multiplied, into the other half of fa and fb.
-  bf16x8 fa[2][TM], fb[2][TB];
+  bf16x8 fa[2][kPl][TM], fb[2][kPl][TB];
   auto read = [&](int buf, auto ks_tag) __attribute__((always_inline)) {
     constexpr int ks = decltype(ks_tag)::value;
     const uint8_t* s = smem + buf * kStage;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fa[ks % 2][i] = TA::Read(s, oa[i], ks);
+    for (int k = kPl - 1; k >= 0; --k) {
 #pragma unroll
-    for (int j = 0; j < TB; ++j) fb[ks % 2][j] = TBt::Read(s, ob[j], ks);
+      for (int i = 0; i < TM; ++i) fa[ks % 2][k][i] = TA::Read(s + k * TA::kBytes, oa[i], ks);
+#pragma unroll
+      for (int j = 0; j < TB; ++j) fb[ks % 2][k][j] = TBt::Read(s + k * TBt::kBytes, ob[j], ks);
+    }
   };
+  // (f32: the six plane products, smallest first.)
+  constexpr int kPairs = kPl == 3 ? 6 : 1;
   auto mfmas = [&](int half) __attribute__((always_inline)) {
+    constexpr int pairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int k = 6 - kPairs; k < 6; ++k)
 #pragma unroll
-      for (int j = 0; j < TB; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[half][j], fa[half][i], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TB; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[half][pairs[k][1]][j], fa[half][pairs[k][0]][i],
+                                                              acc[i][j], 0, 0, 0);
   };
   // The next step's reads spread over the products of this one.
-  constexpr int kMfmas = TM * TB, kReads = TM * TA::kReads + TB * TBt::kReads;
+  constexpr int kMfmas = kPairs * TM * TB, kReads = kPl * (TM * TA::kReads + TB * TBt::kReads);
   constexpr int kPerSlot = (kReads + kMfmas - 1) / kMfmas;
   auto interleave = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -690,18 +711,22 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   // kStages buffers: one multiplied, one taking loads, the others in flight or
   // landed.  Before the last step of stage `it` every wave has its fragments of
   // it and stage it + 1 has landed.
-  for (int s = 0; s < kStages - 1; ++s) {
+  // f32's short stages take a buffer's next loads as soon as it is free.
+  constexpr bool kEarly = kPl == 3;
+  constexpr int kAhead = kEarly ? kStages : kStages - 1;
+  for (int s = 0; s < kAhead; ++s) {
     Each<kParts>([&](auto part) __attribute__((always_inline)) { issue(s, part); });
     advance();
   }
-  WaitVm<(kStages - 2) * kPerStage>();
+  WaitVm<(kAhead - 1) * kPerStage>();
   Barrier();
   read(0, std::integral_constant<int, 0>{});
   for (int it = 0; it < last; ++it) {
-    steps(it % kStages, (it + kStages - 1) % kStages, std::true_type{});
+    steps(it % kStages, (it + kStages - 1) % kStages, std::bool_constant<!kEarly>{});
     WaitVm<(kStages - 2) * kPerStage>();
     WaitLds();
     Barrier();
+    if constexpr (kEarly) issue(it % kStages, std::integral_constant<int, 0>{});
     advance();
     read((it + 1) % kStages, std::integral_constant<int, 0>{});
     mfmas((kSub - 1) % 2);
@@ -976,43 +1001,49 @@ struct Plan {
   int tiles = 0, whole = 0, splits = 1, per_split = 0;
 };
 struct TileShape {
-  int bm, bn, bn_dual, per_cu;  // rows, output columns, workgroups a CU holds
+  int rows, cols, rows_dual, cols_dual, per_cu;  // output's; workgroups a CU holds
+  int bm(bool dual) const { return dual ? rows_dual : rows; }
+  int bn(bool dual) const { return dual ? cols_dual : cols; }
   // us of a stage of one product and of two side by side: on an idle chip, and
   // more for every workgroup a CU holds.
   double alone, shared, alone_dual, shared_dual;
 };
-// Fitted to some 600 timings (three tiles, K shared out over 1 to 32, 39
-// products from 1 x 5632 x 2048 to 8192 x 2048 x 5632, both types), mean error
-// 12 %; the tile and sharing it picks were within 6 % of the best on average
-// (16 % the worst that was no outlier).  Few tokens take the 64-row tile with
-// K shared out -- 24 x 2048 x 5632: 10 us over 8, 25 us over 1, 95 us on 256 x
-// 256 -- many the 256 x 256: 8192 x 2048 x 11264 333 us against 443 on 128 x 128.
-constexpr TileShape kTiles[3] = {{256, 256, 128, 1, 1.07, 0.37, 1.11, 0.43},
-                                 {128, 128, 64, 2, 0.47, 0.21, 0.58, 0.24},
-                                 {64, 64, 64, 2, 0.18, 0.10, 0.27, 0.29}};
-constexpr int kDeep = 64;
+// bf16, fitted to some 600 timings (K shared out over 1 to 32, 39 products from
+// 1 x 5632 x 2048 to 8192 x 2048 x 5632), mean error 12 %; the tile and sharing
+// it picks were within 6 % of the best on average (16 % the worst that was no
+// outlier).  Few tokens take the 64-row tile with K shared out -- 24 x 2048 x
+// 5632: 10 us over 8, 25 us over 1, 95 us on 256 x 256 -- many the 256 x 256:
+// 8192 x 2048 x 11264 333 us against 443 on 128 x 128.
+constexpr TileShape kTiles[3] = {{256, 256, 256, 128, 1, 1.07, 0.37, 1.11, 0.43},
+                                 {128, 128, 128, 64, 2, 0.47, 0.21, 0.58, 0.24},
+                                 {64, 64, 64, 64, 2, 0.18, 0.10, 0.27, 0.29}};
+// f32, stages of 32 with all three planes of each operand in LDS, fitted to 490
+// timings (K shared out over 1 to 16, ten blocks from 150 x 128 x 512 to 200 x
+// 2048 x 5632), mean error 15 %.  dW of 1001 x 776 x 2048: 73 us (103 with a
+// stage a plane product on 128 x 128 x 64, which loads each plane twice).
+constexpr TileShape kTiles32[2] = {{256, 128, 128, 128, 1, 1.5, 1.5, 1.44, 1.5},
+                                   {64, 128, 64, 64, 2, 0.56, 0.52, 0.68, 0.55}};
+constexpr int Deep(bool f32) { return f32 ? 32 : 64; }
+const TileShape& TileOf(bool f32, int tile) { return f32 ? kTiles32[tile] : kTiles[tile]; }
 constexpr size_t kMostPart = size_t{64} << 20;  // bytes of shared-out sums
 struct Shape {
   size_t M, N;
 };
-// (f32's gradient epilogue, nine planes an eight, is past the registers beside 256 x 256.)
-constexpr int FirstTile(Epilogue epi, bool bf16) { return epi == kGrad && !bf16 ? 1 : 0; }
 // Either every tile's K is shared out, or, with more tiles than the chip holds
 // at once, that of the tiles left over after whole rounds: 528 tiles of the
 // weights' gradients run as two rounds and a sixteenth instead of three.
-// (`from`: the first tile of kTiles the kernel comes in.)
-Plan Choose(int from, bool dual, std::initializer_list<Shape> products, size_t K, int nseg) {
-  const double stages = static_cast<double>((K + kDeep - 1) / kDeep) * nseg;
+Plan Choose(bool f32, bool dual, std::initializer_list<Shape> products, size_t K, int nseg) {
+  const double stages = static_cast<double>((K + Deep(f32) - 1) / Deep(f32)) * nseg;
   Plan best;
   double least = 1e30;
-  for (int t = from; t < 3; ++t) {
-    const TileShape& s = kTiles[t];
-    const int bn = dual ? s.bn_dual : s.bn;
+  for (int t = 0; t < (f32 ? 2 : 3); ++t) {
+    const TileShape& s = TileOf(f32, t);
+    const int bm = s.bm(dual), bn = s.bn(dual);
     const double alone = dual ? s.alone_dual : s.alone, shared = dual ? s.shared_dual : s.shared;
-    const double tile_bytes = s.bm * bn * (dual ? 2 : 1) * 4.0, chip = 256.0 * s.per_cu;
+    const double tile_bytes = bm * bn * (dual ? 2 : 1) * 4.0, chip = 256.0 * s.per_cu;
     double tiles = 0;
     for (const Shape& q : products)
-      tiles += std::ceil(static_cast<double>(q.M) / s.bm) * std::ceil(static_cast<double>(q.N) / bn);
+      tiles += std::ceil(static_cast<double>(q.M) / bm) * std::ceil(static_cast<double>(q.N) / bn);
     // us of `wgs` workgroups of `per` stages.
     auto run = [&](double wgs, double per) {
       return std::ceil(wgs / chip) * per * (alone + std::min<double>(s.per_cu, wgs / 256.0) * shared);
@@ -1038,14 +1069,14 @@ Plan Choose(int from, bool dual, std::initializer_list<Shape> products, size_t K
   }
   return best;
 }
-size_t PartBytes(const Plan& plan, bool dual) {
-  const TileShape& s = kTiles[plan.tile];
-  return static_cast<size_t>(plan.tiles - plan.whole) * plan.splits * s.bm * (dual ? 2 * s.bn_dual : s.bn) * 4;
+size_t PartBytes(bool f32, const Plan& plan, bool dual) {
+  const TileShape& s = TileOf(f32, plan.tile);
+  return static_cast<size_t>(plan.tiles - plan.whole) * plan.splits * s.bm(dual) * s.bn(dual) * (dual ? 8 : 4);
 }
 
 template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
 hipError_t LaunchTile(const MmaArgs& a, hipStream_t s) {
-  static_assert(BK == kDeep, "per_split counts such stages");
+  static_assert(BK == Deep(sizeof(T) == 4), "per_split counts such stages");
   const unsigned grid = a.whole + static_cast<unsigned>(a.tiles - a.whole) * a.splits;
   auto* kernel = &FfnMma<T, kEpi, kAS, kBS, BM, BN, BK, WGM, WGN, kStages>;
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(WGM * WGN * kWave), 0, s, a);
@@ -1059,26 +1090,29 @@ hipError_t Mma(MmaArgs a, float* part, hipStream_t s) {
   const Shape shape[3] = {{static_cast<size_t>(a.q[0].M), static_cast<size_t>(a.q[0].N)},
                           {static_cast<size_t>(a.q[1].M), static_cast<size_t>(a.q[1].N)},
                           {static_cast<size_t>(a.q[2].M), static_cast<size_t>(a.q[2].N)}};
-  constexpr int from = FirstTile(static_cast<Epilogue>(kEpi), sizeof(T) == 2);
-  const Plan plan = a.count == 1 ? Choose(from, dual, {shape[0]}, a.K, a.nseg)
-                                 : Choose(from, dual, {shape[0], shape[1], shape[2]}, a.K, a.nseg);
-  const TileShape& t = kTiles[plan.tile];
-  const int bn = dual ? t.bn_dual : t.bn;
+  constexpr bool f32 = sizeof(T) == 4;
+  const Plan plan = a.count == 1 ? Choose(f32, dual, {shape[0]}, a.K, a.nseg)
+                                 : Choose(f32, dual, {shape[0], shape[1], shape[2]}, a.K, a.nseg);
+  const TileShape& t = TileOf(f32, plan.tile);
+  const int bm = t.bm(dual), bn = t.bn(dual);
   for (int i = 0, first = 0; i < a.count; ++i) {
     a.q[i].first = first;
-    first += ((a.q[i].M + t.bm - 1) / t.bm) * ((a.q[i].N + bn - 1) / bn);
+    first += ((a.q[i].M + bm - 1) / bm) * ((a.q[i].N + bn - 1) / bn);
   }
   a.tiles = plan.tiles, a.whole = plan.whole, a.splits = plan.splits, a.per_split = plan.per_split;
   a.part = part;
-  hipError_t e = hipErrorInvalidValue;
-  if constexpr (from == 0) {
+  hipError_t e;
+  if constexpr (f32) {
+    if (plan.tile == 0) e = LaunchTile<T, kEpi, kAS, kBS, dual ? 128 : 256, dual ? 256 : 128, 32, dual ? 2 : 4, dual ? 4 : 2, 2>(a, s);
+    else e = LaunchTile<T, kEpi, kAS, kBS, 64, 128, 32, 2, 2, 2>(a, s);
+  } else {
     if (plan.tile == 0) e = LaunchTile<T, kEpi, kAS, kBS, 256, 256, 64, 2, 4, 2>(a, s);
+    else if (plan.tile == 1) e = LaunchTile<T, kEpi, kAS, kBS, 128, 128, 64, 2, 2, 2>(a, s);
+    else e = LaunchTile<T, kEpi, kAS, kBS, 64, dual ? 128 : 64, 64, 2, 2, dual ? 3 : 4>(a, s);
   }
-  if (plan.tile == 1) e = LaunchTile<T, kEpi, kAS, kBS, 128, 128, 64, 2, 2, 2>(a, s);
-  if (plan.tile == 2) e = LaunchTile<T, kEpi, kAS, kBS, 64, dual ? 128 : 64, 64, 2, 2, dual ? 3 : 4>(a, s);
   if (e != hipSuccess || plan.whole == plan.tiles) return e;
   auto* kernel = &FfnJoin<T, kEpi>;
-  hipLaunchKernelGGL(kernel, dim3(plan.tiles - plan.whole, t.bm * bn / 2048), dim3(256), 0, s, a, t.bm, bn);
+  hipLaunchKernelGGL(kernel, dim3(plan.tiles - plan.whole, bm * bn / 2048), dim3(256), 0, s, a, bm, bn);
   return hipGetLastError();
 }
 
@@ -1193,14 +1227,12 @@ Layout Lay(void* ws, int planes, size_t M, size_t D, size_t F, bool backward) {
     l.dg = s.Take(M, F, planes);
     l.du = s.Take(M, F, planes);
   }
-  const int nseg = planes == 1 ? 1 : 6;
-  auto part = [&](Epilogue epi, std::initializer_list<Shape> q, size_t k, int segs) {
-    const bool dual = epi == kGate;
-    return PartBytes(Choose(FirstTile(epi, planes == 1), dual, q, k, segs), dual);
+  auto part = [&](bool dual, std::initializer_list<Shape> q, size_t k, int segs) {
+    return PartBytes(planes == 3, Choose(planes == 3, dual, q, k, segs), dual);
   };
-  l.part = s.Floats(backward ? std::max({part(kGrad, {{M, F}}, D, nseg), part(kPlain, {{M, D}}, F, 2 * nseg),
-                                         part(kPlain, {{D, F}, {D, F}, {F, D}}, M, nseg)})
-                             : std::max(part(kGate, {{M, F}}, D, nseg), part(kPlain, {{M, D}}, F, nseg)));
+  l.part = s.Floats(backward ? std::max({part(false, {{M, F}}, D, 1), part(false, {{M, D}}, F, 2),
+                                         part(false, {{D, F}, {D, F}, {F, D}}, M, 1)})
+                             : std::max(part(true, {{M, F}}, D, 1), part(false, {{M, D}}, F, 1)));
   l.bytes = s.used();
   return l;
 }
@@ -1234,29 +1266,16 @@ bool Octs(size_t N, std::initializer_list<const void*> ptrs) {
   return N % 8 == 0 && (at & 15) == 0;
 }
 
-// The plane products of A B (and A B2), smallest first, as segments.
-template <class T>
-Product& AddSegments(MmaArgs& a, Product& q, const Planes& A, const Planes& B, const Planes* B2 = nullptr) {
-  constexpr int pairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-  for (int i = sizeof(T) == 2 ? 5 : 0; i < 6; ++i) {
-    q.A[a.nseg] = A.p + pairs[i][0] * A.plane;
-    q.B[a.nseg] = B.p + pairs[i][1] * B.plane;
-    if (B2) q.B2[a.nseg] = B2->p + pairs[i][1] * B2->plane;
-    ++a.nseg;
-  }
-  return q;
-}
-
-// A launch's next product, its segments the plane products of A B (and A B2),
-// smallest first.
-template <class T>
+// A launch's next product, its first segment A B (and A B2).
 Product& AddProduct(MmaArgs& a, size_t M, size_t N, const Planes& A, const Planes& B,
                     const Planes* B2 = nullptr) {
   Product& q = a.q[a.count++];
   q.M = static_cast<int>(M), q.N = static_cast<int>(N);
   q.lda = A.ld, q.ldb = B.ld;
-  a.nseg = 0;
-  return AddSegments<T>(a, q, A, B, B2);
+  q.A[0] = A.p, q.B[0] = B.p, q.B2[0] = B2 ? B2->p : nullptr;
+  q.a_plane = A.plane, q.b_plane = B.plane;
+  a.nseg = 1;
+  return q;
 }
 
 MmaArgs Launch(size_t K) {
@@ -1335,12 +1354,12 @@ hipError_t Fwd(const FfnArgs& f, hipStream_t s) {
   Take<T>(f.wd, f.F, f.D, l.wd, pieces);
   FFN_TRY(Pack<T>(pieces, s));
   MmaArgs a = Launch(f.D);
-  Product& gate = AddProduct<T>(a, f.M, f.F, l.x, l.wg, &l.wu);
+  Product& gate = AddProduct(a, f.M, f.F, l.x, l.wg, &l.wu);
   gate.o1 = f.gate, gate.o2 = f.up, gate.vec = Octs<T>(f.F, {f.gate, f.up});
   a.act = f.act, a.h = l.h;
   FFN_TRY((Mma<T, kGate, false, true>(a, l.part, s)));
   a = Launch(f.F);
-  Product& down = AddProduct<T>(a, f.M, f.D, l.h, l.wd);
+  Product& down = AddProduct(a, f.M, f.D, l.h, l.wd);
   down.o1 = f.y, down.vec = Octs<T>(f.D, {f.y});
   return Mma<T, kPlain, false, true>(a, l.part, s);
 }
@@ -1366,12 +1385,12 @@ hipError_t Bwd(const FfnArgs& f, hipStream_t s) {
   Take<T>(f.dy, f.M, f.D, l.dy, pieces);
   FFN_TRY(Pack<T>(pieces, s));
   MmaArgs a = Launch(f.D);
-  AddProduct<T>(a, f.M, f.F, l.dy, l.wd).vec = Octs<T>(f.F, {f.gate, f.up});
+  AddProduct(a, f.M, f.F, l.dy, l.wd).vec = Octs<T>(f.F, {f.gate, f.up});
   a.act = f.act, a.g = f.gate, a.u = f.up, a.h = l.h, a.dg = l.dg, a.du = l.du;
   FFN_TRY((Mma<T, kGrad, false, false>(a, l.part, s)));
   a = Launch(f.F);
-  Product& dx = AddProduct<T>(a, f.M, f.D, l.dg, l.wg);
-  AddSegments<T>(a, dx, l.du, l.wu);
+  Product& dx = AddProduct(a, f.M, f.D, l.dg, l.wg);
+  dx.A[1] = l.du.p, dx.B[1] = l.wu.p, a.nseg = 2;
   dx.o1 = f.dx, dx.vec = Octs<T>(f.D, {f.dx});
   FFN_TRY((Mma<T, kPlain, false, false>(a, l.part, s)));
   a = Launch(f.M);
@@ -1380,7 +1399,7 @@ hipError_t Bwd(const FfnArgs& f, hipStream_t s) {
   void* out[3] = {f.dwg, f.dwu, f.dwd};
   for (int i = 0; i < 3; ++i) {
     const size_t M = i == 2 ? f.F : f.D, N = i == 2 ? f.D : f.F;
-    Product& q = AddProduct<T>(a, M, N, *left[i], *right[i]);
+    Product& q = AddProduct(a, M, N, *left[i], *right[i]);
     q.o1 = out[i], q.vec = Octs<T>(N, {out[i]});
   }
   return Mma<T, kPlain, true, true>(a, l.part, s);
