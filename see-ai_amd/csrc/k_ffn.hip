@@ -229,19 +229,6 @@ __device__ __forceinline__ void PutPlanes(const Planes& out, size_t at, float (&
   }
 }
 
-// One element into the planes.
-template <class T, bool kWhole = false>
-__device__ __forceinline__ void PutPlane(const Planes& out, size_t at, float v) {
-  if constexpr (kWhole) {
-    reinterpret_cast<float*>(out.p)[at] = v;
-  } else if constexpr (sizeof(T) == 2) {
-    out.p[at] = F32ToBf16(v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 3; ++k) out.p[k * out.plane + at] = static_cast<uint16_t>(TakePlane(v));
-  }
-}
-
 // rows x cols (packed) into padded planes: operands whose rows or base are off
 // 16 bytes, and every f32 operand; all of a call's in one launch.
 struct Piece {
@@ -444,17 +431,18 @@ struct Tile {
   static constexpr int kReads = kStrided ? 2 : 1;  // LDS reads of a fragment
 };
 
-// Eight neighbours of an output row from their sums: c of A B, d of A B2.
+// Eight neighbours of an output row from their sums: c of A B, d of A B2.  Off
+// 16 bytes (!q.vec) what is stored there is Finish1's, the planes' rows are not.
 template <class T, int kEpi, bool kWhole = false>
 __device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m, int n, float (&c)[8],
                                        float (&d)[8]) {
   const int cnt = q.N - n;
   const size_t o = static_cast<size_t>(m) * q.N + n;
-  if constexpr (kEpi == kPlain) Store8(static_cast<T*>(q.o1) + o, q.vec, cnt, c);
+  if constexpr (kEpi == kPlain) Store8(static_cast<T*>(q.o1) + o, true, cnt, c);
   if constexpr (kEpi == kGate) {
-    if (q.o1) {
-      Store8(static_cast<T*>(q.o1) + o, q.vec, cnt, c);
-      Store8(static_cast<T*>(q.o2) + o, q.vec, cnt, d);
+    if (q.o1 && q.vec) {
+      Store8(static_cast<T*>(q.o1) + o, true, cnt, c);
+      Store8(static_cast<T*>(q.o2) + o, true, cnt, d);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -483,33 +471,16 @@ __device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m
     PutPlanes<T, kWhole>(p.h, w, u);
   }
 }
-// The same of one element, for rows off 16 bytes (a lane a column: a lane of
+// The outputs of one element, for rows off 16 bytes (a lane a column: a lane of
 // eight would touch a line of its own with every access).
-template <class T, int kEpi, bool kWhole = false>
-__device__ __forceinline__ void Finish1(const MmaArgs& p, const Product& q, int m, int n, float c, float d) {
-  const bool in = n < q.N;
+template <class T, int kEpi>
+__device__ __forceinline__ void Finish1(const Product& q, int m, int n, float c, float d) {
   const size_t o = static_cast<size_t>(m) * q.N + n;
-  float a = 0.0f, da = 0.0f;
-  if constexpr (kEpi == kPlain) {
-    if (in) Put(static_cast<T*>(q.o1) + o, c);
-  }
+  if constexpr (kEpi == kPlain) Put(static_cast<T*>(q.o1) + o, c);
   if constexpr (kEpi == kGate) {
-    if (in && q.o1) {
-      Put(static_cast<T*>(q.o1) + o, c);
-      Put(static_cast<T*>(q.o2) + o, d);
-    }
-    Activate<sizeof(T) == 2>(p.act, c, a, da);
-    if (n < p.h.ld) PutPlane<T, kWhole>(p.h, static_cast<size_t>(m) * p.h.ld + n, in ? a * d : 0.0f);
-  }
-  if constexpr (kEpi == kGrad) {
-    if (n >= p.h.ld) return;
-    const float g = in ? One(static_cast<const T*>(p.g) + o) : 0.0f;
-    const float u = in ? One(static_cast<const T*>(p.u) + o) : 0.0f;
-    Activate<sizeof(T) == 2>(p.act, g, a, da);
-    const size_t w = static_cast<size_t>(m) * p.h.ld + n;
-    PutPlane<T, kWhole>(p.dg, w, in ? c * u * da : 0.0f);
-    PutPlane<T, kWhole>(p.du, w, in ? c * a : 0.0f);
-    PutPlane<T, kWhole>(p.h, w, in ? a * u : 0.0f);
+    if (!q.o1) return;
+    Put(static_cast<T*>(q.o1) + o, c);
+    Put(static_cast<T*>(q.o2) + o, d);
   }
 }
 
@@ -540,19 +511,19 @@ __global__ void __launch_bounds__(256) FfnJoin(MmaArgs p, int bm, int bn) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[b][e] += k0 + k < p.splits ? v[k][b][e] : 0.0f;
   }
-  if (q.vec) {
-    if (in) Finish<T, kEpi, kWhole>(p, q, m0 + r, n0 + col, s[0], s[1]);
-    return;
-  }
+  if (kEpi != kGrad && !q.vec) {
 #pragma unroll
-  for (int b = 0; b < kBoth; ++b) Store8(&st[b][threadIdx.x * 8], true, 8, s[b]);
-  __syncthreads();
+    for (int b = 0; b < kBoth; ++b) Store8(&st[b][threadIdx.x * 8], true, 8, s[b]);
+    __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int x = e * 256 + threadIdx.x, j = blockIdx.y * 2048 + x;
-    if (j < bm * bn && m0 + j / bn < q.M)
-      Finish1<T, kEpi, kWhole>(p, q, m0 + j / bn, n0 + j % bn, st[0][x], st[kBoth - 1][x]);
+    for (int e = 0; e < 8; ++e) {
+      const int x = e * 256 + threadIdx.x, j = blockIdx.y * 2048 + x;
+      if (j < bm * bn && m0 + j / bn < q.M && n0 + j % bn < q.N)
+        Finish1<T, kEpi>(q, m0 + j / bn, n0 + j % bn, st[0][x], st[kBoth - 1][x]);
+    }
+    if constexpr (kEpi == kPlain) return;
   }
+  if (in) Finish<T, kEpi, kWhole>(p, q, m0 + r, n0 + col, s[0], s[1]);
 }
 
 template <class T, int kEpi, bool kAS, bool kBS, int BM, int BN, int BK, int WGM, int WGN, int kStages>
@@ -759,13 +730,13 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
           }
       __builtin_amdgcn_wave_barrier();
       const int mb = m0 + wm + i * 32, nb = n0 + wn + jb * kW;
-      if (!q.vec && !shared) {
+      if (kEpi != kGrad && !q.vec && !shared) {
         const int n = nb + lane % kW;
         for (int r = lane / kW; r < 32; r += kWave / kW)
-          if (mb + r < q.M)
-            Finish1<T, kEpi>(p, q, mb + r, n, st[r * kPad + lane % kW],
-                             kDual ? st[(32 + r) * kPad + lane % kW] : 0.0f);
-      } else {
+          if (mb + r < q.M && n < q.N)
+            Finish1<T, kEpi>(q, mb + r, n, st[r * kPad + lane % kW], kDual ? st[(32 + r) * kPad + lane % kW] : 0.0f);
+      }
+      if (kEpi != kPlain || q.vec || shared) {
         const int n = nb + (lane % kPerRow) * 8;
 #pragma unroll
         for (int t = 0; t < 32 / kRows; ++t) {
@@ -808,6 +779,26 @@ __device__ __forceinline__ void Row4(const float* p, bool vec, int left, float (
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = !kGuard || e < left ? p[e] : 0.0f;
+  }
+}
+// An element's epilogue, H, dG and dU in f32.
+template <int kEpi>
+__device__ __forceinline__ void FinishWhole(const MmaArgs& p, const Product& q, int m, int n, float c, float d) {
+  const bool in = n < q.N;
+  if (kEpi != kGrad && in) Finish1<float, kEpi>(q, m, n, c, d);
+  if (kEpi == kPlain || n >= p.h.ld) return;
+  const size_t at = static_cast<size_t>(m) * p.h.ld + n, o = static_cast<size_t>(m) * q.N + n;
+  auto put = [&](const Planes& out, float v) { reinterpret_cast<float*>(out.p)[at] = in ? v : 0.0f; };
+  float a, da;
+  if constexpr (kEpi == kGate) {
+    Activate<false>(p.act, c, a, da);
+    put(p.h, a * d);
+  } else if constexpr (kEpi == kGrad) {
+    const float g = in ? static_cast<const float*>(p.g)[o] : 0.0f, u = in ? static_cast<const float*>(p.u)[o] : 0.0f;
+    Activate<false>(p.act, g, a, da);
+    put(p.dg, c * u * da);
+    put(p.du, c * a);
+    put(p.h, a * u);
   }
 }
 template <bool kGuard, bool kVec, int kC>
@@ -927,7 +918,7 @@ __global__ void __launch_bounds__(kRowsWaves * kWave) FfnRows32(MmaArgs p) {
 #pragma unroll
         for (int b = 0; b < kBoth; ++b) out[b * BN] = v[b][e];
       } else {
-        Finish1<float, kEpi, true>(p, q, m0 + m, n0 + n, v[0][e], v[kBoth - 1][e]);
+        FinishWhole<kEpi>(p, q, m0 + m, n0 + n, v[0][e], v[kBoth - 1][e]);
       }
     }
   });
