@@ -18,8 +18,11 @@ namespace seeai {
 // The widest row (D, F) of a feed-forward block: a tile's 256 rows stay inside
 // one buffer descriptor's 32-bit range.
 constexpr uint64_t kFfnMaxWidth = uint64_t{1} << 20;
-// Rows, columns and tokens: the kernels' row indices are 32-bit.
+// Rows and columns of a norm: the kernels' column indices are 32-bit.
 constexpr uint64_t kBlockMaxRows = (uint64_t{1} << 31) - 1;
+// Tokens: a row tile past the last stays a 32-bit index, and 64-row tiles of a
+// narrow block one launch.
+constexpr uint64_t kFfnMaxTokens = uint64_t{1} << 29;
 
 // An operand: its elements, their size, and whether the call writes it.
 struct Operand {
@@ -87,8 +90,8 @@ inline const char* CheckNormBwd(int kind, int dtype, const void* dy, const void*
 inline const char* CheckFfnShape(int dtype, int act, uint64_t M, uint64_t D, uint64_t F) {
   if (dtype < 0 || dtype > 1) return "dtype is 0 (f32) or 1 (bf16)";
   if (act < 0 || act > 3) return "act is 0 (none), 1 (relu), 2 (gelu) or 3 (silu)";
-  if (D == 0 || F == 0 || D > kFfnMaxWidth || F > kFfnMaxWidth || M > kBlockMaxRows)
-    return "bad shape (widths from 1 to 1048576)";
+  if (D == 0 || F == 0 || D > kFfnMaxWidth || F > kFfnMaxWidth || M > kFfnMaxTokens)
+    return "bad shape (widths from 1 to 1048576, tokens to 536870912)";
   return nullptr;
 }
 

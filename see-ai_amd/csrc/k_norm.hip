@@ -517,7 +517,8 @@ hipError_t Long(const NormCall& a, bool bwd, hipStream_t s) {
                        a.mean, a.rstd, static_cast<T*>(a.out), a.rows, a.cols);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  const size_t bands = a.rows / 64 < 1 ? 1 : a.rows / 64 < 64 ? a.rows / 64 : 64;
+  // (Past 2^24 the columns fill the chip by themselves.)
+  const size_t bands = a.rows < 128 || a.cols >> 24 ? 1 : a.rows / 64 < 64 ? a.rows / 64 : 64;
   hipLaunchKernelGGL((NormDwLongKernel<T>),
                      dim3(static_cast<unsigned>((a.cols + 255) / 256), static_cast<unsigned>(bands)),
                      dim3(256), 0, s, a.rms, dy, x, a.mean, a.rstd, a.o1, a.o2, a.part, a.rows,

@@ -283,26 +283,54 @@ class AdamWGroup:
     with ``n`` (default: p's elements) and ``decay`` (default 1).  The group
     keeps the tensors alive; the context outlives it."""
 
+    # A field's element size, by state bits or gradient type.
+    _SIZES = {"p": 4, "m": {32: 4, 8: 1}, "v": {32: 4, 8: 1}, "m_scale": 4, "v_scale": 4,
+              "p_bf16": 2, "g": {"f32": 4, "bf16": 2}}
+
     def __init__(self, ctx: Context, tensors, state_bits: int = 32, grads: str = "f32",
                  seed: int = 0):
+        self.h, self.ctx, self.tensors = None, ctx, list(tensors)
+        if state_bits not in (8, 32) or grads not in ("f32", "bf16"):
+            raise ValueError("state_bits is 8 or 32, grads 'f32' or 'bf16'")
         table = (AdamWTensor * max(len(tensors), 1))()
         for row, t in zip(table, tensors):
+            self._check(t, state_bits, grads)
             for name in ("p", "g", "m", "v", "m_scale", "v_scale", "p_bf16"):
                 setattr(row, name, ptr(t.get(name)))
             row.n = t["n"] if "n" in t else t["p"].numel()
             row.decay = t.get("decay", 1.0)
         h = _P()
-        self.h, self.ctx, self.tensors = None, ctx, list(tensors)
         ctx.call("seeai_adamw_group_create", table, len(tensors), state_bits,
                  {"f32": 0, "bf16": 1}[grads], seed, C.byref(h))
         self.h = h
 
+    def _check(self, t, state_bits, grads):
+        n = t["n"] if "n" in t else t["p"].numel()
+        for name, size in self._SIZES.items():
+            x = t.get(name)
+            if x is None:
+                continue  # the call itself refuses what is missing
+            if isinstance(size, dict):
+                size = size[grads if name == "g" else state_bits]
+            least = (n + 127) // 128 if name.endswith("_scale") else n
+            if name.endswith("_scale") and state_bits == 32:
+                continue
+            if (not x.is_cuda or x.element_size() != size or not x.is_contiguous()
+                    or x.numel() < least):
+                raise ValueError(f"{name}: {least} contiguous elements of {size} bytes on the "
+                                 "device wanted")
+
+    def _live(self):
+        if not self.h or not self.ctx.h:
+            raise BackendError(INVALID, "the AdamW group or its context is closed")
+        return self.h
+
     def step(self, params: StepParams | None = None):
         self.ctx.check(_lib.seeai_adamw_group_step(
-            self.h, C.byref(params) if params is not None else None))
+            self._live(), C.byref(params) if params is not None else None))
 
     def hold(self, params: StepParams):
-        self.ctx.check(_lib.seeai_adamw_group_hold(self.h, C.byref(params)))
+        self.ctx.check(_lib.seeai_adamw_group_hold(self._live(), C.byref(params)))
 
     def close(self):
         if self.h and self.ctx.h:

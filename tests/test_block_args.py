@@ -122,7 +122,8 @@ def test_ffn_refusals(checks):
     p[5] = 1 << 20
     assert b"both or neither" in fwd(p=p)
     assert b"act" in fwd(act=4) and b"dtype" in fwd(dt=-1)
-    for bad in (dict(D=0), dict(F=0), dict(D=(1 << 20) + 1), dict(F=1 << 21), dict(M=1 << 31)):
+    for bad in (dict(D=0), dict(F=0), dict(D=(1 << 20) + 1), dict(F=1 << 21), dict(M=1 << 31),
+                dict(M=(1 << 29) + 1)):
         assert b"shape" in fwd(**bad)
     assert b"workspace" in fwd(wsb=63)
     for i in (0, 1, 2, 3, 6, 7):
@@ -190,3 +191,61 @@ def test_workspace_sizes(hip):
             assert lib.seeai_ffn_workspace(dtype, 64, 96, 160, backward) >= 64 * 160 * size
     assert lib.seeai_ffn_workspace(1, 4, 0, 8, 0) == 0
     assert lib.seeai_ffn_workspace(2, 4, 8, 8, 0) == 0
+
+
+class Fake:
+    """What the group's own checks ask of a tensor."""
+
+    def __init__(self, n, size, contiguous=True, device=True):
+        self.n, self.size, self.contiguous, self.is_cuda = n, size, contiguous, device
+
+    def numel(self):
+        return self.n
+
+    def element_size(self):
+        return self.size
+
+    def is_contiguous(self):
+        return self.contiguous
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+class Recorder:
+    h = None
+
+    def call(self, name, *args):
+        raise LookupError(name)
+
+    check = call
+
+
+def test_group_wrapper_refuses_short_and_mistyped_tensors(hip):
+    def make(bits=8, grads="f32", **over):
+        t = {"p": Fake(300, 4), "g": Fake(300, 4), "m": Fake(300, 1), "v": Fake(300, 1),
+             "m_scale": Fake(3, 4), "v_scale": Fake(3, 4), "p_bf16": Fake(300, 2)} | over
+        return hip.AdamWGroup(Recorder(), [t], bits, grads)
+
+    with pytest.raises(LookupError):  # complete: the call is made
+        make()
+    with pytest.raises(LookupError):
+        make(g=Fake(300, 2), grads="bf16")
+    with pytest.raises(LookupError):
+        make(bits=32, m=Fake(300, 4), v=Fake(300, 4), m_scale=None, v_scale=None, p_bf16=None)
+    for over in (dict(n=301), dict(g=Fake(299, 4)), dict(g=Fake(300, 2)), dict(m=Fake(300, 4)),
+                 dict(v_scale=Fake(2, 4)), dict(p_bf16=Fake(300, 4)), dict(p=Fake(300, 4, False)),
+                 dict(v=Fake(300, 1, True, False))):
+        with pytest.raises(ValueError):
+            make(**over)
+    for over in (dict(bits=16), dict(grads="f16")):
+        with pytest.raises(ValueError):
+            make(**over)
+
+
+def test_a_closed_group_refuses(hip):
+    group = hip.AdamWGroup.__new__(hip.AdamWGroup)
+    group.h, group.ctx = None, Recorder()
+    for call in (group.step, lambda: group.hold(hip.StepParams())):
+        with pytest.raises(hip.BackendError, match="closed"):
+            call()
