@@ -8,13 +8,23 @@
 // rest: the forward's first launch holds a gate tile and the up tile of the
 // same columns side by side and stores act(G) U; the backward's first forms
 // dG, dU and H from its dH accumulators, so dH is never stored.  Two launches
-// forward (G and U; Y), three backward (dH; dX; the three weights' gradients).
+// forward (G and U; Y), three backward (dH; dX; the three weights' gradients),
+// besides the joins of shared-out K and the packing of operands.
 //
-// bf16: the operands as they are.  f32: each operand is split into three bf16
+// Many tokens are bound by the matrix unit's power: 8192 x 2048 x 5632 bf16 runs
+// 528 us forward and 1039 backward, 1,070 and 1,090 TFLOP/s (a library product
+// of these layouts 1,100 to 1,250), at 1.7 of 2.4 GHz; the down projection alone
+// 164 us, the gate's launch 365 for twice its work and 277 MB stored.  Few are
+// bound by the weights' bytes: one token of the same block 25 us for 69 MB.
+//
+// bf16: the operands as they are; what passes between launches (H, dG, dU) is
+// rounded to bf16 once, as the stored G and U are, because the next product's
+// operands are bf16: each costs 2^-9 of its value, what the inputs' own rounding
+// costs.  f32: each operand is split into three bf16
 // planes (x = hi + mid + lo, eight bits each, truncated, so exactly x), and a
 // product is the six plane products down to 2^-16 of it, all into the same f32
 // accumulators: f32's accuracy at a sixth of the bf16 rate, 1.6 times the f32
-// MFMA's.  An infinity's remainder is a NaN, so what an infinity reaches is
+// MFMA's (up to 128 tokens the f32 MFMA itself, below).  An infinity's remainder is a NaN, so what an infinity reaches is
 // not finite but may be a NaN where f32 arithmetic has an infinity.
 #include <algorithm>
 #include <cmath>
@@ -138,6 +148,21 @@ __device__ __forceinline__ void Activate(int act, float x, float& a, float& da) 
   }
 }
 
+// Eight of them, the activation chosen once.
+template <bool kFast>
+__device__ __forceinline__ void Activate8(int act, const float (&x)[8], float (&a)[8], float (&da)[8]) {
+  if (act == 3) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) Activate<kFast>(3, x[e], a[e], da[e]);
+  } else if (act == 2) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) Activate<kFast>(2, x[e], a[e], da[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) Activate<kFast>(act, x[e], a[e], da[e]);
+  }
+}
+
 // Up to eight neighbours of a row, 16 bytes at a time where they may be.
 __device__ __forceinline__ void Load8(const float* p, bool vec, int cnt, float (&v)[8]) {
   if (vec && cnt >= 8) {
@@ -188,6 +213,18 @@ __device__ __forceinline__ void Store8(uint16_t* p, bool vec, int cnt, const flo
       if (e < cnt) p[e] = F32ToBf16(v[e]);
   }
 }
+// Eight neighbours as they lie in memory, for loads that run ahead.
+template <class T>
+struct Raw8 {
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void Load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void Get(float (&v)[8]) const {
+    Load8(reinterpret_cast<const T*>(q), true, 8, v);
+  }
+};
 __device__ __forceinline__ float One(const float* p) { return *p; }
 __device__ __forceinline__ float One(const uint16_t* p) { return Bf16ToF32(*p); }
 __device__ __forceinline__ void Put(float* p, float v) { *p = v; }
@@ -301,17 +338,21 @@ struct Product {
   void *o1, *o2;  // plain: o1; gate: G and U or null
   int first;      // its first tile in the launch
 };
+// What an epilogue works on beside its sums.
+struct Side {
+  int act;
+  const void *g, *u;  // gradient: G and U
+  Planes h, dg, du;
+};
 // A launch's products share K, segments and kind.  Tiles [0, whole) are a
 // workgroup each; the rest share K out over `splits` workgroups, `per_split`
 // stages each, whose f32 sums [tile][split][rows][columns, of both operands]
 // FfnJoin adds and finishes.  (FfnRows32's tiles all share K out.)
-struct MmaArgs {
+struct MmaArgs : Side {
   Product q[3];
-  int count, nseg, K, act;
+  int count, nseg, K;
   int tiles, whole, splits, per_split;
   float* part;
-  const void *g, *u;  // gradient: G and U
-  Planes h, dg, du;
 };
 
 enum Epilogue {
@@ -431,10 +472,28 @@ struct Tile {
   static constexpr int kReads = kStrided ? 2 : 1;  // LDS reads of a fragment
 };
 
+// The gradient's eight from dH, G and U.
+template <class T, bool kWhole>
+__device__ __forceinline__ void FinishGrad(const Side& p, int m, int n, int cnt, const float (&c)[8],
+                                           const float (&g)[8], float (&u)[8]) {
+  float a[8], da[8];
+  Activate8<sizeof(T) == 2>(p.act, g, a, da);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool in = e < cnt;
+    da[e] = in ? c[e] * u[e] * da[e] : 0.0f;
+    u[e] = in ? a[e] * u[e] : 0.0f;
+    a[e] = in ? c[e] * a[e] : 0.0f;
+  }
+  const size_t w = static_cast<size_t>(m) * p.h.ld + n;
+  PutPlanes<T, kWhole>(p.dg, w, da);
+  PutPlanes<T, kWhole>(p.du, w, a);
+  PutPlanes<T, kWhole>(p.h, w, u);
+}
 // Eight neighbours of an output row from their sums: c of A B, d of A B2.  Off
 // 16 bytes (!q.vec) what is stored there is Finish1's, the planes' rows are not.
 template <class T, int kEpi, bool kWhole = false>
-__device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m, int n, float (&c)[8],
+__device__ __forceinline__ void Finish(const Side& p, const Product& q, int m, int n, float (&c)[8],
                                        float (&d)[8]) {
   const int cnt = q.N - n;
   const size_t o = static_cast<size_t>(m) * q.N + n;
@@ -444,31 +503,17 @@ __device__ __forceinline__ void Finish(const MmaArgs& p, const Product& q, int m
       Store8(static_cast<T*>(q.o1) + o, true, cnt, c);
       Store8(static_cast<T*>(q.o2) + o, true, cnt, d);
     }
+    float a[8], da[8];
+    Activate8<sizeof(T) == 2>(p.act, c, a, da);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float a, da;
-      Activate<sizeof(T) == 2>(p.act, c[e], a, da);
-      c[e] = e < cnt ? a * d[e] : 0.0f;
-    }
+    for (int e = 0; e < 8; ++e) c[e] = e < cnt ? a[e] * d[e] : 0.0f;
     PutPlanes<T, kWhole>(p.h, static_cast<size_t>(m) * p.h.ld + n, c);
   }
   if constexpr (kEpi == kGrad) {
-    float g[8], u[8], y[8];
+    float g[8], u[8];
     Load8(static_cast<const T*>(p.g) + o, q.vec, cnt, g);
     Load8(static_cast<const T*>(p.u) + o, q.vec, cnt, u);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float a, da;
-      Activate<sizeof(T) == 2>(p.act, g[e], a, da);
-      const bool in = e < cnt;
-      g[e] = in ? c[e] * u[e] * da : 0.0f;
-      y[e] = in ? c[e] * a : 0.0f;
-      u[e] = in ? a * u[e] : 0.0f;
-    }
-    const size_t w = static_cast<size_t>(m) * p.h.ld + n;
-    PutPlanes<T, kWhole>(p.dg, w, g);
-    PutPlanes<T, kWhole>(p.du, w, y);
-    PutPlanes<T, kWhole>(p.h, w, u);
+    FinishGrad<T, kWhole>(p, m, n, cnt, c, g, u);
   }
 }
 // The outputs of one element, for rows off 16 bytes (a lane a column: a lane of
@@ -558,6 +603,8 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
     first = split * p.per_split;
     stages = min(total - first, p.per_split);
   }
+  // (Copied: the arguments stay in their own memory only while few places use them.)
+  const Side side = p;
   int m0, n0;
   const Product& q = p.q[ProductOf(p, tile, BM, BNs, m0, n0)];
   TA ta;
@@ -710,13 +757,31 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   // The epilogue: kW columns of 32 rows at a time through this wave's slice of
   // LDS.  Accumulator element 4 q + e of block (i, j) is row lane % 32, column
   // 8 q + 4 (lane / 32) + e; a lane takes eight neighbours of a row away.
-  Barrier();  // every wave is done with the stages
   constexpr int kW = WN >= 64 ? 64 : 32, kPad = kW + 4, kBoth = kDual ? 2 : 1;
   static_assert(kWaves * kBoth * 32 * kPad * 4 <= kStages * kStage, "staging fits");
   constexpr int kPerRow = kW / 8, kRows = kWave / kPerRow;
   float* st = reinterpret_cast<float*>(smem) + wave * kBoth * 32 * kPad;
   const int h = lane / 32;
-  Each<TM * (WN / kW)>([&](auto part) __attribute__((always_inline)) {
+  // The gradient's G and U, a part ahead of their use: nothing else covers
+  // their latency (8192 x 2048 x 5632 bf16: 251 us, 316 with the loads where
+  // they are used; the product alone is 165).
+  constexpr int kT = 32 / kRows, kEpiParts = TM * (WN / kW);
+  Raw8<T> rg[2][kT], ru[2][kT];
+  const bool ahead = kEpi == kGrad && q.vec && !shared;
+  auto fetch = [&](auto part) __attribute__((always_inline)) {
+    constexpr int i = decltype(part)::value / (WN / kW), jb = decltype(part)::value % (WN / kW);
+    const int n = min(n0 + wn + jb * kW + (lane % kPerRow) * 8, q.N - 8);
+    Each<kT>([&](auto t) __attribute__((always_inline)) {
+      const size_t o = static_cast<size_t>(min(m0 + wm + i * 32 + lane / kPerRow + t * kRows, q.M - 1)) * q.N + n;
+      rg[decltype(part)::value % 2][t].Load(static_cast<const T*>(side.g) + o);
+      ru[decltype(part)::value % 2][t].Load(static_cast<const T*>(side.u) + o);
+    });
+  };
+  if constexpr (kEpi == kGrad) {
+    if (ahead) fetch(std::integral_constant<int, 0>{});
+  }
+  Barrier();  // every wave is done with the stages
+  Each<kEpiParts>([&](auto part) __attribute__((always_inline)) {
       constexpr int i = decltype(part)::value / (WN / kW), jb = decltype(part)::value % (WN / kW);
 #pragma unroll
       for (int b = 0; b < kBoth; ++b)
@@ -736,7 +801,22 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
           if (mb + r < q.M && n < q.N)
             Finish1<T, kEpi>(q, mb + r, n, st[r * kPad + lane % kW], kDual ? st[(32 + r) * kPad + lane % kW] : 0.0f);
       }
-      if (kEpi != kPlain || q.vec || shared) {
+      if (ahead) {
+        if constexpr (kEpi == kGrad) {
+          if constexpr (decltype(part)::value + 1 < kEpiParts)
+            fetch(std::integral_constant<int, decltype(part)::value + 1>{});
+          const int n = nb + (lane % kPerRow) * 8;
+          Each<kT>([&](auto t) __attribute__((always_inline)) {
+            const int r = lane / kPerRow + t * kRows, m = mb + r;
+            if (m >= q.M || n >= q.N) return;
+            float c[8], g[8], u[8];
+            Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
+            rg[decltype(part)::value % 2][t].Get(g);
+            ru[decltype(part)::value % 2][t].Get(u);
+            FinishGrad<T, false>(side, m, n, 8, c, g, u);
+          });
+        }
+      } else if (kEpi != kPlain || q.vec || shared) {
         const int n = nb + (lane % kPerRow) * 8;
 #pragma unroll
         for (int t = 0; t < 32 / kRows; ++t) {
@@ -751,7 +831,7 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
             Store8(out, true, 8, c);
             if constexpr (kDual) Store8(out + BNs, true, 8, d);
           } else {
-            Finish<T, kEpi>(p, q, m, n, c, d);
+            Finish<T, kEpi>(side, q, m, n, c, d);
           }
         }
       }
