@@ -19,13 +19,14 @@
 //
 // bf16: the operands as they are; what passes between launches (H, dG, dU) is
 // rounded to bf16 once, as the stored G and U are, because the next product's
-// operands are bf16: each costs 2^-9 of its value, what the inputs' own rounding
-// costs.  f32: each operand is split into three bf16
-// planes (x = hi + mid + lo, eight bits each, truncated, so exactly x), and a
-// product is the six plane products down to 2^-16 of it, all into the same f32
+// operands are bf16: at most 2^-8 of each value, as the inputs' own rounding.
+// f32: each operand is split into three bf16 planes (x = hi + mid + lo, eight
+// bits each, truncated, so exactly x), and a product is the six plane products
+// down to 2^-16 of it (what is left out is 2^-24 of it), all into the same f32
 // accumulators: f32's accuracy at a sixth of the bf16 rate, 1.6 times the f32
-// MFMA's (up to 128 tokens the f32 MFMA itself, below).  An infinity's remainder is a NaN, so what an infinity reaches is
-// not finite but may be a NaN where f32 arithmetic has an infinity.
+// MFMA's (up to 128 tokens the f32 MFMA itself, below).  An infinity's remainder
+// is a NaN, so what an infinity reaches is not finite but may be a NaN where f32
+// arithmetic has an infinity.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
