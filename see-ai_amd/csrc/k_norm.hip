@@ -12,6 +12,8 @@
 // held in registers (kE elements a lane) between its statistics and its
 // output, so it is read once; the variance is taken about the mean in a
 // second sweep of the registers.  Statistics and sums are f32 for both types.
+// 8192 x 2048 bf16 on MI355X: RMS forward 12.9 us (5.2 TB/s, a copy's rate),
+// layer backward 29.8, of which the fold below 4.3 (the copy rate would be 19).
 //
 // The weight's gradient runs down the columns while dx needs sums along the
 // rows: a workgroup walks rows strided over the grid, a lane keeps the same
