@@ -27,6 +27,10 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// Sixteen bytes on a float's or a bf16's own alignment: global memory takes them.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4), may_alias));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2), may_alias));
+
 template <class T> struct Io;
 template <> struct Io<float> {
   static constexpr int kV = 4;  // elements of a 16-byte access
@@ -36,6 +40,13 @@ template <> struct Io<float> {
   }
   static __device__ __forceinline__ void Store(float* p, const float* v) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+  static __device__ __forceinline__ void LoadAny(const float* p, float* v) {
+    const f32x4u a = *reinterpret_cast<const f32x4u*>(p);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  }
+  static __device__ __forceinline__ void StoreAny(float* p, const float* v) {
+    *reinterpret_cast<f32x4u*>(p) = f32x4u{v[0], v[1], v[2], v[3]};
   }
   static __device__ __forceinline__ float Get(const float* p) { return *p; }
   static __device__ __forceinline__ void Put(float* p, float v) { *p = v; }
@@ -51,11 +62,26 @@ template <> struct Io<uint16_t> {  // bf16
       v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
   }
-  static __device__ __forceinline__ void Store(uint16_t* p, const float* v) {
+  static __device__ __forceinline__ bf16x8 Pack(const float* v) {
     bf16x8 o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = static_cast<__bf16>(v[i]);
-    *reinterpret_cast<bf16x8*>(p) = o;
+    return o;
+  }
+  static __device__ __forceinline__ void Store(uint16_t* p, const float* v) {
+    *reinterpret_cast<bf16x8*>(p) = Pack(v);
+  }
+  static __device__ __forceinline__ void LoadAny(const uint16_t* p, float* v) {
+    const u32x4u a = *reinterpret_cast<const u32x4u*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ void StoreAny(uint16_t* p, const float* v) {
+    *reinterpret_cast<u32x4u*>(p) = __builtin_bit_cast(u32x4u, Pack(v));
   }
   static __device__ __forceinline__ float Get(const uint16_t* p) { return Bf16ToF32(*p); }
   static __device__ __forceinline__ void Put(uint16_t* p, float v) { *p = F32ToBf16(v); }
@@ -63,16 +89,29 @@ template <> struct Io<uint16_t> {  // bf16
 
 // Where lane t's element e of a row lies, and whether it lies in the row.
 // kVec: groups of kV neighbours, kTPR groups apart (16-byte accesses, rows a
-// multiple of kV long); else single elements kTPR apart.
+// multiple of kV long); else single elements kTPR apart.  kAny, with kVec: the
+// same groups where rows are of any length and begin anywhere, the row's last,
+// short group element by element.
 template <class T, int kTPR, bool kVec>
 __device__ __forceinline__ int ColOf(int t, int e) {
   constexpr int kV = Io<T>::kV;
   return kVec ? ((e / kV) * kTPR + t) * kV + e % kV : e * kTPR + t;
 }
-template <class T, int kTPR, int kE, bool kVec>
+template <class T, int kTPR, int kE, bool kVec, bool kAny>
 __device__ __forceinline__ void LoadRow(const T* row, int t, int cols, float (&v)[kE]) {
   constexpr int kV = Io<T>::kV;
-  if constexpr (kVec) {
+  if constexpr (kAny) {
+#pragma unroll
+    for (int e = 0; e < kE; e += kV) {
+      const int c = ColOf<T, kTPR, true>(t, e);
+      if (c + kV <= cols) {
+        Io<T>::LoadAny(row + c, v + e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) v[e + i] = c + i < cols ? Io<T>::Get(row + c + i) : 0.0f;
+      }
+    }
+  } else if constexpr (kVec) {
 #pragma unroll
     for (int e = 0; e < kE; e += kV) {
       const int c = ColOf<T, kTPR, true>(t, e);
@@ -91,10 +130,22 @@ __device__ __forceinline__ void LoadRow(const T* row, int t, int cols, float (&v
     }
   }
 }
-template <class T, int kTPR, int kE, bool kVec>
+template <class T, int kTPR, int kE, bool kVec, bool kAny = false>
 __device__ __forceinline__ void StoreRow(T* row, int t, int cols, const float (&v)[kE]) {
   constexpr int kV = Io<T>::kV;
-  if constexpr (kVec) {
+  if constexpr (kAny) {
+#pragma unroll
+    for (int e = 0; e < kE; e += kV) {
+      const int c = ColOf<T, kTPR, true>(t, e);
+      if (c + kV <= cols) {
+        Io<T>::StoreAny(row + c, v + e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+          if (c + i < cols) Io<T>::Put(row + c + i, v[e + i]);
+      }
+    }
+  } else if constexpr (kVec) {
 #pragma unroll
     for (int e = 0; e < kE; e += kV) {
       const int c = ColOf<T, kTPR, true>(t, e);
@@ -109,9 +160,20 @@ __device__ __forceinline__ void StoreRow(T* row, int t, int cols, const float (&
   }
 }
 // The f32 vector at the same columns.
-template <class T, int kTPR, int kE, bool kVec>
+template <class T, int kTPR, int kE, bool kVec, bool kAny = false>
 __device__ __forceinline__ void LoadVec(const float* w, int t, int cols, float (&v)[kE]) {
-  if constexpr (kVec) {
+  if constexpr (kAny) {
+#pragma unroll
+    for (int e = 0; e < kE; e += 4) {
+      const int c = ColOf<T, kTPR, true>(t, e);
+      if (c + 4 <= cols) {
+        Io<float>::LoadAny(w + c, v + e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[e + i] = c + i < cols ? w[c + i] : 0.0f;
+      }
+    }
+  } else if constexpr (kVec) {
 #pragma unroll
     for (int e = 0; e < kE; e += 4) {
       const int c = ColOf<T, kTPR, true>(t, e);
@@ -159,7 +221,7 @@ constexpr int Threads(int tpr) { return tpr > 256 ? tpr : 256; }
 constexpr int kBwdPerSimd = 4;
 constexpr int BwdThreads(int tpr) { return tpr > 512 ? tpr : 512; }
 
-template <class T, int kTPR, int kE, bool kVec>
+template <class T, int kTPR, int kE, bool kVec, bool kAny>
 __global__ void __launch_bounds__(Threads(kTPR))
 NormFwdKernel(int rms, const T* __restrict__ x, const float* __restrict__ w,
               const float* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
@@ -173,7 +235,7 @@ NormFwdKernel(int rms, const T* __restrict__ x, const float* __restrict__ w,
     const size_t r = base + threadIdx.x / kTPR;
     const bool in = r < rows;
     float v[kE];
-    LoadRow<T, kTPR, kE, kVec>(x + r * cols, t, in ? cols : 0, v);
+    LoadRow<T, kTPR, kE, kVec, kAny>(x + r * cols, t, in ? cols : 0, v);
     float mu[1] = {0.0f};
     if (!rms) {
 #pragma unroll
@@ -190,16 +252,16 @@ NormFwdKernel(int rms, const T* __restrict__ x, const float* __restrict__ w,
     RowSum<kTPR>(sq, lds);
     const float rs = 1.0f / sqrtf(sq[0] / static_cast<float>(cols) + eps);
     float ww[kE];
-    LoadVec<T, kTPR, kE, kVec>(w, t, cols, ww);
+    LoadVec<T, kTPR, kE, kVec, kAny>(w, t, cols, ww);
 #pragma unroll
     for (int e = 0; e < kE; ++e) v[e] = v[e] * rs * ww[e];
     if (b) {
-      LoadVec<T, kTPR, kE, kVec>(b, t, cols, ww);
+      LoadVec<T, kTPR, kE, kVec, kAny>(b, t, cols, ww);
 #pragma unroll
       for (int e = 0; e < kE; ++e) v[e] += ww[e];
     }
     if (!in) continue;
-    StoreRow<T, kTPR, kE, kVec>(y + r * cols, t, cols, v);
+    StoreRow<T, kTPR, kE, kVec, kAny>(y + r * cols, t, cols, v);
     if (t == 0) {
       if (mean) mean[r] = mu[0];
       if (rstd) rstd[r] = rs;
@@ -468,13 +530,13 @@ struct NormCall {
   float eps;
 };
 
-template <class T, int kTPR, int kE, bool kVec>
+template <class T, int kTPR, int kE, bool kVec, bool kAny>
 hipError_t Run(const NormCall& a, bool bwd, hipStream_t s) {
   const int cols = static_cast<int>(a.cols);
-  if (!bwd) {
+  if (kAny || !bwd) {  // (kAny: Dispatch asks for the forward alone)
     constexpr int kRows = Threads(kTPR) / kTPR;
     const size_t groups = (a.rows + kRows - 1) / kRows;
-    hipLaunchKernelGGL((NormFwdKernel<T, kTPR, kE, kVec>), Grid(groups), dim3(Threads(kTPR)), 0, s, a.rms,
+    hipLaunchKernelGGL((NormFwdKernel<T, kTPR, kE, kVec, kAny>), Grid(groups), dim3(Threads(kTPR)), 0, s, a.rms,
                        static_cast<const T*>(a.x), a.w, a.b,
                        static_cast<T*>(a.out), a.o1, a.o2, a.rows, cols, a.eps);
     return hipGetLastError();
@@ -493,17 +555,17 @@ hipError_t Run(const NormCall& a, bool bwd, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <class T, bool kVec>
+template <class T, bool kVec, bool kAny>
 hipError_t Pick(const NormCall& a, bool bwd, hipStream_t s) {
   // Eight elements a lane: four waves a SIMD.  With sixteen the backward's sums
   // and the row in flight leave it two (8192 x 2048 bf16: 30 us either way;
   // 3001 x 1023 f32, single elements: 17 us against 16).
-  if (a.cols <= 512) return Run<T, 64, 8, kVec>(a, bwd, s);
-  if (a.cols <= 1024) return Run<T, 128, 8, kVec>(a, bwd, s);
-  if (a.cols <= 2048) return Run<T, 256, 8, kVec>(a, bwd, s);
-  if (a.cols <= 4096) return Run<T, 512, 8, kVec>(a, bwd, s);
-  if (a.cols <= 8192) return Run<T, 1024, 8, kVec>(a, bwd, s);
-  return Run<T, 1024, 16, kVec>(a, bwd, s);
+  if (a.cols <= 512) return Run<T, 64, 8, kVec, kAny>(a, bwd, s);
+  if (a.cols <= 1024) return Run<T, 128, 8, kVec, kAny>(a, bwd, s);
+  if (a.cols <= 2048) return Run<T, 256, 8, kVec, kAny>(a, bwd, s);
+  if (a.cols <= 4096) return Run<T, 512, 8, kVec, kAny>(a, bwd, s);
+  if (a.cols <= 8192) return Run<T, 1024, 8, kVec, kAny>(a, bwd, s);
+  return Run<T, 1024, 16, kVec, kAny>(a, bwd, s);
 }
 
 template <class T>
@@ -540,8 +602,15 @@ hipError_t Dispatch(const NormCall& a, bool bwd, hipStream_t s) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.x) |
                        reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.b) |
                        reinterpret_cast<uintptr_t>(a.out);
-  if (a.cols % Io<T>::kV == 0 && (at & 15) == 0) return Pick<T, true>(a, bwd, s);
-  return Pick<T, false>(a, bwd, s);
+  if (a.cols % Io<T>::kV == 0 && (at & 15) == 0) return Pick<T, true, false>(a, bwd, s);
+  // Off that, the forward of wide rows still takes 16 bytes at a time, against
+  // single elements, us (layer): bf16 30000 x 500 19.8 and 23.6, 4000 x 4095 26
+  // and 42, but 30000 x 77 17.7 and 12.8 (most lanes have the short group); f32
+  // 4000 x 4095 25 and 29, but 16384 x 1001 23.7 and 22.8.  The backward loses at
+  // every width (bf16 4000 x 4095 52 and 32): its rows in flight would wait for
+  // the short group's branch.
+  if (!bwd && a.cols > (sizeof(T) == 2 ? 256 : 2048)) return Pick<T, true, true>(a, bwd, s);
+  return Pick<T, false, false>(a, bwd, s);
 }
 
 }  // namespace
