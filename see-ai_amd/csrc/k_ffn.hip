@@ -783,60 +783,60 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   }
   Barrier();  // every wave is done with the stages
   Each<kEpiParts>([&](auto part) __attribute__((always_inline)) {
-      constexpr int i = decltype(part)::value / (WN / kW), jb = decltype(part)::value % (WN / kW);
+    constexpr int i = decltype(part)::value / (WN / kW), jb = decltype(part)::value % (WN / kW);
 #pragma unroll
-      for (int b = 0; b < kBoth; ++b)
+    for (int b = 0; b < kBoth; ++b)
 #pragma unroll
-        for (int jj = 0; jj < kW / 32; ++jj)
+      for (int jj = 0; jj < kW / 32; ++jj)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const v16f& c = acc[i][b * TN + jb * (kW / 32) + jj];
-            *reinterpret_cast<float4*>(st + (b * 32 + lane % 32) * kPad + jj * 32 + 8 * q + 4 * h) =
-                make_float4(c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]);
-          }
-      __builtin_amdgcn_wave_barrier();
-      const int mb = m0 + wm + i * 32, nb = n0 + wn + jb * kW;
-      if (kEpi != kGrad && !q.vec && !shared) {
-        const int n = nb + lane % kW;
-        for (int r = lane / kW; r < 32; r += kWave / kW)
-          if (mb + r < q.M && n < q.N)
-            Finish1<T, kEpi>(q, mb + r, n, st[r * kPad + lane % kW], kDual ? st[(32 + r) * kPad + lane % kW] : 0.0f);
-      }
-      if (ahead) {
-        if constexpr (kEpi == kGrad) {
-          if constexpr (decltype(part)::value + 1 < kEpiParts)
-            fetch(std::integral_constant<int, decltype(part)::value + 1>{});
-          const int n = nb + (lane % kPerRow) * 8;
-          Each<kT>([&](auto t) __attribute__((always_inline)) {
-            const int r = lane / kPerRow + t * kRows, m = mb + r;
-            if (m >= q.M || n >= q.N) return;
-            float c[8], g[8], u[8];
-            Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
-            rg[decltype(part)::value % 2][t].Get(g);
-            ru[decltype(part)::value % 2][t].Get(u);
-            FinishGrad<T, false>(side, m, n, 8, c, g, u);
-          });
+        for (int q = 0; q < 4; ++q) {
+          const v16f& c = acc[i][b * TN + jb * (kW / 32) + jj];
+          *reinterpret_cast<float4*>(st + (b * 32 + lane % 32) * kPad + jj * 32 + 8 * q + 4 * h) =
+              make_float4(c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]);
         }
-      } else if (kEpi != kPlain || q.vec || shared) {
+    __builtin_amdgcn_wave_barrier();
+    const int mb = m0 + wm + i * 32, nb = n0 + wn + jb * kW;
+    if (kEpi != kGrad && !q.vec && !shared) {
+      const int n = nb + lane % kW;
+      for (int r = lane / kW; r < 32; r += kWave / kW)
+        if (mb + r < q.M && n < q.N)
+          Finish1<T, kEpi>(q, mb + r, n, st[r * kPad + lane % kW], kDual ? st[(32 + r) * kPad + lane % kW] : 0.0f);
+    }
+    if (ahead) {
+      if constexpr (kEpi == kGrad) {
+        if constexpr (decltype(part)::value + 1 < kEpiParts)
+          fetch(std::integral_constant<int, decltype(part)::value + 1>{});
         const int n = nb + (lane % kPerRow) * 8;
-#pragma unroll
-        for (int t = 0; t < 32 / kRows; ++t) {
+        Each<kT>([&](auto t) __attribute__((always_inline)) {
           const int r = lane / kPerRow + t * kRows, m = mb + r;
-          if (m >= q.M || n >= q.N) continue;
-          float c[8], d[8];
+          if (m >= q.M || n >= q.N) return;
+          float c[8], g[8], u[8];
           Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
-          if constexpr (kDual) Load8(st + (32 + r) * kPad + (lane % kPerRow) * 8, true, 8, d);
-          if (shared) {
-            float* out = p.part + ((static_cast<size_t>(tile - p.whole) * p.splits + split) * BM + (m - m0)) *
-                                      (kBoth * BNs) + (n - n0);
-            Store8(out, true, 8, c);
-            if constexpr (kDual) Store8(out + BNs, true, 8, d);
-          } else {
-            Finish<T, kEpi>(side, q, m, n, c, d);
-          }
+          rg[decltype(part)::value % 2][t].Get(g);
+          ru[decltype(part)::value % 2][t].Get(u);
+          FinishGrad<T, false>(side, m, n, 8, c, g, u);
+        });
+      }
+    } else if (kEpi != kPlain || q.vec || shared) {
+      const int n = nb + (lane % kPerRow) * 8;
+#pragma unroll
+      for (int t = 0; t < 32 / kRows; ++t) {
+        const int r = lane / kPerRow + t * kRows, m = mb + r;
+        if (m >= q.M || n >= q.N) continue;
+        float c[8], d[8];
+        Load8(st + r * kPad + (lane % kPerRow) * 8, true, 8, c);
+        if constexpr (kDual) Load8(st + (32 + r) * kPad + (lane % kPerRow) * 8, true, 8, d);
+        if (shared) {
+          float* out = p.part + ((static_cast<size_t>(tile - p.whole) * p.splits + split) * BM + (m - m0)) *
+                                    (kBoth * BNs) + (n - n0);
+          Store8(out, true, 8, c);
+          if constexpr (kDual) Store8(out + BNs, true, 8, d);
+        } else {
+          Finish<T, kEpi>(side, q, m, n, c, d);
         }
       }
-      __builtin_amdgcn_wave_barrier();
+    }
+    __builtin_amdgcn_wave_barrier();
   });
 }
 

@@ -67,7 +67,8 @@ def within(torch, got, want, bound):
 
 NORM_SHAPES = [(1, 1), (3, 7), (1, 768), (5, 64), (70, 512), (9, 513), (130, 1000), (33, 1023),
                (2100, 1024), (64, 1030), (40, 2048), (7, 2050), (600, 4096), (5, 5001), (3, 8192),
-               (4, 8193), (3, 16384), (2, 16385), (130, 20000), (6, 2051), (4, 6143), (3, 257), (2, 12289)]
+               (4, 8193), (3, 16384), (2, 16385), (130, 20000), (6, 2051), (4, 6143), (3, 257),
+               (2, 12289)]
 DEPTH = 260  # f32 additions behind one sum over a row's or a column's partials
 
 
