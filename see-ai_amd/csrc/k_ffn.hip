@@ -753,7 +753,10 @@ __global__ void __launch_bounds__(WGM * WGN * kWave) FfnMma(MmaArgs p) {
   }
   steps(last % kStages, 0, std::false_type{});
   mfmas((kSub - 1) % 2);
-  WaitVm<0>();  // the repeated loads have landed
+  // The repeated loads have landed and this wave's fragments are in registers:
+  // past the next barrier other waves write over the stages.
+  WaitVm<0>();
+  WaitLds();
 
   // The epilogue: kW columns of 32 rows at a time through this wave's slice of
   // LDS.  Accumulator element 4 q + e of block (i, j) is row lane % 32, column
