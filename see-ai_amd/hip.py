@@ -289,18 +289,20 @@ class AdamWGroup:
 
     def __init__(self, ctx: Context, tensors, state_bits: int = 32, grads: str = "f32",
                  seed: int = 0):
-        self.h, self.ctx, self.tensors = None, ctx, list(tensors)
+        # Dicts of its own: the device's table holds the tensors' addresses,
+        # whatever becomes of the caller's.
+        self.h, self.ctx, self.tensors = None, ctx, [dict(t) for t in tensors]
         if state_bits not in (8, 32) or grads not in ("f32", "bf16"):
             raise ValueError("state_bits is 8 or 32, grads 'f32' or 'bf16'")
-        table = (AdamWTensor * max(len(tensors), 1))()
-        for row, t in zip(table, tensors):
+        table = (AdamWTensor * max(len(self.tensors), 1))()
+        for row, t in zip(table, self.tensors):
             self._check(t, state_bits, grads)
             for name in ("p", "g", "m", "v", "m_scale", "v_scale", "p_bf16"):
                 setattr(row, name, ptr(t.get(name)))
             row.n = t["n"] if "n" in t else t["p"].numel()
             row.decay = t.get("decay", 1.0)
         h = _P()
-        ctx.call("seeai_adamw_group_create", table, len(tensors), state_bits,
+        ctx.call("seeai_adamw_group_create", table, len(self.tensors), state_bits,
                  {"f32": 0, "bf16": 1}[grads], seed, C.byref(h))
         self.h = h
 

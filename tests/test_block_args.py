@@ -249,3 +249,24 @@ def test_a_closed_group_refuses(hip):
     for call in (group.step, lambda: group.hold(hip.StepParams())):
         with pytest.raises(hip.BackendError, match="closed"):
             call()
+
+
+class Accepting(Recorder):
+    """A context whose calls succeed."""
+
+    def call(self, name, *args):
+        return None
+
+
+def test_a_group_keeps_the_tensors_it_was_made_of(hip):
+    """The device's table holds addresses: what the caller does to its dicts afterwards must not
+    free the memory behind them."""
+    t = {"p": Fake(300, 4), "g": Fake(300, 4), "m": Fake(300, 4), "v": Fake(300, 4), "decay": 0.5}
+    given = [t]
+    group = hip.AdamWGroup(Accepting(), given, 32, "f32")
+    p, g, m = t["p"], t["g"], t["m"]
+    t["g"] = Fake(300, 4)
+    del t["m"]
+    given.clear()
+    held = list(group.tensors[0].values())
+    assert all(any(x is y for y in held) for x in (p, g, m, t["v"]))
