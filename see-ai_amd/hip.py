@@ -278,14 +278,18 @@ class Context:
 class AdamWGroup:
     """A group of tensors stepped together (seeai_adamw_group_*).
 
-    ``tensors``: dicts of device tensors -- ``p`` (f32), ``g``, ``m``, ``v``,
-    with 8-bit states ``m_scale`` and ``v_scale``, optionally ``p_bf16`` --
-    with ``n`` (default: p's elements) and ``decay`` (default 1).  The group
-    keeps the tensors alive; the context outlives it."""
+    ``tensors``: dicts of device tensors -- ``p`` (f32), ``g`` (of ``grads``),
+    ``m``, ``v`` (f32, or uint8 / float8_e4m3fn codes), with 8-bit states
+    ``m_scale`` and ``v_scale`` (f32), optionally ``p_bf16`` -- with ``n``
+    (default: p's elements) and ``decay`` (default 1).  bf16 is bfloat16 or its
+    bits in 16-bit integers.  The group keeps the tensors alive; the context
+    outlives it."""
 
-    # A field's element size, by state bits or gradient type.
-    _SIZES = {"p": 4, "m": {32: 4, 8: 1}, "v": {32: 4, 8: 1}, "m_scale": 4, "v_scale": 4,
-              "p_bf16": 2, "g": {"f32": 4, "bf16": 2}}
+    # A field's element size and types, by state bits or gradient type.
+    _F32, _BF16 = (4, ("float32",)), (2, ("bfloat16", "int16", "uint16"))
+    _STATE = {32: _F32, 8: (1, ("uint8", "float8_e4m3fn"))}
+    _FIELDS = {"p": _F32, "m": _STATE, "v": _STATE, "m_scale": _F32, "v_scale": _F32,
+               "p_bf16": _BF16, "g": {"f32": _F32, "bf16": _BF16}}
 
     def __init__(self, ctx: Context, tensors, state_bits: int = 32, grads: str = "f32",
                  seed: int = 0):
@@ -308,12 +312,11 @@ class AdamWGroup:
 
     def _check(self, t, state_bits, grads):
         n = t["n"] if "n" in t else t["p"].numel()
-        for name, size in self._SIZES.items():
+        for name, kind in self._FIELDS.items():
             x = t.get(name)
             if x is None:
                 continue  # the call itself refuses what is missing
-            if isinstance(size, dict):
-                size = size[grads if name == "g" else state_bits]
+            size, types = kind[grads if name == "g" else state_bits] if isinstance(kind, dict) else kind
             least = (n + 127) // 128 if name.endswith("_scale") else n
             if name.endswith("_scale") and state_bits == 32:
                 continue
@@ -321,6 +324,9 @@ class AdamWGroup:
                     or x.numel() < least):
                 raise ValueError(f"{name}: {least} contiguous elements of {size} bytes on the "
                                  "device wanted")
+            dtype = str(getattr(x, "dtype", types[0])).removeprefix("torch.")
+            if dtype not in types:
+                raise ValueError(f"{name}: {' or '.join(types)} wanted, not {dtype}")
 
     def _live(self):
         if not self.h or not self.ctx.h:

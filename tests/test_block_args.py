@@ -270,3 +270,30 @@ def test_a_group_keeps_the_tensors_it_was_made_of(hip):
     given.clear()
     held = list(group.tensors[0].values())
     assert all(any(x is y for y in held) for x in (p, g, m, t["v"]))
+
+
+class Typed(Fake):
+    """A tensor that says its type, as a device tensor does."""
+
+    def __init__(self, n, dtype):
+        super().__init__(n, {"32": 4, "16": 2, "t8": 1, "fn": 1}[dtype[-2:]])
+        self.dtype = "torch." + dtype
+
+
+def test_group_wrapper_refuses_wrong_types_of_the_right_size(hip):
+    def make(bits=8, grads="f32", **over):
+        code = "uint8" if bits == 8 else "float32"
+        types = {"p": "float32", "g": "float32" if grads == "f32" else "bfloat16", "m": code, "v": code,
+                 "m_scale": "float32", "v_scale": "float32", "p_bf16": "bfloat16"} | over
+        return hip.AdamWGroup(Accepting(), [{k: Typed(300, t) for k, t in types.items()}], bits, grads)
+
+    for bits in (8, 32):
+        for grads in ("f32", "bf16"):
+            make(bits, grads)
+    make(m="float8_e4m3fn", v="float8_e4m3fn")  # what the codes are
+    make(g="int16", p_bf16="uint16", grads="bf16")  # bf16 bits
+    for over in (dict(p="int32"), dict(g="int32"), dict(g="float16", grads="bf16"), dict(m="int8"),
+                 dict(v="int8"), dict(m_scale="int32"), dict(v_scale="int32"), dict(p_bf16="float16"),
+                 dict(m="int32", bits=32), dict(v="int32", bits=32)):
+        with pytest.raises(ValueError, match=next(k for k in over if k not in ("grads", "bits"))):
+            make(**over)
