@@ -327,6 +327,9 @@ class AdamWGroup:
             dtype = str(getattr(x, "dtype", types[0])).removeprefix("torch.")
             if dtype not in types:
                 raise ValueError(f"{name}: {' or '.join(types)} wanted, not {dtype}")
+            here = getattr(self.ctx, "device_index", None)
+            if here is not None and getattr(getattr(x, "device", None), "index", here) != here:
+                raise ValueError(f"{name}: on device {x.device.index}, the context on device {here}")
 
     def _live(self):
         if not self.h or not self.ctx.h:

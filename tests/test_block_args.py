@@ -297,3 +297,23 @@ def test_group_wrapper_refuses_wrong_types_of_the_right_size(hip):
                  dict(m="int32", bits=32), dict(v="int32", bits=32)):
         with pytest.raises(ValueError, match=next(k for k in over if k not in ("grads", "bits"))):
             make(**over)
+
+
+def test_group_wrapper_refuses_tensors_of_another_device(hip):
+    """A step runs on its context's device; another device's memory may be out of its reach."""
+    class At:
+        def __init__(self, index):
+            self.index = index
+
+    def make(**over):
+        t = {k: Typed(300, "float32") for k in ("p", "g", "m", "v")}
+        for k, x in t.items():
+            x.device = At(over.get(k, 1))
+        ctx = Accepting()
+        ctx.device_index = 1
+        return hip.AdamWGroup(ctx, [t], 32, "f32")
+
+    make()
+    for name in ("p", "g", "m", "v"):
+        with pytest.raises(ValueError, match=f"{name}: .*device 1"):
+            make(**{name: 0})
