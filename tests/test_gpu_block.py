@@ -145,6 +145,28 @@ def test_norm(ctx, torch_cuda, kind, bf16, off):
         assert torch.equal(again.t, dw.t), "the weight's gradient differs run to run"
 
 
+@pytest.mark.parametrize("rows,cols,off", [(8192, 1024, 0), (8199, 1023, 1), (16411, 520, 0),
+                                           (8203, 2048, 0)])
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_norm_backward_over_two_workgroups_a_cu(ctx, torch_cuda, bf16, rows, cols, off):
+    """Rows enough for 512 workgroups' partial sums, the last of them without a full share."""
+    torch = torch_cuda
+    t, step = types(torch, bf16)
+    rnd = gen(torch, rows + cols)
+    x = put(torch, rnd(rows, cols) * 2 + rnd(rows, 1) * 3, t, off)
+    w, dy = put(torch, 1 + 0.3 * rnd(cols), torch.float32, off), put(torch, rnd(rows, cols), t, off)
+    mean = x.double().mean(1).float()
+    rstd = (x.double().var(1, unbiased=False) + EPS).rsqrt().float()
+    dx = Guarded(torch, (rows, cols), t, off)
+    dw, db = (Guarded(torch, (cols,), torch.float32) for _ in range(2))
+    ws = norm_bwd(ctx, 0, bf16, dy, x, w, mean, rstd, dx.t, dw.t, db.t)
+    r = norm_backward_reference(torch, 0, x, w, dy, mean, rstd)
+    within(torch, dx.t, r[0], r[1] + step * r[0].abs())
+    within(torch, dw.t, r[2], r[3])
+    within(torch, db.t, r[4], r[5])
+    assert all(g.intact() for g in (dx, dw, db, ws))
+
+
 def call_norm_fwd(ctx, kind, bf16, x, w, b, y, mean, rstd, eps=EPS):
     p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     ctx.call("seeai_norm_fwd", kind, bf16, p(x), p(w), p(b), p(y), p(mean), p(rstd), *x.shape, eps)
@@ -334,6 +356,34 @@ def test_ffn_sizes_a_rule_turns_at(hip, ctx, torch_cuda, bf16, M, D, F):
     dy = put(torch, gen(torch, 5)(M, D), t, 0)
     grads = ffn_bwd(hip, ctx, torch, bf16, 3, *ins, gate, up, dy)
     check_ffn_bwd(torch, 3, step, *ins, gate, up, dy, *grads)
+
+
+# Sizes that between them take every tile the block's products can run on, with several stages of K,
+# rows on and off 16 bytes, K whole, shared out, and shared out for the tiles past whole rounds alone
+# (tests/test_ffn_plan.py holds the list to that).
+TILE_SHAPES = [(300, 260, 515), (512, 1024, 4096), (700, 1000, 1500), (1001, 776, 2056),
+               (1001, 777, 2050), (1500, 1033, 4107), (3000, 1000, 3000), (1024, 2048, 5632),
+               (4096, 2048, 1408), (4097, 1030, 2055), (4000, 2050, 4100), (8190, 2050, 5630),
+               (8192, 2048, 5632)]
+
+
+@pytest.mark.parametrize("bf16", [1, 0])
+@pytest.mark.parametrize("M,D,F", TILE_SHAPES)
+def test_ffn_on_every_tile(hip, ctx, torch_cuda, M, D, F, bf16):
+    torch = torch_cuda
+    t, step = types(torch, bf16)
+    for off in (0, 1) if M < 4000 else (0,):
+        print(f"ffn tiles bf16={bf16} off={off} M={M} D={D} F={F}", flush=True)
+        ins = ffn_inputs(torch, M, D, F, t, off, M + D + F)
+        gate, up, y = ffn_fwd(hip, ctx, torch, bf16, 3, *ins, True, off)
+        check_ffn_fwd(torch, 3, step, *ins, gate, up, y)
+        dy = put(torch, gen(torch, 5)(M, D), t, off)
+        grads = ffn_bwd(hip, ctx, torch, bf16, 3, *ins, gate, up, dy, off)
+        check_ffn_bwd(torch, 3, step, *ins, gate, up, dy, *grads)
+        for a, b in zip(ffn_fwd(hip, ctx, torch, bf16, 3, *ins, True, off)
+                        + ffn_bwd(hip, ctx, torch, bf16, 3, *ins, gate, up, dy, off),
+                        [gate, up, y, *grads]):
+            assert torch.equal(a, b), "an output differs run to run"
 
 
 def test_ffn_gradients_against_differences(hip, ctx, torch_cuda):
