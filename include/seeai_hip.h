@@ -368,7 +368,8 @@ int seeai_norm_bwd(seeai_ctx* ctx, int kind, int dtype, const void* d_dy, const 
                    uint64_t ws_bytes);
 
 /* The gated feed-forward block: G = x wg, U = x wu, y = (act(G) * U) wd, with
- * x, y [M, D], wg, wu [D, F], wd [F, D] in `dtype`; act as in seeai_gemm_f32.
+ * x, y [M, D], wg, wu [D, F], wd [F, D] in `dtype`; act as in seeai_gemm_f32,
+ * but a NaN gate stays a NaN with relu too.
  * Products accumulate in f32; in bf16 the product act(G) U rounds once before
  * the down projection.  d_gate and d_up [M, F] receive G and U for the
  * backward pass, or are both NULL.  D and F up to 1048576, M to 536870912. */

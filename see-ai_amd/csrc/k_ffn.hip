@@ -122,8 +122,9 @@ __device__ __forceinline__ void Barrier() {
   asm volatile("" ::: "memory");
 }
 
-// The activation (ActExpr's functions) and its derivative.  GELU's 1 + tanh(t)
-// is 2 sigmoid(2 t), so both smooth ones are x s(.) with one exponential.
+// The activation (ActExpr's functions, but a NaN passes ReLU) and its derivative.
+// GELU's 1 + tanh(t) is 2 sigmoid(2 t), so both smooth ones are x s(.) with one
+// exponential.
 // kFast: the hardware's exponential and reciprocal, a few f32 steps off, for
 // results that leave in bf16.
 template <bool kFast>
@@ -145,9 +146,9 @@ __device__ __forceinline__ void Activate(int act, float x, float& a, float& da) 
     a = x * s;
     da = s + x * s * (1.0f - s) * (2.0f * kC * (1.0f + 3.0f * kA * x * x));
   } else {
-    const bool on = act == 0 || x > 0.0f;
-    a = on ? x : 0.0f;
-    da = on ? 1.0f : 0.0f;
+    const bool off = act == 1 && x <= 0.0f;
+    a = off ? 0.0f : x;
+    da = off ? 0.0f : act == 1 && x != x ? x : 1.0f;
   }
 }
 

@@ -440,6 +440,31 @@ def test_ffn_values_that_are_not_finite(hip, ctx, torch_cuda):
             assert y[1].isnan().all() and not torch.isfinite(y[3]).any()
 
 
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_ffn_nan_gates_reach_every_result(hip, ctx, torch_cuda, bf16, act):
+    """A NaN in the gate's weights reaches y of every token, with every activation; one in a saved
+    gate reaches the gradients that depend on it and no others.  (The derivative without an
+    activation is 1 whatever the gate, so there the gate's weights' gradient stays finite.)"""
+    torch = torch_cuda
+    t, _ = types(torch, bf16)
+    for M in (4, 40, 300):
+        x, wg, wu, wd = ffn_inputs(torch, M, 128, 192, t, 0, 3)
+        gate, up, _ = ffn_fwd(hip, ctx, torch, bf16, act, x, wg, wu, wd, True)
+        dy = put(torch, gen(torch, 5)(M, 128), t)
+        gate[2, 7] = float("nan")
+        dx, dwg, dwu, dwd = ffn_bwd(hip, ctx, torch, bf16, act, x, wg, wu, wd, gate, up, dy)
+        keep = [i for i in range(M) if i != 2]
+        assert dx[2].isnan().all() and torch.isfinite(dx[keep]).all()
+        cols = [i for i in range(192) if i != 7]
+        assert act == 0 or dwg[:, 7].isnan().all()
+        assert dwu[:, 7].isnan().all() and dwd[7].isnan().all()
+        assert all(torch.isfinite(v).all() for v in (dwg[:, cols], dwu[:, cols], dwd[cols]))
+        wg[5, 7] = float("nan")
+        y = ffn_fwd(hip, ctx, torch, bf16, act, x, wg, wu, wd, False)[2]
+        assert y.isnan().all()
+
+
 # --- AdamW over a group ---------------------------------------------------------------------------
 
 PARAMS = dict(lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.05)
