@@ -144,7 +144,9 @@ __device__ __forceinline__ void Activate(int act, float x, float& a, float& da) 
   } else if (act == 2) {
     const float s = Sigmoid<kFast>(2.0f * (kC * (x + kA * x * x * x)));
     a = x * s;
-    da = s + x * s * (1.0f - s) * (2.0f * kC * (1.0f + 3.0f * kA * x * x));
+    // Past 32 either way s is 0 or 1 and the second term 0, x^2 short of infinity or not.
+    const float y = fminf(fmaxf(x, -32.0f), 32.0f);
+    da = s + y * s * (1.0f - s) * (2.0f * kC * (1.0f + 3.0f * kA * y * y));
   } else {
     const bool off = act == 1 && x <= 0.0f;
     a = off ? 0.0f : x;

@@ -465,6 +465,22 @@ def test_ffn_nan_gates_reach_every_result(hip, ctx, torch_cuda, bf16, act):
         assert y.isnan().all()
 
 
+@pytest.mark.parametrize("act", [1, 2, 3])
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_ffn_gradients_at_large_gates(hip, ctx, torch_cuda, bf16, act):
+    """Finite gates have finite derivatives, 0 or 1 far out, also where the gate's square is past
+    f32."""
+    torch = torch_cuda
+    t, step = types(torch, bf16)
+    for M in (4, 40, 300):
+        ins = ffn_inputs(torch, M, 128, 192, t, 0, 3)
+        gate, up = (put(torch, gen(torch, i)(M, 192), t) for i in (8, 9))
+        gate[0, 1], gate[1, 3], gate[2, 5], gate[3, 2] = 1e25, 1e20, -1e20, -3e37
+        dy = put(torch, gen(torch, 5)(M, 128), t)
+        grads = ffn_bwd(hip, ctx, torch, bf16, act, *ins, gate, up, dy)
+        check_ffn_bwd(torch, act, step, *ins, gate, up, dy, *grads)
+
+
 # --- AdamW over a group ---------------------------------------------------------------------------
 
 PARAMS = dict(lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.05)
