@@ -170,4 +170,15 @@ inline const char* CheckAdamWGroup(const seeai_adamw_tensor* t, uint64_t count, 
   return nullptr;
 }
 
+// The values of 8-bit moments: as many as a group can hold (one launch of
+// 2048 elements a workgroup, below 2^32 threads).
+inline const char* CheckAdamWValues(int which, int dtype, const void* codes, const float* scales,
+                                    uint64_t n, const void* out) {
+  if (which < 0 || which > 1) return "which is 0 (m) or 1 (v)";
+  if (dtype < 0 || dtype > 1) return "dtype is 0 (f32) or 1 (bf16)";
+  if (n >> 36 || (n + 2047) / 2048 >> 24) return "operand too large";
+  return CheckOperands({{codes, n, 1, false}, {scales, (n + 127) / 128, 4, false},
+                        {out, n, TypeSize(dtype), true}});
+}
+
 }  // namespace seeai

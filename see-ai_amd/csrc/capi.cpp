@@ -3336,10 +3336,7 @@ int seeai_adamw_group_hold(seeai_adamw_group* g, const seeai_step_params* params
 int seeai_adamw_state_values(seeai_ctx* c, int which, int dtype, const uint8_t* codes,
                              const float* scales, uint64_t n, void* out) {
   if (!c) return SEEAI_INVALID;
-  if (which < 0 || which > 1 || dtype < 0 || dtype > 1 || n >> 35)
-    return Fail(c, SEEAI_INVALID, "adamw_state_values: bad which, dtype or size");
-  if (const char* e = CheckOperands({{codes, n, 1, false}, {scales, (n + 127) / 128, 4, false},
-                                     {out, n, TypeSize(dtype), true}}))
+  if (const char* e = CheckAdamWValues(which, dtype, codes, scales, n, out))
     return Fail(c, SEEAI_INVALID, "adamw_state_values: %s", e);
   OnDevice on(c->device);
   SEEAI_TRY(c, on.status(), "adamw_state_values");

@@ -317,3 +317,32 @@ def test_group_wrapper_refuses_tensors_of_another_device(hip):
     for name in ("p", "g", "m", "v"):
         with pytest.raises(ValueError, match=f"{name}: .*device 1"):
             make(**{name: 0})
+
+
+def test_values_refusals(tmp_path):
+    """As many values as one launch takes: a workgroup of 256 threads to 2048, below 2^32 threads."""
+    src, lib = tmp_path / "v.cc", tmp_path / "v.so"
+    src.write_text(r"""
+#include "see-ai_amd/csrc/block_args.h"
+extern "C" const char* values(int which, int dt, const uint64_t* p, uint64_t n) {
+  return seeai::CheckAdamWValues(which, dt, reinterpret_cast<const void*>(p[0]),
+                                 reinterpret_cast<const float*>(p[1]), n, reinterpret_cast<const void*>(p[2]));
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", f"-I{ROOT}", str(src), "-o", str(lib)], check=True)
+    h = C.CDLL(str(lib))
+    h.values.restype = C.c_char_p
+
+    def ask(which=0, dt=0, p=(1 << 40, 2 << 40, 3 << 40), n=300):
+        return h.values(which, dt, (C.c_uint64 * 3)(*p), u(n))
+    assert ask() is None and ask(1, 1) is None and ask(n=0, p=(0, 0, 0)) is None
+    assert b"which" in ask(2) and b"dtype" in ask(dt=2)
+    most = ((1 << 24) - 1) * 2048
+    assert ask(n=most) is None and most // 2048 * 256 < 1 << 32
+    assert all(b"large" in ask(n=n) for n in (most + 1, (1 << 35) - 1, 1 << 35, 1 << 63, (1 << 64) - 1))
+    for i in range(3):
+        p = [1 << 40, 2 << 40, 3 << 40]
+        p[i] = 0
+        assert b"null" in ask(p=p)
+    assert b"alignment" in ask(p=(1 << 40, (2 << 40) + 2, 3 << 40))
+    assert b"overlaps" in ask(p=(1 << 40, 2 << 40, (1 << 40) + 256))
