@@ -289,13 +289,15 @@ struct Pieces {
 };
 template <class T>
 __global__ void __launch_bounds__(256) FfnPackKernel(Pieces p) {
+  const unsigned block = blockIdx.y * gridDim.x + blockIdx.x;
+  if (block >= p.blocks) return;
   int k = 0;
-  while (k + 1 < p.count && blockIdx.x >= p.q[k + 1].first) ++k;
+  while (k + 1 < p.count && block >= p.q[k + 1].first) ++k;
   const Piece& q = p.q[k];
   // 2048 elements of the padded rows a workgroup, eight a thread; rows off 16
   // bytes come a lane an element through LDS.
   __shared__ float st[256 * 8];
-  const size_t base = static_cast<size_t>(blockIdx.x - q.first) * 2048, r0 = base / q.out.ld;
+  const size_t base = static_cast<size_t>(block - q.first) * 2048, r0 = base / q.out.ld;
   const uint32_t ld = q.out.ld, c0 = static_cast<uint32_t>(base - r0 * ld);
   if (!q.vec) {
 #pragma unroll
@@ -1259,7 +1261,9 @@ template <class T>
 hipError_t Pack(const Pieces& pieces, hipStream_t s) {
   if (pieces.count == 0) return hipSuccess;
   auto* kernel = &FfnPackKernel<T>;
-  hipLaunchKernelGGL(kernel, dim3(pieces.blocks), dim3(256), 0, s, pieces);
+  // In rows of workgroups: past 2^35 elements one row would be over 2^32 threads.
+  const unsigned row = std::min(pieces.blocks, 1u << 16);
+  hipLaunchKernelGGL(kernel, dim3(row, (pieces.blocks + row - 1) / row), dim3(256), 0, s, pieces);
   return hipGetLastError();
 }
 

@@ -386,6 +386,20 @@ def test_ffn_on_every_tile(hip, ctx, torch_cuda, M, D, F, bf16):
             assert torch.equal(a, b), "an output differs run to run"
 
 
+@pytest.mark.parametrize("bf16", [1, 0])
+def test_ffn_packing_past_a_row_of_workgroups(hip, ctx, torch_cuda, bf16):
+    """Operands off 16 bytes of more than 2^27 elements together: packed by several rows of workgroups."""
+    torch = torch_cuda
+    t, step = types(torch, bf16)
+    M, D, F = 70001, 2050, 9
+    ins = ffn_inputs(torch, M, D, F, t, 0, 1)
+    gate, up, y = ffn_fwd(hip, ctx, torch, bf16, 3, *ins, True)
+    check_ffn_fwd(torch, 3, step, *ins, gate, up, y)
+    dy = put(torch, gen(torch, 5)(M, D), t)
+    grads = ffn_bwd(hip, ctx, torch, bf16, 3, *ins, gate, up, dy)
+    check_ffn_bwd(torch, 3, step, *ins, gate, up, dy, *grads)
+
+
 def test_ffn_gradients_against_differences(hip, ctx, torch_cuda):
     """Central differences of the block's own forward, f32: the loss sum(y c) along random
     directions of x and of each weight.  A difference at h is off by h^2 of the third
