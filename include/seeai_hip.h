@@ -390,13 +390,15 @@ int seeai_ffn_bwd(seeai_ctx* ctx, int dtype, int act, const void* d_x, const voi
  * v_scale one float per 128 elements (the last block may be short); m stands
  * for code * scale, v for (code * scale)^2, a code being an e4m3 float (bias 7,
  * no infinities, 0x7F / 0xFF a NaN).  All-zero bytes are zero moments.  The new
- * moments round stochastically -- m and sqrt(v) right on average, v itself up
- * to 1/16 above -- by bits drawn from `seed`, the step's number (its low 32
- * bits) and the element's number (tensors end to end, each from a multiple of
- * 128): the same group, seed and step give the same bytes.  A NaN
- * or infinite moment becomes the NaN code of its element alone.  decay
- * multiplies the step's weight_decay; p_bf16, where given, receives the new
- * p rounded to bf16. */
+ * moments round stochastically, by bits drawn from `seed`, the step's number
+ * (its low 32 bits) and the element's number (tensors end to end, each from a
+ * multiple of 128): the same group, seed and step give the same bytes.  A code
+ * is right on average for m, and for sqrt(v) from the smallest code on (2^-9 of
+ * the scale: 1/115,000 to 1/230,000 of the block's largest); below it every
+ * v > 0 is held as that code, however small.  v itself comes out up to 1/16
+ * above, up to half above under eight smallest codes.  A NaN or infinite moment
+ * becomes the NaN code of its element alone.  decay multiplies the step's
+ * weight_decay; p_bf16, where given, receives the new p rounded to bf16. */
 typedef struct seeai_adamw_tensor {
   float* p;
   const void* g; /* f32, or bf16 with grad_dtype 1 */

@@ -15,8 +15,12 @@
 // Mix draws from (seed, step, the element's number in the group) -- the mean
 // is right and the same call gives the same bytes.  A power of two scales
 // without rounding, so the codes hold the f32 moments' own leading bits.
-// r > 0 keeps at least the smallest code: no element with a gradient behind
-// it divides by eps alone.  A NaN or infinite moment takes the NaN code and
+// r > 0 keeps at least the smallest code, 2^-9 of the scale: no element with a
+// gradient behind it divides by eps alone, and below that code r is held too
+// large (at 0.3 of it v is eleven times itself), so such an element's steps
+// are smaller than f32 moments would make them.  v = r^2 gains r's variance: of
+// what it climbs up to gap / 2r, 1/16 among the normal codes, half among the
+// subnormal.  A NaN or infinite moment takes the NaN code and
 // stays with its element; it does not count towards the block's scale.
 //
 // Bound by HBM: per element p in and out, g in, m and v in and out.  A lane

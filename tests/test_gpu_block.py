@@ -682,6 +682,37 @@ def test_8_bit_moments_are_right_on_average(hip, ctx, torch_cuda):
         assert least < float(rest.mean()) / want - 1 < most, name
 
 
+def test_8_bit_moments_near_the_smallest_code(hip, ctx, torch_cuda):
+    """From the smallest code on r = sqrt(v) is right on average and v high by its variance; below it
+    every r > 0 is that code.  From zero moments one step leaves r = sqrt(1 - beta2) |g|; a block's
+    largest, 300, is the scale's 300, so the others, in smallest codes of 2^-9, are q.  N = 8128
+    elements a q, each off by up to half a code at a spread of one half: means within 5 / (2 sqrt(N))
+    = 0.028 codes, v's within (2 q + 1) times that."""
+    torch = torch_cuda
+    blocks, qs = 64 * 5, (0.3, 0.9, 1.5, 3.3, 7.5)
+    n = 128 * blocks
+    root = math.sqrt(1.0 - float(np.float32(0.999)))
+    q = torch.tensor(qs, device="cuda").repeat_interleave(64)
+    r = (q / 512)[:, None].repeat(1, 128)
+    r[:, 0] = 300.0
+    t = {"p": torch.zeros(n, device="cuda"), "g": (r / root).flatten().contiguous(),
+         "m": torch.zeros(n, dtype=torch.uint8, device="cuda"),
+         "v": torch.zeros(n, dtype=torch.uint8, device="cuda"),
+         "m_scale": torch.zeros(blocks, device="cuda"), "v_scale": torch.zeros(blocks, device="cuda")}
+    hip.AdamWGroup(ctx, [t], 8, "f32", seed=6).step(params(hip, 1))
+    assert (t["v_scale"] == 1).all()
+    out = torch.empty(n, device="cuda")
+    ctx.call("seeai_adamw_state_values", 1, 0, t["v"].data_ptr(), t["v_scale"].data_ptr(), n, out.data_ptr())
+    v = out.view(5, 64, 128)[:, :, 1:].double() * 512 ** 2  # in smallest codes, squared
+    for i, want in enumerate(qs):
+        if want < 1:
+            assert (v[i] == 1).all()
+            continue
+        f, slack = want - math.floor(want), 2.5 / math.sqrt(64 * 127)
+        assert abs(float(v[i].sqrt().mean()) - want) < slack
+        assert abs(float(v[i].mean()) - (want ** 2 + f * (1 - f))) < (2 * want + 1) * slack
+
+
 def test_8_bit_moments_with_values_that_are_not_finite(hip, ctx, torch_cuda):
     torch = torch_cuda
     ts = tensors(torch, [300], 8, "f32", False)
