@@ -371,7 +371,10 @@ int seeai_norm_bwd(seeai_ctx* ctx, int kind, int dtype, const void* d_dy, const 
  * x, y [M, D], wg, wu [D, F], wd [F, D] in `dtype`; act as in seeai_gemm_f32,
  * but a NaN gate stays a NaN with relu too.
  * Products accumulate in f32; in bf16 the product act(G) U rounds once before
- * the down projection.  d_gate and d_up [M, F] receive G and U for the
+ * the down projection, in the backward pass dG and dU too.  In f32 past 128
+ * tokens a product's term loses up to 2^-21 of itself (0.7 2^-24 on average), an
+ * operand its bits below 2^-133, and what an infinity reaches may be a NaN where
+ * f32 arithmetic has an infinity.  d_gate and d_up [M, F] receive G and U for the
  * backward pass, or are both NULL.  D and F up to 1048576, M to 536870912. */
 uint64_t seeai_ffn_workspace(int dtype, uint64_t M, uint64_t D, uint64_t F, int backward);
 int seeai_ffn_fwd(seeai_ctx* ctx, int dtype, int act, const void* d_x, const void* d_wg,

@@ -21,12 +21,16 @@
 // rounded to bf16 once, as the stored G and U are, because the next product's
 // operands are bf16: at most 2^-8 of each value, as the inputs' own rounding.
 // f32: each operand is split into three bf16 planes (x = hi + mid + lo, eight
-// bits each, truncated, so exactly x), and a product is the six plane products
-// down to 2^-16 of it (what is left out is 2^-24 of it), all into the same f32
-// accumulators: f32's accuracy at a sixth of the bf16 rate, 1.6 times the f32
-// MFMA's (up to 128 tokens the f32 MFMA itself, below).  An infinity's remainder
-// is a NaN, so what an infinity reaches is not finite but may be a NaN where f32
-// arithmetic has an infinity.
+// bits each, truncated, so exactly x), and a product is its six largest plane
+// products, all into the same f32 accumulators.  What is left out
+// (mid lo, lo mid, lo lo; mid < 2^-7 and lo < 2^-15 of x's leading bit) is below
+// 2^-21 of the term and has its sign: 0.7 2^-24 of it on average over random
+// operands, 7.8 2^-24 for the square of 1 + 2^-7 - 2^-23.  So f32's accuracy but
+// for a loss of that size towards zero, at a sixth of the bf16 rate, 1.6 times
+// the f32 MFMA's (up to 128 tokens the f32 MFMA itself, below, which leaves
+// nothing out).  Bits of an operand below 2^-133 are past bf16's last.  An
+// infinity's remainder is a NaN, so past 128 tokens what an infinity reaches is
+// not finite but may be a NaN where f32 arithmetic has an infinity.
 #include <algorithm>
 #include <type_traits>
 #include <utility>

@@ -400,6 +400,27 @@ def test_ffn_packing_past_a_row_of_workgroups(hip, ctx, torch_cuda, bf16):
     check_ffn_bwd(torch, 3, step, *ins, gate, up, dy, *grads)
 
 
+@pytest.mark.parametrize("e", [0, -110, -120])
+@pytest.mark.parametrize("M", [100, 200])
+def test_ffn_f32_products_leave_out_less_than_2_to_the_minus_21(hip, ctx, torch_cuda, M, e):
+    """Past 128 tokens a term loses less than 2^-21 of itself, towards zero (here 7.8 2^-24, about the
+    most there is), and an operand its bits below 2^-133, bf16's last; up to 128 tokens nothing.  The
+    sum of D equal terms adds (D + 1) U for its own roundings."""
+    torch = torch_cuda
+    D, F, v = 16, 24, 1 + 2.0 ** -7 - 2.0 ** -23
+    x, wg, wu, wd = (torch.full(s, v, device="cuda") for s in ((M, D), (D, F), (D, F), (F, D)))
+    x *= 2.0 ** e
+    x[1::2] *= -1
+    gate, up, _ = ffn_fwd(hip, ctx, torch, 0, 0, x, wg, wu, wd, True)
+    want = D * v * v * 2.0 ** e
+    for got in (gate.double(), up.double()):
+        assert (got[0::2] > 0).all() and (got[1::2] < 0).all()
+        short = want - got.abs()  # (towards zero)
+        assert (short >= -(D + 1) * U * want).all()
+        left_out = (M > 128) * (2.0 ** -21 * want + D * v * 2.0 ** -133)
+        assert (short <= left_out + (D + 1) * U * want).all()
+
+
 def test_ffn_gradients_against_differences(hip, ctx, torch_cuda):
     """Central differences of the block's own forward, f32: the loss sum(y c) along random
     directions of x and of each weight.  A difference at h is off by h^2 of the third
