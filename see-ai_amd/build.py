@@ -7,9 +7,10 @@ Flags:
   -ffp-contract=off   the epilogue, optimizer and elementwise expressions
                       round where the reference's x86-64 build rounds them
   -Xclang -target-feature -Xclang -packed-fp32-ops
-                      keeps the compiler from forming packed-f32 VALU ops
-                      (this pool's rule; the host pass warns it does not know
-                      the feature, which is harmless)
+                      keeps the compiler from forming packed-f32 VALU ops,
+                      some forms of which have given wrong results (the host
+                      pass warns it does not know the feature, which is
+                      harmless)
   -mllvm -amdgpu-mfma-vgpr-form  (k_flash.hip, k_attn16.hip, k_attn3.hip)
                       MFMA accumulators in VGPRs: the attention kernels run
                       VALU softmax on every score tile, and AGPR-resident

@@ -12,10 +12,11 @@
 // besides the joins of shared-out K and the packing of operands.
 //
 // Many tokens are bound by the matrix unit's power: 8192 x 2048 x 5632 bf16 runs
-// 528 us forward and 1039 backward, 1,070 and 1,090 TFLOP/s (a library product
-// of these layouts 1,100 to 1,250), at 1.7 of 2.4 GHz; the down projection alone
-// 164 us, the gate's launch 365 for twice its work and 277 MB stored.  Few are
-// bound by the weights' bytes: one token of the same block 25 us for 69 MB.
+// 528 us forward and 1039 backward, 1,070 and 1,090 TFLOP/s (the same products
+// of a library, without what the epilogues do, 472 and 947 us; 1,030 to 1,550
+// TFLOP/s by layout and K), at 1.7 of 2.4 GHz; the down projection alone 161 us,
+// the gate's launch 361 for twice its work and 277 MB stored.  Few are bound by
+// the weights' bytes: one token of the same block 25 us for 69 MB.
 //
 // bf16: the operands as they are; what passes between launches (H, dG, dU) is
 // rounded to bf16 once, as the stored G and U are, because the next product's
