@@ -245,10 +245,8 @@ def prepare(case, seed):
         return case, x
     hip, ctx = _framework()
     lib, byte = hip.lib(), lambda n: torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
-    if case["op"] in ("logp", "pref"):
-        x["ws"] = byte(lib.seeai_token_logp_workspace(case["rows"], case["vocab"]))
-        if case["op"] == "pref":
-            x["ws_pref"] = byte(lib.seeai_pref_workspace(case["seqs"] // 2))
+    if case["op"] == "pref":
+        x["ws"] = byte(lib.seeai_pref_workspace(case["seqs"] // 2))
     elif case["op"] == "policy":
         x["ws"] = byte(lib.seeai_policy_workspace(case["rows"], case["vocab"]))
     elif case["op"].startswith("join"):
@@ -259,7 +257,7 @@ def prepare(case, seed):
             int(case["dtype"] == "bf16"), RES, EPS)
         if case["op"] == "join_bwd":
             x["ws"] = byte(lib.seeai_block_join_workspace(case["rows"], case["cols"], case["gate_rows"]))
-    else:
+    elif case["op"] == "clip":
         sizes, at = _sizes(case)
         x["grads"] = hip.GradGroup(ctx, [x["g"][a:a + n] for n, a in zip(sizes, at)])
         if case["step"]:
@@ -292,14 +290,14 @@ def _own(case, x):
         R, V, ld = case["rows"], case["vocab"], case["ld"]
         logp, stats = new32(R), new32(R, 2)
         ctx.call("seeai_token_logp_fwd", bf16, p(x["logits"]), ld, p(x["labels"]), p(logp), p(stats),
-                 R, V, p(x["ws"]), x["ws"].numel())
+                 R, V)
         if case["op"] == "logp":
             return {"logp": logp}
         pairs = case["seqs"] // 2
         loss, margin, dlogp, dlogits = new32(1), new32(pairs), new32(R), new(x["logits"])
         ctx.call("seeai_pref_loss", p(logp), p(x["ref"]), p(x["labels"]), p(x["starts"]), R, pairs,
                  PREF["beta"], 0.0, PREF["smoothing"], int(case["average"]), 1.0 / pairs, p(loss),
-                 p(margin), p(dlogp), p(x["ws_pref"]), x["ws_pref"].numel())
+                 p(margin), p(dlogp), p(x["ws"]), x["ws"].numel())
         ctx.call("seeai_token_logp_bwd", bf16, p(x["logits"]), ld, p(x["labels"]), p(stats), p(dlogp),
                  p(dlogits), R, V)
         return {"loss": loss, "logp": logp, "margin": margin, "dlogits": dlogits[:, :V]}
