@@ -431,11 +431,140 @@ int seeai_adamw_group_step(seeai_adamw_group* group, const seeai_step_params* pa
 /* Puts a step's values on the device, stream-ordered, for the steps with NULL
  * params after it.  Not while the stream is captured. */
 int seeai_adamw_group_hold(seeai_adamw_group* group, const seeai_step_params* params);
+/* seeai_adamw_group_step with every gradient multiplied by *d_factor (one f32 on
+ * the device: seeai_grad_group_norm's clip factor, or a loss scale's inverse)
+ * as it is read, so that clipping costs no pass of its own. */
+int seeai_adamw_group_step_scaled(seeai_adamw_group* group, const seeai_step_params* params,
+                                  const float* d_factor);
 /* The moments that 8-bit codes stand for: which 0 = m, 1 = v; dtype of d_out
  * 0 = f32, 1 = bf16 (which holds every code's value exactly where its exponent
  * range does); scales one per 128 elements from the first. */
 int seeai_adamw_state_values(seeai_ctx* ctx, int which, int dtype, const uint8_t* d_codes,
                              const float* d_scales, uint64_t n, void* d_out);
+/* The global norm of a step's gradients: many tensors, f32 and bf16 beside each
+ * other, in two launches.  The verdicts are those of seeai_adamw_step's clip. */
+typedef struct seeai_grad_tensor {
+  void* g;
+  uint64_t n;
+  int dtype; /* 0 f32, 1 bf16 */
+  uint32_t reserved;
+} seeai_grad_tensor;
+typedef struct seeai_grad_group seeai_grad_group;
+/* Checks the tensors (device pointers, none sharing memory with another: status
+ * 2) and keeps their table, and the norm's partial sums, on the device.  Not
+ * while the stream is captured. */
+int seeai_grad_group_create(seeai_ctx* ctx, const seeai_grad_tensor* tensors, uint64_t count,
+                            seeai_grad_group** out);
+/* Waits for the device; the context outlives its groups. */
+void seeai_grad_group_destroy(seeai_grad_group* group);
+/* *d_norm (NULL: not wanted) = the 2-norm of all gradients, squares summed in
+ * f64 in a fixed order, and *d_factor = min(1, max_norm / norm).  max_norm that
+ * is not a finite positive float is status 1 (kClipThresholdRefusal), except 0:
+ * the norm alone (d_factor NULL).  With a max_norm a norm that is not finite is
+ * a refusal: the factor is 1, no optimizer step behind it on the stream writes
+ * anything, and the next seeai_flush reports it.  Calls of one group that may
+ * run at the same time (a replayed graph beside an eager call) race. */
+int seeai_grad_group_norm(seeai_grad_group* group, float max_norm, float* d_norm, float* d_factor);
+/* Every gradient times *d_factor, in place; untouched where it is 1 or after a
+ * refusal. */
+int seeai_grad_group_scale(seeai_grad_group* group, const float* d_factor);
+
+/* What stands between two blocks: the norm after a block, its gate, the scaled
+ * residual, and the norm before the next block, in one pass (kinds, types and
+ * norms as in seeai_norm_fwd):
+ *   n = norm(o) post_w + post_b,  y = res_scale x + gate n,
+ *   h = norm(y) pre_w + pre_b
+ * post_w NULL: n = o; gate NULL: ones; pre_w NULL: no h; one of the norms has to
+ * be there.  A layer norm's bias may be NULL; root mean square has none.  Row r
+ * takes the gate's row r / gate_rows: gate [ceil(rows / gate_rows), cols], one
+ * row a sequence, or one for all with gate_rows >= rows.  The second norm takes
+ * y before its rounding to bf16.  cols up to 16384. */
+typedef struct seeai_block_join {
+  const void* o;       /* [rows, cols], the block's output */
+  const void* x;       /* [rows, cols], the residual stream (not read backward) */
+  const float* post_w; /* [cols], as all vectors */
+  const float* post_b;
+  const float* gate;
+  const float* pre_w;
+  const float* pre_b;
+  uint64_t rows, cols, gate_rows;
+  int kind, dtype;
+  float res_scale, eps;
+} seeai_block_join;
+/* d_y may be x, in place; d_stats [rows, 4], for the backward pass (or NULL):
+ * mean and 1 / deviation of o, then of y (0 where there is none). */
+int seeai_block_join_fwd(seeai_ctx* ctx, const seeai_block_join* join, void* d_y, void* d_h,
+                         float* d_stats);
+/* Its backward pass from d_y and d_stats (d_y is not read without pre_w): d_dh
+ * the gradient of h (NULL without pre_w), d_dy what reaches y past h (NULL:
+ * nothing).  dx may be d_dy, in place.  The vectors' gradients are f32 and the
+ * same bits every run; those of absent vectors are NULL, those of present ones
+ * may be, but not post_w's and pre_w's.  Zero rows give zeros. */
+typedef struct seeai_block_join_grads {
+  void* dx;
+  void* d_o;
+  float* dpost_w;
+  float* dpost_b;
+  float* dgate;
+  float* dpre_w;
+  float* dpre_b;
+} seeai_block_join_grads;
+/* gate_rows 0: without a gate. */
+uint64_t seeai_block_join_workspace(uint64_t rows, uint64_t cols, uint64_t gate_rows);
+int seeai_block_join_bwd(seeai_ctx* ctx, const seeai_block_join* join, const void* d_y,
+                         const float* d_stats, const void* d_dh, const void* d_dy,
+                         const seeai_block_join_grads* grads, void* d_ws, uint64_t ws_bytes);
+
+/* --- Learning from preferences -------------------------------------------
+ * Losses on the labels' log-probabilities, with their gradients, beside
+ * seeai_xent_*; memory, streams and dtype as for a block's own weights above.
+ * No reference counterpart.  Logits [N, C] in `dtype`, rows `ld` >= C elements
+ * apart (what lies between rows is neither read nor written), of any alignment;
+ * the gradients likewise, and they may take the logits' place (d_dlogits =
+ * d_logits).  A row whose label is negative is not judged: its logits are not
+ * read, its log-probability is 0 and its gradient zero.  A label from C on makes
+ * its row's results NaN. */
+
+/* logp[r] = log softmax(logits[r])[label], d_stats [N, 2] (or NULL) the row's
+ * maximum and sum of exp(logit - maximum), for the backward pass. */
+int seeai_token_logp_fwd(seeai_ctx* ctx, int dtype, const void* d_logits, uint64_t ld,
+                         const int32_t* d_labels, float* d_logp, float* d_stats, uint64_t N,
+                         uint64_t C);
+/* dlogits = dlogp (one-hot(label) - softmax). */
+int seeai_token_logp_bwd(seeai_ctx* ctx, int dtype, const void* d_logits, uint64_t ld,
+                         const int32_t* d_labels, const float* d_stats, const float* d_dlogp,
+                         void* d_dlogits, uint64_t N, uint64_t C);
+
+/* A loss on pairs of answers: sequence q is rows d_starts[q] to d_starts[q + 1]
+ * (2 pairs + 1 of them, rising; they are kept within [0, N]), pair i the chosen
+ * answer 2 i and the rejected one 2 i + 1.  An answer's log ratio is the sum over
+ * its judged rows of logp - ref_logp (d_ref_logp NULL: of logp), with `average`
+ * their mean (0 without any);
+ *   margin = beta (chosen - rejected) - offset,
+ *   loss = scale sum of (1 - smoothing) -log sigmoid(margin)
+ *                       + smoothing -log sigmoid(-margin)
+ * d_margin [pairs] and d_dlogp [N], the loss's gradient, may be NULL; rows that
+ * are not judged or in no sequence have a gradient of zero.  Sums are f64. */
+uint64_t seeai_pref_workspace(uint64_t pairs);
+int seeai_pref_loss(seeai_ctx* ctx, const float* d_logp, const float* d_ref_logp,
+                    const int32_t* d_labels, const int32_t* d_starts, uint64_t N, uint64_t pairs,
+                    float beta, float offset, float smoothing, int average, float scale,
+                    float* d_loss, float* d_margin, float* d_dlogp, void* d_ws, uint64_t ws_bytes);
+
+/* The clipped policy loss on sampled answers, from logits to their gradient in
+ * one call: with ratio = exp(logp - old_logp), A the row's advantage, and
+ * e = exp(ref_logp - logp),
+ *   l = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (e - (ref_logp - logp) - 1)
+ *   loss = scale sum over judged rows of weight l
+ * d_ref_logp NULL: without the KL term (kl_coef 0); d_weight NULL: ones; d_logp
+ * [N] and d_dlogits may be NULL. */
+uint64_t seeai_policy_workspace(uint64_t N, uint64_t C);
+int seeai_policy_loss(seeai_ctx* ctx, int dtype, const void* d_logits, uint64_t ld,
+                      const int32_t* d_labels, const float* d_old_logp, const float* d_ref_logp,
+                      const float* d_adv, const float* d_weight, uint64_t N, uint64_t C,
+                      float clip_low, float clip_high, float kl_coef, float scale, float* d_loss,
+                      float* d_logp, void* d_dlogits, void* d_ws, uint64_t ws_bytes);
 /* The eval argmax, first maximum wins (update_engine.cc:537-565). */
 int seeai_argmax_rows(seeai_ctx* ctx, const float* d_probs, uint64_t rows,
                       uint64_t cols, int32_t* d_out);

@@ -1,5 +1,6 @@
 // block_args.h -- the argument checks of the trained-block entry points
-// (seeai_norm_*, seeai_ffn_*, seeai_adamw_group_*): what the kernels assume of
+// (seeai_norm_*, seeai_ffn_*, seeai_block_join_*, seeai_adamw_group_*,
+// seeai_grad_group_*): what the kernels assume of
 // their operands, decided on the host before anything is launched.  Plain C++
 // without HIP, so the checks run where there is no GPU.  A check returns null,
 // or why the call is refused.
@@ -9,6 +10,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <initializer_list>
+#include <utility>
 #include <vector>
 
 #include "../../include/seeai_hip.h"
@@ -168,6 +170,85 @@ inline const char* CheckAdamWGroup(const seeai_adamw_tensor* t, uint64_t count, 
     if (r.out) written = std::max(written, r.e);
   }
   return nullptr;
+}
+
+// A step's gradients: each complete and aligned, none sharing memory with
+// another (the clip in place takes each once).
+inline const char* CheckGradGroup(const seeai_grad_tensor* t, uint64_t count) {
+  if (count > 1 << 24) return "too many tensors";
+  if (count && !t) return "null operand";
+  std::vector<std::pair<uintptr_t, uintptr_t>> runs;
+  uint64_t chunks = 0;
+  for (uint64_t i = 0; i < count; ++i) {
+    const seeai_grad_tensor& x = t[i];
+    if (x.n == 0) continue;
+    if (x.dtype < 0 || x.dtype > 1) return "dtype is 0 (f32) or 1 (bf16)";
+    if (x.n >> 36) return "operand too large";
+    if (!x.g) return "null operand";
+    const uintptr_t b = reinterpret_cast<uintptr_t>(x.g);
+    if (b % TypeSize(x.dtype)) return "operand off its element's alignment";
+    runs.push_back({b, b + x.n * TypeSize(x.dtype)});
+    if ((chunks += (x.n + 2047) / 2048) >> 24) return "group too large";
+  }
+  std::sort(runs.begin(), runs.end());
+  for (size_t i = 1; i < runs.size(); ++i)
+    if (runs[i].first < runs[i - 1].second) return "two gradients share memory";
+  return nullptr;
+}
+
+// Rows of a join are held in registers.
+constexpr uint64_t kJoinMaxCols = 16384;
+
+inline const char* CheckJoinShape(uint64_t rows, uint64_t cols) {
+  return cols == 0 || cols > kJoinMaxCols || rows > kBlockMaxRows ? "bad shape (columns from 1 to 16384)" : nullptr;
+}
+inline uint64_t JoinGates(const seeai_block_join& j) {
+  return j.gate ? (j.rows + j.gate_rows - 1) / j.gate_rows : 0;
+}
+inline const char* CheckJoin(const seeai_block_join& j) {
+  if (j.kind < 0 || j.kind > 1) return "kind is 0 (layer) or 1 (root mean square)";
+  if (j.dtype < 0 || j.dtype > 1) return "dtype is 0 (f32) or 1 (bf16)";
+  if (const char* e = CheckJoinShape(j.rows, j.cols)) return e;
+  if (!(j.eps >= 0.0f) || j.eps > 3.4028234663852886e38f) return "eps is a finite number from zero";
+  if (!(j.res_scale - j.res_scale == 0.0f)) return "res_scale is finite";
+  if (!j.post_w && !j.pre_w) return "neither norm is there";
+  if ((j.post_b && !j.post_w) || (j.pre_b && !j.pre_w)) return "a bias without its norm";
+  if (j.kind == 1 && (j.post_b || j.pre_b)) return "a root-mean-square norm has no bias";
+  if (j.gate && (j.gate_rows == 0 || j.gate_rows >> 62)) return "gate_rows is at least 1";
+  return nullptr;
+}
+
+inline const char* CheckJoinFwd(const seeai_block_join& j, const void* y, const void* h,
+                                const float* stats) {
+  if (const char* e = CheckJoin(j)) return e;
+  if (!j.pre_w && h) return "no norm to give h";
+  const uint64_t n = j.rows * j.cols, size = TypeSize(j.dtype), c = j.cols;
+  return CheckOperands({{j.o, n, size, false}, {j.x, j.x == y ? 0 : n, size, false},
+                        {j.post_w, j.post_w ? c : 0, 4, false}, {j.post_b, j.post_b ? c : 0, 4, false},
+                        {j.gate, JoinGates(j) * c, 4, false}, {j.pre_w, j.pre_w ? c : 0, 4, false},
+                        {j.pre_b, j.pre_b ? c : 0, 4, false}, {y, n, size, true},
+                        {h, j.pre_w ? n : 0, size, true}, {stats, stats ? 4 * j.rows : 0, 4, true}});
+}
+
+inline const char* CheckJoinBwd(const seeai_block_join& j, const void* y, const float* stats,
+                                const void* dh, const void* dy, const seeai_block_join_grads& g,
+                                const void* ws, uint64_t ws_bytes, uint64_t need) {
+  if (const char* e = CheckJoin(j)) return e;
+  if (!j.pre_w && dh) return "no norm that gave h";
+  if ((g.dpost_w && !j.post_w) || (g.dpost_b && !j.post_b) || (g.dgate && !j.gate) ||
+      (g.dpre_w && !j.pre_w) || (g.dpre_b && !j.pre_b))
+    return "the gradient of an absent vector";
+  if (ws_bytes < need) return "workspace too small (seeai_block_join_workspace)";
+  const uint64_t n = j.rows * j.cols, size = TypeSize(j.dtype), c = j.cols;
+  const uint64_t post = j.post_w ? c : 0, pre = j.pre_w ? c : 0, gates = JoinGates(j) * c;
+  return CheckOperands({{j.o, post || gates ? n : 0, size, false}, {y, pre ? n : 0, size, false},
+                        {stats, 4 * j.rows, 4, false}, {dh, pre ? n : 0, size, false},
+                        {dy, dy && dy != g.dx ? n : 0, size, false}, {j.post_w, post, 4, false},
+                        {j.post_b, j.post_b ? c : 0, 4, false}, {j.gate, gates, 4, false},
+                        {j.pre_w, pre, 4, false}, {g.dx, n, size, true}, {g.d_o, n, size, true},
+                        {g.dpost_w, post, 4, true}, {g.dpost_b, g.dpost_b ? c : 0, 4, true},
+                        {g.dgate, g.dgate ? gates : 0, 4, true}, {g.dpre_w, pre, 4, true},
+                        {g.dpre_b, g.dpre_b ? c : 0, 4, true}, {ws, (need + 15) / 16, 16, true}});
 }
 
 // The values of 8-bit moments: as many as a group can hold (one launch of

@@ -28,6 +28,7 @@
 #include "block_args.h"
 #include "common.h"
 #include "operands.h"
+#include "pref_args.h"
 
 using namespace seeai;
 
@@ -3150,6 +3151,14 @@ int Capturing(seeai_ctx* c, bool* yes) {
   return SEEAI_OK;
 }
 
+// What both directions of a join take.
+JoinArgs JoinOf(const seeai_block_join& j) {
+  JoinArgs a{};
+  a.rms = j.kind, a.o = j.o, a.post_w = j.post_w, a.post_b = j.post_b, a.gate = j.gate, a.pre_w = j.pre_w;
+  a.rows = j.rows, a.cols = j.cols, a.gate_rows = j.gate_rows, a.res = j.res_scale, a.eps = j.eps;
+  return a;
+}
+
 }  // namespace
 
 uint64_t seeai_norm_bwd_workspace(uint64_t rows, uint64_t cols) {
@@ -3177,6 +3186,39 @@ int seeai_norm_bwd(seeai_ctx* c, int kind, int dtype, const void* dy, const void
   SEEAI_TRY(c, on.status(), "norm_bwd");
   SEEAI_TRY(c, LaunchNormBwd(kind, dtype, dy, x, w, mean, rstd, dx, dw, db, rows, cols, ws, c->stream),
             "norm_bwd");
+  return SEEAI_OK;
+}
+
+uint64_t seeai_block_join_workspace(uint64_t rows, uint64_t cols, uint64_t gate_rows) {
+  if (CheckJoinShape(rows, cols)) return 0;
+  return JoinWorkspaceBytes(rows, cols, gate_rows);
+}
+int seeai_block_join_fwd(seeai_ctx* c, const seeai_block_join* j, void* y, void* h, float* stats) {
+  if (!c) return SEEAI_INVALID;
+  if (!j) return Fail(c, SEEAI_INVALID, "block_join_fwd: null argument");
+  if (const char* e = CheckJoinFwd(*j, y, h, stats)) return Fail(c, SEEAI_INVALID, "block_join_fwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "block_join_fwd");
+  JoinArgs a = JoinOf(*j);
+  a.x = j->x, a.pre_b = j->pre_b, a.y = y, a.h = h, a.stats = stats;
+  SEEAI_TRY(c, LaunchJoinFwd(j->dtype, a, c->stream), "block_join_fwd");
+  return SEEAI_OK;
+}
+int seeai_block_join_bwd(seeai_ctx* c, const seeai_block_join* j, const void* y, const float* stats,
+                         const void* dh, const void* dy, const seeai_block_join_grads* g, void* ws,
+                         uint64_t ws_bytes) {
+  if (!c) return SEEAI_INVALID;
+  if (!j || !g) return Fail(c, SEEAI_INVALID, "block_join_bwd: null argument");
+  const uint64_t need = seeai_block_join_workspace(j->rows, j->cols, j->gate ? j->gate_rows : 0);
+  if (const char* e = CheckJoinBwd(*j, y, stats, dh, dy, *g, ws, ws_bytes, need))
+    return Fail(c, SEEAI_INVALID, "block_join_bwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "block_join_bwd");
+  JoinArgs a = JoinOf(*j);
+  a.y = const_cast<void*>(y), a.stats = const_cast<float*>(stats), a.dh = dh, a.dy = dy;
+  a.dx = g->dx, a.d_o = g->d_o, a.dpost_w = g->dpost_w, a.dpost_b = g->dpost_b, a.dgate = g->dgate;
+  a.dpre_w = g->dpre_w, a.dpre_b = g->dpre_b, a.part = static_cast<float*>(ws);
+  SEEAI_TRY(c, LaunchJoinBwd(j->dtype, a, c->stream), "block_join_bwd");
   return SEEAI_OK;
 }
 
@@ -3237,6 +3279,26 @@ AdamWGroupStep GroupStep(const seeai_adamw_group* g, const seeai_step_params& P)
   float hy[3];
   StepHyper(P, hy);
   return {P.lr, P.beta1, P.beta2, P.eps, P.weight_decay, hy[1], hy[2], AdamWGroupKey(g->seed, P.step)};
+}
+
+// One step, the gradients multiplied by *factor where it is given.
+int GroupRun(seeai_adamw_group* g, const seeai_step_params* params, const float* factor, const char* what) {
+  if (!g) return SEEAI_INVALID;
+  seeai_ctx* c = g->ctx;
+  if (!params && !g->holds)
+    return Fail(c, SEEAI_INVALID, "%s: no params, and none held (seeai_adamw_group_hold)", what);
+  if (params && params->step == 0) return Fail(c, SEEAI_INVALID, "%s: steps count from 1", what);
+  bool capturing;
+  if (int rc = Capturing(c, &capturing)) return rc;
+  if (capturing && params)
+    return Fail(c, SEEAI_INVALID, "%s: a captured step takes held params (NULL)", what);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), what);
+  SEEAI_TRY(c, LaunchAdamWGroup(g->table, g->count, g->chunks, g->bits, g->grads_bf16,
+                                params ? GroupStep(g, *params) : AdamWGroupStep{},
+                                params ? nullptr : g->held, factor, c->flag(), c->stream),
+            what);
+  return SEEAI_OK;
 }
 
 }  // namespace
@@ -3301,22 +3363,14 @@ void seeai_adamw_group_destroy(seeai_adamw_group* g) {
 }
 
 int seeai_adamw_group_step(seeai_adamw_group* g, const seeai_step_params* params) {
+  return GroupRun(g, params, nullptr, "adamw_group_step");
+}
+int seeai_adamw_group_step_scaled(seeai_adamw_group* g, const seeai_step_params* params,
+                                  const float* factor) {
   if (!g) return SEEAI_INVALID;
-  seeai_ctx* c = g->ctx;
-  if (!params && !g->holds)
-    return Fail(c, SEEAI_INVALID, "adamw_group_step: no params, and none held (seeai_adamw_group_hold)");
-  if (params && params->step == 0) return Fail(c, SEEAI_INVALID, "adamw_group_step: steps count from 1");
-  bool capturing;
-  if (int rc = Capturing(c, &capturing)) return rc;
-  if (capturing && params)
-    return Fail(c, SEEAI_INVALID, "adamw_group_step: a captured step takes held params (NULL)");
-  OnDevice on(c->device);
-  SEEAI_TRY(c, on.status(), "adamw_group_step");
-  SEEAI_TRY(c, LaunchAdamWGroup(g->table, g->count, g->chunks, g->bits, g->grads_bf16,
-                                params ? GroupStep(g, *params) : AdamWGroupStep{},
-                                params ? nullptr : g->held, c->flag(), c->stream),
-            "adamw_group_step");
-  return SEEAI_OK;
+  if (const char* e = CheckOperands({{factor, 1, 4, false}}))
+    return Fail(g->ctx, SEEAI_INVALID, "adamw_group_step_scaled: %s", e);
+  return GroupRun(g, params, factor, "adamw_group_step_scaled");
 }
 
 int seeai_adamw_group_hold(seeai_adamw_group* g, const seeai_step_params* params) {
@@ -3341,6 +3395,157 @@ int seeai_adamw_state_values(seeai_ctx* c, int which, int dtype, const uint8_t* 
   OnDevice on(c->device);
   SEEAI_TRY(c, on.status(), "adamw_state_values");
   SEEAI_TRY(c, LaunchAdamWValues(which, dtype, codes, scales, n, out, c->stream), "adamw_state_values");
+  return SEEAI_OK;
+}
+
+// --- The gradients of a step ----------------------------------------------------------------------
+
+}  // extern "C" (the group's definition)
+
+struct seeai_grad_group {
+  seeai_ctx* ctx = nullptr;
+  GradGroupTensor* table = nullptr;  // device, behind the norm's partial sums
+  double* part = nullptr;
+  int count = 0;
+  uint64_t chunks = 0;
+};
+
+extern "C" {
+
+int seeai_grad_group_create(seeai_ctx* c, const seeai_grad_tensor* t, uint64_t count,
+                            seeai_grad_group** out) try {
+  if (!c || !out) return Fail(c, SEEAI_INVALID, "grad_group_create: null argument");
+  *out = nullptr;
+  if (const char* e = CheckGradGroup(t, count)) return Fail(c, SEEAI_INVALID, "grad_group_create: %s", e);
+  bool capturing;
+  if (int rc = Capturing(c, &capturing)) return rc;
+  if (capturing) return Fail(c, SEEAI_INVALID, "grad_group_create: the stream is being captured");
+  std::vector<GradGroupTensor> rows;
+  uint64_t chunks = 0;
+  for (uint64_t i = 0; i < count; ++i) {
+    const seeai_grad_tensor& x = t[i];
+    if (x.n == 0) continue;
+    rows.push_back({x.g, x.n, chunks, x.dtype, (reinterpret_cast<uintptr_t>(x.g) & 15) == 0});
+    chunks += (x.n + kGradChunk - 1) / kGradChunk;
+  }
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "grad_group_create");
+  const size_t parts = static_cast<size_t>(GradNormParts(chunks)) * sizeof(double);
+  const size_t bytes = rows.size() * sizeof(GradGroupTensor);
+  auto g = std::make_unique<seeai_grad_group>();
+  void* mem = nullptr;
+  SEEAI_TRY(c, hipMalloc(&mem, parts + bytes + 16), "grad_group table");
+  uint8_t* table = static_cast<uint8_t*>(mem) + parts;
+  if (bytes)
+    if (hipError_t e = hipMemcpy(table, rows.data(), bytes, hipMemcpyHostToDevice); e != hipSuccess) {
+      (void)hipFree(mem);
+      return Hip(c, e, "grad_group table copy");
+    }
+  g->ctx = c;
+  g->part = static_cast<double*>(mem);
+  g->table = reinterpret_cast<GradGroupTensor*>(table);
+  g->count = static_cast<int>(rows.size());
+  g->chunks = chunks;
+  *out = g.release();
+  return SEEAI_OK;
+} catch (const std::bad_alloc&) {
+  return Fail(c, SEEAI_INVALID, "grad_group_create: out of host memory");
+}
+
+void seeai_grad_group_destroy(seeai_grad_group* g) {
+  if (!g) return;
+  OnDevice on(g->ctx->device);
+  if (g->part) (void)hipFree(g->part);  // waits for the device
+  delete g;
+}
+
+int seeai_grad_group_norm(seeai_grad_group* g, float max_norm, float* norm, float* factor) {
+  if (!g) return SEEAI_INVALID;
+  seeai_ctx* c = g->ctx;
+  if (max_norm != 0.0f && (!std::isfinite(max_norm) || !(max_norm > 0.0f)))
+    return Fail(c, SEEAI_REFUSED, "%s", kClipThresholdRefusal);
+  if (max_norm == 0.0f && factor) return Fail(c, SEEAI_INVALID, "grad_group_norm: a factor needs a max_norm");
+  if (const char* e = CheckOperands({{norm, norm || !factor ? 1u : 0u, 4, true},
+                                     {factor, max_norm > 0.0f ? 1u : 0u, 4, true}}))
+    return Fail(c, SEEAI_INVALID, "grad_group_norm: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "grad_group_norm");
+  SEEAI_TRY(c, LaunchGradNorm(g->table, g->count, g->chunks, g->part, max_norm, norm, factor, c->flag(),
+                              c->stream),
+            "grad_group_norm");
+  return SEEAI_OK;
+}
+
+int seeai_grad_group_scale(seeai_grad_group* g, const float* factor) {
+  if (!g) return SEEAI_INVALID;
+  seeai_ctx* c = g->ctx;
+  if (const char* e = CheckOperands({{factor, 1, 4, false}}))
+    return Fail(c, SEEAI_INVALID, "grad_group_scale: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "grad_group_scale");
+  SEEAI_TRY(c, LaunchGradScale(g->table, g->count, g->chunks, factor, c->flag(), c->stream),
+            "grad_group_scale");
+  return SEEAI_OK;
+}
+
+// --- Learning from preferences --------------------------------------------------------------------
+
+int seeai_token_logp_fwd(seeai_ctx* c, int dtype, const void* z, uint64_t ld, const int32_t* labels,
+                         float* logp, float* stats, uint64_t N, uint64_t C) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckTokenLogpFwd(dtype, z, ld, labels, logp, stats, N, C))
+    return Fail(c, SEEAI_INVALID, "token_logp_fwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "token_logp_fwd");
+  SEEAI_TRY(c, LaunchTokenLogpFwd(dtype, z, ld, labels, logp, stats, N, C, c->stream), "token_logp_fwd");
+  return SEEAI_OK;
+}
+int seeai_token_logp_bwd(seeai_ctx* c, int dtype, const void* z, uint64_t ld, const int32_t* labels,
+                         const float* stats, const float* dlogp, void* dz, uint64_t N, uint64_t C) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckTokenLogpBwd(dtype, z, ld, labels, stats, dlogp, dz, N, C))
+    return Fail(c, SEEAI_INVALID, "token_logp_bwd: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "token_logp_bwd");
+  SEEAI_TRY(c, LaunchTokenLogpBwd(dtype, z, ld, labels, stats, dlogp, dz, N, C, c->stream),
+            "token_logp_bwd");
+  return SEEAI_OK;
+}
+
+uint64_t seeai_pref_workspace(uint64_t pairs) {
+  return pairs > kPrefMaxPairs ? 0 : PrefWorkspaceBytes(pairs);
+}
+int seeai_pref_loss(seeai_ctx* c, const float* logp, const float* ref, const int32_t* labels,
+                    const int32_t* starts, uint64_t N, uint64_t pairs, float beta, float offset,
+                    float smoothing, int average, float scale, float* loss, float* margin, float* dlogp,
+                    void* ws, uint64_t ws_bytes) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckPrefLoss(logp, ref, labels, starts, N, pairs, beta, offset, smoothing, average,
+                                    scale, loss, margin, dlogp, ws, ws_bytes, seeai_pref_workspace(pairs)))
+    return Fail(c, SEEAI_INVALID, "pref_loss: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "pref_loss");
+  const PrefArgs a{logp, ref, labels, starts, N, pairs, beta, offset, smoothing, scale, average, margin, dlogp};
+  SEEAI_TRY(c, LaunchPrefLoss(a, loss, ws, c->stream), "pref_loss");
+  return SEEAI_OK;
+}
+
+uint64_t seeai_policy_workspace(uint64_t N, uint64_t C) {
+  if (CheckLogitsShape(0, C, N, C)) return 0;
+  return PolicyWorkspaceBytes(N);
+}
+int seeai_policy_loss(seeai_ctx* c, int dtype, const void* z, uint64_t ld, const int32_t* labels,
+                      const float* old_logp, const float* ref, const float* adv, const float* weight,
+                      uint64_t N, uint64_t C, float low, float high, float kl, float scale, float* loss,
+                      float* logp, void* dz, void* ws, uint64_t ws_bytes) {
+  if (!c) return SEEAI_INVALID;
+  if (const char* e = CheckPolicyLoss(dtype, z, ld, labels, old_logp, ref, adv, weight, N, C, low, high, kl,
+                                      scale, loss, logp, dz, ws, ws_bytes, seeai_policy_workspace(N, C)))
+    return Fail(c, SEEAI_INVALID, "policy_loss: %s", e);
+  OnDevice on(c->device);
+  SEEAI_TRY(c, on.status(), "policy_loss");
+  const PolicyTerms P{old_logp, ref, adv, weight, low, high, kl, scale};
+  SEEAI_TRY(c, LaunchPolicyLoss(dtype, z, ld, labels, P, loss, logp, dz, N, C, ws, c->stream), "policy_loss");
   return SEEAI_OK;
 }
 

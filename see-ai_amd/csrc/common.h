@@ -310,6 +310,56 @@ hipError_t LaunchNormBwd(int rms, int bf16, const void* dy, const void* x, const
                          const float* mean, const float* rstd, void* dx, float* dw, float* db,
                          size_t rows, size_t cols, void* ws, hipStream_t s);
 
+// Learning from preferences (k_pref.hip): logits f32 or bf16, rows ld apart; a
+// negative label is not judged.  stats [N, 2]: a row's maximum and exp sum.
+// dz may be z.
+hipError_t LaunchTokenLogpFwd(int bf16, const void* z, size_t ld, const int32_t* labels, float* logp,
+                              float* stats, size_t N, size_t C, hipStream_t s);
+hipError_t LaunchTokenLogpBwd(int bf16, const void* z, size_t ld, const int32_t* labels,
+                              const float* stats, const float* dlogp, void* dz, size_t N, size_t C,
+                              hipStream_t s);
+struct PrefArgs {
+  const float *logp, *ref_logp;  // ref_logp null: zeros
+  const int32_t *labels, *starts;
+  size_t N, pairs;
+  float beta, offset, smoothing, scale;
+  int average;
+  float *margin, *dlogp;  // either null: not wanted
+};
+size_t PrefWorkspaceBytes(size_t pairs);
+hipError_t LaunchPrefLoss(const PrefArgs& a, float* loss, void* ws, hipStream_t s);
+struct PolicyTerms {
+  const float *old_logp, *ref_logp, *adv, *weight;  // ref_logp null: no KL; weight null: ones
+  float low, high, kl, scale;
+};
+size_t PolicyWorkspaceBytes(size_t N);
+// logp and dz may be null.
+hipError_t LaunchPolicyLoss(int bf16, const void* z, size_t ld, const int32_t* labels,
+                            const PolicyTerms& P, float* loss, float* logp, void* dz, size_t N, size_t C,
+                            void* ws, hipStream_t s);
+
+// Between two blocks (k_join.hip): n = norm(o) post_w + post_b, y = res x +
+// gate n, h = norm(y) pre_w + pre_b; tensors f32 or bf16, vectors f32, stats
+// [rows, 4].  post_w, gate, pre_w null: without that part.  A row r takes gate
+// row r / gate_rows.  y may be x, dx may be dy.
+struct JoinArgs {
+  int rms;
+  const void *o, *x;
+  const float *post_w, *post_b, *gate, *pre_w, *pre_b;
+  size_t rows, cols, gate_rows;
+  float res, eps;
+  void *y, *h;
+  float* stats;
+  // the backward's: y and stats are inputs
+  const void *dh, *dy;  // dy null: zeros
+  void *dx, *d_o;
+  float *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
+  float* part;
+};
+size_t JoinWorkspaceBytes(size_t rows, size_t cols, size_t gate_rows);
+hipError_t LaunchJoinFwd(int bf16, const JoinArgs& a, hipStream_t s);
+hipError_t LaunchJoinBwd(int bf16, const JoinArgs& a, hipStream_t s);
+
 // The gated feed-forward block (k_ffn.hip): x, y, dy, dx [M, D], wg, wu and
 // their gradients [D, F], wd and its gradient [F, D], gate, up [M, F], all f32
 // or all bf16.  ws: FfnWorkspaceBytes.
@@ -350,12 +400,32 @@ struct AdamWGroupStep {
 };
 uint32_t AdamWGroupKey(uint32_t seed, uint64_t step);
 // held: null, or device memory whose step takes the place of args.
+// factor: null, or what every gradient is multiplied by first.
 hipError_t LaunchAdamWGroup(const AdamWGroupTensor* tab, int count, uint64_t chunks, int bits,
                             int grads_bf16, const AdamWGroupStep& args, const AdamWGroupStep* held,
-                            const int* flag, hipStream_t s);
+                            const float* factor, const int* flag, hipStream_t s);
 hipError_t LaunchAdamWGroupHold(AdamWGroupStep* held, const AdamWGroupStep& args, hipStream_t s);
 hipError_t LaunchAdamWValues(int second, int bf16, const uint8_t* codes, const float* scales,
                              uint64_t n, void* out, hipStream_t s);
+
+// The gradients of a step (k_grad_group.hip): the device table's rows; a
+// tensor's chunks of kGradChunk elements are numbered through the group from
+// first_chunk.  part: GradNormParts doubles.
+constexpr int kGradChunk = 2048;
+struct GradGroupTensor {
+  void* g;
+  uint64_t n, first_chunk;
+  int bf16;
+  int vec;  // g takes 16-byte accesses
+};
+int GradNormParts(uint64_t chunks);
+// norm (null: not wanted) = sqrt(sum of squares); with max_norm > 0 also factor
+// = min(1, max_norm / norm), and a norm that is not finite sets flag.
+hipError_t LaunchGradNorm(const GradGroupTensor* tab, int count, uint64_t chunks, double* part,
+                          float max_norm, float* norm, float* factor, int* flag, hipStream_t s);
+// g *= factor, in place, but where it is 1 or flag is set.
+hipError_t LaunchGradScale(const GradGroupTensor* tab, int count, uint64_t chunks,
+                           const float* factor, const int* flag, hipStream_t s);
 
 // Optimizer family (k_optim.hip).  `flag` is the device refusal word that
 // every parameter-writing kernel honours; `scale` a device float slot.

@@ -143,7 +143,8 @@ __device__ __forceinline__ void StoreCodes(uint8_t* p, bool vec, int cnt, const 
 template <int kBits, class G>
 __global__ void __launch_bounds__(kThreads)
 AdamWGroupKernel(const AdamWGroupTensor* __restrict__ tab, int count, AdamWGroupStep args,
-                 const AdamWGroupStep* __restrict__ held, const int* __restrict__ flag) {
+                 const AdamWGroupStep* __restrict__ held, const float* __restrict__ factor,
+                 const int* __restrict__ flag) {
   if (*flag) return;
   const AdamWGroupStep P = held ? *held : args;
   // The tensor this chunk lies in: the last whose first chunk is not past it.
@@ -171,6 +172,11 @@ AdamWGroupKernel(const AdamWGroupTensor* __restrict__ tab, int count, AdamWGroup
     Decode8(LoadCodes(static_cast<const uint8_t*>(T.v) + at, vec, cnt), vs, v);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) v[e] = v[e] * v[e];
+  }
+  if (factor) {  // a clipped step
+    const float f = *factor;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) g[e] *= f;
   }
   const float om_b1 = 1.0f - P.beta1, om_b2 = 1.0f - P.beta2, wd = P.weight_decay * T.decay;
 #pragma unroll
@@ -269,11 +275,11 @@ uint32_t AdamWGroupKey(uint32_t seed, uint64_t step) {
 
 hipError_t LaunchAdamWGroup(const AdamWGroupTensor* tab, int count, uint64_t chunks, int bits,
                             int grads_bf16, const AdamWGroupStep& args, const AdamWGroupStep* held,
-                            const int* flag, hipStream_t s) {
+                            const float* factor, const int* flag, hipStream_t s) {
   if (chunks == 0) return hipSuccess;
   auto go = [&](auto* kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(chunks)), dim3(kThreads), 0, s, tab,
-                       count, args, held, flag);
+                       count, args, held, factor, flag);
     return hipGetLastError();
   };
   if (bits == 32) return grads_bf16 ? go(AdamWGroupKernel<32, uint16_t>) : go(AdamWGroupKernel<32, float>);

@@ -1,0 +1,150 @@
+// k_grad_group.hip -- the global norm of a step's gradients over many tensors
+// (f32 and bf16 beside each other), the factor that clips it, and the clip in
+// place.
+//
+//   norm = sqrt(sum of g^2 over all tensors),  factor = min(1, max_norm / norm)
+//
+// The verdicts are the per-tensor clip's (k_optim.hip; optimizer.cc:40-85): a
+// norm that is not finite sets the refusal word, and no step behind it writes
+// anything.  Squares are f64 (an f32 square overflows from 1.8e19 on) and so
+// are their sums: workgroup b adds its share of the chunks, one workgroup the
+// shares, both in an order that the group's sizes alone decide -- no atomics,
+// the same bits every run.  Bound by HBM: every gradient read once.  The factor
+// stays on the device, where the step multiplies by it (k_adamw_group.hip), so
+// that clipping costs no pass of its own.
+#include "rows.h"
+
+namespace seeai {
+namespace {
+
+constexpr int kThreads = 256, kPer = 8;
+static_assert(kThreads * kPer == kGradChunk, "a chunk is a workgroup's turn");
+
+__device__ __forceinline__ int TensorOf(const GradGroupTensor* tab, int count, uint64_t chunk) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (tab[mid].first_chunk <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Eight neighbours from element `at` on, zeros past the tensor.
+__device__ __forceinline__ void Load(const GradGroupTensor& T, uint64_t at, float (&v)[kPer]) {
+  const bool whole = T.vec && at + kPer <= T.n;
+  if (T.bf16) {
+    const uint16_t* g = static_cast<const uint16_t*>(T.g) + at;
+    if (whole) {
+      Io<uint16_t>::Load(g, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[e] = at + e < T.n ? Bf16ToF32(g[e]) : 0.0f;
+    }
+  } else {
+    const float* g = static_cast<const float*>(T.g) + at;
+    if (whole) {
+      Io<float>::Load(g, v);
+      Io<float>::Load(g + 4, v + 4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[e] = at + e < T.n ? g[e] : 0.0f;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+GradNormKernel(const GradGroupTensor* __restrict__ tab, int count, uint64_t chunks,
+               double* __restrict__ part) {
+  __shared__ double red[kThreads / kWave];
+  const uint64_t first = chunks * blockIdx.x / gridDim.x, last = chunks * (blockIdx.x + 1) / gridDim.x;
+  int i = TensorOf(tab, count, first);
+  GradGroupTensor T = tab[i];
+  double sq = 0.0;
+  for (uint64_t c = first; c < last; ++c) {
+    while (i + 1 < count && tab[i + 1].first_chunk <= c) T = tab[++i];
+    float v[kPer];
+    Load(T, (c - T.first_chunk) * kGradChunk + threadIdx.x * kPer, v);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sq += static_cast<double>(v[e]) * static_cast<double>(v[e]);
+  }
+  sq = BlockSumD<kThreads>(sq, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = sq;
+}
+
+constexpr int kFoldThreads = 1024;
+__global__ void __launch_bounds__(kFoldThreads)
+GradFactorKernel(const double* __restrict__ part, int n, float max_norm, float* __restrict__ norm,
+                 float* __restrict__ factor, int* __restrict__ flag) {
+  __shared__ double red[kFoldThreads / kWave];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kFoldThreads) s += part[i];
+  s = sqrt(BlockSumD<kFoldThreads>(s, red));
+  if (threadIdx.x != 0) return;
+  if (norm) *norm = static_cast<float>(s);
+  if (!(max_norm > 0.0f)) return;
+  const double cap = static_cast<double>(max_norm);
+  if (!isfinite(s)) *flag = 1;
+  *factor = isfinite(s) && s > cap ? static_cast<float>(cap / s) : 1.0f;
+}
+
+__global__ void __launch_bounds__(kThreads)
+GradScaleKernel(const GradGroupTensor* __restrict__ tab, int count, const float* __restrict__ factor,
+                const int* __restrict__ flag) {
+  const float f = *factor;
+  if (*flag || f == 1.0f) return;
+  const GradGroupTensor T = tab[TensorOf(tab, count, blockIdx.x)];
+  const uint64_t at = (blockIdx.x - T.first_chunk) * kGradChunk + threadIdx.x * kPer;
+  if (at >= T.n) return;
+  float v[kPer];
+  Load(T, at, v);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) v[e] *= f;
+  const bool whole = T.vec && at + kPer <= T.n;
+  if (T.bf16) {
+    uint16_t* g = static_cast<uint16_t*>(T.g) + at;
+    if (whole) {
+      Io<uint16_t>::Store(g, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (at + e < T.n) g[e] = F32ToBf16(v[e]);
+    }
+  } else {
+    float* g = static_cast<float*>(T.g) + at;
+    if (whole) {
+      Io<float>::Store(g, v);
+      Io<float>::Store(g + 4, v + 4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (at + e < T.n) g[e] = v[e];
+    }
+  }
+}
+
+}  // namespace
+
+int GradNormParts(uint64_t chunks) { return static_cast<int>(chunks < 2048 ? chunks : 2048); }
+
+hipError_t LaunchGradNorm(const GradGroupTensor* tab, int count, uint64_t chunks, double* part,
+                          float max_norm, float* norm, float* factor, int* flag, hipStream_t s) {
+  const int n = GradNormParts(chunks);
+  if (n) {
+    hipLaunchKernelGGL(GradNormKernel, dim3(n), dim3(kThreads), 0, s, tab, count, chunks, part);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(GradFactorKernel, dim3(1), dim3(kFoldThreads), 0, s, part, n, max_norm, norm,
+                     factor, flag);
+  return hipGetLastError();
+}
+
+hipError_t LaunchGradScale(const GradGroupTensor* tab, int count, uint64_t chunks,
+                           const float* factor, const int* flag, hipStream_t s) {
+  if (chunks == 0) return hipSuccess;
+  hipLaunchKernelGGL(GradScaleKernel, dim3(static_cast<unsigned>(chunks)), dim3(kThreads), 0, s, tab,
+                     count, factor, flag);
+  return hipGetLastError();
+}
+
+}  // namespace seeai

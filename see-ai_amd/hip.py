@@ -77,6 +77,27 @@ class AdamWTensor(C.Structure):
                 ("n", C.c_uint64), ("decay", C.c_float), ("reserved", C.c_uint32)]
 
 
+class GradTensor(C.Structure):
+    """seeai_grad_tensor: one tensor of a gradient group (device pointer)."""
+    _fields_ = [("g", C.c_void_p), ("n", C.c_uint64), ("dtype", C.c_int), ("reserved", C.c_uint32)]
+
+
+class BlockJoin(C.Structure):
+    """seeai_block_join: what stands between two blocks (device pointers; the
+    caller keeps their tensors alive)."""
+    _fields_ = [("o", C.c_void_p), ("x", C.c_void_p), ("post_w", C.c_void_p), ("post_b", C.c_void_p),
+                ("gate", C.c_void_p), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p),
+                ("rows", C.c_uint64), ("cols", C.c_uint64), ("gate_rows", C.c_uint64),
+                ("kind", C.c_int), ("dtype", C.c_int), ("res_scale", C.c_float), ("eps", C.c_float)]
+
+
+class BlockJoinGrads(C.Structure):
+    """seeai_block_join_grads: its gradients (device pointers)."""
+    _fields_ = [("dx", C.c_void_p), ("d_o", C.c_void_p), ("dpost_w", C.c_void_p),
+                ("dpost_b", C.c_void_p), ("dgate", C.c_void_p), ("dpre_w", C.c_void_p),
+                ("dpre_b", C.c_void_p)]
+
+
 # Every exported symbol with its ctypes signature: the header, one to one.
 EXPORTS = {
     "seeai_create": (_I, [_I, C.POINTER(_P)]),
@@ -145,6 +166,22 @@ EXPORTS = {
     "seeai_adamw_group_destroy": (None, [_P]),
     "seeai_adamw_group_step": (_I, [_P, C.POINTER(StepParams)]),
     "seeai_adamw_group_hold": (_I, [_P, C.POINTER(StepParams)]),
+    "seeai_adamw_group_step_scaled": (_I, [_P, C.POINTER(StepParams), _P]),
+    "seeai_grad_group_create": (_I, [_P, C.POINTER(GradTensor), _U64, C.POINTER(_P)]),
+    "seeai_grad_group_destroy": (None, [_P]),
+    "seeai_grad_group_norm": (_I, [_P, _F, _P, _P]),
+    "seeai_grad_group_scale": (_I, [_P, _P]),
+    "seeai_block_join_fwd": (_I, [_P, C.POINTER(BlockJoin), _P, _P, _P]),
+    "seeai_block_join_workspace": (_U64, [_U64, _U64, _U64]),
+    "seeai_block_join_bwd": (_I, [_P, C.POINTER(BlockJoin), _P, _P, _P, _P,
+                                  C.POINTER(BlockJoinGrads), _P, _U64]),
+    "seeai_token_logp_fwd": (_I, [_P, _I, _P, _U64, _P, _P, _P, _U64, _U64]),
+    "seeai_token_logp_bwd": (_I, [_P, _I, _P, _U64, _P, _P, _P, _P, _U64, _U64]),
+    "seeai_pref_workspace": (_U64, [_U64]),
+    "seeai_pref_loss": (_I, [_P, _P, _P, _P, _P, _U64, _U64, _F, _F, _F, _I, _F, _P, _P, _P, _P, _U64]),
+    "seeai_policy_workspace": (_U64, [_U64, _U64]),
+    "seeai_policy_loss": (_I, [_P, _I, _P, _U64, _P, _P, _P, _P, _P, _U64, _U64, _F, _F, _F, _F, _P, _P,
+                               _P, _P, _U64]),
     "seeai_adamw_state_values": (_I, [_P, _I, _I, _P, _P, _U64, _P]),
     "seeai_argmax_rows": (_I, [_P, _P, _U64, _U64, _P]),
     "seeai_argmax_tally": (_I, [_P, _P, _P, _U64, _U64, C.POINTER(_U64), C.POINTER(_U64)]),
@@ -336,9 +373,15 @@ class AdamWGroup:
             raise BackendError(INVALID, "the AdamW group or its context is closed")
         return self.h
 
-    def step(self, params: StepParams | None = None):
-        self.ctx.check(_lib.seeai_adamw_group_step(
-            self._live(), C.byref(params) if params is not None else None))
+    def step(self, params: StepParams | None = None, factor=None):
+        """One step; with ``factor`` (one f32 on the device) every gradient is
+        multiplied by it as it is read (GradGroup.norm's clip factor)."""
+        by = C.byref(params) if params is not None else None
+        if factor is None:
+            self.ctx.check(_lib.seeai_adamw_group_step(self._live(), by))
+        else:
+            _one_float("factor", factor, self.ctx)
+            self.ctx.check(_lib.seeai_adamw_group_step_scaled(self._live(), by, ptr(factor)))
 
     def hold(self, params: StepParams):
         self.ctx.check(_lib.seeai_adamw_group_hold(self._live(), C.byref(params)))
@@ -346,6 +389,73 @@ class AdamWGroup:
     def close(self):
         if self.h and self.ctx.h:
             _lib.seeai_adamw_group_destroy(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 -- interpreter shutdown
+            pass
+
+
+def _one_float(name, t, ctx):
+    """A device scalar of the context's device: one f32."""
+    index = getattr(getattr(t, "device", None), "index", None)
+    here = getattr(ctx, "device_index", None)
+    if (not t.is_cuda or t.numel() != 1 or str(getattr(t, "dtype", "float32")).removeprefix("torch.")
+            != "float32" or (here is not None and index not in (None, here))):
+        raise ValueError(f"{name}: one float32 on the context's device wanted")
+
+
+class GradGroup:
+    """The gradients of a step (seeai_grad_group_*): their global norm, and the
+    clip by it.
+
+    ``tensors``: contiguous device tensors, float32 and bfloat16 (or its bits in
+    16-bit integers) beside each other.  The group keeps them alive; the context
+    outlives it."""
+
+    _TYPES = {"float32": 0, "bfloat16": 1, "int16": 1, "uint16": 1}
+
+    def __init__(self, ctx: Context, tensors):
+        self.h, self.ctx, self.tensors = None, ctx, list(tensors)
+        table = (GradTensor * max(len(self.tensors), 1))()
+        here = getattr(ctx, "device_index", None)
+        for row, t in zip(table, self.tensors):
+            dtype = str(t.dtype).removeprefix("torch.")
+            if dtype not in self._TYPES:
+                raise ValueError(f"gradient: {' or '.join(self._TYPES)} wanted, not {dtype}")
+            if not t.is_cuda or not t.is_contiguous():
+                raise ValueError("gradient: a contiguous tensor on the device wanted")
+            if here is not None and getattr(getattr(t, "device", None), "index", here) != here:
+                raise ValueError(f"gradient: on device {t.device.index}, the context on device {here}")
+            row.g, row.n, row.dtype = ptr(t), t.numel(), self._TYPES[dtype]
+        h = _P()
+        ctx.call("seeai_grad_group_create", table, len(self.tensors), C.byref(h))
+        self.h = h
+
+    def _live(self):
+        if not self.h or not self.ctx.h:
+            raise BackendError(INVALID, "the gradient group or its context is closed")
+        return self.h
+
+    def norm(self, max_norm: float = 0.0, norm=None, factor=None):
+        """The gradients' 2-norm into ``norm`` and, with a ``max_norm``, the clip
+        factor min(1, max_norm / norm) into ``factor`` (one f32 each, on the
+        device)."""
+        for name, t in (("norm", norm), ("factor", factor)):
+            if t is not None:
+                _one_float(name, t, self.ctx)
+        self.ctx.check(_lib.seeai_grad_group_norm(self._live(), max_norm, ptr(norm), ptr(factor)))
+
+    def scale(self, factor):
+        """Every gradient times ``factor``, in place."""
+        _one_float("factor", factor, self.ctx)
+        self.ctx.check(_lib.seeai_grad_group_scale(self._live(), ptr(factor)))
+
+    def close(self):
+        if self.h and self.ctx.h:
+            _lib.seeai_grad_group_destroy(self.h)
         self.h = None
 
     def __del__(self):
