@@ -28,72 +28,233 @@
 namespace seeai {
 namespace {
 
+constexpr int kRsrcWord3 = 0x00020000;  // raw buffer, out-of-range reads give 0
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ u32x4 ReadBuffer(__amdgpu_buffer_rsrc_t rs, int byte) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, byte, 0, 0));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t Buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, kRsrcWord3);
+}
+
+__device__ __forceinline__ float UniformF(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
+// A row of T over kTPR threads, 16 bytes an access: lane t's group i holds the
+// kV columns from (i kTPR + t) kV on.  A row is its wave's own, so its address
+// is a scalar.  Rows on dwords (f32; bf16 of an even width) go through a buffer
+// range of exactly the row: a dword past it reads as zero and is not stored, each
+// dword by itself, so no access asks where the row ends.  Other bf16 rows
+// (kOff) are read 16 bytes at a time from wherever they lie; the row's last,
+// short group reads the row's last 16 bytes and is shifted into place, so its
+// load, too, can run ahead of its use.
+template <class T, int kTPR, int kE, bool kOff>
+struct Row {
+  static constexpr int kV = Io<T>::kV, kN = kE / kV;
+  u32x4 q[kN];
+  static __device__ __forceinline__ int Col(int t, int i) { return (i * kTPR + t) * kV; }
+  // here: the row's columns, or 0 for a row that is not there (zeros).
+  __device__ __forceinline__ void Load(const T* row, int t, int here) {
+    if constexpr (!kOff) {
+      const auto rs = Buffer(row, here * static_cast<int>(sizeof(T)));
+#pragma unroll
+      for (int i = 0; i < kN; ++i) q[i] = ReadBuffer(rs, Col(t, i) * static_cast<int>(sizeof(T)));
+    } else if (here >= kV) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int c = Col(t, i), last = here - kV;
+        q[i] = *reinterpret_cast<const u32x4u*>(row + (c < last ? c : last));
+      }
+    } else {  // fewer columns than a group, the first lane's
+#pragma unroll
+      for (int i = 0; i < kN; ++i) q[i] = u32x4{0, 0, 0, 0};
+      if (t == 0) {
+#pragma unroll
+        for (int c = 0; c < kV - 1; ++c)
+          if (c < here) q[0][c / 2] |= static_cast<uint32_t>(row[c]) << (16 * (c % 2));
+      }
+    }
+  }
+  __device__ __forceinline__ void Get(int t, int here, float (&v)[kE]) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      u32x4 w = q[i];
+      if constexpr (kOff) {
+        const int by = here >= kV ? Col(t, i) - (here - kV) : 0;  // elements to shift out
+        if (by & 4) w = u32x4{w[2], w[3], 0, 0};
+        if (by & 2) w = u32x4{w[1], w[2], w[3], 0};
+        if (by & 1)
+          w = u32x4{__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16),
+                    __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
+        if (by >= kV) w = u32x4{0, 0, 0, 0};
+        // (a group before the last: by is negative)
+        if (by <= 0) w = q[i];
+      }
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i * kV + k] = __uint_as_float(w[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[i * kV + 2 * k] = __uint_as_float(w[k] << 16);
+          v[i * kV + 2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void Store(T* row, int t, int cols, const float (&v)[kE]) {
+    const auto rs = Buffer(row, cols * static_cast<int>(sizeof(T)));
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = Col(t, i);
+      const float* at = v + i * kV;
+      if constexpr (kOff) {
+        if (c + kV <= cols) {
+          Io<T>::StoreAny(row + c, at);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kV; ++k)
+            if (c + k < cols) Io<T>::Put(row + c + k, at[k]);
+        }
+      } else if constexpr (sizeof(T) == 4) {
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4{__float_as_uint(at[0]), __float_as_uint(at[1]), __float_as_uint(at[2]), __float_as_uint(at[3])},
+            rs, c * 4, 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, Io<uint16_t>::Pack(at)), rs, c * 2, 0, 0);
+      }
+    }
+  }
+};
+
+// The f32 vector at the same columns, zeros past it.
+template <class T, int kTPR, int kE>
+__device__ __forceinline__ void Vector(const float* w, int t, int cols, float (&v)[kE]) {
+  const auto rs = Buffer(w, cols * 4);
+#pragma unroll
+  for (int e = 0; e < kE; e += 4) {
+    const u32x4 x = ReadBuffer(rs, ColOf<T, kTPR, true>(t, e) * 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[e + k] = __uint_as_float(x[k]);
+  }
+}
+
+template <class T, int kTPR, int kE>
+__device__ __forceinline__ void StoreVector(float* w, int t, int cols, const float (&v)[kE]) {
+  const auto rs = Buffer(w, cols * 4);
+#pragma unroll
+  for (int e = 0; e < kE; e += 4)
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v[e]), __float_as_uint(v[e + 1]),
+                                                 __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3])},
+                                           rs, ColOf<T, kTPR, true>(t, e) * 4, 0, 0);
+}
+
 constexpr int FwdThreads(int tpr) { return tpr > 256 ? tpr : 256; }
-constexpr int BwdThreads(int tpr) { return tpr > 512 ? tpr : 512; }
+// The backward's workgroup, one a CU: few bands, and few sums for the fold.
+constexpr int kBwdThreads = 1024;
+
+// Sum over the wave's lanes by lane moves within registers; all lanes get it.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ float MoveAdd(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, kRows, 0xf, false));
+}
+__device__ __forceinline__ float LaneSum(float v) {
+  v = MoveAdd<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8 within rows of 16
+  v = MoveAdd<0x112, 0xf>(v);
+  v = MoveAdd<0x114, 0xf>(v);
+  v = MoveAdd<0x118, 0xf>(v);
+  v = MoveAdd<0x142, 0xa>(v);  // lane 15 of a row to the next row
+  v = MoveAdd<0x143, 0xc>(v);  // lane 31 to the upper half
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+// Two sums over the kTPR threads of each row; `lds` [2][2 x 16], used in turn,
+// so that one barrier keeps a sum's reads from the next one's writes.
+template <int kTPR>
+__device__ __forceinline__ float2 RowSum2(float a, float b, float* lds, int& turn) {
+  a = LaneSum(a), b = LaneSum(b);
+  if constexpr (kTPR > kWave) {
+    constexpr int kWaves = kTPR / kWave;
+    const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
+    float* at = lds + 32 * turn;
+    turn ^= 1;
+    if (threadIdx.x % kWave == 0) at[2 * w] = a, at[2 * w + 1] = b;
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) a += at[2 * (first + k)], b += at[2 * (first + k) + 1];
+  }
+  return make_float2(a, b);
+}
 
 // v normalised in place; its mean and 1 / deviation.
-template <class T, int kTPR, int kE, bool kVec>
+template <class T, int kTPR, int kE>
 __device__ __forceinline__ float2 Normalise(float (&v)[kE], int rms, int t, int cols, float eps,
-                                            float* lds) {
-  float mu[1] = {0.0f}, sq[1] = {0.0f};
+                                            float* lds, int& turn) {
+  float mu = 0.0f, sq = 0.0f;
   if (!rms) {
 #pragma unroll
-    for (int e = 0; e < kE; ++e) mu[0] += v[e];
-    RowSum<kTPR>(mu, lds);
-    mu[0] /= static_cast<float>(cols);
+    for (int e = 0; e < kE; ++e) mu += v[e];
+    mu = RowSum2<kTPR>(mu, 0.0f, lds, turn).x / static_cast<float>(cols);
 #pragma unroll
-    for (int e = 0; e < kE; ++e) v[e] = ColOf<T, kTPR, kVec>(t, e) < cols ? v[e] - mu[0] : 0.0f;
+    for (int e = 0; e < kE; ++e) v[e] = ColOf<T, kTPR, true>(t, e) < cols ? v[e] - mu : 0.0f;
   }
 #pragma unroll
-  for (int e = 0; e < kE; ++e) sq[0] += v[e] * v[e];
-  RowSum<kTPR>(sq, lds);
-  const float rs = 1.0f / sqrtf(sq[0] / static_cast<float>(cols) + eps);
+  for (int e = 0; e < kE; ++e) sq += v[e] * v[e];
+  sq = RowSum2<kTPR>(sq, 0.0f, lds, turn).x;
+  const float rs = 1.0f / sqrtf(sq / static_cast<float>(cols) + eps);
 #pragma unroll
   for (int e = 0; e < kE; ++e) v[e] *= rs;
-  return make_float2(mu[0], rs);
+  return make_float2(mu, rs);
 }
 
 // v = v w + b (b null: without).
-template <class T, int kTPR, int kE, bool kVec, bool kAny>
+template <class T, int kTPR, int kE>
 __device__ __forceinline__ void Scale(float (&v)[kE], const float* w, const float* b, int t, int cols) {
   float u[kE];
-  LoadVec<T, kTPR, kE, kVec, kAny>(w, t, cols, u);
+  Vector<T, kTPR, kE>(w, t, cols, u);
 #pragma unroll
   for (int e = 0; e < kE; ++e) v[e] *= u[e];
   if (!b) return;
-  LoadVec<T, kTPR, kE, kVec, kAny>(b, t, cols, u);
+  Vector<T, kTPR, kE>(b, t, cols, u);
 #pragma unroll
   for (int e = 0; e < kE; ++e) v[e] += u[e];
 }
 
-template <class T, int kTPR, int kE, bool kVec, bool kAny>
+template <class T, int kTPR, int kE, bool kOff>
 __global__ void __launch_bounds__(FwdThreads(kTPR))
 JoinFwdKernel(JoinArgs a) {
-  __shared__ float lds[16];
+  using R = Row<T, kTPR, kE, kOff>;
+  __shared__ float lds[64];
   constexpr int kRows = FwdThreads(kTPR) / kTPR;
-  const int t = threadIdx.x % kTPR, cols = static_cast<int>(a.cols);
+  const int t = threadIdx.x % kTPR, sub = Uniform(threadIdx.x / kTPR), cols = static_cast<int>(a.cols);
+  int turn = 0;
   // (the loop is uniform over the workgroup, its barriers too)
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < a.rows;
        base += static_cast<size_t>(gridDim.x) * kRows) {
-    const size_t r = base + threadIdx.x / kTPR;
+    const size_t r = base + sub, off = r * cols;
     const bool in = r < a.rows;
     const int here = in ? cols : 0;
+    R ro, rx;
+    ro.Load(static_cast<const T*>(a.o) + off, t, here);
+    rx.Load(static_cast<const T*>(a.x) + off, t, here);
     float v[kE], x[kE];
-    LoadRow<T, kTPR, kE, kVec, kAny>(static_cast<const T*>(a.o) + r * cols, t, here, v);
-    LoadRow<T, kTPR, kE, kVec, kAny>(static_cast<const T*>(a.x) + r * cols, t, here, x);
+    ro.Get(t, here, v);
     float2 so = make_float2(0.0f, 0.0f), sy = so;
     if (a.post_w) {
-      so = Normalise<T, kTPR, kE, kVec>(v, a.rms, t, cols, a.eps, lds);
-      Scale<T, kTPR, kE, kVec, kAny>(v, a.post_w, a.post_b, t, cols);
+      so = Normalise<T, kTPR, kE>(v, a.rms, t, cols, a.eps, lds, turn);
+      Scale<T, kTPR, kE>(v, a.post_w, a.post_b, t, cols);
     }
-    if (a.gate) Scale<T, kTPR, kE, kVec, kAny>(v, a.gate + (in ? r : 0) / a.gate_rows * cols, nullptr, t, cols);
+    if (a.gate) Scale<T, kTPR, kE>(v, a.gate + (in ? r : 0) / a.gate_rows * cols, nullptr, t, cols);
+    rx.Get(t, here, x);
 #pragma unroll
     for (int e = 0; e < kE; ++e) v[e] = a.res * x[e] + v[e];
-    if (in) StoreRow<T, kTPR, kE, kVec, kAny>(static_cast<T*>(a.y) + r * cols, t, cols, v);
+    if (in) R::Store(static_cast<T*>(a.y) + off, t, cols, v);
     if (a.pre_w) {
-      sy = Normalise<T, kTPR, kE, kVec>(v, a.rms, t, cols, a.eps, lds);
-      Scale<T, kTPR, kE, kVec, kAny>(v, a.pre_w, a.pre_b, t, cols);
-      if (in) StoreRow<T, kTPR, kE, kVec, kAny>(static_cast<T*>(a.h) + r * cols, t, cols, v);
+      sy = Normalise<T, kTPR, kE>(v, a.rms, t, cols, a.eps, lds, turn);
+      Scale<T, kTPR, kE>(v, a.pre_w, a.pre_b, t, cols);
+      if (in) R::Store(static_cast<T*>(a.h) + off, t, cols, v);
     }
     if (in && t == 0 && a.stats) {
       float* s = a.stats + 4 * r;
@@ -105,173 +266,246 @@ JoinFwdKernel(JoinArgs a) {
 // How the rows are shared out: `bands` of `len` rows, `per` to a gate, or of
 // `gates` whole gates' rows.
 struct Plan {
-  size_t bands, len, per, gates;
+  unsigned bands, per;
+  size_t len, gates;
 };
 // A row's threads, for rows of `cols`.
 int RowThreads(size_t cols) {
   return cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
 }
-constexpr size_t kBands = 512;
+constexpr size_t kBands = 256;
 Plan PlanOf(size_t rows, size_t cols, size_t gate_rows) {
-  if (rows == 0) return {1, 0, 1, 0};  // sums of zero
-  const int tpr = RowThreads(cols), threads = BwdThreads(tpr);
-  const size_t slots = static_cast<size_t>(threads / tpr), turns = (rows + slots - 1) / slots;
-  const size_t most = threads > 512 || turns < 4 * kBands ? kBands / 2 : kBands;
+  if (rows == 0) return {1, 1, 0, 0};  // sums of zero
+  const size_t slots = static_cast<size_t>(kBwdThreads / RowThreads(cols));
   const auto whole = [&](size_t n) { return (n + slots - 1) / slots * slots; };
-  size_t len = whole((rows + most - 1) / most);
+  size_t len = whole((rows + kBands - 1) / kBands);
   const size_t gr = gate_rows == 0 || gate_rows > rows ? rows : gate_rows, groups = (rows + gr - 1) / gr;
   if (gr < len) {
     const size_t k = len / gr;
-    return {(groups + k - 1) / k, k * gr, 1, k};
+    return {static_cast<unsigned>((groups + k - 1) / k), 1, k * gr, k};
   }
   const size_t per = (gr + len - 1) / len;
   len = whole((gr + per - 1) / per);
-  return {groups * per, len, per, 0};
+  return {static_cast<unsigned>(groups * per), static_cast<unsigned>(per), len, 0};
 }
 
 // bands' sums: [bands][4][cols]: dw', db', S1 and S0 (or dw and db where a
 // band's gates are whole), or the gradients themselves where there is one band.
-template <class T, int kTPR, int kE, bool kVec>
-__global__ void __launch_bounds__(BwdThreads(kTPR), BwdThreads(kTPR) / 256)
+// A row's loads go out while the row before it is reduced (kAhead).
+template <class T, int kTPR, int kE, bool kOff, bool kRms>
+__global__ void __launch_bounds__(kBwdThreads, kBwdThreads / 256)
 JoinBwdKernel(JoinArgs a, Plan plan) {
-  constexpr int kRows = BwdThreads(kTPR) / kTPR;
-  __shared__ float lds[32];
-  __shared__ float own[kRows > 1 ? kTPR * kE : 4];  // element e of thread t at ((e / 4) kTPR + t) 4 + e % 4
-  const int t = threadIdx.x % kTPR, sub = threadIdx.x / kTPR, cols = static_cast<int>(a.cols);
+  using R = Row<T, kTPR, kE, kOff>;
+  constexpr int kRows = kBwdThreads / kTPR;
+  constexpr bool kAhead = kE == 8;  // (with 16 the registers are full)
+  __shared__ float lds[64];
+  // Element e of thread t at ((e / 4) kTPR + t) 4 + e % 4: w', and gate w.
+  __shared__ float wpre[kTPR * kE], wpost[kTPR * kE];
+  const int t = threadIdx.x % kTPR, sub = Uniform(threadIdx.x / kTPR), cols = static_cast<int>(a.cols);
+  const auto slot = [&](int e) { return (e / 4 * kTPR + t) * 4 + e % 4; };
   const float inv = 1.0f / static_cast<float>(cols);
-  const bool pre = a.pre_w != nullptr, post = a.post_w != nullptr;
+  const bool pre = a.pre_w != nullptr, post = a.post_w != nullptr, tail = post || a.gate;
   const size_t all = a.rows ? a.rows : 1, gr = !a.gate || a.gate_rows > all ? all : a.gate_rows;
   const bool whole = plan.gates > 0;  // whole gates in a band
+  int turn = 0;
   // This band's rows.
   size_t first, last;
   if (whole) {
     first = blockIdx.x * plan.len, last = first + plan.len;
   } else {
-    const size_t g = blockIdx.x / plan.per, k = blockIdx.x % plan.per;
+    const unsigned g = blockIdx.x / plan.per, k = blockIdx.x % plan.per;
     first = g * gr + k * plan.len;
     last = first + plan.len < (g + 1) * gr ? first + plan.len : (g + 1) * gr;
   }
   if (last > a.rows) last = a.rows;
   // The row groups' sums add up in order; the last group holds them.
-  auto join = [&](float (&s)[kE]) {
+  auto join = [&](float (&s)[kE], float* own) {
     if constexpr (kRows > 1) {
       for (int g = 0; g < kRows; ++g) {
         __syncthreads();
         if (sub == g) {
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            float* at = own + (e / 4 * kTPR + t) * 4 + e % 4;
-            if (g > 0) s[e] = *at + s[e];
-            *at = s[e];
+            if (g > 0) s[e] = own[slot(e)] + s[e];
+            own[slot(e)] = s[e];
           }
         }
       }
     }
   };
+  auto four = [&](const float* own, int e, float (&w)[4]) {  // from column e on
+    const float4 q = *reinterpret_cast<const float4*>(own + slot(e));
+    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+  };
   float* part = a.part + static_cast<size_t>(blockIdx.x) * 4 * cols;
   const bool one = gridDim.x == 1;
-  float pw[kE], pb[kE];
+  float pw[kE], pb[kRms ? 1 : kE];
 #pragma unroll
-  for (int e = 0; e < kE; ++e) pw[e] = pb[e] = 0.0f;
+  for (int e = 0; e < kE; ++e) pw[e] = 0.0f;
+  if constexpr (!kRms) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) pb[e] = 0.0f;
+  }
+  R rh, ry, ro, rd;
+  float4 st;
+  size_t base = first;
+  auto fetch = [&](size_t end) {  // (past the gate's last row: zeros, which add nothing)
+    const size_t r = base + sub, off = r * cols;
+    const int here = r < end ? cols : 0;
+    rh.Load(static_cast<const T*>(a.dh) + off, t, pre ? here : 0);
+    ry.Load(static_cast<const T*>(a.y) + off, t, pre ? here : 0);
+    rd.Load(static_cast<const T*>(a.dy) + off, t, a.dy ? here : 0);
+    ro.Load(static_cast<const T*>(a.o) + off, t, tail ? here : 0);
+    st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (here) {
+      const float* s = a.stats + 4 * r;
+      st = make_float4(s[0], s[1], s[2], s[3]);
+    }
+  };
+  if (pre && sub == 0) {
+    float v[kE];
+    Vector<T, kTPR, kE>(a.pre_w, t, cols, v);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) wpre[slot(e)] = v[e];
+  }
   for (size_t at = first;;) {  // a gate's rows in this band (at least one turn: no rows, sums of zero)
     const size_t g = at / gr, end = whole && (g + 1) * gr < last ? (g + 1) * gr : last;
     const float* gate = a.gate && at < a.rows ? a.gate + g * cols : nullptr;
-    float s1[kE], s0[kE];
+    base = at;
+    if constexpr (kAhead) fetch(end);
+    __syncthreads();  // (the gate before has been read)
+    if (sub == 0) {
+      float v[kE], u[kE];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) s1[e] = s0[e] = 0.0f;
-    for (size_t base = at; base < end; base += kRows) {  // (uniform over the workgroup, its barriers too)
-      const size_t r = base + sub;
+      for (int e = 0; e < kE; ++e) v[e] = u[e] = 1.0f;
+      if (post) Vector<T, kTPR, kE>(a.post_w, t, cols, v);
+      if (gate) Vector<T, kTPR, kE>(gate, t, cols, u);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) wpost[slot(e)] = v[e] * u[e];
+    }
+    __syncthreads();
+    float s1[kE], s0[kRms ? 1 : kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) s1[e] = 0.0f;
+    if constexpr (!kRms) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) s0[e] = 0.0f;
+    }
+    while (base < end) {  // (uniform over the workgroup, its barriers too)
+      const size_t r = base + sub, off = r * cols;
       const bool in = r < end;
       const int here = in ? cols : 0;
-      const size_t off = r * cols;
-      float d[kE], v[kE], w[kE];
-      float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (in) {
-        const float* s = a.stats + 4 * r;
-        st = make_float4(s[0], s[1], s[2], s[3]);
-      }
-#pragma unroll
-      for (int e = 0; e < kE; ++e) d[e] = 0.0f;
+      if constexpr (!kAhead) fetch(end);
+      const float4 q = make_float4(UniformF(st.x), UniformF(st.y), UniformF(st.z), UniformF(st.w));
+      float d[kE], v[kE];
+      const R md = rd, mo = ro;
+      rh.Get(t, pre ? here : 0, d);
+      ry.Get(t, pre ? here : 0, v);
+      base += kRows;
+      if constexpr (kAhead) fetch(end);
       if (pre) {
-        float s[2] = {0.0f, 0.0f};
-        LoadRow<T, kTPR, kE, kVec>(static_cast<const T*>(a.dh) + off, t, here, d);
-        LoadRow<T, kTPR, kE, kVec>(static_cast<const T*>(a.y) + off, t, here, v);
-        LoadVec<T, kTPR, kE, kVec>(a.pre_w, t, cols, w);
-        const float mu = a.rms ? 0.0f : st.z;
+        float c1 = 0.0f, c2 = 0.0f;
+        const float mu = kRms ? 0.0f : q.z;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {  // (columns past the row: d = 0, so no term)
-          v[e] = (v[e] - mu) * st.w;
-          pw[e] += d[e] * v[e];
-          pb[e] += d[e];
-          d[e] *= w[e];
-          s[0] += d[e];
-          s[1] += d[e] * v[e];
+        for (int e = 0; e < kE; e += 4) {  // (columns past the row: d = 0, so no term)
+          float ww[4];
+          four(wpre, e, ww);
+#pragma unroll
+          for (int i = e; i < e + 4; ++i) {
+            v[i] = (v[i] - mu) * q.w;
+            pw[i] += d[i] * v[i];
+            if constexpr (!kRms) pb[i] += d[i];
+            d[i] *= ww[i - e];
+            c1 += d[i];
+            c2 += d[i] * v[i];
+          }
         }
-        RowSum<kTPR>(s, lds);
-        const float c1 = a.rms ? 0.0f : s[0] * inv, c2 = s[1] * inv;
+        const float2 c = RowSum2<kTPR>(c1, c2, lds, turn);
+        c1 = kRms ? 0.0f : c.x * inv, c2 = c.y * inv;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) d[e] = ColOf<T, kTPR, kVec>(t, e) < here ? st.w * (d[e] - c1 - v[e] * c2) : 0.0f;
+        for (int e = 0; e < kE; ++e) {
+          d[e] = q.w * (d[e] - c1 - v[e] * c2);
+          // (a layer norm's columns past the row would hold its mean's part)
+          if (!kRms && ColOf<T, kTPR, true>(t, e) >= cols) d[e] = 0.0f;
+        }
       }
-      if (a.dy) {
-        LoadRow<T, kTPR, kE, kVec>(static_cast<const T*>(a.dy) + off, t, here, v);
+      md.Get(t, a.dy ? here : 0, v);
 #pragma unroll
-        for (int e = 0; e < kE; ++e) d[e] += v[e];
-      }
+      for (int e = 0; e < kE; ++e) d[e] += v[e];
 #pragma unroll
       for (int e = 0; e < kE; ++e) v[e] = a.res * d[e];
-      if (in) StoreRow<T, kTPR, kE, kVec>(static_cast<T*>(a.dx) + off, t, cols, v);
-      if (post || gate) {
-        LoadRow<T, kTPR, kE, kVec>(static_cast<const T*>(a.o) + off, t, here, v);
+      if (in) R::Store(static_cast<T*>(a.dx) + off, t, cols, v);
+      if (tail) {
+        mo.Get(t, here, v);
         if (post) {
-          const float mu = a.rms ? 0.0f : st.x;
+          const float mu = kRms ? 0.0f : q.x;
 #pragma unroll
-          for (int e = 0; e < kE; ++e) v[e] = (v[e] - mu) * st.y;
+          for (int e = 0; e < kE; ++e) v[e] = (v[e] - mu) * q.y;
         }
+        float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) s1[e] += d[e] * v[e], s0[e] += d[e];
-      }
-      if (gate) {
-        LoadVec<T, kTPR, kE, kVec>(gate, t, cols, w);
+        for (int e = 0; e < kE; e += 4) {
+          float ww[4];
+          four(wpost, e, ww);
 #pragma unroll
-        for (int e = 0; e < kE; ++e) d[e] *= w[e];
-      }
-      if (post) {
-        float s[2] = {0.0f, 0.0f};
-        LoadVec<T, kTPR, kE, kVec>(a.post_w, t, cols, w);
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          d[e] *= w[e];
-          s[0] += d[e];
-          s[1] += d[e] * v[e];
-        }
-        RowSum<kTPR>(s, lds);
-        const float c1 = a.rms ? 0.0f : s[0] * inv, c2 = s[1] * inv;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) d[e] = st.y * (d[e] - c1 - v[e] * c2);
-      }
-      if (in) StoreRow<T, kTPR, kE, kVec>(static_cast<T*>(a.d_o) + off, t, cols, d);
-    }
-    if (post || gate) {
-      join(s1);
-      join(s0);
-      if (sub == kRows - 1) {
-        const bool mine = whole || plan.per == 1;  // all of the gate's rows
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const int c = ColOf<T, kTPR, kVec>(t, e);
-          if (c >= cols) continue;
-          if (a.dgate && mine && at < a.rows)
-            a.dgate[g * cols + c] = post ? a.post_w[c] * s1[e] + (a.post_b ? a.post_b[c] * s0[e] : 0.0f) : s1[e];
-          if (whole || one) {
-            const float by = gate ? gate[c] : 1.0f;
-            float* ow = one ? a.dpost_w : part + 2 * cols;
-            float* ob = one ? a.dpost_b : part + 3 * cols;
-            if (post) ow[c] = by * s1[e] + (at == first ? 0.0f : ow[c]);
-            if (post && a.dpost_b) ob[c] = by * s0[e] + (at == first ? 0.0f : ob[c]);
-          } else {
-            part[2 * cols + c] = s1[e];
-            part[3 * cols + c] = s0[e];
+          for (int i = e; i < e + 4; ++i) {
+            s1[i] += d[i] * v[i];
+            if constexpr (!kRms) s0[i] += d[i];
+            d[i] *= ww[i - e];
+            c1 += d[i];
+            c2 += d[i] * v[i];
           }
+        }
+        if (post) {
+          const float2 c = RowSum2<kTPR>(c1, c2, lds, turn);
+          c1 = kRms ? 0.0f : c.x * inv, c2 = c.y * inv;
+#pragma unroll
+          for (int e = 0; e < kE; ++e) d[e] = q.y * (d[e] - c1 - v[e] * c2);
+        }
+      }
+      if (in) R::Store(static_cast<T*>(a.d_o) + off, t, cols, d);
+    }
+    if (tail) {
+      // (the gate's product has been read by every row group behind a barrier)
+      join(s1, wpost);
+      if constexpr (!kRms) join(s0, wpost);
+      if (sub == kRows - 1) {
+        float v[kE], u[kE];
+        if (a.dgate && (whole || plan.per == 1) && at < a.rows) {  // all of the gate's rows are here
+          if (post) {
+            Vector<T, kTPR, kE>(a.post_w, t, cols, v);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) v[e] *= s1[e];
+            if constexpr (!kRms) {
+              if (a.post_b) {
+                Vector<T, kTPR, kE>(a.post_b, t, cols, u);
+#pragma unroll
+                for (int e = 0; e < kE; ++e) v[e] += u[e] * s0[e];
+              }
+            }
+            StoreVector<T, kTPR, kE>(a.dgate + g * cols, t, cols, v);
+          } else {
+            StoreVector<T, kTPR, kE>(a.dgate + g * cols, t, cols, s1);
+          }
+        }
+        if (whole || one) {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) v[e] = 1.0f;
+          if (gate) Vector<T, kTPR, kE>(gate, t, cols, v);
+          auto add = [&](float* to, const auto& s) {  // onto the gates' before
+#pragma unroll
+            for (int e = 0; e < kE; ++e) u[e] = 0.0f;
+            if (at != first) Vector<T, kTPR, kE>(to, t, cols, u);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) u[e] += v[e] * s[e];
+            StoreVector<T, kTPR, kE>(to, t, cols, u);
+          };
+          if (post) add(one ? a.dpost_w : part + 2 * cols, s1);
+          if constexpr (!kRms)
+            if (a.dpost_b) add(one ? a.dpost_b : part + 3 * cols, s0);
+        } else {
+          StoreVector<T, kTPR, kE>(part + 2 * cols, t, cols, s1);
+          if constexpr (!kRms) StoreVector<T, kTPR, kE>(part + 3 * cols, t, cols, s0);
         }
       }
     }
@@ -279,107 +513,122 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
     if (!whole || at >= last) break;
   }
   if (pre) {
-    join(pw);
-    join(pb);
+    join(pw, wpre);
+    if constexpr (!kRms) join(pb, wpre);
     if (sub == kRows - 1) {
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const int c = ColOf<T, kTPR, kVec>(t, e);
-        if (c >= cols) continue;
-        (one ? a.dpre_w : part)[c] = pw[e];
-        if (a.dpre_b) (one ? a.dpre_b : part + cols)[c] = pb[e];
-      }
+      StoreVector<T, kTPR, kE>(one ? a.dpre_w : part, t, cols, pw);
+      if constexpr (!kRms)
+        if (a.dpre_b) StoreVector<T, kTPR, kE>(one ? a.dpre_b : part + cols, t, cols, pb);
     }
   }
 }
 
-// The bands' sums, 32 columns a workgroup, eight threads a column, each over
-// every eighth band, joined in order.  blockIdx.y: 0 dw', 1 db', 2 dw, 3 db,
-// 4 + g gate g.
-constexpr int kFoldCols = 32, kFoldParts = 8;
+// The bands' sums, 32 columns a workgroup, 32 threads a column, each over every
+// 32nd band, joined in order.  blockIdx.y, of what there is: the norm before the
+// next block's gradients; the norm after the block's, and the gate's where there
+// is one for all rows; every other gate's.
+constexpr int kFoldCols = 32, kFoldParts = 32;
 __global__ void __launch_bounds__(kFoldCols * kFoldParts)
-JoinFoldKernel(JoinArgs a, Plan plan) {
-  __shared__ float lds[2][kFoldParts][kFoldCols];
+JoinFoldKernel(JoinArgs a, Plan plan, unsigned gates) {
+  __shared__ float lds[2][kFoldParts][kFoldCols + 1];
   const int i = threadIdx.x % kFoldCols, k = threadIdx.x / kFoldCols;
   const size_t cols = a.cols, c = static_cast<size_t>(blockIdx.x) * kFoldCols + i;
-  const unsigned job = blockIdx.y;
-  float* out = job == 0 ? a.dpre_w : job == 1 ? a.dpre_b : job == 2 ? a.dpost_w : job == 3 ? a.dpost_b
-                                                                              : a.dgate;
-  if (!out) return;  // (uniform)
-  const bool by_gate = (job == 2 || job == 3) && a.gate && plan.gates == 0;
-  const size_t b0 = job >= 4 ? (job - 4) * plan.per : 0, b1 = job >= 4 ? b0 + plan.per : plan.bands;
-  const float* row = a.part + (job >= 4 ? 2 : job) * cols + c;
-  float s = 0.0f, s0 = 0.0f;
+  unsigned job = blockIdx.y + (a.pre_w ? 0 : 1);
+  if (job > 0 && !a.post_w && !(a.dgate && gates == 1)) ++job;
+  const unsigned g = job - 2;  // from job 2 on
+  const unsigned b0 = job < 2 ? 0 : g * plan.per, b1 = job < 2 ? plan.bands : b0 + plan.per;
+  // A band's sums count as its gate times them where its gate is one of several.
+  const bool weigh = job == 1 && a.gate && plan.gates == 0 && gates > 1;
+  const float* row = a.part + (job == 0 ? 0 : 2) * cols + c;
+  const bool both = !a.rms && (job == 0 ? a.dpre_b != nullptr : a.post_b != nullptr);
+  float s = 0.0f, z = 0.0f;
   if (c < cols) {
+    unsigned at = plan.per > 1 ? k % plan.per : 0, of = k / plan.per;  // the band within its gate, the gate
 #pragma unroll 8
-    for (size_t b = b0 + k; b < b1; b += kFoldParts) {
-      const float v = row[b * 4 * cols];
-      s += by_gate ? a.gate[b / plan.per * cols + c] * v : v;
-      if (job >= 4 && a.post_b) s0 += row[(b * 4 + 1) * cols];
+    for (unsigned b = b0 + k; b < b1; b += kFoldParts) {
+      const size_t off = static_cast<size_t>(b) * 4 * cols;
+      float v = row[off], u = both ? row[off + cols] : 0.0f;
+      if (weigh) {
+        const float by = a.gate[of * cols + c];
+        v *= by, u *= by;
+        for (at += kFoldParts; at >= plan.per; at -= plan.per) ++of;
+      }
+      s += v, z += u;
     }
   }
-  lds[0][k][i] = s, lds[1][k][i] = s0;
+  lds[0][k][i] = s, lds[1][k][i] = z;
+  __syncthreads();
+  // Eight threads a column join four parts each, then one the eight.
+  if (k < 8) {
+#pragma unroll
+    for (int j = 8; j < kFoldParts; j += 8) s += lds[0][k + j][i], z += lds[1][k + j][i];
+    lds[0][k][i] = s, lds[1][k][i] = z;
+  }
   __syncthreads();
   if (k != 0 || c >= cols) return;
 #pragma unroll
-  for (int j = 1; j < kFoldParts; ++j) s += lds[0][j][i], s0 += lds[1][j][i];
-  if (job < 4) {
-    out[c] = s;
-  } else {
-    out[(job - 4) * cols + c] = a.post_w ? a.post_w[c] * s + (a.post_b ? a.post_b[c] * s0 : 0.0f) : s;
+  for (int j = 1; j < 8; ++j) s += lds[0][j][i], z += lds[1][j][i];
+  if (job == 0) {
+    a.dpre_w[c] = s;
+    if (a.dpre_b) a.dpre_b[c] = z;
+    return;
   }
+  const float gate = a.gate && gates == 1 && plan.gates == 0 ? a.gate[c] : 1.0f;
+  if (job == 1 && a.post_w) {
+    a.dpost_w[c] = gate * s;
+    if (a.dpost_b) a.dpost_b[c] = gate * z;
+  }
+  if (a.dgate && (job > 1 || (gates == 1 && plan.gates == 0)))
+    a.dgate[(job > 1 ? g : 0) * cols + c] = a.post_w ? a.post_w[c] * s + (a.post_b ? a.post_b[c] * z : 0.0f) : s;
 }
 
 dim3 Grid(size_t groups) {  // a launch's workgroups (the kernels walk the rows past them)
   return dim3(static_cast<unsigned>(groups < (1u << 20) ? groups : 1u << 20));
 }
 
-template <class T, int kTPR, int kE, bool kVec, bool kAny>
+template <class T, int kTPR, int kE, bool kOff>
 hipError_t Run(const JoinArgs& a, bool bwd, hipStream_t s) {
-  if (kAny || !bwd) {  // (kAny: Dispatch asks for the forward alone)
+  if (!bwd) {
     constexpr int kThreads = FwdThreads(kTPR), kRows = kThreads / kTPR;
-    hipLaunchKernelGGL((JoinFwdKernel<T, kTPR, kE, kVec, kAny>), Grid((a.rows + kRows - 1) / kRows),
+    hipLaunchKernelGGL((JoinFwdKernel<T, kTPR, kE, kOff>), Grid((a.rows + kRows - 1) / kRows),
                        dim3(kThreads), 0, s, a);
     return hipGetLastError();
   }
   const Plan plan = PlanOf(a.rows, a.cols, a.gate ? a.gate_rows : 0);
-  hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kVec>), dim3(static_cast<unsigned>(plan.bands)),
-                     dim3(BwdThreads(kTPR)), 0, s, a, plan);
+  if (a.rms)
+    hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, true>), dim3(plan.bands), dim3(kBwdThreads), 0, s, a, plan);
+  else
+    hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, false>), dim3(plan.bands), dim3(kBwdThreads), 0, s, a, plan);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || plan.bands == 1) return e;
-  if (!a.pre_w && !a.post_w && !(a.dgate && plan.per > 1)) return hipSuccess;
-  const size_t gates = a.dgate && plan.per > 1 ? plan.bands / plan.per : 0;
+  // Gates whose rows lie in several bands.
+  const unsigned gates = a.gate && plan.gates == 0 ? plan.bands / plan.per : 0;
+  const unsigned shared = a.dgate && plan.per > 1 ? gates : 0;
+  const unsigned jobs = (a.pre_w ? 1 : 0) + (a.post_w || shared == 1 ? 1 : 0) + (shared > 1 ? shared : 0);
+  if (jobs == 0) return hipSuccess;
   hipLaunchKernelGGL(JoinFoldKernel,
-                     dim3(static_cast<unsigned>((a.cols + kFoldCols - 1) / kFoldCols),
-                          static_cast<unsigned>(4 + gates)),
-                     dim3(kFoldCols * kFoldParts), 0, s, a, plan);
+                     dim3(static_cast<unsigned>((a.cols + kFoldCols - 1) / kFoldCols), jobs),
+                     dim3(kFoldCols * kFoldParts), 0, s, a, plan, gates);
   return hipGetLastError();
 }
 
-template <class T, bool kVec, bool kAny>
+template <class T, bool kOff>
 hipError_t Pick(const JoinArgs& a, bool bwd, hipStream_t s) {
   switch (RowThreads(a.cols)) {
-    case 64: return Run<T, 64, 8, kVec, kAny>(a, bwd, s);
-    case 128: return Run<T, 128, 8, kVec, kAny>(a, bwd, s);
-    case 256: return Run<T, 256, 8, kVec, kAny>(a, bwd, s);
-    case 512: return Run<T, 512, 8, kVec, kAny>(a, bwd, s);
-    default:
-      return a.cols <= 8192 ? Run<T, 1024, 8, kVec, kAny>(a, bwd, s) : Run<T, 1024, 16, kVec, kAny>(a, bwd, s);
+    case 64: return Run<T, 64, 8, kOff>(a, bwd, s);
+    case 128: return Run<T, 128, 8, kOff>(a, bwd, s);
+    case 256: return Run<T, 256, 8, kOff>(a, bwd, s);
+    case 512: return Run<T, 512, 8, kOff>(a, bwd, s);
+    default: return a.cols <= 8192 ? Run<T, 1024, 8, kOff>(a, bwd, s) : Run<T, 1024, 16, kOff>(a, bwd, s);
   }
 }
 
-template <class T>
-hipError_t Dispatch(const JoinArgs& a, bool bwd, hipStream_t s) {
-  // 16-byte accesses where every row and vector begins on 16 bytes.
-  uintptr_t at = 0;
-  for (const void* p : {a.o, a.x, static_cast<const void*>(a.post_w), static_cast<const void*>(a.post_b),
-                        static_cast<const void*>(a.gate), static_cast<const void*>(a.pre_w),
-                        static_cast<const void*>(a.pre_b), static_cast<const void*>(a.y),
-                        static_cast<const void*>(a.h), a.dh, a.dy, static_cast<const void*>(a.dx),
-                        static_cast<const void*>(a.d_o)})
+hipError_t Dispatch(int bf16, const JoinArgs& a, bool bwd, hipStream_t s) {
+  if (!bf16) return Pick<float, false>(a, bwd, s);
+  uintptr_t at = 2 * a.cols;  // every row on a dword
+  for (const void* p : {a.o, a.x, static_cast<const void*>(a.y), static_cast<const void*>(a.h), a.dh, a.dy,
+                        static_cast<const void*>(a.dx), static_cast<const void*>(a.d_o)})
     at |= reinterpret_cast<uintptr_t>(p);
-  if (a.cols % Io<T>::kV == 0 && (at & 15) == 0) return Pick<T, true, false>(a, bwd, s);
-  if (!bwd && a.cols > (sizeof(T) == 2 ? 256 : 2048)) return Pick<T, true, true>(a, bwd, s);
-  return Pick<T, false, false>(a, bwd, s);
+  return at & 3 ? Pick<uint16_t, true>(a, bwd, s) : Pick<uint16_t, false>(a, bwd, s);
 }
 
 }  // namespace
@@ -391,11 +640,11 @@ size_t JoinWorkspaceBytes(size_t rows, size_t cols, size_t gate_rows) {
 
 hipError_t LaunchJoinFwd(int bf16, const JoinArgs& a, hipStream_t s) {
   if (a.rows == 0) return hipSuccess;
-  return bf16 ? Dispatch<uint16_t>(a, false, s) : Dispatch<float>(a, false, s);
+  return Dispatch(bf16, a, false, s);
 }
 
 hipError_t LaunchJoinBwd(int bf16, const JoinArgs& a, hipStream_t s) {
-  return bf16 ? Dispatch<uint16_t>(a, true, s) : Dispatch<float>(a, true, s);
+  return Dispatch(bf16, a, true, s);
 }
 
 }  // namespace seeai
