@@ -43,24 +43,51 @@ __device__ __forceinline__ float UniformF(float v) {
 }
 
 // A row of T over kTPR threads, 16 bytes an access: lane t's group i holds the
-// kV columns from (i kTPR + t) kV on.  A row is its wave's own, so its address
-// is a scalar.  Rows on dwords (f32; bf16 of an even width) go through a buffer
-// range of exactly the row: a dword past it reads as zero and is not stored, each
-// dword by itself, so no access asks where the row ends.  Other bf16 rows
-// (kOff) are read 16 bytes at a time from wherever they lie; the row's last,
-// short group reads the row's last 16 bytes and is shifted into place, so its
-// load, too, can run ahead of its use.
+// kV columns from (i kTPR + t) kV on.  Rows on dwords (f32; bf16 of an even
+// width) go through buffer ranges.  With a wave or more a row the range is
+// exactly the row, its address a scalar: a dword past it reads as zero and is
+// not stored, each dword by itself, so no access asks where the row ends.  With
+// several rows a wave (kTPR 16 or 32, one group a lane) the range is the wave's
+// rows, neighbours in memory, lanes past their row's columns point past it, and
+// a row's last, short group is cut by hand.  Other bf16 rows (kOff) are read 16
+// bytes at a time from wherever they lie; the row's last, short group reads the
+// row's last 16 bytes and is shifted into place, so its load, too, can run ahead
+// of its use.
 template <class T, int kTPR, int kE, bool kOff>
 struct Row {
-  static constexpr int kV = Io<T>::kV, kN = kE / kV;
+  static constexpr int kV = Io<T>::kV, kN = kE / kV, kSize = sizeof(T);
+  static constexpr bool kNarrow = kTPR < kWave;
   u32x4 q[kN];
   static __device__ __forceinline__ int Col(int t, int i) { return (i * kTPR + t) * kV; }
-  // here: the row's columns, or 0 for a row that is not there (zeros).
-  __device__ __forceinline__ void Load(const T* row, int t, int here) {
-    if constexpr (!kOff) {
-      const auto rs = Buffer(row, here * static_cast<int>(sizeof(T)));
+  static constexpr int kPast = 0x40000000;  // past every range
+  // The wave's rows from its first on, and where this lane's group i lies.
+  static __device__ __forceinline__ size_t First(size_t r) {
+    const size_t lane_row = (threadIdx.x % kWave) / kTPR;
+    const size_t f = r - lane_row;
+    return (static_cast<size_t>(Uniform(static_cast<int>(f >> 32))) << 32) |
+           static_cast<uint32_t>(Uniform(static_cast<int>(f)));
+  }
+  static __device__ __forceinline__ int Byte(int t, int i, int cols) {
+    const int c = Col(t, i), lane_row = (threadIdx.x % kWave) / kTPR;
+    return c < cols ? (lane_row * cols + c) * kSize : kPast;
+  }
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t Rows(const T* x, size_t r, size_t end, int cols) {
+    const size_t f = First(r), left = f < end ? end - f : 0;
+    const int n = left < kWave / kTPR ? static_cast<int>(left) : kWave / kTPR;
+    return Buffer(x + f * cols, n * cols * kSize);
+  }
+  // Row r of x, zeros where it is not before `end`.
+  __device__ __forceinline__ void Load(const T* x, size_t r, size_t end, int t, int cols) {
+    const T* row = x + r * cols;
+    const int here = r < end ? cols : 0;
+    if constexpr (!kOff && kNarrow) {
+      const auto rs = Rows(x, r, end, cols);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) q[i] = ReadBuffer(rs, Col(t, i) * static_cast<int>(sizeof(T)));
+      for (int i = 0; i < kN; ++i) q[i] = ReadBuffer(rs, Byte(t, i, cols));
+    } else if constexpr (!kOff) {
+      const auto rs = Buffer(row, here * kSize);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) q[i] = ReadBuffer(rs, Col(t, i) * kSize);
     } else if (here >= kV) {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
@@ -77,22 +104,21 @@ struct Row {
       }
     }
   }
-  __device__ __forceinline__ void Get(int t, int here, float (&v)[kE]) const {
+  __device__ __forceinline__ void Get(int t, int cols, float (&v)[kE]) const {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       u32x4 w = q[i];
       if constexpr (kOff) {
-        const int by = here >= kV ? Col(t, i) - (here - kV) : 0;  // elements to shift out
+        const int by = cols >= kV ? Col(t, i) - (cols - kV) : 0;  // elements to shift out
         if (by & 4) w = u32x4{w[2], w[3], 0, 0};
         if (by & 2) w = u32x4{w[1], w[2], w[3], 0};
         if (by & 1)
           w = u32x4{__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16),
                     __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
         if (by >= kV) w = u32x4{0, 0, 0, 0};
-        // (a group before the last: by is negative)
-        if (by <= 0) w = q[i];
+        if (by <= 0) w = q[i];  // a group before the last
       }
-      if constexpr (sizeof(T) == 4) {
+      if constexpr (kSize == 4) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[i * kV + k] = __uint_as_float(w[k]);
       } else {
@@ -102,15 +128,48 @@ struct Row {
           v[i * kV + 2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
         }
       }
+      if constexpr (!kOff && kNarrow) {
+#pragma unroll
+        for (int k = 1; k < kV; ++k)
+          if (Col(t, i) + k >= cols) v[i * kV + k] = 0.0f;
+      }
     }
   }
-  static __device__ __forceinline__ void Store(T* row, int t, int cols, const float (&v)[kE]) {
-    const auto rs = Buffer(row, cols * static_cast<int>(sizeof(T)));
+  static __device__ __forceinline__ u32x4 Bits(const float* v) {
+    if constexpr (kSize == 4)
+      return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    else
+      return __builtin_bit_cast(u32x4, Io<uint16_t>::Pack(v));
+  }
+  static __device__ __forceinline__ void Store(T* x, size_t r, size_t end, int t, int cols, const float (&v)[kE]) {
+    if constexpr (!kOff && kNarrow) {
+      const auto rs = Rows(x, r, end, cols);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int c = Col(t, i);
-      const float* at = v + i * kV;
-      if constexpr (kOff) {
+      for (int i = 0; i < kN; ++i) {
+        const u32x4 w = Bits(v + i * kV);
+        const int c = Col(t, i), byte = Byte(t, i, cols);
+        if (c + kV <= cols) {
+          __builtin_amdgcn_raw_buffer_store_b128(w, rs, byte, 0, 0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c + k * 4 / kSize < cols) __builtin_amdgcn_raw_buffer_store_b32(w[k], rs, byte + 4 * k, 0, 0);
+        }
+      }
+      return;
+    }
+    if (r >= end) return;
+    T* row = x + r * cols;
+    if constexpr (!kOff) {
+      const auto rs = Buffer(row, cols * kSize);
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        __builtin_amdgcn_raw_buffer_store_b128(Bits(v + i * kV), rs, Col(t, i) * kSize, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int c = Col(t, i);
+        const float* at = v + i * kV;
         if (c + kV <= cols) {
           Io<T>::StoreAny(row + c, at);
         } else {
@@ -118,16 +177,22 @@ struct Row {
           for (int k = 0; k < kV; ++k)
             if (c + k < cols) Io<T>::Put(row + c + k, at[k]);
         }
-      } else if constexpr (sizeof(T) == 4) {
-        __builtin_amdgcn_raw_buffer_store_b128(
-            u32x4{__float_as_uint(at[0]), __float_as_uint(at[1]), __float_as_uint(at[2]), __float_as_uint(at[3])},
-            rs, c * 4, 0, 0);
-      } else {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, Io<uint16_t>::Pack(at)), rs, c * 2, 0, 0);
       }
     }
   }
 };
+
+// The row group of a thread: a scalar where a row has whole waves.
+template <int kTPR>
+__device__ __forceinline__ int RowGroup() {
+  if constexpr (kTPR >= kWave) return Uniform(threadIdx.x / kTPR);
+  else return threadIdx.x / kTPR;
+}
+template <int kTPR>
+__device__ __forceinline__ float RowFloat(float v) {  // a value of a row
+  if constexpr (kTPR >= kWave) return UniformF(v);
+  else return v;
+}
 
 // The f32 vector at the same columns, zeros past it.
 template <class T, int kTPR, int kE>
@@ -141,39 +206,39 @@ __device__ __forceinline__ void Vector(const float* w, int t, int cols, float (&
   }
 }
 
-template <class T, int kTPR, int kE>
-__device__ __forceinline__ void StoreVector(float* w, int t, int cols, const float (&v)[kE]) {
-  const auto rs = Buffer(w, cols * 4);
-#pragma unroll
-  for (int e = 0; e < kE; e += 4)
-    __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v[e]), __float_as_uint(v[e + 1]),
-                                                 __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3])},
-                                           rs, ColOf<T, kTPR, true>(t, e) * 4, 0, 0);
-}
-
 constexpr int FwdThreads(int tpr) { return tpr > 256 ? tpr : 256; }
 // The backward's workgroup, one a CU: few bands, and few sums for the fold.
 constexpr int kBwdThreads = 1024;
 
-// Sum over the wave's lanes by lane moves within registers; all lanes get it.
-template <int kCtrl, int kRows>
+// Sums by lane moves within registers.
+template <int kCtrl, int kRows = 0xf>
 __device__ __forceinline__ float MoveAdd(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, kRows, 0xf, false));
 }
+template <int kTPR>
 __device__ __forceinline__ float LaneSum(float v) {
-  v = MoveAdd<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8 within rows of 16
-  v = MoveAdd<0x112, 0xf>(v);
-  v = MoveAdd<0x114, 0xf>(v);
-  v = MoveAdd<0x118, 0xf>(v);
-  v = MoveAdd<0x142, 0xa>(v);  // lane 15 of a row to the next row
-  v = MoveAdd<0x143, 0xc>(v);  // lane 31 to the upper half
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  if constexpr (kTPR < kWave) {  // over 16 or 32 lanes, each of them gets it
+    v = MoveAdd<0xB1>(v);   // the neighbour's
+    v = MoveAdd<0x4E>(v);   // the neighbouring pair's
+    v = MoveAdd<0x141>(v);  // the other four of eight
+    v = MoveAdd<0x140>(v);  // the other eight of sixteen
+    if constexpr (kTPR == 32) v += __shfl_xor(v, 16, kWave);
+    return v;
+  } else {
+    v = MoveAdd<0x111>(v);  // from 1, 2, 4, 8 lanes before, within rows of 16
+    v = MoveAdd<0x112>(v);
+    v = MoveAdd<0x114>(v);
+    v = MoveAdd<0x118>(v);
+    v = MoveAdd<0x142, 0xa>(v);  // lane 15 of a row to the next row
+    v = MoveAdd<0x143, 0xc>(v);  // lane 31 to the upper half
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  }
 }
 // Two sums over the kTPR threads of each row; `lds` [2][2 x 16], used in turn,
 // so that one barrier keeps a sum's reads from the next one's writes.
 template <int kTPR>
 __device__ __forceinline__ float2 RowSum2(float a, float b, float* lds, int& turn) {
-  a = LaneSum(a), b = LaneSum(b);
+  a = LaneSum<kTPR>(a), b = LaneSum<kTPR>(b);
   if constexpr (kTPR > kWave) {
     constexpr int kWaves = kTPR / kWave;
     const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
@@ -228,33 +293,43 @@ JoinFwdKernel(JoinArgs a) {
   using R = Row<T, kTPR, kE, kOff>;
   __shared__ float lds[64];
   constexpr int kRows = FwdThreads(kTPR) / kTPR;
-  const int t = threadIdx.x % kTPR, sub = Uniform(threadIdx.x / kTPR), cols = static_cast<int>(a.cols);
+  const int t = threadIdx.x % kTPR, sub = RowGroup<kTPR>(), cols = static_cast<int>(a.cols);
   int turn = 0;
   // (the loop is uniform over the workgroup, its barriers too)
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < a.rows;
        base += static_cast<size_t>(gridDim.x) * kRows) {
-    const size_t r = base + sub, off = r * cols;
+    const size_t r = base + sub;
     const bool in = r < a.rows;
-    const int here = in ? cols : 0;
     R ro, rx;
-    ro.Load(static_cast<const T*>(a.o) + off, t, here);
-    rx.Load(static_cast<const T*>(a.x) + off, t, here);
+    ro.Load(static_cast<const T*>(a.o), r, a.rows, t, cols);
+    rx.Load(static_cast<const T*>(a.x), r, a.rows, t, cols);
     float v[kE], x[kE];
-    ro.Get(t, here, v);
+    ro.Get(t, cols, v);
     float2 so = make_float2(0.0f, 0.0f), sy = so;
     if (a.post_w) {
       so = Normalise<T, kTPR, kE>(v, a.rms, t, cols, a.eps, lds, turn);
       Scale<T, kTPR, kE>(v, a.post_w, a.post_b, t, cols);
     }
-    if (a.gate) Scale<T, kTPR, kE>(v, a.gate + (in ? r : 0) / a.gate_rows * cols, nullptr, t, cols);
-    rx.Get(t, here, x);
+    if (a.gate) {
+      const size_t g = (in ? r : 0) / a.gate_rows;
+      if constexpr (kTPR >= kWave) {
+        Scale<T, kTPR, kE>(v, a.gate + g * cols, nullptr, t, cols);
+      } else {  // rows of one wave may differ in their gates
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          const int c = ColOf<T, kTPR, true>(t, e);
+          v[e] *= c < cols ? a.gate[g * cols + c] : 0.0f;
+        }
+      }
+    }
+    rx.Get(t, cols, x);
 #pragma unroll
     for (int e = 0; e < kE; ++e) v[e] = a.res * x[e] + v[e];
-    if (in) R::Store(static_cast<T*>(a.y) + off, t, cols, v);
+    R::Store(static_cast<T*>(a.y), r, a.rows, t, cols, v);
     if (a.pre_w) {
       sy = Normalise<T, kTPR, kE>(v, a.rms, t, cols, a.eps, lds, turn);
       Scale<T, kTPR, kE>(v, a.pre_w, a.pre_b, t, cols);
-      if (in) R::Store(static_cast<T*>(a.h) + off, t, cols, v);
+      R::Store(static_cast<T*>(a.h), r, a.rows, t, cols, v);
     }
     if (in && t == 0 && a.stats) {
       float* s = a.stats + 4 * r;
@@ -271,7 +346,7 @@ struct Plan {
 };
 // A row's threads, for rows of `cols`.
 int RowThreads(size_t cols) {
-  return cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
+  return cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
 }
 constexpr size_t kBands = 256;
 Plan PlanOf(size_t rows, size_t cols, size_t gate_rows) {
@@ -301,7 +376,11 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
   __shared__ float lds[64];
   // Element e of thread t at ((e / 4) kTPR + t) 4 + e % 4: w', and gate w.
   __shared__ float wpre[kTPR * kE], wpost[kTPR * kE];
-  const int t = threadIdx.x % kTPR, sub = Uniform(threadIdx.x / kTPR), cols = static_cast<int>(a.cols);
+  // Sums of the row groups' columns; over wpost, which is read no more by then,
+  // where there is one group.
+  __shared__ float groups[kRows > 1 ? kRows * kTPR * kE : 4];
+  float* stage = kRows > 1 ? groups : wpost;
+  const int t = threadIdx.x % kTPR, sub = RowGroup<kTPR>(), cols = static_cast<int>(a.cols);
   const auto slot = [&](int e) { return (e / 4 * kTPR + t) * 4 + e % 4; };
   const float inv = 1.0f / static_cast<float>(cols);
   const bool pre = a.pre_w != nullptr, post = a.post_w != nullptr, tail = post || a.gate;
@@ -318,19 +397,19 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
     last = first + plan.len < (g + 1) * gr ? first + plan.len : (g + 1) * gr;
   }
   if (last > a.rows) last = a.rows;
-  // The row groups' sums add up in order; the last group holds them.
-  auto join = [&](float (&s)[kE], float* own) {
-    if constexpr (kRows > 1) {
-      for (int g = 0; g < kRows; ++g) {
-        __syncthreads();
-        if (sub == g) {
+  // Column sums over the row groups, in order, a thread a column: `use(c, sum)`.
+  auto join = [&](const auto& s, auto&& use) {
+    __syncthreads();  // what the memory held has been read
 #pragma unroll
-          for (int e = 0; e < kE; ++e) {
-            if (g > 0) s[e] = own[slot(e)] + s[e];
-            own[slot(e)] = s[e];
-          }
-        }
-      }
+    for (int e = 0; e < kE; e += 4)
+      *reinterpret_cast<float4*>(stage + sub * (kTPR * kE) + ColOf<T, kTPR, true>(t, e)) =
+          make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += kBwdThreads) {
+      float sum = stage[c];
+#pragma unroll
+      for (int g = 1; g < kRows; ++g) sum += stage[g * (kTPR * kE) + c];
+      use(c, sum);
     }
   };
   auto four = [&](const float* own, int e, float (&w)[4]) {  // from column e on
@@ -350,14 +429,13 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
   float4 st;
   size_t base = first;
   auto fetch = [&](size_t end) {  // (past the gate's last row: zeros, which add nothing)
-    const size_t r = base + sub, off = r * cols;
-    const int here = r < end ? cols : 0;
-    rh.Load(static_cast<const T*>(a.dh) + off, t, pre ? here : 0);
-    ry.Load(static_cast<const T*>(a.y) + off, t, pre ? here : 0);
-    rd.Load(static_cast<const T*>(a.dy) + off, t, a.dy ? here : 0);
-    ro.Load(static_cast<const T*>(a.o) + off, t, tail ? here : 0);
+    const size_t r = base + sub;
+    rh.Load(static_cast<const T*>(a.dh), r, pre ? end : 0, t, cols);
+    ry.Load(static_cast<const T*>(a.y), r, pre ? end : 0, t, cols);
+    rd.Load(static_cast<const T*>(a.dy), r, a.dy ? end : 0, t, cols);
+    ro.Load(static_cast<const T*>(a.o), r, tail ? end : 0, t, cols);
     st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (here) {
+    if (r < end) {
       const float* s = a.stats + 4 * r;
       st = make_float4(s[0], s[1], s[2], s[3]);
     }
@@ -392,15 +470,14 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
       for (int e = 0; e < kE; ++e) s0[e] = 0.0f;
     }
     while (base < end) {  // (uniform over the workgroup, its barriers too)
-      const size_t r = base + sub, off = r * cols;
-      const bool in = r < end;
-      const int here = in ? cols : 0;
+      const size_t r = base + sub;
       if constexpr (!kAhead) fetch(end);
-      const float4 q = make_float4(UniformF(st.x), UniformF(st.y), UniformF(st.z), UniformF(st.w));
+      const float4 q = make_float4(RowFloat<kTPR>(st.x), RowFloat<kTPR>(st.y), RowFloat<kTPR>(st.z),
+                                   RowFloat<kTPR>(st.w));
       float d[kE], v[kE];
       const R md = rd, mo = ro;
-      rh.Get(t, pre ? here : 0, d);
-      ry.Get(t, pre ? here : 0, v);
+      rh.Get(t, cols, d);
+      ry.Get(t, cols, v);
       base += kRows;
       if constexpr (kAhead) fetch(end);
       if (pre) {
@@ -429,14 +506,14 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
           if (!kRms && ColOf<T, kTPR, true>(t, e) >= cols) d[e] = 0.0f;
         }
       }
-      md.Get(t, a.dy ? here : 0, v);
+      md.Get(t, cols, v);
 #pragma unroll
       for (int e = 0; e < kE; ++e) d[e] += v[e];
 #pragma unroll
       for (int e = 0; e < kE; ++e) v[e] = a.res * d[e];
-      if (in) R::Store(static_cast<T*>(a.dx) + off, t, cols, v);
+      R::Store(static_cast<T*>(a.dx), r, end, t, cols, v);
       if (tail) {
-        mo.Get(t, here, v);
+        mo.Get(t, cols, v);
         if (post) {
           const float mu = kRms ? 0.0f : q.x;
 #pragma unroll
@@ -463,49 +540,25 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
           for (int e = 0; e < kE; ++e) d[e] = q.y * (d[e] - c1 - v[e] * c2);
         }
       }
-      if (in) R::Store(static_cast<T*>(a.d_o) + off, t, cols, d);
+      R::Store(static_cast<T*>(a.d_o), r, end, t, cols, d);
     }
     if (tail) {
-      // (the gate's product has been read by every row group behind a barrier)
-      join(s1, wpost);
-      if constexpr (!kRms) join(s0, wpost);
-      if (sub == kRows - 1) {
-        float v[kE], u[kE];
-        if (a.dgate && (whole || plan.per == 1) && at < a.rows) {  // all of the gate's rows are here
-          if (post) {
-            Vector<T, kTPR, kE>(a.post_w, t, cols, v);
-#pragma unroll
-            for (int e = 0; e < kE; ++e) v[e] *= s1[e];
-            if constexpr (!kRms) {
-              if (a.post_b) {
-                Vector<T, kTPR, kE>(a.post_b, t, cols, u);
-#pragma unroll
-                for (int e = 0; e < kE; ++e) v[e] += u[e] * s0[e];
-              }
-            }
-            StoreVector<T, kTPR, kE>(a.dgate + g * cols, t, cols, v);
-          } else {
-            StoreVector<T, kTPR, kE>(a.dgate + g * cols, t, cols, s1);
-          }
-        }
-        if (whole || one) {
-#pragma unroll
-          for (int e = 0; e < kE; ++e) v[e] = 1.0f;
-          if (gate) Vector<T, kTPR, kE>(gate, t, cols, v);
-          auto add = [&](float* to, const auto& s) {  // onto the gates' before
-#pragma unroll
-            for (int e = 0; e < kE; ++e) u[e] = 0.0f;
-            if (at != first) Vector<T, kTPR, kE>(to, t, cols, u);
-#pragma unroll
-            for (int e = 0; e < kE; ++e) u[e] += v[e] * s[e];
-            StoreVector<T, kTPR, kE>(to, t, cols, u);
-          };
-          if (post) add(one ? a.dpost_w : part + 2 * cols, s1);
-          if constexpr (!kRms)
-            if (a.dpost_b) add(one ? a.dpost_b : part + 3 * cols, s0);
-        } else {
-          StoreVector<T, kTPR, kE>(part + 2 * cols, t, cols, s1);
-          if constexpr (!kRms) StoreVector<T, kTPR, kE>(part + 3 * cols, t, cols, s0);
+      const bool mine = a.dgate && (whole || plan.per == 1) && at < a.rows;  // all of the gate's rows are here
+      const bool weighted = whole || one;
+      float* o1 = one ? a.dpost_w : part + 2 * cols;
+      float* o0 = one ? a.dpost_b : part + 3 * cols;
+      join(s1, [&](int c, float sum) {
+        if (mine) a.dgate[g * cols + c] = post ? a.post_w[c] * sum : sum;
+        if (!weighted) o1[c] = sum;
+        else if (post) o1[c] = (gate ? gate[c] : 1.0f) * sum + (at == first ? 0.0f : o1[c]);
+      });
+      if constexpr (!kRms) {
+        if (a.post_b) {
+          join(s0, [&](int c, float sum) {
+            if (mine) a.dgate[g * cols + c] += a.post_b[c] * sum;
+            if (!weighted) o0[c] = sum;
+            else if (a.dpost_b) o0[c] = (gate ? gate[c] : 1.0f) * sum + (at == first ? 0.0f : o0[c]);
+          });
         }
       }
     }
@@ -513,12 +566,13 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
     if (!whole || at >= last) break;
   }
   if (pre) {
-    join(pw, wpre);
-    if constexpr (!kRms) join(pb, wpre);
-    if (sub == kRows - 1) {
-      StoreVector<T, kTPR, kE>(one ? a.dpre_w : part, t, cols, pw);
-      if constexpr (!kRms)
-        if (a.dpre_b) StoreVector<T, kTPR, kE>(one ? a.dpre_b : part + cols, t, cols, pb);
+    float* o1 = one ? a.dpre_w : part;
+    join(pw, [&](int c, float sum) { o1[c] = sum; });
+    if constexpr (!kRms) {
+      if (a.dpre_b) {
+        float* o0 = one ? a.dpre_b : part + cols;
+        join(pb, [&](int c, float sum) { o0[c] = sum; });
+      }
     }
   }
 }
@@ -614,6 +668,8 @@ hipError_t Run(const JoinArgs& a, bool bwd, hipStream_t s) {
 template <class T, bool kOff>
 hipError_t Pick(const JoinArgs& a, bool bwd, hipStream_t s) {
   switch (RowThreads(a.cols)) {
+    case 16: return Run<T, 16, 8, kOff>(a, bwd, s);
+    case 32: return Run<T, 32, 8, kOff>(a, bwd, s);
     case 64: return Run<T, 64, 8, kOff>(a, bwd, s);
     case 128: return Run<T, 128, 8, kOff>(a, bwd, s);
     case 256: return Run<T, 256, 8, kOff>(a, bwd, s);
