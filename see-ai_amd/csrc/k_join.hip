@@ -207,8 +207,11 @@ __device__ __forceinline__ void Vector(const float* w, int t, int cols, float (&
 }
 
 constexpr int FwdThreads(int tpr) { return tpr > 256 ? tpr : 256; }
-// The backward's workgroup, one a CU: few bands, and few sums for the fold.
-constexpr int kBwdThreads = 1024;
+// The backward's workgroup, and its bands: two workgroups a CU, whose turns of
+// load, sum and store interleave.  us, against one of 1024 threads a CU (half the
+// bands): 20000 x 200 bf16 with gates of 300 rows 25 and 35, 4000 x 4095 bf16 51
+// and 54, 8192 x 2048 bf16 39 both, 3001 x 1023 f32 27 and 25.
+constexpr int BwdThreads(int tpr) { return tpr > 512 ? tpr : 512; }
 
 // Sums by lane moves within registers.
 template <int kCtrl, int kRows = 0xf>
@@ -348,14 +351,15 @@ struct Plan {
 int RowThreads(size_t cols) {
   return cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
 }
-constexpr size_t kBands = 256;
+constexpr size_t kBands = 512;
 Plan PlanOf(size_t rows, size_t cols, size_t gate_rows) {
   if (rows == 0) return {1, 1, 0, 0};  // sums of zero
-  const size_t slots = static_cast<size_t>(kBwdThreads / RowThreads(cols));
+  const int tpr = RowThreads(cols), threads = BwdThreads(tpr);
+  const size_t slots = static_cast<size_t>(threads / tpr), most = threads > 512 ? kBands / 2 : kBands;
   const auto whole = [&](size_t n) { return (n + slots - 1) / slots * slots; };
-  size_t len = whole((rows + kBands - 1) / kBands);
+  size_t len = whole((rows + most - 1) / most);
   const size_t gr = gate_rows == 0 || gate_rows > rows ? rows : gate_rows, groups = (rows + gr - 1) / gr;
-  if (gr < len) {
+  if (gr <= len) {
     const size_t k = len / gr;
     return {static_cast<unsigned>((groups + k - 1) / k), 1, k * gr, k};
   }
@@ -368,10 +372,10 @@ Plan PlanOf(size_t rows, size_t cols, size_t gate_rows) {
 // band's gates are whole), or the gradients themselves where there is one band.
 // A row's loads go out while the row before it is reduced (kAhead).
 template <class T, int kTPR, int kE, bool kOff, bool kRms>
-__global__ void __launch_bounds__(kBwdThreads, kBwdThreads / 256)
+__global__ void __launch_bounds__(BwdThreads(kTPR), 4)
 JoinBwdKernel(JoinArgs a, Plan plan) {
   using R = Row<T, kTPR, kE, kOff>;
-  constexpr int kRows = kBwdThreads / kTPR;
+  constexpr int kThreads = BwdThreads(kTPR), kRows = kThreads / kTPR;
   constexpr bool kAhead = kE == 8;  // (with 16 the registers are full)
   __shared__ float lds[64];
   // Element e of thread t at ((e / 4) kTPR + t) 4 + e % 4: w', and gate w.
@@ -405,7 +409,7 @@ JoinBwdKernel(JoinArgs a, Plan plan) {
       *reinterpret_cast<float4*>(stage + sub * (kTPR * kE) + ColOf<T, kTPR, true>(t, e)) =
           make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
     __syncthreads();
-    for (int c = threadIdx.x; c < cols; c += kBwdThreads) {
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
       float sum = stage[c];
 #pragma unroll
       for (int g = 1; g < kRows; ++g) sum += stage[g * (kTPR * kE) + c];
@@ -597,15 +601,13 @@ JoinFoldKernel(JoinArgs a, Plan plan, unsigned gates) {
   const bool both = !a.rms && (job == 0 ? a.dpre_b != nullptr : a.post_b != nullptr);
   float s = 0.0f, z = 0.0f;
   if (c < cols) {
-    unsigned at = plan.per > 1 ? k % plan.per : 0, of = k / plan.per;  // the band within its gate, the gate
 #pragma unroll 8
     for (unsigned b = b0 + k; b < b1; b += kFoldParts) {
       const size_t off = static_cast<size_t>(b) * 4 * cols;
       float v = row[off], u = both ? row[off + cols] : 0.0f;
       if (weigh) {
-        const float by = a.gate[of * cols + c];
+        const float by = a.gate[b / plan.per * cols + c];
         v *= by, u *= by;
-        for (at += kFoldParts; at >= plan.per; at -= plan.per) ++of;
       }
       s += v, z += u;
     }
@@ -650,9 +652,9 @@ hipError_t Run(const JoinArgs& a, bool bwd, hipStream_t s) {
   }
   const Plan plan = PlanOf(a.rows, a.cols, a.gate ? a.gate_rows : 0);
   if (a.rms)
-    hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, true>), dim3(plan.bands), dim3(kBwdThreads), 0, s, a, plan);
+    hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, true>), dim3(plan.bands), dim3(BwdThreads(kTPR)), 0, s, a, plan);
   else
-    hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, false>), dim3(plan.bands), dim3(kBwdThreads), 0, s, a, plan);
+    hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, false>), dim3(plan.bands), dim3(BwdThreads(kTPR)), 0, s, a, plan);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || plan.bands == 1) return e;
   // Gates whose rows lie in several bands.
   const unsigned gates = a.gate && plan.gates == 0 ? plan.bands / plan.per : 0;

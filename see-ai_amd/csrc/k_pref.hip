@@ -35,22 +35,120 @@ __device__ __forceinline__ float ExpNeg(float x) { return __builtin_amdgcn_exp2f
 struct Lse {
   float m = -INFINITY, s = 0.0f;
   __device__ __forceinline__ float Base() const { return m == -INFINITY ? 0.0f : m; }
-  template <int n>
-  __device__ __forceinline__ void Take(const float (&v)[n]) {
-    float top = m;
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A row on 16-byte groups of kV elements: wherever the row begins, the groups
+// begin on 16 bytes, the first with `skip` elements before the row, the last
+// with what lies behind it.  A softmax asks nothing of which lane holds which
+// column, so rows of any alignment cost no more than aligned ones; a group's
+// elements outside the row, which share 16 aligned bytes with one of the row's,
+// are read and become -inf, and are never written.
+template <class T>
+struct Line {
+  static constexpr int kV = 16 / sizeof(T);
+  const u32x4* base;
+  size_t groups, end;  // end: skip + C
+  int skip;
+  __device__ __forceinline__ Line(const T* row, size_t C) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+    skip = static_cast<int>(at % 16 / sizeof(T));
+    base = reinterpret_cast<const u32x4*>(at & ~uintptr_t{15});
+    end = C + skip;
+    groups = (end + kV - 1) / kV;
+  }
+  __device__ __forceinline__ bool Whole(size_t g) const { return (g > 0 || skip == 0) && (g + 1) * kV <= end; }
+  // Group g's elements outside the row become -inf, all of them past the row.
+  __device__ __forceinline__ u32x4 Mask(u32x4 w, size_t g) const {
+    const size_t c = g * kV;
+    const int first = g == 0 ? skip : 0, last = c >= end ? 0 : end - c < kV ? static_cast<int>(end - c) : kV;
 #pragma unroll
-    for (int i = 0; i < n; ++i) top = fmaxf(top, v[i]);
-    const float was = m;
-    m = top;
-    const float base = Base();
-    s *= ExpNeg(was - base);
+    for (int k = 0; k < kV; ++k) {
+      const bool out = k < first || k >= last;
+      if constexpr (sizeof(T) == 4) {
+        w[k] = out ? 0xFF800000u : w[k];
+      } else if (k % 2) {
+        w[k / 2] = out ? (w[k / 2] & 0xFFFFu) | 0xFF800000u : w[k / 2];
+      } else {
+        w[k / 2] = out ? (w[k / 2] & 0xFFFF0000u) | 0xFF80u : w[k / 2];
+      }
+    }
+    return w;
+  }
+  static __device__ __forceinline__ void Floats(u32x4 w, float (&v)[kV]) {
 #pragma unroll
-    for (int i = 0; i < n; ++i) s += ExpNeg(v[i] - base);
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[k] = __uint_as_float(w[k]);
+      } else {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+      }
+    }
+  }
+  static __device__ __forceinline__ u32x4 Bits(const float (&v)[kV]) {
+    if constexpr (sizeof(T) == 4)
+      return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    else
+      return __builtin_bit_cast(u32x4, Io<uint16_t>::Pack(v));
+  }
+  // Group from + g (from a scalar, g a lane's): an address of a scalar and 32 bits.
+  __device__ __forceinline__ u32x4 Read(size_t from, unsigned g) const {
+    return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + from) + g * 16u);
+  }
+  // A whole group to the row `out`, whose own group it is where `same` (out lies
+  // on 16 bytes as the row does).
+  __device__ __forceinline__ void Store(T* out, bool same, size_t from, unsigned g, const float (&v)[kV]) const {
+    char* at = reinterpret_cast<char*>(out - skip + from * kV) + g * 16u;
+    if (same) *reinterpret_cast<u32x4*>(at) = Bits(v);
+    else Io<T>::StoreAny(reinterpret_cast<T*>(at), v);
+  }
+  // The column that thread t sees to of the first and the last group where they
+  // are not whole (kV threads each), or C for none.
+  __device__ __forceinline__ size_t Edge(int t, size_t C) const {
+    if (t >= 2 * kV || (t >= kV && groups == 1)) return C;
+    const size_t g = t < kV ? 0 : groups - 1, c = g * kV + t % kV;
+    return Whole(g) || c < static_cast<size_t>(skip) || c >= end ? C : c - skip;
   }
 };
 
-// The row's, from its kTPR threads'; `label` of the row's first thread (the
-// label's logit, read before any thread may write over it) comes to all of them.
+// Keeps what is formed from w before from being kept for what is formed of it
+// behind: unpacked twice it takes a quarter of the registers.
+__device__ __forceinline__ void Forget(u32x4& w) { asm volatile("" : "+v"(w)); }
+
+// Several groups at once: one new maximum for all of them.
+template <class T, int n>
+__device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n]) {
+  constexpr int kV = Line<T>::kV;
+  float top = a.m;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    float v[kV];
+    Line<T>::Floats(w[i], v);
+#pragma unroll
+    for (int k = 0; k < kV; ++k) top = fmaxf(top, v[k]);
+    Forget(w[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const float was = a.m;
+  a.m = top;
+  const float base = a.Base();
+  a.s *= ExpNeg(was - base);
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    float v[kV];
+    Line<T>::Floats(w[i], v);
+#pragma unroll
+    for (int k = 0; k < kV; ++k) a.s += ExpNeg(v[k] - base);
+    Forget(w[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The row's maximum and sum from its kTPR threads'; `label` of the row's first
+// thread (the label's logit, read before any thread may write over it) comes to
+// all of them.
 template <int kTPR>
 __device__ __forceinline__ Lse RowLse(Lse a, float* lds, float& label) {
   Lse r;
@@ -76,68 +174,95 @@ __device__ __forceinline__ Lse RowLse(Lse a, float* lds, float& label) {
   return r;
 }
 
-// kV neighbours from column c on, -inf past the row.
-template <class T>
-__device__ __forceinline__ void Columns(const T* row, size_t c, size_t C, float (&v)[Io<T>::kV]) {
-  constexpr int kV = Io<T>::kV;
-  if (c + kV <= C) {
-    Io<T>::LoadAny(row + c, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kV; ++i) v[i] = c + i < C ? Io<T>::Get(row + c + i) : -INFINITY;
-  }
-}
+constexpr int kAhead = 4;  // groups a lane reads before it uses them
 
+// This thread's share of a row: kAhead loads go out at a time; what may lie
+// outside the row (the first turn's first group, the last turn) is masked.
 template <class T, int kTPR>
-__device__ __forceinline__ Lse SweepLse(const T* row, int t, size_t C) {
-  constexpr int kV = Io<T>::kV;
+__device__ __forceinline__ Lse SweepLse(const Line<T>& line, int t) {
   Lse a;
-  for (size_t c = static_cast<size_t>(t) * kV; c < C; c += kTPR * kV) {
-    float v[kV];
-    Columns(row, c, C, v);
-    a.Take(v);
+  for (size_t at = 0; at < line.groups; at += kAhead * kTPR) {
+    u32x4 w[kAhead];
+    const bool last = at + kAhead * kTPR >= line.groups;
+    const unsigned left = last ? static_cast<unsigned>(line.groups - at) : kAhead * kTPR;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const unsigned g = u * kTPR + t;
+      w[u] = line.Read(at, g < left ? g : left - 1);
+    }
+    if (at == 0 && !last) w[0] = line.Mask(w[0], t);
+    if (last) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) w[u] = line.Mask(w[u], at + u * kTPR + t);
+    }
+    Take<T>(a, w);
   }
   return a;
 }
 
-// dz = d (1[c = l] - exp(z - m) inv): columns of a lane are read before they are
-// written, so out may be row.
+// dz = d (1[c = l] - exp(z - m) / s) for a group: by = -d / s; `label` counts
+// from the line's first group.
+template <class T>
+__device__ __forceinline__ void GroupGrad(u32x4 w, unsigned g, size_t label, float d, float by, float m,
+                                          float (&v)[Line<T>::kV]) {
+  constexpr int kV = Line<T>::kV;
+  Line<T>::Floats(w, v);
+#pragma unroll
+  for (int k = 0; k < kV; ++k) v[k] = by * ExpNeg(v[k] - m);
+  if (label / kV <= 0xFFFFFFFFu && g == static_cast<unsigned>(label / kV)) {
+    const int at = static_cast<int>(label % kV);
+#pragma unroll
+    for (int k = 0; k < kV; ++k)
+      if (k == at) v[k] += d;
+  }
+}
+
+// One column's gradient, by itself: what groups that are not whole hold.
+template <class T>
+__device__ __forceinline__ void EdgeGrad(const Line<T>& line, const T* row, T* out, int t, size_t C, size_t label,
+                                         float d, float by, float m) {
+  const size_t c = line.Edge(t, C);
+  if (c >= C) return;
+  const float v = by * ExpNeg(Io<T>::Get(row + c) - m);
+  Io<T>::Put(out + c, c == label ? v + d : v);
+}
+
+// A lane's groups are read before they are written, so out may be the row.
 template <class T, int kTPR>
-__device__ __forceinline__ void SweepGrad(const T* row, T* out, int t, size_t C, size_t label, float d,
-                                          float m, float inv) {
-  constexpr int kV = Io<T>::kV;
-  for (size_t c = static_cast<size_t>(t) * kV; c < C; c += kTPR * kV) {
-    float v[kV];
-    Columns(row, c, C, v);
+__device__ __forceinline__ void SweepGrad(const Line<T>& line, const T* row, T* out, bool same, int t, size_t C,
+                                          size_t label, float d, float m, float s) {
+  constexpr int kV = Line<T>::kV;
+  const float by = -d / s;
+  for (size_t at = 0; at < line.groups; at += kAhead * kTPR) {
+    u32x4 w[kAhead];
+    const size_t rest = line.groups - at;
+    const unsigned left = rest < kAhead * kTPR ? static_cast<unsigned>(rest) : kAhead * kTPR;
+    // This turn's groups that are whole, and the label's among them.
+    const unsigned from = at == 0 && line.skip ? 1 : 0, to = left - (at + left == line.groups && line.end % kV ? 1 : 0);
+    const size_t lab = label + line.skip - at * kV;  // (far past this turn's where it lies before)
 #pragma unroll
-    for (int i = 0; i < kV; ++i) v[i] = -d * (ExpNeg(v[i] - m) * inv);
-    if (label - c < kV) {
-#pragma unroll
-      for (int i = 0; i < kV; ++i)
-        if (label == c + i) v[i] = d + v[i];
+    for (int u = 0; u < kAhead; ++u) {
+      const unsigned g = u * kTPR + t;
+      w[u] = line.Read(at, g < left ? g : left - 1);
     }
-    if (c + kV <= C) {
-      Io<T>::StoreAny(out + c, v);
-    } else {
 #pragma unroll
-      for (int i = 0; i < kV; ++i)
-        if (c + i < C) Io<T>::Put(out + c + i, v[i]);
+    for (int u = 0; u < kAhead; ++u) {
+      const unsigned g = u * kTPR + t;
+      float v[kV];
+      GroupGrad<T>(w[u], g, lab, d, by, m, v);
+      if (g >= from && g < to) line.Store(out, same, at, g, v);
     }
   }
+  EdgeGrad(line, row, out, t, C, label, d, by, m);
 }
 template <class T, int kTPR>
 __device__ __forceinline__ void SweepZero(T* out, int t, size_t C) {
-  constexpr int kV = Io<T>::kV;
-  const float v[kV] = {};
-  for (size_t c = static_cast<size_t>(t) * kV; c < C; c += kTPR * kV) {
-    if (c + kV <= C) {
-      Io<T>::StoreAny(out + c, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kV; ++i)
-        if (c + i < C) Io<T>::Put(out + c + i, 0.0f);
-    }
-  }
+  const Line<T> line(out, C);
+  const float v[Line<T>::kV] = {};
+  for (size_t at = 0; at < line.groups; at += kTPR)
+    if (line.Whole(at + t)) line.Store(out, true, at, t, v);
+  const size_t c = line.Edge(t, C);
+  if (c < C) Io<T>::Put(out + c, 0.0f);
 }
 
 // A label's logit; one past the vocabulary has none.
@@ -147,6 +272,14 @@ __device__ __forceinline__ float LabelLogit(const T* row, int label, size_t C) {
 }
 
 constexpr int GroupOf(int tpr) { return tpr > 256 ? tpr : 256; }
+// The row group of a thread, a scalar: a row has whole waves.
+template <int kTPR>
+__device__ __forceinline__ int RowGroup() { return Uniform(threadIdx.x / kTPR); }
+// Whether two rows begin at the same place within 16 bytes.
+template <class T>
+__device__ __forceinline__ bool SameGroups(const T* a, const T* b) {
+  return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
 
 template <class T, int kTPR>
 __global__ void __launch_bounds__(GroupOf(kTPR))
@@ -157,11 +290,13 @@ TokenLogpKernel(const T* __restrict__ z, size_t ld, const int32_t* __restrict__ 
   const int t = threadIdx.x % kTPR;
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < N;
        base += static_cast<size_t>(gridDim.x) * kRows) {
-    const size_t r = base + threadIdx.x / kTPR;
-    const int label = r < N ? labels[r] : -1;
+    const size_t r = base + RowGroup<kTPR>();
+    const int label = r < N ? Uniform(labels[r]) : -1;
     const T* row = z + r * ld;
     float zl = t == 0 ? LabelLogit(row, label, C) : 0.0f;
-    const Lse a = RowLse<kTPR>(SweepLse<T, kTPR>(row, t, label < 0 ? 0 : C), lds, zl);
+    Lse a;
+    if (label >= 0) a = SweepLse<T, kTPR>(Line<T>(row, C), t);
+    a = RowLse<kTPR>(a, lds, zl);
     if (t == 0 && r < N) {
       logp[r] = label < 0 ? 0.0f : (zl - a.m) - logf(a.s);
       if (stats) stats[2 * r] = label < 0 ? 0.0f : a.m, stats[2 * r + 1] = label < 0 ? 0.0f : a.s;
@@ -169,6 +304,8 @@ TokenLogpKernel(const T* __restrict__ z, size_t ld, const int32_t* __restrict__ 
   }
 }
 
+// The last rows first: of logits that the forward pass has just read, they are
+// what the chip's last cache still holds.
 template <class T, int kTPR>
 __global__ void __launch_bounds__(GroupOf(kTPR))
 TokenLogpBwdKernel(const T* z, size_t ld, const int32_t* __restrict__ labels,
@@ -176,65 +313,125 @@ TokenLogpBwdKernel(const T* z, size_t ld, const int32_t* __restrict__ labels,
                    size_t C) {
   constexpr int kRows = GroupOf(kTPR) / kTPR;
   const int t = threadIdx.x % kTPR;
-  for (size_t r = static_cast<size_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; r < N;
-       r += static_cast<size_t>(gridDim.x) * kRows) {
-    const int label = labels[r];
+  for (size_t i = static_cast<size_t>(blockIdx.x) * kRows + RowGroup<kTPR>(); i < N;
+       i += static_cast<size_t>(gridDim.x) * kRows) {
+    const size_t r = N - 1 - i;
+    const int label = Uniform(labels[r]);
+    T* out = dz + r * ld;
     if (label < 0) {
-      SweepZero<T, kTPR>(dz + r * ld, t, C);
+      SweepZero<T, kTPR>(out, t, C);
     } else {
+      const T* row = z + r * ld;
       const float d = static_cast<size_t>(label) < C ? dlogp[r] : NAN;
-      SweepGrad<T, kTPR>(z + r * ld, dz + r * ld, t, C, label, d, stats[2 * r], 1.0f / stats[2 * r + 1]);
+      SweepGrad<T, kTPR>(Line<T>(row, C), row, out, SameGroups(row, out), t, C, label, d, stats[2 * r],
+                         stats[2 * r + 1]);
     }
   }
 }
 
-// A judged token's loss and the loss's derivative by its log-probability.
-__device__ __forceinline__ float2 PolicyToken(const PolicyTerms& P, size_t r, float logp) {
-  const float ratio = expf(logp - P.old_logp[r]), adv = P.adv[r];
-  // (a NaN passes both bounds)
-  const float held = ratio < 1.0f - P.low ? 1.0f - P.low : ratio > 1.0f + P.high ? 1.0f + P.high : ratio;
-  const float whole = ratio * adv, cut = held * adv;
-  float loss = cut < whole ? -cut : -whole, d = cut < whole ? 0.0f : -whole;
-  if (P.ref_logp) {
-    const float back = P.ref_logp[r] - logp, e = expf(back);
-    loss += P.kl * ((e - back) - 1.0f);
-    d += P.kl * (1.0f - e);
+// A judged token's numbers, read ahead of its log-probability, and its loss with
+// the derivative by it.
+struct PolicyToken {
+  float old, ref, adv, weight;
+  __device__ PolicyToken() {}
+  __device__ __forceinline__ PolicyToken(const PolicyTerms& P, size_t r)
+      : old(P.old_logp[r]), ref(P.ref_logp ? P.ref_logp[r] : 0.0f), adv(P.adv[r]),
+        weight((P.weight ? P.weight[r] : 1.0f) * P.scale) {}
+  __device__ __forceinline__ float2 At(const PolicyTerms& P, float logp) const {
+    const float ratio = expf(logp - old);
+    // (a NaN passes both bounds)
+    const float held = ratio < 1.0f - P.low ? 1.0f - P.low : ratio > 1.0f + P.high ? 1.0f + P.high : ratio;
+    const float whole = ratio * adv, cut = held * adv;
+    float loss = cut < whole ? -cut : -whole, d = cut < whole ? 0.0f : -whole;
+    if (P.ref_logp) {
+      const float back = ref - logp, e = expf(back);
+      loss += P.kl * ((e - back) - 1.0f);
+      d += P.kl * (1.0f - e);
+    }
+    return make_float2(loss, d);
   }
-  return make_float2(loss, d);
-}
+};
 
-template <class T, int kTPR>
-__global__ void __launch_bounds__(GroupOf(kTPR))
+// A row of at most kT kN groups in registers: the logits are read once and their
+// gradient written once.  kN = 0: rows of any length, read a second time (from
+// the caches, mostly) for the gradient.
+template <class T, int kT, int kN>
+__global__ void __launch_bounds__(GroupOf(kT))
 PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTerms P,
              float* __restrict__ logp, T* dz, double* __restrict__ part, size_t N, size_t C) {
-  constexpr int kRows = GroupOf(kTPR) / kTPR;
+  constexpr int kRows = GroupOf(kT) / kT, kV = Line<T>::kV;
   __shared__ float lds[33];
   __shared__ double sum[kRows];
-  const int t = threadIdx.x % kTPR;
   double mine = 0.0;  // of the row's first thread
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < N;
        base += static_cast<size_t>(gridDim.x) * kRows) {
-    const size_t r = base + threadIdx.x / kTPR;
-    const int label = r < N ? labels[r] : -1;
+    int t = threadIdx.x % kT;
+    asm volatile("" : "+v"(t));  // (its groups' offsets are formed where they are used, not kept)
+    const size_t r = base + RowGroup<kT>();
+    const int label = r < N ? Uniform(labels[r]) : -1;
     const T* row = z + r * ld;
-    float zl = t == 0 ? LabelLogit(row, label, C) : 0.0f;
-    const Lse a = RowLse<kTPR>(SweepLse<T, kTPR>(row, t, label < 0 ? 0 : C), lds, zl);
+    const Line<T> line(row, C);
+    Lse a;
+    u32x4 q[kN ? kN : 1];
+    float zl = 0.0f;
+    PolicyToken tok;
+    if (label >= 0) {
+      if (t == 0) zl = LabelLogit(row, label, C);
+      tok = PolicyToken(P, r);
+      if constexpr (kN > 0) {
+        const unsigned groups = static_cast<unsigned>(line.groups);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const unsigned g = i * kT + t;
+          q[i] = line.Read(0, g < groups ? g : groups - 1);
+        }
+        // (outside the row: -inf; groups past it all of it)
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          if (i == 0 || (i + 1u) * kT >= groups) {
+            q[i] = line.Mask(q[i], i * kT + t);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        Take<T>(a, q);
+      } else {
+        a = SweepLse<T, kT>(line, t);
+      }
+    }
+    a = RowLse<kT>(a, lds, zl);
     if (r >= N) continue;  // (no barrier is left in this turn)
+    T* out = dz + r * ld;
     if (label < 0) {
       if (t == 0 && logp) logp[r] = 0.0f;
-      if (dz) SweepZero<T, kTPR>(dz + r * ld, t, C);
+      if (dz) SweepZero<T, kT>(out, t, C);
       continue;
     }
     const float lp = (zl - a.m) - logf(a.s);
-    const float2 term = PolicyToken(P, r, lp);
-    const float w = (P.weight ? P.weight[r] : 1.0f) * P.scale;
+    const float2 term = tok.At(P, lp);
     if (t == 0) {
       if (logp) logp[r] = lp;
-      mine += static_cast<double>(w) * static_cast<double>(term.x);
+      mine += static_cast<double>(tok.weight) * static_cast<double>(term.x);
     }
-    if (dz) SweepGrad<T, kTPR>(row, dz + r * ld, t, C, label, w * term.y, a.m, 1.0f / a.s);
+    if (!dz) continue;
+    const bool same = SameGroups(row, out);
+    const float d = tok.weight * term.y;
+    if constexpr (kN > 0) {
+      const float by = -d / a.s;
+      const size_t at = static_cast<size_t>(label) + line.skip;
+      const unsigned from = line.skip ? 1 : 0, to = static_cast<unsigned>(line.end / kV);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const unsigned g = i * kT + t;
+        float v[kV];
+        GroupGrad<T>(q[i], g, at, d, by, a.m, v);
+        if (g >= from && g < to) line.Store(out, same, 0, g, v);
+        __builtin_amdgcn_sched_barrier(0);  // one group's numbers at a time
+      }
+      EdgeGrad(line, row, out, t, C, label, d, by, a.m);
+    } else {
+      SweepGrad<T, kT>(line, row, out, same, t, C, label, d, a.m, a.s);
+    }
   }
-  if (t == 0) sum[threadIdx.x / kTPR] = mine;
+  if (threadIdx.x % kT == 0) sum[threadIdx.x / kT] = mine;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int k = 1; k < kRows; ++k) mine += sum[k];
@@ -314,11 +511,30 @@ unsigned Groups(size_t rows, int per) {
   return static_cast<unsigned>(g < kMaxGroups ? g : kMaxGroups);
 }
 
+// A row's threads in the kernels that walk along it.
 template <class F>
 hipError_t ByRow(size_t N, size_t C, F&& go) {
   if (C <= 2048) return go(std::integral_constant<int, 64>{});
   if (N >= 2048) return go(std::integral_constant<int, 256>{});
   return go(std::integral_constant<int, 1024>{});
+}
+
+// A row's threads and groups a thread in registers, for rows of up to `groups`
+// 16-byte groups (one more where rows begin anywhere).
+template <class F>
+hipError_t ByRegisters(size_t N, size_t groups, F&& go) {
+#define SEEAI_ROW(t, n) go(std::integral_constant<int, t>{}, std::integral_constant<int, n>{})
+  if (groups <= 64 * 4) return SEEAI_ROW(64, 4);
+  if (groups <= 256 * 4) return SEEAI_ROW(256, 4);
+  if (N >= 512) {
+    if (groups <= 256 * 8) return SEEAI_ROW(256, 8);
+    if (groups <= 512 * 8) return SEEAI_ROW(512, 8);
+  }
+  if (groups <= 1024 * 4) return SEEAI_ROW(1024, 4);
+  if (groups <= 1024 * 8) return SEEAI_ROW(1024, 8);
+  if (groups <= 1024 * 16) return SEEAI_ROW(1024, 16);
+  return SEEAI_ROW(1024, 0);
+#undef SEEAI_ROW
 }
 
 }  // namespace
@@ -371,28 +587,32 @@ hipError_t LaunchPrefLoss(const PrefArgs& a, float* loss, void* ws, hipStream_t 
   return hipGetLastError();
 }
 
+template <class T>
+hipError_t RunPolicy(const void* z, size_t ld, const int32_t* labels, const PolicyTerms& P, float* logp,
+                     void* dz, size_t N, size_t C, double* part, size_t* parts, hipStream_t s) {
+  constexpr size_t kV = 16 / sizeof(T);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(z) | (ld * sizeof(T));
+  return ByRegisters(N, (C + kV - 1) / kV + (at % 16 ? 1 : 0), [&](auto tpr, auto held) {
+    constexpr int kT = decltype(tpr)::value, kN = decltype(held)::value, kG = GroupOf(kT);
+    const unsigned groups = Groups(N, kG / kT);
+    hipLaunchKernelGGL((PolicyKernel<T, kT, kN>), dim3(groups), dim3(kG), 0, s, static_cast<const T*>(z), ld,
+                       labels, P, logp, static_cast<T*>(dz), part, N, C);
+    *parts = groups;
+    return hipGetLastError();
+  });
+}
+
 hipError_t LaunchPolicyLoss(int bf16, const void* z, size_t ld, const int32_t* labels,
                             const PolicyTerms& P, float* loss, float* logp, void* dz, size_t N, size_t C,
                             void* ws, hipStream_t s) {
   double* part = static_cast<double*>(ws);
-  size_t groups = 0;
+  size_t parts = 0;
   if (N) {
-    const hipError_t e = ByRow(N, C, [&](auto tpr) {
-      constexpr int kT = decltype(tpr)::value, kG = GroupOf(kT);
-      groups = Groups(N, kG / kT);
-      if (bf16)
-        hipLaunchKernelGGL((PolicyKernel<uint16_t, kT>), dim3(static_cast<unsigned>(groups)), dim3(kG), 0,
-                           s, static_cast<const uint16_t*>(z), ld, labels, P, logp,
-                           static_cast<uint16_t*>(dz), part, N, C);
-      else
-        hipLaunchKernelGGL((PolicyKernel<float, kT>), dim3(static_cast<unsigned>(groups)), dim3(kG), 0, s,
-                           static_cast<const float*>(z), ld, labels, P, logp, static_cast<float*>(dz),
-                           part, N, C);
-      return hipGetLastError();
-    });
+    const hipError_t e = bf16 ? RunPolicy<uint16_t>(z, ld, labels, P, logp, dz, N, C, part, &parts, s)
+                              : RunPolicy<float>(z, ld, labels, P, logp, dz, N, C, part, &parts, s);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(SumTermsKernel, dim3(1), dim3(kSumThreads), 0, s, part, groups, 1.0, loss);
+  hipLaunchKernelGGL(SumTermsKernel, dim3(1), dim3(kSumThreads), 0, s, part, parts, 1.0, loss);
   return hipGetLastError();
 }
 
