@@ -213,28 +213,17 @@ constexpr int FwdThreads(int tpr) { return tpr > 256 ? tpr : 256; }
 // and 54, 8192 x 2048 bf16 39 both, 3001 x 1023 f32 27 and 25.
 constexpr int BwdThreads(int tpr) { return tpr > 512 ? tpr : 512; }
 
-// Sums by lane moves within registers.
-template <int kCtrl, int kRows = 0xf>
-__device__ __forceinline__ float MoveAdd(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, kRows, 0xf, false));
-}
 template <int kTPR>
 __device__ __forceinline__ float LaneSum(float v) {
-  if constexpr (kTPR < kWave) {  // over 16 or 32 lanes, each of them gets it
+  if constexpr (kTPR >= kWave) {
+    return LanesSum(v);
+  } else {  // over 16 or 32 lanes, each of them gets it
     v = MoveAdd<0xB1>(v);   // the neighbour's
     v = MoveAdd<0x4E>(v);   // the neighbouring pair's
     v = MoveAdd<0x141>(v);  // the other four of eight
     v = MoveAdd<0x140>(v);  // the other eight of sixteen
     if constexpr (kTPR == 32) v += __shfl_xor(v, 16, kWave);
     return v;
-  } else {
-    v = MoveAdd<0x111>(v);  // from 1, 2, 4, 8 lanes before, within rows of 16
-    v = MoveAdd<0x112>(v);
-    v = MoveAdd<0x114>(v);
-    v = MoveAdd<0x118>(v);
-    v = MoveAdd<0x142, 0xa>(v);  // lane 15 of a row to the next row
-    v = MoveAdd<0x143, 0xc>(v);  // lane 31 to the upper half
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
   }
 }
 // Two sums over the kTPR threads of each row; `lds` [2][2 x 16], used in turn,

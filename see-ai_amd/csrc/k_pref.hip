@@ -117,13 +117,14 @@ struct Line {
 // behind: unpacked twice it takes a quarter of the registers.
 __device__ __forceinline__ void Forget(u32x4& w) { asm volatile("" : "+v"(w)); }
 
-// Several groups at once: one new maximum for all of them.
+// The first `used` (a scalar) of several groups at once: one new maximum for all.
 template <class T, int n>
-__device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n]) {
+__device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n], int used) {
   constexpr int kV = Line<T>::kV;
   float top = a.m;
 #pragma unroll
   for (int i = 0; i < n; ++i) {
+    if (i >= used) break;
     float v[kV];
     Line<T>::Floats(w[i], v);
 #pragma unroll
@@ -137,6 +138,7 @@ __device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n]) {
   a.s *= ExpNeg(was - base);
 #pragma unroll
   for (int i = 0; i < n; ++i) {
+    if (i >= used) break;
     float v[kV];
     Line<T>::Floats(w[i], v);
 #pragma unroll
@@ -152,17 +154,17 @@ __device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n]) {
 template <int kTPR>
 __device__ __forceinline__ Lse RowLse(Lse a, float* lds, float& label) {
   Lse r;
-  r.m = WaveMaxF(a.m);
-  r.s = WaveSumF(a.s * ExpNeg(a.m - r.Base()));
-  label = __shfl(label, 0, kWave);
+  r.m = LanesMax(a.m);
+  r.s = LanesSum(a.s * ExpNeg(a.m - r.Base()));
+  label = __int_as_float(Uniform(__float_as_int(label)));
   if constexpr (kTPR > kWave) {
     constexpr int kWaves = kTPR / kWave;
     const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
     __syncthreads();  // the sums before these have been read
     if (threadIdx.x % kWave == 0) lds[2 * w] = r.m, lds[2 * w + 1] = r.s;
-    if (w == first && threadIdx.x % kWave == 0) lds[32] = label;
+    if (w == first && threadIdx.x % kWave == 0) lds[32 + w] = label;
     __syncthreads();
-    label = lds[32];
+    label = lds[32 + first];
     Lse all;
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) all.m = fmaxf(all.m, lds[2 * (first + k)]);
@@ -174,12 +176,15 @@ __device__ __forceinline__ Lse RowLse(Lse a, float* lds, float& label) {
   return r;
 }
 
-constexpr int kAhead = 4;  // groups a lane reads before it uses them
+
+// Groups a lane reads before it uses them: sixteen waves are alone on a CU.
+constexpr int Ahead(int tpr) { return tpr > 256 ? 8 : 4; }
 
 // This thread's share of a row: kAhead loads go out at a time; what may lie
 // outside the row (the first turn's first group, the last turn) is masked.
 template <class T, int kTPR>
 __device__ __forceinline__ Lse SweepLse(const Line<T>& line, int t) {
+  constexpr int kAhead = Ahead(kTPR);
   Lse a;
   for (size_t at = 0; at < line.groups; at += kAhead * kTPR) {
     u32x4 w[kAhead];
@@ -190,12 +195,14 @@ __device__ __forceinline__ Lse SweepLse(const Line<T>& line, int t) {
       const unsigned g = u * kTPR + t;
       w[u] = line.Read(at, g < left ? g : left - 1);
     }
-    if (at == 0 && !last) w[0] = line.Mask(w[0], t);
+    const int used = last ? static_cast<int>((left + kTPR - 1) / kTPR) : kAhead;
+    if (at == 0 && t == 0) w[0] = line.Mask(w[0], 0);
     if (last) {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) w[u] = line.Mask(w[u], at + u * kTPR + t);
+      for (int u = 0; u < kAhead; ++u)
+        if (u < used && u * kTPR + t + 1u >= left) w[u] = line.Mask(w[u], at + u * kTPR + t);
     }
-    Take<T>(a, w);
+    Take<T>(a, w, used);
   }
   return a;
 }
@@ -231,9 +238,11 @@ __device__ __forceinline__ void EdgeGrad(const Line<T>& line, const T* row, T* o
 template <class T, int kTPR>
 __device__ __forceinline__ void SweepGrad(const Line<T>& line, const T* row, T* out, bool same, int t, size_t C,
                                           size_t label, float d, float m, float s) {
-  constexpr int kV = Line<T>::kV;
+  constexpr int kV = Line<T>::kV, kAhead = Ahead(kTPR);
   const float by = -d / s;
-  for (size_t at = 0; at < line.groups; at += kAhead * kTPR) {
+  constexpr size_t kTurn = kAhead * kTPR;
+  for (size_t i = (line.groups + kTurn - 1) / kTurn; i-- > 0;) {  // the end, read last, first
+    const size_t at = i * kTurn;
     u32x4 w[kAhead];
     const size_t rest = line.groups - at;
     const unsigned left = rest < kAhead * kTPR ? static_cast<unsigned>(rest) : kAhead * kTPR;
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(GroupOf(kTPR))
 TokenLogpKernel(const T* __restrict__ z, size_t ld, const int32_t* __restrict__ labels,
                 float* __restrict__ logp, float* __restrict__ stats, size_t N, size_t C) {
   constexpr int kRows = GroupOf(kTPR) / kTPR;
-  __shared__ float lds[33];
+  __shared__ float lds[48];
   const int t = threadIdx.x % kTPR;
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < N;
        base += static_cast<size_t>(gridDim.x) * kRows) {
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(GroupOf(kT))
 PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTerms P,
              float* __restrict__ logp, T* dz, double* __restrict__ part, size_t N, size_t C) {
   constexpr int kRows = GroupOf(kT) / kT, kV = Line<T>::kV;
-  __shared__ float lds[33];
+  __shared__ float lds[48];
   __shared__ double sum[kRows];
   double mine = 0.0;  // of the row's first thread
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < N;
@@ -380,19 +389,22 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
       tok = PolicyToken(P, r);
       if constexpr (kN > 0) {
         const unsigned groups = static_cast<unsigned>(line.groups);
+const int used = static_cast<int>((groups + kT - 1) / kT);
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
+          if (i >= used) break;
           const unsigned g = i * kT + t;
           q[i] = line.Read(0, g < groups ? g : groups - 1);
         }
         // (outside the row: -inf; groups past it all of it)
+        if (t == 0) q[0] = line.Mask(q[0], 0);
 #pragma unroll
-        for (int i = 0; i < kN; ++i)
-          if (i == 0 || (i + 1u) * kT >= groups) {
-            q[i] = line.Mask(q[i], i * kT + t);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        Take<T>(a, q);
+        for (int i = 0; i < kN; ++i) {
+          if (i >= used) break;
+          if (i * kT + t + 1u >= groups) q[i] = line.Mask(q[i], i * kT + t);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        Take<T>(a, q, used);
       } else {
         a = SweepLse<T, kT>(line, t);
       }
@@ -420,6 +432,7 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
       const unsigned from = line.skip ? 1 : 0, to = static_cast<unsigned>(line.end / kV);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
+        if (static_cast<size_t>(i) * kT >= line.groups) break;
         const unsigned g = i * kT + t;
         float v[kV];
         GroupGrad<T>(q[i], g, at, d, by, a.m, v);
@@ -444,10 +457,23 @@ __global__ void __launch_bounds__(kSumThreads)
 SumTermsKernel(const double* __restrict__ part, size_t n, double scale, float* __restrict__ loss) {
   __shared__ double red[kSumThreads / kWave];
   double s = 0.0;
-#pragma unroll 4
-  for (size_t i = threadIdx.x; i < n; i += kSumThreads) s += part[i];
-  s = BlockSumD<kSumThreads>(s, red);
-  if (threadIdx.x == 0) *loss = static_cast<float>(scale * s);
+  for (size_t i = threadIdx.x; i < n; i += 8 * kSumThreads) {  // eight loads at a time
+    double v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const size_t at = i + k * kSumThreads;
+      v[k] = part[at < n ? at : 0];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += i + k * kSumThreads < n ? v[k] : 0.0;
+  }
+  s = WaveSumD(s);
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int k = 1; k < kSumThreads / kWave; ++k) s += red[k];
+  *loss = static_cast<float>(scale * s);
 }
 
 __device__ __forceinline__ double Softplus(double x) {
@@ -511,20 +537,27 @@ unsigned Groups(size_t rows, int per) {
   return static_cast<unsigned>(g < kMaxGroups ? g : kMaxGroups);
 }
 
-// A row's threads in the kernels that walk along it.
+// The 16-byte groups that a row of C may lie on.
+size_t RowGroups(int bf16, const void* z, size_t ld, size_t C) {
+  const size_t kV = bf16 ? 8 : 4, size = bf16 ? 2 : 4;
+  return (C + kV - 1) / kV + ((reinterpret_cast<uintptr_t>(z) | (ld * size)) % 16 ? 1 : 0);
+}
+
+// A row's threads in the kernels that walk along it: four groups each, then as
+// many as fill the chip.
 template <class F>
-hipError_t ByRow(size_t N, size_t C, F&& go) {
-  if (C <= 2048) return go(std::integral_constant<int, 64>{});
-  if (N >= 2048) return go(std::integral_constant<int, 256>{});
+hipError_t ByRow(size_t N, size_t groups, F&& go) {
+  if (groups <= 256) return go(std::integral_constant<int, 64>{});
+  if (groups <= 1024 || N >= 2048) return go(std::integral_constant<int, 256>{});
   return go(std::integral_constant<int, 1024>{});
 }
 
-// A row's threads and groups a thread in registers, for rows of up to `groups`
-// 16-byte groups (one more where rows begin anywhere).
+// A row's threads and groups a thread in registers.
 template <class F>
 hipError_t ByRegisters(size_t N, size_t groups, F&& go) {
 #define SEEAI_ROW(t, n) go(std::integral_constant<int, t>{}, std::integral_constant<int, n>{})
   if (groups <= 64 * 4) return SEEAI_ROW(64, 4);
+  if (groups <= 128 * 4) return SEEAI_ROW(128, 4);
   if (groups <= 256 * 4) return SEEAI_ROW(256, 4);
   if (N >= 512) {
     if (groups <= 256 * 8) return SEEAI_ROW(256, 8);
@@ -532,8 +565,7 @@ hipError_t ByRegisters(size_t N, size_t groups, F&& go) {
   }
   if (groups <= 1024 * 4) return SEEAI_ROW(1024, 4);
   if (groups <= 1024 * 8) return SEEAI_ROW(1024, 8);
-  if (groups <= 1024 * 16) return SEEAI_ROW(1024, 16);
-  return SEEAI_ROW(1024, 0);
+  return SEEAI_ROW(512, 0);
 #undef SEEAI_ROW
 }
 
@@ -545,7 +577,7 @@ size_t PrefWorkspaceBytes(size_t pairs) { return pairs * sizeof(double); }
 hipError_t LaunchTokenLogpFwd(int bf16, const void* z, size_t ld, const int32_t* labels, float* logp,
                               float* stats, size_t N, size_t C, hipStream_t s) {
   if (N == 0) return hipSuccess;
-  return ByRow(N, C, [&](auto tpr) {
+  return ByRow(N, RowGroups(bf16, z, ld, C), [&](auto tpr) {
     constexpr int kT = decltype(tpr)::value, kG = GroupOf(kT);
     if (bf16)
       hipLaunchKernelGGL((TokenLogpKernel<uint16_t, kT>), dim3(Groups(N, kG / kT)), dim3(kG), 0, s,
@@ -561,7 +593,7 @@ hipError_t LaunchTokenLogpBwd(int bf16, const void* z, size_t ld, const int32_t*
                               const float* stats, const float* dlogp, void* dz, size_t N, size_t C,
                               hipStream_t s) {
   if (N == 0) return hipSuccess;
-  return ByRow(N, C, [&](auto tpr) {
+  return ByRow(N, RowGroups(bf16, z, ld, C), [&](auto tpr) {
     constexpr int kT = decltype(tpr)::value, kG = GroupOf(kT);
     if (bf16)
       hipLaunchKernelGGL((TokenLogpBwdKernel<uint16_t, kT>), dim3(Groups(N, kG / kT)), dim3(kG), 0, s,
@@ -590,9 +622,7 @@ hipError_t LaunchPrefLoss(const PrefArgs& a, float* loss, void* ws, hipStream_t 
 template <class T>
 hipError_t RunPolicy(const void* z, size_t ld, const int32_t* labels, const PolicyTerms& P, float* logp,
                      void* dz, size_t N, size_t C, double* part, size_t* parts, hipStream_t s) {
-  constexpr size_t kV = 16 / sizeof(T);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(z) | (ld * sizeof(T));
-  return ByRegisters(N, (C + kV - 1) / kV + (at % 16 ? 1 : 0), [&](auto tpr, auto held) {
+  return ByRegisters(N, RowGroups(sizeof(T) == 2, z, ld, C), [&](auto tpr, auto held) {
     constexpr int kT = decltype(tpr)::value, kN = decltype(held)::value, kG = GroupOf(kT);
     const unsigned groups = Groups(N, kG / kT);
     hipLaunchKernelGGL((PolicyKernel<T, kT, kN>), dim3(groups), dim3(kG), 0, s, static_cast<const T*>(z), ld,

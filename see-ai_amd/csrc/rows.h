@@ -174,6 +174,38 @@ __device__ __forceinline__ void LoadVec(const float* w, int t, int cols, float (
   }
 }
 
+// Sums and maxima by lane moves within registers: MoveAdd adds what the DPP
+// control brings (0 where it brings nothing).
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ float MoveAdd(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, kRows, 0xf, false));
+}
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ float MoveMax(float v) {
+  const int i = __float_as_int(v);
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(i, i, kCtrl, kRows, 0xf, false)));
+}
+__device__ __forceinline__ float Lane63(float v) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+// Over the wave; every lane gets it.
+__device__ __forceinline__ float LanesSum(float v) {
+  v = MoveAdd<0x111>(v);  // from 1, 2, 4, 8 lanes before, within rows of 16
+  v = MoveAdd<0x112>(v);
+  v = MoveAdd<0x114>(v);
+  v = MoveAdd<0x118>(v);
+  v = MoveAdd<0x142, 0xa>(v);  // lane 15 of a row to the next row
+  return Lane63(MoveAdd<0x143, 0xc>(v));  // lane 31 to the upper half
+}
+__device__ __forceinline__ float LanesMax(float v) {  // (a NaN is passed over)
+  v = MoveMax<0x111>(v);
+  v = MoveMax<0x112>(v);
+  v = MoveMax<0x114>(v);
+  v = MoveMax<0x118>(v);
+  v = MoveMax<0x142, 0xa>(v);
+  return Lane63(MoveMax<0x143, 0xc>(v));
+}
+
 // Sums over the kTPR threads of each row of a workgroup: within the wave, then
 // over a row's waves through LDS (two floats a wave).
 template <int kTPR, int kN>
