@@ -3404,8 +3404,10 @@ int seeai_adamw_state_values(seeai_ctx* c, int which, int dtype, const uint8_t* 
 
 struct seeai_grad_group {
   seeai_ctx* ctx = nullptr;
-  GradGroupTensor* table = nullptr;  // device, behind the norm's partial sums
+  // Device memory: the norm's partial sums, its count of workgroups done, the table.
   double* part = nullptr;
+  unsigned* done = nullptr;
+  GradGroupTensor* table = nullptr;
   int count = 0;
   uint64_t chunks = 0;
 };
@@ -3434,16 +3436,18 @@ int seeai_grad_group_create(seeai_ctx* c, const seeai_grad_tensor* t, uint64_t c
   const size_t bytes = rows.size() * sizeof(GradGroupTensor);
   auto g = std::make_unique<seeai_grad_group>();
   void* mem = nullptr;
-  SEEAI_TRY(c, hipMalloc(&mem, parts + bytes + 16), "grad_group table");
-  uint8_t* table = static_cast<uint8_t*>(mem) + parts;
-  if (bytes)
-    if (hipError_t e = hipMemcpy(table, rows.data(), bytes, hipMemcpyHostToDevice); e != hipSuccess) {
-      (void)hipFree(mem);
-      return Hip(c, e, "grad_group table copy");
-    }
+  std::vector<uint8_t> image(16 + bytes);  // a count of zero, then the table
+  if (bytes) std::memcpy(image.data() + 16, rows.data(), bytes);
+  SEEAI_TRY(c, hipMalloc(&mem, parts + image.size()), "grad_group table");
+  uint8_t* at = static_cast<uint8_t*>(mem) + parts;
+  if (hipError_t e = hipMemcpy(at, image.data(), image.size(), hipMemcpyHostToDevice); e != hipSuccess) {
+    (void)hipFree(mem);
+    return Hip(c, e, "grad_group table copy");
+  }
   g->ctx = c;
   g->part = static_cast<double*>(mem);
-  g->table = reinterpret_cast<GradGroupTensor*>(table);
+  g->done = reinterpret_cast<unsigned*>(at);
+  g->table = reinterpret_cast<GradGroupTensor*>(at + 16);
   g->count = static_cast<int>(rows.size());
   g->chunks = chunks;
   *out = g.release();
@@ -3470,8 +3474,8 @@ int seeai_grad_group_norm(seeai_grad_group* g, float max_norm, float* norm, floa
     return Fail(c, SEEAI_INVALID, "grad_group_norm: %s", e);
   OnDevice on(c->device);
   SEEAI_TRY(c, on.status(), "grad_group_norm");
-  SEEAI_TRY(c, LaunchGradNorm(g->table, g->count, g->chunks, g->part, max_norm, norm, factor, c->flag(),
-                              c->stream),
+  SEEAI_TRY(c, LaunchGradNorm(g->table, g->count, g->chunks, g->part, g->done, max_norm, norm, factor,
+                              c->flag(), c->stream),
             "grad_group_norm");
   return SEEAI_OK;
 }

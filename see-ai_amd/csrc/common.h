@@ -410,7 +410,8 @@ hipError_t LaunchAdamWValues(int second, int bf16, const uint8_t* codes, const f
 
 // The gradients of a step (k_grad_group.hip): the device table's rows; a
 // tensor's chunks of kGradChunk elements are numbered through the group from
-// first_chunk.  part: GradNormParts doubles.
+// first_chunk.  part: GradNormParts doubles; done: a zero before the first call,
+// and again after each.
 constexpr int kGradChunk = 2048;
 struct GradGroupTensor {
   void* g;
@@ -422,7 +423,8 @@ int GradNormParts(uint64_t chunks);
 // norm (null: not wanted) = sqrt(sum of squares); with max_norm > 0 also factor
 // = min(1, max_norm / norm), and a norm that is not finite sets flag.
 hipError_t LaunchGradNorm(const GradGroupTensor* tab, int count, uint64_t chunks, double* part,
-                          float max_norm, float* norm, float* factor, int* flag, hipStream_t s);
+                          unsigned* done, float max_norm, float* norm, float* factor, int* flag,
+                          hipStream_t s);
 // g *= factor, in place, but where it is 1 or flag is set.
 hipError_t LaunchGradScale(const GradGroupTensor* tab, int count, uint64_t chunks,
                            const float* factor, const int* flag, hipStream_t s);

@@ -226,6 +226,22 @@ __device__ __forceinline__ float LaneSum(float v) {
     return v;
   }
 }
+template <int kTPR>
+__device__ __forceinline__ float RowSum1(float a, float* lds, int& turn) {
+  a = LaneSum<kTPR>(a);
+  if constexpr (kTPR > kWave) {
+    constexpr int kWaves = kTPR / kWave;
+    const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
+    float* at = lds + 32 * turn;
+    turn ^= 1;
+    if (threadIdx.x % kWave == 0) at[w] = a;
+    __syncthreads();
+    a = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) a += at[first + k];
+  }
+  return a;
+}
 // Two sums over the kTPR threads of each row; `lds` [2][2 x 16], used in turn,
 // so that one barrier keeps a sum's reads from the next one's writes.
 template <int kTPR>
@@ -247,20 +263,19 @@ __device__ __forceinline__ float2 RowSum2(float a, float b, float* lds, int& tur
 
 // v normalised in place; its mean and 1 / deviation.
 template <class T, int kTPR, int kE>
-__device__ __forceinline__ float2 Normalise(float (&v)[kE], int rms, int t, int cols, float eps,
+__device__ __forceinline__ float2 Normalise(float (&v)[kE], int rms, int t, int cols, float inv, float eps,
                                             float* lds, int& turn) {
   float mu = 0.0f, sq = 0.0f;
   if (!rms) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) mu += v[e];
-    mu = RowSum2<kTPR>(mu, 0.0f, lds, turn).x / static_cast<float>(cols);
+    mu = RowSum1<kTPR>(mu, lds, turn) * inv;
 #pragma unroll
     for (int e = 0; e < kE; ++e) v[e] = ColOf<T, kTPR, true>(t, e) < cols ? v[e] - mu : 0.0f;
   }
 #pragma unroll
   for (int e = 0; e < kE; ++e) sq += v[e] * v[e];
-  sq = RowSum2<kTPR>(sq, 0.0f, lds, turn).x;
-  const float rs = 1.0f / sqrtf(sq / static_cast<float>(cols) + eps);
+  const float rs = rsqrtf(RowSum1<kTPR>(sq, lds, turn) * inv + eps);
 #pragma unroll
   for (int e = 0; e < kE; ++e) v[e] *= rs;
   return make_float2(mu, rs);
@@ -286,6 +301,7 @@ JoinFwdKernel(JoinArgs a) {
   __shared__ float lds[64];
   constexpr int kRows = FwdThreads(kTPR) / kTPR;
   const int t = threadIdx.x % kTPR, sub = RowGroup<kTPR>(), cols = static_cast<int>(a.cols);
+  const float inv = 1.0f / static_cast<float>(cols);
   int turn = 0;
   // (the loop is uniform over the workgroup, its barriers too)
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < a.rows;
@@ -299,7 +315,7 @@ JoinFwdKernel(JoinArgs a) {
     ro.Get(t, cols, v);
     float2 so = make_float2(0.0f, 0.0f), sy = so;
     if (a.post_w) {
-      so = Normalise<T, kTPR, kE>(v, a.rms, t, cols, a.eps, lds, turn);
+      so = Normalise<T, kTPR, kE>(v, a.rms, t, cols, inv, a.eps, lds, turn);
       Scale<T, kTPR, kE>(v, a.post_w, a.post_b, t, cols);
     }
     if (a.gate) {
@@ -319,7 +335,7 @@ JoinFwdKernel(JoinArgs a) {
     for (int e = 0; e < kE; ++e) v[e] = a.res * x[e] + v[e];
     R::Store(static_cast<T*>(a.y), r, a.rows, t, cols, v);
     if (a.pre_w) {
-      sy = Normalise<T, kTPR, kE>(v, a.rms, t, cols, a.eps, lds, turn);
+      sy = Normalise<T, kTPR, kE>(v, a.rms, t, cols, inv, a.eps, lds, turn);
       Scale<T, kTPR, kE>(v, a.pre_w, a.pre_b, t, cols);
       R::Store(static_cast<T*>(a.h), r, a.rows, t, cols, v);
     }
