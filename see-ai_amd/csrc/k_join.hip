@@ -648,13 +648,14 @@ dim3 Grid(size_t groups) {  // a launch's workgroups (the kernels walk the rows 
 }
 
 template <class T, int kTPR, int kE, bool kOff>
-hipError_t Run(const JoinArgs& a, bool bwd, hipStream_t s) {
-  if (!bwd) {
-    constexpr int kThreads = FwdThreads(kTPR), kRows = kThreads / kTPR;
-    hipLaunchKernelGGL((JoinFwdKernel<T, kTPR, kE, kOff>), Grid((a.rows + kRows - 1) / kRows),
-                       dim3(kThreads), 0, s, a);
-    return hipGetLastError();
-  }
+hipError_t RunFwd(const JoinArgs& a, hipStream_t s) {
+  constexpr int kThreads = FwdThreads(kTPR), kRows = kThreads / kTPR;
+  hipLaunchKernelGGL((JoinFwdKernel<T, kTPR, kE, kOff>), Grid((a.rows + kRows - 1) / kRows), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+template <class T, int kTPR, int kE, bool kOff>
+hipError_t RunBwd(const JoinArgs& a, hipStream_t s) {
   const Plan plan = PlanOf(a.rows, a.cols, a.gate ? a.gate_rows : 0);
   if (a.rms)
     hipLaunchKernelGGL((JoinBwdKernel<T, kTPR, kE, kOff, true>), dim3(plan.bands), dim3(BwdThreads(kTPR)), 0, s, a, plan);
@@ -672,17 +673,38 @@ hipError_t Run(const JoinArgs& a, bool bwd, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Past 256 columns the forward holds 16 elements a lane: fewer waves meet in a
+// row's sums and share its vectors' loads (8 a lane and 16, bf16, us: layer norms
+// 2000 x 8192 35 and 28, 4000 x 4095 34 and 33, 8000 x 2048 26 both; 32768 x 128,
+// half the lanes without columns, 7.8 and 9.9).
+template <class T, bool kOff>
+hipError_t Forward(const JoinArgs& a, hipStream_t s) {
+  if (a.cols <= 128) return RunFwd<T, 16, 8, kOff>(a, s);
+  if (a.cols <= 256) return RunFwd<T, 32, 8, kOff>(a, s);
+  if (a.cols <= 512) return RunFwd<T, 32, 16, kOff>(a, s);
+  if (a.cols <= 1024) return RunFwd<T, 64, 16, kOff>(a, s);
+  if (a.cols <= 2048) return RunFwd<T, 128, 16, kOff>(a, s);
+  if (a.cols <= 4096) return RunFwd<T, 256, 16, kOff>(a, s);
+  if (a.cols <= 8192) return RunFwd<T, 512, 16, kOff>(a, s);
+  return RunFwd<T, 1024, 16, kOff>(a, s);
+}
+
+template <class T, bool kOff>
+hipError_t Backward(const JoinArgs& a, hipStream_t s) {
+  switch (RowThreads(a.cols)) {
+    case 16: return RunBwd<T, 16, 8, kOff>(a, s);
+    case 32: return RunBwd<T, 32, 8, kOff>(a, s);
+    case 64: return RunBwd<T, 64, 8, kOff>(a, s);
+    case 128: return RunBwd<T, 128, 8, kOff>(a, s);
+    case 256: return RunBwd<T, 256, 8, kOff>(a, s);
+    case 512: return RunBwd<T, 512, 8, kOff>(a, s);
+    default: return a.cols <= 8192 ? RunBwd<T, 1024, 8, kOff>(a, s) : RunBwd<T, 1024, 16, kOff>(a, s);
+  }
+}
+
 template <class T, bool kOff>
 hipError_t Pick(const JoinArgs& a, bool bwd, hipStream_t s) {
-  switch (RowThreads(a.cols)) {
-    case 16: return Run<T, 16, 8, kOff>(a, bwd, s);
-    case 32: return Run<T, 32, 8, kOff>(a, bwd, s);
-    case 64: return Run<T, 64, 8, kOff>(a, bwd, s);
-    case 128: return Run<T, 128, 8, kOff>(a, bwd, s);
-    case 256: return Run<T, 256, 8, kOff>(a, bwd, s);
-    case 512: return Run<T, 512, 8, kOff>(a, bwd, s);
-    default: return a.cols <= 8192 ? Run<T, 1024, 8, kOff>(a, bwd, s) : Run<T, 1024, 16, kOff>(a, bwd, s);
-  }
+  return bwd ? Backward<T, kOff>(a, s) : Forward<T, kOff>(a, s);
 }
 
 hipError_t Dispatch(int bf16, const JoinArgs& a, bool bwd, hipStream_t s) {

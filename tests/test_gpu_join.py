@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 # and 16, odd widths, gates of one row, a few, a part of a band, all rows.
 SHAPES = [(1, 1, 0), (1, 768, 1), (3, 7, 2), (5, 64, 5), (70, 512, 7), (9, 513, 1), (130, 1000, 50),
           (33, 1023, 0), (2100, 1024, 700), (2100, 96, 3), (64, 1030, 64), (40, 2048, 11), (7, 2050, 2), (37, 128, 5), (70, 130, 9), (300, 255, 100), (41, 256, 0), (9, 126, 2),
-          (600, 4096, 1000), (5, 5001, 3), (3, 8192, 2), (4, 8193, 0), (3, 16384, 1), (2, 16383, 2),
+          (600, 4096, 1000), (5, 5001, 3), (3, 8192, 2), (4, 8193, 0), (3, 16384, 1), (35, 511, 6), (20, 1025, 0), (11, 4097, 3), (2, 16383, 2),
           (4100, 320, 1025), (5000, 40, 1), (5000, 17, 33), (129, 6, 4), (6000, 202, 1500), (2049, 2048, 1)]
 # kind, post norm, pre norm, biases
 FORMS = [(0, 1, 1, 1), (1, 1, 1, 0), (0, 1, 0, 0), (1, 0, 1, 0), (0, 0, 1, 1), (1, 1, 0, 0)]
