@@ -218,6 +218,32 @@ def test_block_join(hip, ctx, torch_cuda, form, bf16, off):
         assert torch.equal(y2, y) and (not pre or torch.equal(h2, h))
 
 
+@pytest.mark.parametrize("which", [("o",), ("y", "h"), ("dx",), ("dh", "do")])
+def test_block_join_of_tensors_that_lie_differently(hip, ctx, torch_cuda, which):
+    """Some operands off a dword, the others on it: the bits of operands all on 16 bytes."""
+    torch = torch_cuda
+    t = torch.bfloat16
+    for rows, cols in ((40, 128), (37, 514), (9, 4098), (300, 30)):
+        d = inputs(torch, 0, 1, 1, 1, rows, cols, 7, t, 0)
+        y, h, st = forward(hip, ctx, torch, 0, 1, d, rows, cols, 7)
+        dh, dy = put(torch, gen(torch, 1)(rows, cols), t), put(torch, gen(torch, 2)(rows, cols), t)
+        want = backward(hip, ctx, torch, 0, 1, d, 7, y, st, dh, dy)
+        at = lambda name: Guarded(torch, (rows, cols), t, int(name in which))  # noqa: E731
+        o, gy, gh, gdx, gdo, gdh = (at(k) for k in ("o", "y", "h", "dx", "do", "dh"))
+        o.t.copy_(d["o"]), gdh.t.copy_(dh)
+        j = struct(hip, 0, 1, d | {"o": o.t}, rows, cols, 7)
+        p = hip.ptr
+        ctx.call("seeai_block_join_fwd", j, p(gy.t), p(gh.t), p(st))
+        assert torch.equal(gy.t, y) and torch.equal(gh.t, h) and gy.intact() and gh.intact()
+        n = hip.lib().seeai_block_join_workspace(rows, cols, 7)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+        grads = {k: torch.empty_like(want[k]) for k in NAMES[2:]}
+        ctx.call("seeai_block_join_bwd", j, p(gy.t), p(st), p(gdh.t), p(dy),
+                 hip.BlockJoinGrads(p(gdx.t), p(gdo.t), *(p(grads[k]) for k in NAMES[2:])), p(ws), n)
+        assert torch.equal(gdx.t, want["dx"]) and torch.equal(gdo.t, want["do"]) and gdx.intact() and gdo.intact()
+        assert all(torch.equal(grads[k], want[k]) for k in NAMES[2:])
+
+
 def test_block_join_without_some_gradients(hip, ctx, torch_cuda):
     torch = torch_cuda
     for rows, cols, gate_rows in ((300, 264, 100), (300, 264, 2), (5, 64, 5)):

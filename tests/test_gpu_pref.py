@@ -88,7 +88,7 @@ def check_logits_grad(torch, got, z, labels, d, e_d, p, e_p, step):
 LOGITS = [(1, 1, 1), (3, 2, 5), (1, 64, 64), (7, 511, 511), (70, 513, 520), (5, 2047, 2050), (9, 2048, 2048),
           (4, 2049, 2049), (33, 4001, 4003), (2, 8192, 8192), (3, 8193, 8200), (2100, 2112, 2112),
           (2, 32000, 32000), (2049, 2051, 2051), (3, 32769, 32770), (2, 65537, 65540), (1, 128000, 128000),
-          (2, 131073, 131080)]
+          (2, 131073, 131080), (600, 9001, 9001), (520, 17000, 17000), (513, 29999, 30002), (1, 40000, 40000)]
 
 
 @pytest.mark.parametrize("off", [0, 1])
@@ -117,6 +117,33 @@ def test_token_logp(ctx, torch_cuda, bf16, off):
         keep = out.t[:, :V].clone()
         token_logp_bwd(ctx, torch, buf.t, ld, labels, stats, dlogp, V, buf.t)  # in place
         assert torch.equal(buf.t[:, :V], keep) and buf.t[:, V:].isnan().all()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_gradients_where_the_logits_lie_otherwise(hip, ctx, torch_cuda, bf16):
+    """A gradient buffer whose rows begin elsewhere within 16 bytes than the logits', and
+    gradients too large for the last cache."""
+    torch = torch_cuda
+    t, step = types(torch, bf16)
+    cases = [(5, 1000, 1000), (3, 9001, 9003), (4, 70000, 70000), (2, 7, 9), (9, 33, 33)]
+    for N, V, ld in cases + ([(4400, 16001, 16001)] if bf16 else [(2200, 16000, 16000)]):
+        buf, labels, old, ref, adv, weight = policy_inputs(torch, N, V, ld, bf16, V)
+        same, other = Guarded(torch, (N, ld), t), Guarded(torch, (N, ld), t, 3)
+        _, stats = token_logp(ctx, torch, buf.t, ld, labels, V)
+        dlogp = gen(torch, 5)(N)
+        for out in (same, other):
+            token_logp_bwd(ctx, torch, buf.t, ld, labels, stats, dlogp, V, out.t)
+            assert out.intact() and (out.t[:, V:] == 7).all()
+        assert torch.equal(same.t, other.t)
+        if N > 1000:
+            rows = list(range(0, N, N // 20))
+            _, _, p, e_p = softmax64(torch, buf.t[rows, :V], labels[rows])
+            check_logits_grad(torch, same.t[rows, :V], buf.t[rows, :V], labels[rows], dlogp[rows],
+                              torch.zeros(len(rows), dtype=torch.float64, device="cuda"), p, e_p, step)
+        for out in (same, other):
+            policy_loss(hip, ctx, torch, buf.t, ld, labels, old, ref, adv, weight, V, 0.1, 1.0, out.t)
+            assert out.intact() and (out.t[:, V:] == 7).all()
+        assert torch.equal(same.t, other.t)
 
 
 def test_token_logp_of_masked_and_odd_logits(ctx, torch_cuda):
@@ -235,7 +262,8 @@ def pref64(torch, logp, ref, labels, starts, beta, offset, eps, average, scale):
 
 # Sequences' lengths: pairs of one token, none, long ones; rows before and behind.
 PAIRS = [([1, 1], 0, 0), ([5, 0], 2, 3), ([0, 0], 1, 0), ([64, 65, 511, 513], 0, 7),
-         ([1000, 3000, 1, 2, 0, 9], 11, 70), ([7] * 130, 0, 0), ([40000, 20000], 5, 1)]
+         ([1000, 3000, 1, 2, 0, 9], 11, 70), ([7] * 130, 0, 0), ([40000, 20000], 5, 1), ([3] * 600, 2, 1),
+         ([511] * 4, 1, 3), ([600, 500, 400, 300, 200, 40], 0, 8), ([90] * 22, 0, 9)]
 
 
 @pytest.mark.parametrize("average", [0, 1])
