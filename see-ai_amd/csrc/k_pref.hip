@@ -17,6 +17,10 @@
 // other rows first) and the gradient written once.  A row whose label is
 // negative is not judged: it is not read, and its gradient is zero.
 // Everything between is f32, sums over rows and the pairs' terms are f64.
+// 8192 x 32000 bf16 with 70 % of the rows judged, on MI355X: log-probabilities 66
+// us (5.5 TB/s; a copy runs 5.1), their backward 147 (6.0, part of the logits from
+// the last cache), the policy loss with its gradient 160 (5.6, VALU issue 68 %
+// busy).
 #include <type_traits>
 
 #include "rows.h"
@@ -178,7 +182,7 @@ __device__ __forceinline__ Lse RowLse(Lse a, float* lds, float& label) {
 }
 
 
-// Groups a lane reads before it uses them: sixteen waves are alone on a CU.
+// Groups a lane reads before it uses them: more where few rows share a CU.
 constexpr int Ahead(int tpr) { return tpr > 256 ? 8 : 4; }
 
 // This thread's share of a row: kAhead loads go out at a time; what may lie
@@ -713,7 +717,8 @@ hipError_t LaunchTokenLogpBwd(int bf16, const void* z, size_t ld, const int32_t*
 
 hipError_t LaunchPrefLoss(const PrefArgs& a, float* loss, void* ws, hipStream_t s) {
   double* terms = static_cast<double*>(ws);
-  // One launch up to here (us, one and two: 8 pairs of 8192 rows 0 and 0).
+  // One launch while one CU's loads keep up (us, one against two kernels: 4 pairs of
+  // 701 rows 6.6 and 5.8 + 2.2, 8 of 8192 12.0 and 7.2 + 1.8, 32 of 16384 20 and 6.5 + 2).
   if (a.pairs && a.pairs <= kOnePairs && a.N <= kOneRows) {
     hipLaunchKernelGGL(PrefOneKernel, dim3(1), dim3(kOneThreads), 0, s, a, loss);
     return hipGetLastError();
