@@ -521,9 +521,9 @@ int seeai_block_join_bwd(seeai_ctx* ctx, const seeai_block_join* join, const voi
  * No reference counterpart.  Logits [N, C] in `dtype`, rows `ld` >= C elements
  * apart, of any alignment; the gradients likewise, and they may take the logits'
  * place (d_dlogits = d_logits).  What lies between rows is left as it is and
- * counts for nothing (a row is read by whole aligned 16 bytes).  A row whose label is negative is not judged: its logits are not
- * read, its log-probability is 0 and its gradient zero.  A label from C on makes
- * its row's results NaN. */
+ * counts for nothing (a row is read by whole aligned 16 bytes).  A row whose
+ * label is negative is not judged: its logits are not read, its log-probability
+ * is 0 and its gradient zero.  A label from C on makes its row's results NaN. */
 
 /* logp[r] = log softmax(logits[r])[label], d_stats [N, 2] (or NULL) the row's
  * maximum and sum of exp(logit - maximum), for the backward pass. */

@@ -35,10 +35,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float ExpNeg(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // A running maximum and the sum of exp(z - max) under it.  While all z are -inf
-// the maximum is, too, and the sum zero; a NaN or +inf makes the sum a NaN.
+// the maximum is, too, and the sum zero; a NaN or +inf makes the sum a NaN.  A
+// group's terms add up in pairs, groups in f64: where one token is nearly sure the
+// sum is 1 and little more, and its logarithm as small as f32's roundings on 1.
 struct Lse {
-  float m = -INFINITY, s = 0.0f;
+  float m = -INFINITY;
+  double s = 0.0;
   __device__ __forceinline__ float Base() const { return m == -INFINITY ? 0.0f : m; }
+  // log softmax of a logit: log s from its leading bits and the rest.
+  __device__ __forceinline__ float Logp(float z) const {
+    const float lead = static_cast<float>(s);
+    const float rest = static_cast<float>(s - static_cast<double>(lead)) / lead;
+    return ((z - m) - logf(lead)) - rest;
+  }
 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -140,14 +149,19 @@ __device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n], int used) {
   const float was = a.m;
   a.m = top;
   const float base = a.Base();
-  a.s *= ExpNeg(was - base);
+  a.s *= static_cast<double>(ExpNeg(was - base));
 #pragma unroll
   for (int i = 0; i < n; ++i) {
     if (i >= used) break;
     float v[kV];
     Line<T>::Floats(w[i], v);
 #pragma unroll
-    for (int k = 0; k < kV; ++k) a.s += ExpNeg(v[k] - base);
+    for (int k = 0; k < kV; ++k) v[k] = ExpNeg(v[k] - base);
+#pragma unroll
+    for (int n2 = kV / 2; n2 > 0; n2 /= 2)
+#pragma unroll
+      for (int k = 0; k < n2; ++k) v[k] += v[k + n2];
+    a.s += static_cast<double>(v[0]);
     Forget(w[i]);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -156,31 +170,33 @@ __device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n], int used) {
 // The row's maximum and sum from its kTPR threads'; `label` of the row's first
 // thread (the label's logit, read before any thread may write over it) comes to
 // all of them.
+struct RowLds {
+  double s[16];
+  float m[16], label[16];
+};
 template <int kTPR>
-__device__ __forceinline__ Lse RowLse(Lse a, float* lds, float& label) {
+__device__ __forceinline__ Lse RowLse(Lse a, RowLds& lds, float& label) {
   Lse r;
   r.m = LanesMax(a.m);
-  r.s = LanesSum(a.s * ExpNeg(a.m - r.Base()));
+  r.s = LanesSumD(a.s * static_cast<double>(ExpNeg(a.m - r.Base())));
   label = __int_as_float(Uniform(__float_as_int(label)));
   if constexpr (kTPR > kWave) {
     constexpr int kWaves = kTPR / kWave;
     const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
     __syncthreads();  // the sums before these have been read
-    if (threadIdx.x % kWave == 0) lds[2 * w] = r.m, lds[2 * w + 1] = r.s;
-    if (w == first && threadIdx.x % kWave == 0) lds[32 + w] = label;
+    if (threadIdx.x % kWave == 0) lds.m[w] = r.m, lds.s[w] = r.s, lds.label[w] = label;
     __syncthreads();
-    label = lds[32 + first];
+    label = lds.label[first];
     Lse all;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) all.m = fmaxf(all.m, lds[2 * (first + k)]);
+    for (int k = 0; k < kWaves; ++k) all.m = fmaxf(all.m, lds.m[first + k]);
     const float base = all.Base();
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) all.s += lds[2 * (first + k) + 1] * ExpNeg(lds[2 * (first + k)] - base);
+    for (int k = 0; k < kWaves; ++k) all.s += lds.s[first + k] * static_cast<double>(ExpNeg(lds.m[first + k] - base));
     r = all;
   }
   return r;
 }
-
 
 // Groups a lane reads before it uses them: more where few rows share a CU.
 constexpr int Ahead(int tpr) { return tpr > 256 ? 8 : 4; }
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(GroupOf(kTPR))
 TokenLogpKernel(const T* __restrict__ z, size_t ld, const int32_t* __restrict__ labels,
                 float* __restrict__ logp, float* __restrict__ stats, size_t N, size_t C) {
   constexpr int kRows = GroupOf(kTPR) / kTPR;
-  __shared__ float lds[48];
+  __shared__ RowLds lds;
   const int t = threadIdx.x % kTPR;
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < N;
        base += static_cast<size_t>(gridDim.x) * kRows) {
@@ -312,8 +328,8 @@ TokenLogpKernel(const T* __restrict__ z, size_t ld, const int32_t* __restrict__ 
     if (label >= 0) a = SweepLse<T, kTPR>(Line<T>(row, C), t);
     a = RowLse<kTPR>(a, lds, zl);
     if (t == 0 && r < N) {
-      logp[r] = label < 0 ? 0.0f : (zl - a.m) - logf(a.s);
-      if (stats) stats[2 * r] = label < 0 ? 0.0f : a.m, stats[2 * r + 1] = label < 0 ? 0.0f : a.s;
+      logp[r] = label < 0 ? 0.0f : a.Logp(zl);
+      if (stats) stats[2 * r] = label < 0 ? 0.0f : a.m, stats[2 * r + 1] = label < 0 ? 0.0f : static_cast<float>(a.s);
     }
   }
 }
@@ -374,7 +390,7 @@ __global__ void __launch_bounds__(GroupOf(kT))
 PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTerms P,
              float* __restrict__ logp, T* dz, bool past, double* __restrict__ part, size_t N, size_t C) {
   constexpr int kRows = GroupOf(kT) / kT, kV = Line<T>::kV;
-  __shared__ float lds[48];
+  __shared__ RowLds lds;
   __shared__ double sum[kRows];
   double mine = 0.0;  // of the row's first thread
   for (size_t base = static_cast<size_t>(blockIdx.x) * kRows; base < N;
@@ -422,7 +438,7 @@ const int used = static_cast<int>((groups + kT - 1) / kT);
       if (dz) SweepZero<T, kT>(out, past, t, C);
       continue;
     }
-    const float lp = (zl - a.m) - logf(a.s);
+    const float lp = a.Logp(zl);
     const float2 term = tok.At(P, lp);
     if (t == 0) {
       if (logp) logp[r] = lp;
@@ -432,7 +448,7 @@ const int used = static_cast<int>((groups + kT - 1) / kT);
     const int how = StoreHow(row, out, past);
     const float d = tok.weight * term.y;
     if constexpr (kN > 0) {
-      const float by = -d / a.s;
+      const float by = -d / static_cast<float>(a.s);
       const size_t at = static_cast<size_t>(label) + line.skip;
       const unsigned from = line.skip ? 1 : 0, to = static_cast<unsigned>(line.end / kV);
 #pragma unroll
@@ -446,7 +462,7 @@ const int used = static_cast<int>((groups + kT - 1) / kT);
       }
       EdgeGrad(line, row, out, t, C, label, d, by, a.m);
     } else {
-      SweepGrad<T, kT>(line, row, out, how, t, C, label, d, a.m, a.s);
+      SweepGrad<T, kT>(line, row, out, how, t, C, label, d, a.m, static_cast<float>(a.s));
     }
   }
   if (threadIdx.x % kT == 0) sum[threadIdx.x / kT] = mine;

@@ -197,6 +197,22 @@ __device__ __forceinline__ float LanesSum(float v) {
   v = MoveAdd<0x142, 0xa>(v);  // lane 15 of a row to the next row
   return Lane63(MoveAdd<0x143, 0xc>(v));  // lane 31 to the upper half
 }
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ double MoveAddD(double v) {
+  const int lo = __double2loint(v), hi = __double2hiint(v);
+  return v + __hiloint2double(__builtin_amdgcn_update_dpp(0, hi, kCtrl, kRows, 0xf, false),
+                              __builtin_amdgcn_update_dpp(0, lo, kCtrl, kRows, 0xf, false));
+}
+__device__ __forceinline__ double LanesSumD(double v) {
+  v = MoveAddD<0x111>(v);
+  v = MoveAddD<0x112>(v);
+  v = MoveAddD<0x114>(v);
+  v = MoveAddD<0x118>(v);
+  v = MoveAddD<0x142, 0xa>(v);
+  v = MoveAddD<0x143, 0xc>(v);
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63),
+                          __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
 __device__ __forceinline__ float LanesMax(float v) {  // (a NaN is passed over)
   v = MoveMax<0x111>(v);
   v = MoveMax<0x112>(v);

@@ -189,6 +189,26 @@ def test_token_logp_of_masked_and_odd_logits(ctx, torch_cuda):
             assert out.t[12, -1] == 0  # a sure token has no gradient
 
 
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_token_logp_of_a_nearly_sure_token(ctx, torch_cuda, bf16):
+    """The sum is 1 and a little: its small logarithm keeps its own digits.  The group that holds
+    the 1 rounds three times, the other terms and their rescalings (to a thread's, a wave's and a
+    row's maximum) by (3 |d| + 2) u each, all else is f64."""
+    torch = torch_cuda
+    t, _ = types(torch, bf16)
+    for N, V in ((64, 40), (64, 4000), (700, 32000), (3, 131000), (64, 32001)):
+        z = (gen(torch, V)(N, V) - math.log(V) - 4.0).to(t)
+        labels = torch.randint(0, V, (N,), device="cuda").to(torch.int32)
+        z[torch.arange(N), labels.long()] = 1.0
+        logp, _ = token_logp(ctx, torch, z, V, labels, V)
+        d = z.double() - 1.0
+        p = torch.exp(d).scatter(1, labels.long()[:, None], 0.0)
+        want = -torch.log1p(p.sum(1))
+        bound = U * (3.5 + (p * (12 * d.abs() + 10)).sum(1) + 6 * want.abs())
+        assert float(bound.max()) < 0.05 * float(want.abs().min())
+        within(torch, logp, want, bound)
+
+
 def test_token_logp_past_32_bit_offsets(ctx, torch_cuda):
     """Over 2^32 bytes and 2^31 elements: the last rows are the formula's."""
     torch = torch_cuda
