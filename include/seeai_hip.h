@@ -442,7 +442,7 @@ int seeai_adamw_group_step_scaled(seeai_adamw_group* group, const seeai_step_par
 int seeai_adamw_state_values(seeai_ctx* ctx, int which, int dtype, const uint8_t* d_codes,
                              const float* d_scales, uint64_t n, void* d_out);
 /* The global norm of a step's gradients: many tensors, f32 and bf16 beside each
- * other, in two launches.  The verdicts are those of seeai_adamw_step's clip. */
+ * other, in one launch or two.  The verdicts are those of seeai_adamw_step's clip. */
 typedef struct seeai_grad_tensor {
   void* g;
   uint64_t n;

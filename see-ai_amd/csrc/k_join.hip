@@ -49,12 +49,11 @@ __device__ __forceinline__ float UniformF(float v) {
 // width) go through buffer ranges.  With a wave or more a row the range is
 // exactly the row, its address a scalar: a dword past it reads as zero and is
 // not stored, each dword by itself, so no access asks where the row ends.  With
-// several rows a wave (kTPR 16 or 32, one group a lane) the range is the wave's
-// rows, neighbours in memory, lanes past their row's columns point past it, and
-// a row's last, short group is cut by hand.  Other bf16 rows (kOff) are read 16
-// bytes at a time from wherever they lie; the row's last, short group reads the
-// row's last 16 bytes and is shifted into place, so its load, too, can run ahead
-// of its use.
+// several rows a wave (kTPR 16 or 32) the range is the wave's rows, neighbours in
+// memory, lanes past their row's columns point past it, and a row's last, short
+// group is cut by hand.  Other bf16 rows (kOff) are read 16 bytes at a time from
+// wherever they lie; the row's last, short group reads the row's last 16 bytes
+// and is shifted into place, so its load, too, can run ahead of its use.
 template <class T, int kTPR, int kE, bool kOff>
 struct Row {
   static constexpr int kV = Io<T>::kV, kN = kE / kV, kSize = sizeof(T);

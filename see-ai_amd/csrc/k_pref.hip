@@ -16,10 +16,11 @@
 // Bound by HBM: the logits read once (twice where a gradient needs a sum over
 // other rows first) and the gradient written once.  A row whose label is
 // negative is not judged: it is not read, and its gradient is zero.
-// Everything between is f32, sums over rows and the pairs' terms are f64.
+// Everything between is f32; sums along a row past its groups of 16 bytes, sums
+// over rows and the pairs' terms are f64.
 // 8192 x 32000 bf16 with 70 % of the rows judged, on MI355X: log-probabilities 66
 // us (5.5 TB/s; a copy runs 5.1), their backward 147 (6.0, part of the logits from
-// the last cache), the policy loss with its gradient 160 (5.6, VALU issue 68 %
+// the last cache), the policy loss with its gradient 161 (5.5, VALU issue 69 %
 // busy).
 #include <type_traits>
 
@@ -410,7 +411,7 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
       tok = PolicyToken(P, r);
       if constexpr (kN > 0) {
         const unsigned groups = static_cast<unsigned>(line.groups);
-const int used = static_cast<int>((groups + kT - 1) / kT);
+        const int used = static_cast<int>((groups + kT - 1) / kT);
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
           if (i >= used) break;
