@@ -375,9 +375,16 @@ struct PolicyToken {
     const float whole = ratio * adv, cut = held * adv;
     float loss = cut < whole ? -cut : -whole, d = cut < whole ? 0.0f : -whole;
     if (P.ref_logp) {
+      // Near the reference e - back - 1 is about back^2 / 2, which differences of
+      // numbers near 1 would lose: there its series, whose first missing term is
+      // back^6 2 / 8!, 2^-26 of the sum at 1/4.
       const float back = ref - logp, e = expf(back);
-      loss += P.kl * ((e - back) - 1.0f);
-      d += P.kl * (1.0f - e);
+      const bool near = fabsf(back) < 0.25f;
+      const float row = 1.0f + back * (1.0f / 3) * (1.0f + back * 0.25f * (1.0f + back * 0.2f *
+                        (1.0f + back * (1.0f / 6) * (1.0f + back * (1.0f / 7)))));
+      const float curve = near ? 0.5f * back * back * row : (e - back) - 1.0f;
+      loss += P.kl * curve;
+      d -= P.kl * (near ? back + curve : e - 1.0f);
     }
     return make_float2(loss, d);
   }

@@ -473,6 +473,31 @@ def test_policy_sides_of_the_clip(hip, ctx, torch_cuda):
     assert abs(float(loss) + float((held * adv).sum())) < 32 * U * float((held * adv).abs().sum())
 
 
+def test_policy_near_the_reference(hip, ctx, torch_cuda):
+    """A KL term is about half the square of a small difference of log-probabilities:
+    it keeps its digits.  The difference is rounded once (twice that in its square),
+    the square twice, the series' end once and its steps by a twelfth of theirs, off
+    by 2^-26 = U / 4, the sum once: within 8 U of the loss; the derivative, the
+    difference and a part of at most a seventh of that, within 4 U."""
+    torch = torch_cuda
+    N, V = 64, 40
+    buf, labels = token_inputs(torch, N, V, V, 0, 77)
+    live, zeros = labels >= 0, torch.zeros(N, device="cuda")
+    call = lambda old, ref, out: policy_loss(hip, ctx, torch, buf.t, V, labels, old, ref, zeros, None,  # noqa: E731
+                                             V, 1.0, 1.0, out)
+    lp = call(zeros, zeros, None)[1]
+    _, _, p, e_p = softmax64(torch, buf.t, labels)
+    for far in (1e-5, 1e-3, 0.1, 0.2499):
+        print(f"policy near the reference {far}", flush=True)
+        ref, out = lp + far * torch.linspace(-1, 1, N, device="cuda"), torch.empty_like(buf.t)
+        loss, again = call(lp, ref, out)
+        assert torch.equal(again, lp)
+        back = torch.where(live, ref.double() - lp.double(), 0.0)
+        L, d = (torch.expm1(back) - back).sum().view(1), -torch.expm1(back)
+        within(torch, loss, L, 8 * U * L)
+        check_logits_grad(torch, out, buf.t, labels, d, 4 * U * d.abs(), p, e_p, U)
+
+
 def test_policy_with_odd_values(hip, ctx, torch_cuda):
     """A NaN or an infinity stays in its row, though not out of the loss."""
     torch = torch_cuda
