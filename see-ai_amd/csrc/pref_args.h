@@ -68,7 +68,7 @@ inline const char* CheckPolicyLoss(int dtype, const void* z, uint64_t ld, const 
   if (N && !ref && kl != 0.0f) return "a KL term needs ref_logp";
   if (ws_bytes < need) return "workspace too small (seeai_policy_workspace)";
   const uint64_t span = LogitsSpan(ld, N, C), size = TypeSize(dtype);
-  return CheckOperands({{z, z == dz ? 0 : span, size, false}, {labels, N, 4, false},
+  return CheckOperands({{z, dz && z == dz ? 0 : span, size, false}, {labels, N, 4, false},
                         {old_logp, N, 4, false}, {ref, ref ? N : 0, 4, false}, {adv, N, 4, false},
                         {weight, weight ? N : 0, 4, false}, {loss, 1, 4, true},
                         {logp, logp ? N : 0, 4, true}, {dz, dz ? span : 0, size, true},

@@ -307,3 +307,18 @@ def test_grad_group_wrapper(hip):
     with pytest.raises(ValueError, match="factor"):
         step.step(hip.StepParams(), Fake(n=2))
     step.h = None
+
+
+def test_policy_logits_are_there_without_a_gradient(checks):
+    """No gradient wanted is not a gradient in the logits' place."""
+    def ask(p, N=4):
+        return checks("policy", 1, p, u(8), u(N), u(8), 0.2, 0.2, 0.1, 1.0, u(32), u(32))
+    p = spread(10)
+    p[0] = p[8] = 0
+    assert b"null" in ask(p)
+    assert ask([0] * 6 + [1 << 30, 0, 0, 2 << 30], N=0) is None
+    p = spread(10)
+    p[8] = 0
+    assert ask(p) is None
+    p[8] = p[0]
+    assert ask(p) is None
