@@ -3548,7 +3548,8 @@ int seeai_policy_loss(seeai_ctx* c, int dtype, const void* z, uint64_t ld, const
     return Fail(c, SEEAI_INVALID, "policy_loss: %s", e);
   OnDevice on(c->device);
   SEEAI_TRY(c, on.status(), "policy_loss");
-  const PolicyTerms P{old_logp, ref, adv, weight, low, high, kl, scale};
+  // (a coefficient of zero takes the reference out, infinite terms and all)
+  const PolicyTerms P{old_logp, kl != 0.0f ? ref : nullptr, adv, weight, low, high, kl, scale};
   SEEAI_TRY(c, LaunchPolicyLoss(dtype, z, ld, labels, P, loss, logp, dz, N, C, ws, c->stream), "policy_loss");
   return SEEAI_OK;
 }

@@ -1,0 +1,50 @@
+"""GPU: where the losses from logits come to the ends of their ranges -- nearly sure
+labels, far margins, coefficients of zero, ratios and KL terms past f32 -- and the
+joins' column sums past 32-bit offsets, against plain float64.
+
+Tolerances are bounds on what the kernels' own roundings may add up to, as in
+test_gpu_pref.py and test_gpu_join.py: u = 2^-24 for each f32 operation, 2^-8 of the
+value for a rounding to bf16, exp(x) within (3 |x| + 2) u of itself."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+from tests.test_gpu_block import U, Guarded, ctx, gen, types, within  # noqa: F401
+from tests.test_gpu_join import DEPTH, NAMES, back64, struct
+from tests.test_gpu_pref import (policy64, policy_loss, pref_loss, softmax64, token_inputs, token_logp,
+                                 token_logp_bwd)
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+# --- coefficients of zero, and terms past f32 -----------------------------------------------------
+
+def rows_of_tokens(hip, ctx, torch, V, N=12):
+    z = gen(torch, V)(N, V)
+    labels = torch.full((N,), 4, dtype=torch.int32, device="cuda")
+    lp, _ = token_logp(ctx, torch, z, V, labels, V)
+    return z, labels, lp, gen(torch, 1)(N), gen(torch, 2)(N).abs() + 0.1
+
+
+def call_policy(hip, ctx, torch, z, labels, old, ref, adv, weight, kl):
+    out = torch.empty_like(z)
+    loss, lp = policy_loss(hip, ctx, torch, z, z.shape[1], labels, old, ref, adv, weight, z.shape[1], kl, 1.0, out)
+    return loss, lp, out
+
+
+@pytest.mark.parametrize("V", [30, 5000, 40000])
+def test_a_kl_coefficient_of_zero_takes_the_reference_out(hip, ctx, torch_cuda, V):
+    """Tokens that the reference rules out, or has far above the policy, and a NaN: the
+    bits of the call without a reference."""
+    torch = torch_cuda
+    z, labels, lp, adv, weight = rows_of_tokens(hip, ctx, torch, V)
+    old, ref = lp + 0.01, lp.clone()
+    ref[1], ref[2], ref[3], ref[4] = -INF, lp[2] + 200, NAN, INF
+    z[5, 4] = -INF  # the policy rules the label out
+    want = call_policy(hip, ctx, torch, z, labels, old, None, adv, weight, 0.0)
+    got = call_policy(hip, ctx, torch, z, labels, old, ref, adv, weight, 0.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.isfinite(v).all() for v in (got[0], got[2]))
