@@ -382,7 +382,8 @@ struct PolicyToken {
       const bool near = fabsf(back) < 0.25f;
       const float row = 1.0f + back * (1.0f / 3) * (1.0f + back * 0.25f * (1.0f + back * 0.2f *
                         (1.0f + back * (1.0f / 6) * (1.0f + back * (1.0f / 7)))));
-      const float curve = near ? 0.5f * back * back * row : (e - back) - 1.0f;
+      // (infinite where back is, on either side)
+      const float curve = near ? 0.5f * back * back * row : e == INFINITY ? e : (e - back) - 1.0f;
       loss += P.kl * curve;
       d -= P.kl * (near ? back + curve : e - 1.0f);
     }

@@ -48,3 +48,20 @@ def test_a_kl_coefficient_of_zero_takes_the_reference_out(hip, ctx, torch_cuda, 
     want = call_policy(hip, ctx, torch, z, labels, old, None, adv, weight, 0.0)
     got = call_policy(hip, ctx, torch, z, labels, old, ref, adv, weight, 0.0)
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.isfinite(v).all() for v in (got[0], got[2]))
+
+
+@pytest.mark.parametrize("V", [30, 5000])
+def test_the_kl_term_of_a_token_that_the_policy_rules_out(hip, ctx, torch_cuda, V):
+    """exp(back) - back - 1 is an infinity where back is, on either side."""
+    torch = torch_cuda
+    for side in (0, 1):
+        z, labels, lp, adv, weight = rows_of_tokens(hip, ctx, torch, V)
+        old, ref = lp + 0.01, lp + 0.02
+        if side:
+            ref[3] = -INF
+        else:
+            z[3, 4] = -INF
+        loss, got, out = call_policy(hip, ctx, torch, z, labels, old, ref, adv, weight, 0.1)
+        assert float(loss) == INF and bool(got[3] == -INF) == (side == 0)
+        others = [i for i in range(12) if i != 3]
+        assert torch.isfinite(out[others]).all() and (side == 0 or torch.isfinite(out[3]).all())
