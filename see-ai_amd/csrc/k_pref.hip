@@ -372,7 +372,8 @@ struct PolicyToken {
     const float ratio = expf(logp - old);
     // (a NaN passes both bounds)
     const float held = ratio < 1.0f - P.low ? 1.0f - P.low : ratio > 1.0f + P.high ? 1.0f + P.high : ratio;
-    const float whole = ratio * adv, cut = held * adv;
+    // (a ratio past f32 beside an advantage of zero: no term)
+    const float whole = adv == 0.0f && ratio == INFINITY ? 0.0f : ratio * adv, cut = held * adv;
     float loss = cut < whole ? -cut : -whole, d = cut < whole ? 0.0f : -whole;
     if (P.ref_logp) {
       // Near the reference e - back - 1 is about back^2 / 2, which differences of

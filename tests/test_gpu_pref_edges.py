@@ -51,6 +51,21 @@ def test_a_kl_coefficient_of_zero_takes_the_reference_out(hip, ctx, torch_cuda, 
 
 
 @pytest.mark.parametrize("V", [30, 5000])
+def test_an_advantage_of_zero_beside_a_far_ratio(hip, ctx, torch_cuda, V):
+    """Answers no better and no worse than the rest of their group: no term, however far
+    the policy has moved (a ratio past f32)."""
+    torch = torch_cuda
+    z, labels, lp, adv, weight = rows_of_tokens(hip, ctx, torch, V)
+    old = lp + 0.01
+    adv[3], adv[5] = 0.0, -0.0
+    want = call_policy(hip, ctx, torch, z, labels, old, None, adv, weight, 0.0)
+    old[3], old[5] = lp[3] - 100, lp[5] - 1e4
+    got = call_policy(hip, ctx, torch, z, labels, old, None, adv, weight, 0.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.isfinite(got[2]).all()
+    assert not got[2][[3, 5]].any()
+
+
+@pytest.mark.parametrize("V", [30, 5000])
 def test_the_kl_term_of_a_token_that_the_policy_rules_out(hip, ctx, torch_cuda, V):
     """exp(back) - back - 1 is an infinity where back is, on either side."""
     torch = torch_cuda
