@@ -558,8 +558,8 @@ int seeai_pref_loss(seeai_ctx* ctx, const float* d_logp, const float* d_ref_logp
  *       + kl_coef (e - (ref_logp - logp) - 1)
  *   loss = scale sum over judged rows of weight l
  * A kl_coef of 0 is without the KL term, whatever d_ref_logp holds; d_ref_logp
- * NULL (kl_coef 0) likewise; d_weight NULL: ones; d_logp [N] and d_dlogits may be
- * NULL. */
+ * NULL (kl_coef 0) likewise; d_weight NULL: ones, and a row of weight 0 takes no
+ * part, whatever its other numbers are; d_logp [N] and d_dlogits may be NULL. */
 uint64_t seeai_policy_workspace(uint64_t N, uint64_t C);
 int seeai_policy_loss(seeai_ctx* ctx, int dtype, const void* d_logits, uint64_t ld,
                       const int32_t* d_labels, const float* d_old_logp, const float* d_ref_logp,

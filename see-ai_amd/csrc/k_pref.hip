@@ -369,6 +369,7 @@ struct PolicyToken {
       : old(P.old_logp[r]), ref(P.ref_logp ? P.ref_logp[r] : 0.0f), adv(P.adv[r]),
         weight((P.weight ? P.weight[r] : 1.0f) * P.scale) {}
   __device__ __forceinline__ float2 At(const PolicyTerms& P, float logp) const {
+    if (weight == 0.0f) return make_float2(0.0f, 0.0f);  // whatever the rest is
     const float ratio = expf(logp - old);
     // (a NaN passes both bounds)
     const float held = ratio < 1.0f - P.low ? 1.0f - P.low : ratio > 1.0f + P.high ? 1.0f + P.high : ratio;

@@ -66,6 +66,24 @@ def test_an_advantage_of_zero_beside_a_far_ratio(hip, ctx, torch_cuda, V):
 
 
 @pytest.mark.parametrize("V", [30, 5000])
+def test_a_weight_of_zero_takes_its_row_out(hip, ctx, torch_cuda, V):
+    """Whatever its other numbers are; its log-probability is given all the same."""
+    torch = torch_cuda
+    z, labels, lp, adv, weight = rows_of_tokens(hip, ctx, torch, V)
+    old, ref = lp + 0.01, lp + 0.02
+    off = [2, 3, 4, 5, 6]
+    weight[off] = 0.0
+    old[2], adv[2] = lp[2] - 100, -1.0  # a term past f32
+    ref[3] = lp[3] + 200
+    old[4], adv[5], ref[6] = NAN, INF, NAN
+    out = call_policy(hip, ctx, torch, z, labels, old, ref, adv, weight, 0.1)
+    labels[off] = -1
+    want = call_policy(hip, ctx, torch, z, labels, old, ref, adv, weight, 0.1)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[2], want[2]) and torch.isfinite(out[2]).all()
+    within(torch, out[1], lp, U * lp.abs())
+
+
+@pytest.mark.parametrize("V", [30, 5000])
 def test_the_kl_term_of_a_token_that_the_policy_rules_out(hip, ctx, torch_cuda, V):
     """exp(back) - back - 1 is an infinity where back is, on either side."""
     torch = torch_cuda
