@@ -524,10 +524,12 @@ struct Pair {
     margin = beta * (chosen - rejected) - P.offset;
     // softplus(x) = max(x, 0) + log(1 + exp(-|x|)), sigmoid by the same exponential.
     const double e = exp(-fabs(margin)), tail = log1p(e), up = margin > 0.0 ? margin : 0.0;
-    const double down = margin < 0.0 ? -margin : 0.0, won = (margin < 0.0 ? e : 1.0) / (1.0 + e);
+    const double down = margin < 0.0 ? -margin : 0.0;
+    const double won = (margin < 0.0 ? e : 1.0) / (1.0 + e), lost = (margin > 0.0 ? e : 1.0) / (1.0 + e);
     // (a smoothing of zero takes no part in an infinite margin)
     term = (eps < 1.0 ? (1.0 - eps) * (down + tail) : 0.0) + (eps > 0.0 ? eps * (up + tail) : 0.0);
-    d = P.scale * beta * (won - (1.0 - eps));
+    // won - (1 - eps), without the difference from 1 where the chosen answer is far ahead.
+    d = P.scale * beta * (eps * won - (1.0 - eps) * lost);
   }
 };
 

@@ -21,6 +21,28 @@ pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
 
 
+# --- far margins ----------------------------------------------------------------------------------
+
+def test_pairs_of_far_margins_keep_their_gradient(hip, ctx, torch_cuda):
+    """scale beta (eps - sigmoid(-margin)) is exp(-margin) where the chosen answer is far
+    ahead and nothing is smoothed: its digits are its own, not those of a difference
+    from 1."""
+    torch = torch_cuda
+    for lengths in ([1, 1] * 9, [700, 700] * 9):  # one workgroup for all pairs, and one a pair
+        margins = torch.tensor([-80.0, -40.0, -20.0, -3.0, 0.0, 3.0, 20.0, 40.0, 80.0], dtype=torch.float64)
+        N = sum(lengths)
+        starts = torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+        logp = torch.zeros(N, device="cuda")
+        logp[starts[0:-1:2].long()] = margins.float().cuda()  # the chosen answers' first tokens
+        labels = torch.zeros(N, dtype=torch.int32, device="cuda")
+        for eps, sign in ((0.0, 1.0), (1.0, -1.0)):
+            got = pref_loss(hip, ctx, torch, logp, None, labels, starts, 1.0, 0.0, eps, 0, 1.0)
+            want = -sign * torch.sigmoid(-sign * margins).cuda()
+            d = got[2][starts[0:-1:2].long()]
+            within(torch, d, want, (U + 1e-14) * want.abs())
+            assert torch.equal(got[2][starts[1::2].long()], -d)
+
+
 # --- coefficients of zero, and terms past f32 -----------------------------------------------------
 
 def rows_of_tokens(hip, ctx, torch, V, N=12):
