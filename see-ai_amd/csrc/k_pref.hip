@@ -35,19 +35,26 @@ constexpr float kLog2e = 1.4426950408889634f;
 // |x| 2^-24 of itself, and terms far down hardly count.
 __device__ __forceinline__ float ExpNeg(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// A running maximum and the sum of exp(z - max) under it.  While all z are -inf
-// the maximum is, too, and the sum zero; a NaN or +inf makes the sum a NaN.  A
-// group's terms add up in pairs, groups in f64: where one token is nearly sure the
-// sum is 1 and little more, and its logarithm as small as f32's roundings on 1.
+// A running maximum and the sum of exp(z - max) under it, of a row's logits but the
+// label's.  While all z are -inf the maximum is, too, and the sum zero; a NaN or
+// +inf makes the sum a NaN.  A group's terms add up in pairs, groups in f64.
 struct Lse {
   float m = -INFINITY;
   double s = 0.0;
   __device__ __forceinline__ float Base() const { return m == -INFINITY ? 0.0f : m; }
-  // log softmax of a logit: log s from its leading bits and the rest.
-  __device__ __forceinline__ float Logp(float z) const {
-    const float lead = static_cast<float>(s);
-    const float rest = static_cast<float>(s - static_cast<double>(lead)) / lead;
-    return ((z - m) - logf(lead)) - rest;
+};
+
+// The whole row, from the sum of the others under the row's maximum and the label's
+// logit: the sum, and the label's log-probability.  Where the label is nearly sure
+// the sum is 1 and a little, and the log-probability as small: the logarithm of the
+// sum's leading bits, and what they leave of that little, which has its own digits as
+// the label stands apart from it.
+struct Soft {
+  float m, s, logp;
+  __device__ __forceinline__ Soft(const Lse& others, float zl) : m(others.m) {
+    const float own = ExpNeg(zl - others.Base());
+    s = static_cast<float>(others.s + static_cast<double>(own));
+    logp = ((zl - m) - logf(s)) - static_cast<float>(others.s - static_cast<double>(s - own)) * __builtin_amdgcn_rcpf(s);
   }
 };
 
@@ -87,6 +94,17 @@ struct Line {
       } else {
         w[k / 2] = out ? (w[k / 2] & 0xFFFF0000u) | 0xFF80u : w[k / 2];
       }
+    }
+    return w;
+  }
+  // Element `at` (a scalar) of a group becomes -inf.
+  static __device__ __forceinline__ u32x4 Without(u32x4 w, int at) {
+    const uint32_t keep = sizeof(T) == 4 ? 0u : at % 2 ? 0xFFFFu : 0xFFFF0000u;
+    const uint32_t low = sizeof(T) == 4 || at % 2 ? 0xFF800000u : 0xFF80u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool here = at * static_cast<int>(sizeof(T)) / 4 == k;
+      w[k] = (w[k] & (here ? keep : ~0u)) | (here ? low : 0u);
     }
     return w;
   }
@@ -132,6 +150,21 @@ struct Line {
 // behind: unpacked twice it takes a quarter of the registers.
 __device__ __forceinline__ void Forget(u32x4& w) { asm volatile("" : "+v"(w)); }
 
+// Of n groups, kStep apart from this thread's on, the one that is group `own` of
+// them all (a scalar) loses its element `at`.  Branches, a scalar's and then a lane's:
+// as selects they would be formed for every group.
+template <class T, int kStep, int n>
+__device__ __forceinline__ void DropLabel(u32x4 (&w)[n], unsigned own, int at, int t) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    if (own / kStep != static_cast<unsigned>(i)) continue;
+    if (t == static_cast<int>(own % kStep)) {
+      Forget(w[i]);
+      w[i] = Line<T>::Without(w[i], at);
+    }
+  }
+}
+
 // The first `used` (a scalar) of several groups at once: one new maximum for all.
 template <class T, int n>
 __device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n], int used) {
@@ -168,9 +201,9 @@ __device__ __forceinline__ void Take(Lse& a, u32x4 (&w)[n], int used) {
   }
 }
 
-// The row's maximum and sum from its kTPR threads'; `label` of the row's first
-// thread (the label's logit, read before any thread may write over it) comes to
-// all of them.
+// The row's maximum and the sum of all but its label under it, from its kTPR threads';
+// `label` of the row's first thread (the label's logit, read before any thread may
+// write over it) comes to all of them.
 struct RowLds {
   double s[16];
   float m[16], label[16];
@@ -178,9 +211,10 @@ struct RowLds {
 template <int kTPR>
 __device__ __forceinline__ Lse RowLse(Lse a, RowLds& lds, float& label) {
   Lse r;
-  r.m = LanesMax(a.m);
-  r.s = LanesSumD(a.s * static_cast<double>(ExpNeg(a.m - r.Base())));
   label = __int_as_float(Uniform(__float_as_int(label)));
+  r.m = LanesMax(a.m);
+  if constexpr (kTPR == kWave) r.m = fmaxf(r.m, label);
+  r.s = LanesSumD(a.s * static_cast<double>(ExpNeg(a.m - r.Base())));
   if constexpr (kTPR > kWave) {
     constexpr int kWaves = kTPR / kWave;
     const int w = threadIdx.x / kWave, first = w / kWaves * kWaves;
@@ -189,6 +223,7 @@ __device__ __forceinline__ Lse RowLse(Lse a, RowLds& lds, float& label) {
     __syncthreads();
     label = lds.label[first];
     Lse all;
+    all.m = fmaxf(all.m, label);
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) all.m = fmaxf(all.m, lds.m[first + k]);
     const float base = all.Base();
@@ -202,11 +237,12 @@ __device__ __forceinline__ Lse RowLse(Lse a, RowLds& lds, float& label) {
 // Groups a lane reads before it uses them: more where few rows share a CU.
 constexpr int Ahead(int tpr) { return tpr > 256 ? 8 : 4; }
 
-// This thread's share of a row: kAhead loads go out at a time; what may lie
-// outside the row (the first turn's first group, the last turn) is masked.
+// This thread's share of a row but its label (`label` from the line's first group
+// on): kAhead loads go out at a time; what may lie outside the row (the first
+// turn's first group, the last turn) is masked.
 template <class T, int kTPR>
-__device__ __forceinline__ Lse SweepLse(const Line<T>& line, int t) {
-  constexpr int kAhead = Ahead(kTPR);
+__device__ __forceinline__ Lse SweepLse(const Line<T>& line, size_t label, int t) {
+  constexpr int kAhead = Ahead(kTPR), kV = Line<T>::kV;
   Lse a;
   for (size_t at = 0; at < line.groups; at += kAhead * kTPR) {
     u32x4 w[kAhead];
@@ -224,6 +260,8 @@ __device__ __forceinline__ Lse SweepLse(const Line<T>& line, int t) {
       for (int u = 0; u < kAhead; ++u)
         if (u < used && u * kTPR + t + 1u >= left) w[u] = line.Mask(w[u], at + u * kTPR + t);
     }
+    if (label / kV - at < kAhead * kTPR)  // (far past this turn's where it lies before)
+      DropLabel<T, kTPR>(w, static_cast<unsigned>(label / kV - at), static_cast<int>(label % kV), t);
     Take<T>(a, w, used);
   }
   return a;
@@ -326,11 +364,15 @@ TokenLogpKernel(const T* __restrict__ z, size_t ld, const int32_t* __restrict__ 
     const T* row = z + r * ld;
     float zl = t == 0 ? LabelLogit(row, label, C) : 0.0f;
     Lse a;
-    if (label >= 0) a = SweepLse<T, kTPR>(Line<T>(row, C), t);
+    if (label >= 0) {
+      const Line<T> line(row, C);
+      a = SweepLse<T, kTPR>(line, static_cast<size_t>(label) + line.skip, t);
+    }
     a = RowLse<kTPR>(a, lds, zl);
     if (t == 0 && r < N) {
-      logp[r] = label < 0 ? 0.0f : a.Logp(zl);
-      if (stats) stats[2 * r] = label < 0 ? 0.0f : a.m, stats[2 * r + 1] = label < 0 ? 0.0f : static_cast<float>(a.s);
+      const Soft all(a, zl);
+      logp[r] = label < 0 ? 0.0f : all.logp;
+      if (stats) stats[2 * r] = label < 0 ? 0.0f : all.m, stats[2 * r + 1] = label < 0 ? 0.0f : all.s;
     }
   }
 }
@@ -416,6 +458,7 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
     u32x4 q[kN ? kN : 1];
     float zl = 0.0f;
     PolicyToken tok;
+    const size_t at = static_cast<size_t>(label) + line.skip;  // (a judged row's)
     if (label >= 0) {
       if (t == 0) zl = LabelLogit(row, label, C);
       tok = PolicyToken(P, r);
@@ -436,9 +479,10 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
           if (i * kT + t + 1u >= groups) q[i] = line.Mask(q[i], i * kT + t);
           __builtin_amdgcn_sched_barrier(0);
         }
+        DropLabel<T, kT>(q, static_cast<unsigned>(at / kV), static_cast<int>(at % kV), t);
         Take<T>(a, q, used);
       } else {
-        a = SweepLse<T, kT>(line, t);
+        a = SweepLse<T, kT>(line, at, t);
       }
     }
     a = RowLse<kT>(a, lds, zl);
@@ -449,31 +493,30 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
       if (dz) SweepZero<T, kT>(out, past, t, C);
       continue;
     }
-    const float lp = a.Logp(zl);
-    const float2 term = tok.At(P, lp);
+    const Soft all(a, zl);
+    const float2 term = tok.At(P, all.logp);
     if (t == 0) {
-      if (logp) logp[r] = lp;
+      if (logp) logp[r] = all.logp;
       mine += static_cast<double>(tok.weight) * static_cast<double>(term.x);
     }
     if (!dz) continue;
     const int how = StoreHow(row, out, past);
     const float d = tok.weight * term.y;
     if constexpr (kN > 0) {
-      const float by = -d / static_cast<float>(a.s);
-      const size_t at = static_cast<size_t>(label) + line.skip;
+      const float by = -d / all.s, own = by * ExpNeg(zl - all.m) + d;
       const unsigned from = line.skip ? 1 : 0, to = static_cast<unsigned>(line.end / kV);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         if (static_cast<size_t>(i) * kT >= line.groups) break;
         const unsigned g = i * kT + t;
         float v[kV];
-        GroupGrad<T>(q[i], g, at, d, by, a.m, v);
+        GroupGrad<T>(q[i], g, at, own, by, all.m, v);
         if (g >= from && g < to) line.Store(out, how, 0, g, v);
         __builtin_amdgcn_sched_barrier(0);  // one group's numbers at a time
       }
-      EdgeGrad(line, row, out, t, C, label, d, by, a.m);
+      EdgeGrad(line, row, out, t, C, label, d, by, all.m);
     } else {
-      SweepGrad<T, kT>(line, row, out, how, t, C, label, d, a.m, static_cast<float>(a.s));
+      SweepGrad<T, kT>(line, row, out, how, t, C, label, d, all.m, all.s);
     }
   }
   if (threadIdx.x % kT == 0) sum[threadIdx.x / kT] = mine;

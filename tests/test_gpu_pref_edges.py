@@ -21,6 +21,57 @@ pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
 
 
+# --- nearly sure labels ---------------------------------------------------------------------------
+
+# Rows of a wave, of four and sixteen waves, walked and in registers; the label's
+# neighbours within 16 bytes are terms like all others, wherever the row begins.
+SURE = [(64, 3, 3, 0), (64, 40, 40, 0), (64, 41, 43, 1), (64, 2000, 2000, 0), (700, 2113, 2113, 1),
+        (64, 4000, 4000, 0), (3, 32001, 32003, 1), (700, 32000, 32000, 0), (520, 50001, 50001, 1),
+        (3, 131000, 131000, 0), (2, 131073, 131080, 1)]
+
+
+def sure_inputs(torch, N, V, ld, off, bf16, gap):
+    """Rows whose labels, anywhere in them, are sure but for about exp(-gap)."""
+    t, step = types(torch, bf16)
+    buf = Guarded(torch, (N, ld), t, off)
+    buf.t.fill_(NAN)
+    z = 0.5 * gen(torch, V + ld)(N, V) - math.log(V) - gap + 1.0
+    labels = torch.randint(0, V, (N,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+    labels[0], labels[-1] = 0, V - 1
+    z[torch.arange(N), labels] = 1.0
+    buf.t[:, :V] = z.to(t)
+    d = buf.t[:, :V].double() - 1.0
+    e = torch.exp(d).scatter(1, labels[:, None], 0.0)  # the others, beside the label's 1
+    return buf, labels.to(torch.int32), d, e, step
+
+
+def sure_logp(d, e):
+    """-log(1 + the others' sum), and its bound: each of the others' terms within
+    (3 |d| + 2) u, the rescalings to higher maxima on their way (together as far, 2 u
+    for each of at most 11), three additions within 16 bytes, then f64; a rounding of the
+    sum and a logarithm good to 4 u."""
+    want = -e.sum(1).log1p()
+    return want, U * ((e * (6 * d.abs() + 30)).sum(1) + 6 * want.abs())
+
+
+@pytest.mark.parametrize("gap", [6.0, 14.0, 21.0])
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_a_nearly_sure_label_beside_its_neighbours(hip, ctx, torch_cuda, bf16, gap):
+    """However little is left beside the label, and wherever it lies, the
+    log-probability keeps its own digits."""
+    torch = torch_cuda
+    for N, V, ld, off in SURE:
+        buf, labels, d, e, _ = sure_inputs(torch, N, V, ld, off, bf16, gap)
+        want, bound = sure_logp(d, e)
+        logp, stats = token_logp(ctx, torch, buf.t, ld, labels, V)
+        within(torch, logp, want, bound)
+        assert (stats[:, 0] == 1).all()
+        within(torch, stats[:, 1], 1 + e.sum(1), bound + 2 * U)
+        zeros = torch.zeros(N, device="cuda")
+        _, again = policy_loss(hip, ctx, torch, buf.t, ld, labels, zeros, None, zeros, None, V, 0.0, 1.0)
+        within(torch, again, want, bound)
+
+
 # --- far margins ----------------------------------------------------------------------------------
 
 def test_pairs_of_far_margins_keep_their_gradient(hip, ctx, torch_cuda):
