@@ -50,8 +50,8 @@ struct Lse {
 // sum's leading bits, and what they leave of that little, which has its own digits as
 // the label stands apart from it.
 struct Soft {
-  float m, s, logp;
-  __device__ __forceinline__ Soft(const Lse& others, float zl) : m(others.m) {
+  float m, s, logp, rest;  // rest: s without the label's term
+  __device__ __forceinline__ Soft(const Lse& others, float zl) : m(others.m), rest(static_cast<float>(others.s)) {
     const float own = ExpNeg(zl - others.Base());
     s = static_cast<float>(others.s + static_cast<double>(own));
     logp = ((zl - m) - logf(s)) - static_cast<float>(others.s - static_cast<double>(s - own)) * __builtin_amdgcn_rcpf(s);
@@ -267,39 +267,54 @@ __device__ __forceinline__ Lse SweepLse(const Line<T>& line, size_t label, int t
   return a;
 }
 
-// dz = d (1[c = l] - exp(z - m) / s) for a group: by = -d / s; `label` counts
-// from the line's first group.
+// dz = -d exp(z - m) / s for a group, by = -d / s; whether the label lies in it, at `at`.
 template <class T>
-__device__ __forceinline__ void GroupGrad(u32x4 w, unsigned g, size_t label, float d, float by, float m,
-                                          float (&v)[Line<T>::kV]) {
+__device__ __forceinline__ bool GroupGrad(u32x4 w, unsigned g, size_t label, float by, float m,
+                                          float (&v)[Line<T>::kV], int& at) {
   constexpr int kV = Line<T>::kV;
   Line<T>::Floats(w, v);
 #pragma unroll
   for (int k = 0; k < kV; ++k) v[k] = by * ExpNeg(v[k] - m);
-  if (label / kV <= 0xFFFFFFFFu && g == static_cast<unsigned>(label / kV)) {
-    const int at = static_cast<int>(label % kV);
+  at = static_cast<int>(label % kV);
+  return label / kV <= 0xFFFFFFFFu && g == static_cast<unsigned>(label / kV);
+}
+template <int kV>
+__device__ __forceinline__ void PutAt(float (&v)[kV], int at, float x) {
 #pragma unroll
-    for (int k = 0; k < kV; ++k)
-      if (k == at) v[k] += d;
+  for (int k = 0; k < kV; ++k)
+    if (k == at) v[k] = x;
+}
+
+// The label's own gradient is d (1 - p), where a nearly sure label's 1 - p has to
+// come from the others' terms: `own`, d rest / s, where that rest is known.
+// Where it is not (kSum), d - d p, and the row's other gradients add up (a thread's
+// in `sum`): they are less than half of d where p is more than a half, and then the
+// label's gradient is minus their sum.  `mine`: this thread has stored the label's.
+struct RowGrad {
+  float d, own, by, m;
+  double sum = 0.0;
+  bool mine = false;
+};
+
+// One column's gradient, by itself: what groups that are not whole hold.
+template <class T, bool kSum>
+__device__ __forceinline__ void EdgeGrad(const Line<T>& line, const T* row, T* out, int t, size_t C, size_t label,
+                                         RowGrad& G) {
+  const size_t c = line.Edge(t, C);
+  if (c >= C) return;
+  const float v = G.by * ExpNeg(Io<T>::Get(row + c) - G.m);
+  Io<T>::Put(out + c, c != label ? v : kSum ? v + G.d : G.own);
+  if constexpr (kSum) {
+    if (c == label) G.mine = true;
+    else G.sum += static_cast<double>(v);
   }
 }
 
-// One column's gradient, by itself: what groups that are not whole hold.
-template <class T>
-__device__ __forceinline__ void EdgeGrad(const Line<T>& line, const T* row, T* out, int t, size_t C, size_t label,
-                                         float d, float by, float m) {
-  const size_t c = line.Edge(t, C);
-  if (c >= C) return;
-  const float v = by * ExpNeg(Io<T>::Get(row + c) - m);
-  Io<T>::Put(out + c, c == label ? v + d : v);
-}
-
 // A lane's groups are read before they are written, so out may be the row.
-template <class T, int kTPR>
+template <class T, int kTPR, bool kSum>
 __device__ __forceinline__ void SweepGrad(const Line<T>& line, const T* row, T* out, int how, int t, size_t C,
-                                          size_t label, float d, float m, float s) {
+                                          size_t label, RowGrad& G) {
   constexpr int kV = Line<T>::kV, kAhead = Ahead(kTPR);
-  const float by = -d / s;
   constexpr size_t kTurn = kAhead * kTPR;
   for (size_t i = (line.groups + kTurn - 1) / kTurn; i-- > 0;) {  // the end, read last, first
     const size_t at = i * kTurn;
@@ -317,12 +332,29 @@ __device__ __forceinline__ void SweepGrad(const Line<T>& line, const T* row, T* 
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const unsigned g = u * kTPR + t;
-      float v[kV];
-      GroupGrad<T>(w[u], g, lab, d, by, m, v);
+      float v[kV], own = G.own;
+      int k;
+      const bool here = GroupGrad<T>(w[u], g, lab, G.by, G.m, v, k);
+      if constexpr (kSum) {
+        if (here) {
+#pragma unroll
+          for (int e = 0; e < kV; ++e)
+            if (e == k) own = v[e] + G.d, v[e] = 0.0f;
+        }
+        float part[kV];
+#pragma unroll
+        for (int e = 0; e < kV; ++e) part[e] = v[e];
+#pragma unroll
+        for (int n = kV / 2; n > 0; n /= 2)
+#pragma unroll
+          for (int e = 0; e < n; ++e) part[e] += part[e + n];
+        if (g >= from && g < to) G.sum += static_cast<double>(part[0]), G.mine |= here;
+      }
+      if (here) PutAt(v, k, own);
       if (g >= from && g < to) line.Store(out, how, at, g, v);
     }
   }
-  EdgeGrad(line, row, out, t, C, label, d, by, m);
+  EdgeGrad<T, kSum>(line, row, out, t, C, label, G);
 }
 template <class T, int kTPR>
 __device__ __forceinline__ void SweepZero(T* out, bool past, int t, size_t C) {
@@ -384,8 +416,11 @@ __global__ void __launch_bounds__(GroupOf(kTPR))
 TokenLogpBwdKernel(const T* z, size_t ld, const int32_t* __restrict__ labels,
                    const float* __restrict__ stats, const float* __restrict__ dlogp, T* dz, bool past,
                    size_t N, size_t C) {
-  constexpr int kRows = GroupOf(kTPR) / kTPR;
+  constexpr int kRows = GroupOf(kTPR) / kTPR, kWaves = kTPR / kWave;
+  static_assert(kWaves == 1 || kRows == 1, "a row's barriers are its workgroup's");
+  __shared__ double lds[2][kWaves];  // used in turn: one barrier a row
   const int t = threadIdx.x % kTPR;
+  int turn = 0;
   for (size_t i = static_cast<size_t>(blockIdx.x) * kRows + RowGroup<kTPR>(); i < N;
        i += static_cast<size_t>(gridDim.x) * kRows) {
     const size_t r = N - 1 - i;
@@ -395,9 +430,19 @@ TokenLogpBwdKernel(const T* z, size_t ld, const int32_t* __restrict__ labels,
       SweepZero<T, kTPR>(out, past, t, C);
     } else {
       const T* row = z + r * ld;
-      const float d = static_cast<size_t>(label) < C ? dlogp[r] : NAN;
-      SweepGrad<T, kTPR>(Line<T>(row, C), row, out, StoreHow(row, out, past), t, C, label, d, stats[2 * r],
-                         stats[2 * r + 1]);
+      RowGrad G{static_cast<size_t>(label) < C ? dlogp[r] : NAN, 0.0f, 0.0f, stats[2 * r]};
+      G.by = -G.d / stats[2 * r + 1];
+      SweepGrad<T, kTPR, true>(Line<T>(row, C), row, out, StoreHow(row, out, past), t, C, label, G);
+      double sum = LanesSumD(G.sum);
+      if constexpr (kWaves > 1) {
+        if (threadIdx.x % kWave == 0) lds[turn][threadIdx.x / kWave] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) sum += lds[turn][k];
+        turn ^= 1;
+      }
+      if (G.mine && fabs(sum) < 0.5 * fabs(static_cast<double>(G.d))) Io<T>::Put(out + label, static_cast<float>(-sum));
     }
   }
 }
@@ -502,21 +547,23 @@ PolicyKernel(const T* z, size_t ld, const int32_t* __restrict__ labels, PolicyTe
     if (!dz) continue;
     const int how = StoreHow(row, out, past);
     const float d = tok.weight * term.y;
+    RowGrad G{d, 0.0f, -d / all.s, all.m};
+    G.own = -G.by * all.rest;
     if constexpr (kN > 0) {
-      const float by = -d / all.s, own = by * ExpNeg(zl - all.m) + d;
       const unsigned from = line.skip ? 1 : 0, to = static_cast<unsigned>(line.end / kV);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         if (static_cast<size_t>(i) * kT >= line.groups) break;
         const unsigned g = i * kT + t;
         float v[kV];
-        GroupGrad<T>(q[i], g, at, own, by, all.m, v);
+        int k;
+        if (GroupGrad<T>(q[i], g, at, G.by, G.m, v, k)) PutAt(v, k, G.own);
         if (g >= from && g < to) line.Store(out, how, 0, g, v);
         __builtin_amdgcn_sched_barrier(0);  // one group's numbers at a time
       }
-      EdgeGrad(line, row, out, t, C, label, d, by, all.m);
+      EdgeGrad<T, false>(line, row, out, t, C, label, G);
     } else {
-      SweepGrad<T, kT>(line, row, out, how, t, C, label, d, all.m, all.s);
+      SweepGrad<T, kT, false>(line, row, out, how, t, C, label, G);
     }
   }
   if (threadIdx.x % kT == 0) sum[threadIdx.x / kT] = mine;

@@ -72,6 +72,38 @@ def test_a_nearly_sure_label_beside_its_neighbours(hip, ctx, torch_cuda, bf16, g
         within(torch, again, want, bound)
 
 
+@pytest.mark.parametrize("gap", [6.0, 14.0, 21.0])
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_a_nearly_sure_label_keeps_its_gradient(hip, ctx, torch_cuda, bf16, gap):
+    """The label's element is d (1 - p): small beside d, but as near to itself as the
+    others' d p, whose sum it is.  Those are within (3 |d| + 2) u, the row's sum and
+    the division 2 u each, a product, three additions within 16 bytes."""
+    torch = torch_cuda
+    t, _ = types(torch, bf16)
+    for N, V, ld, off in SURE:
+        buf, labels, d, e, step = sure_inputs(torch, N, V, ld, off, bf16, gap)
+        row = torch.arange(N, device="cuda")
+        p = e / (1 + e.sum(1, keepdim=True))
+        rest, e_rest = p.sum(1), U * (p * (3 * d.abs() + 12)).sum(1)
+        _, stats = token_logp(ctx, torch, buf.t, ld, labels, V)
+        dlogp = gen(torch, 5)(N)
+        out = Guarded(torch, (N, ld), t, off)
+        token_logp_bwd(ctx, torch, buf.t, ld, labels, stats, dlogp, V, out.t)
+        got, dd = out.t[row, labels.long()], dlogp.double()
+        within(torch, got, dd * rest, dd.abs() * (e_rest + step * (rest + e_rest)))
+        assert out.intact() and (out.t[:, V:] == 7).all()
+        # The policy loss, from the log-probabilities that it gives itself.
+        adv, old = gen(torch, 6)(N), torch.full((N,), -0.05, device="cuda")
+        _, lp = policy_loss(hip, ctx, torch, buf.t, ld, labels, old, None, adv, None, V, 0.0, 1.0, out.t)
+        _, _, dd, e_d = policy64(torch, lp, torch.zeros_like(dd), labels, old, None, adv, None, 0.0, 1.0)
+        rest = -torch.expm1(lp.double())
+        bound = e_d * rest + dd.abs() * 8 * U * rest
+        within(torch, out.t[row, labels.long()], dd * rest, bound + step * ((dd * rest).abs() + bound))
+        keep = out.t.clone()
+        policy_loss(hip, ctx, torch, buf.t, ld, labels, old, None, adv, None, V, 0.0, 1.0, buf.t)
+        assert torch.equal(buf.t[:, :V], keep[:, :V])
+
+
 # --- far margins ----------------------------------------------------------------------------------
 
 def test_pairs_of_far_margins_keep_their_gradient(hip, ctx, torch_cuda):
