@@ -104,6 +104,21 @@ def test_a_nearly_sure_label_keeps_its_gradient(hip, ctx, torch_cuda, bf16, gap)
         assert torch.equal(buf.t[:, :V], keep[:, :V])
 
 
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_wide_rows_add_up_in_64_bits(ctx, torch_cuda, bf16):
+    """Of a sum's roundings only the exponentials' own count, and three additions
+    within 16 bytes, however wide the row is."""
+    torch = torch_cuda
+    for N, V, ld, off in ((600, 9001, 9001, 1), (520, 50001, 50001, 0), (2, 131073, 131080, 1), (1, 262144, 262144, 0)):
+        buf, labels = token_inputs(torch, N, V, ld, bf16, V, skip=0.0, off=off)
+        logp, _ = token_logp(ctx, torch, buf.t, ld, labels, V)
+        want, _, p, _ = softmax64(torch, buf.t[:, :V], labels)
+        z = buf.t[:, :V].double()
+        d = (z - z.amax(1, keepdim=True)).abs()
+        picked, log_s = d.gather(1, labels.long()[:, None])[:, 0], d.gather(1, labels.long()[:, None])[:, 0] + want
+        within(torch, logp, want, U * ((p * (6 * d + 30)).sum(1) + picked + 4 * log_s.abs() + 2 * want.abs() + 2))
+
+
 # --- far margins ----------------------------------------------------------------------------------
 
 def test_pairs_of_far_margins_keep_their_gradient(hip, ctx, torch_cuda):
@@ -203,3 +218,48 @@ def test_the_kl_term_of_a_token_that_the_policy_rules_out(hip, ctx, torch_cuda, 
         assert float(loss) == INF and bool(got[3] == -INF) == (side == 0)
         others = [i for i in range(12) if i != 3]
         assert torch.isfinite(out[others]).all() and (side == 0 or torch.isfinite(out[3]).all())
+
+
+# --- the joins' column sums -----------------------------------------------------------------------
+
+def test_block_join_column_sums_past_32_bit_offsets(hip, ctx, torch_cuda):
+    """Over 2^32 bytes and 2^31 elements, the last gate's rows few: the vectors' gradients
+    against float64 sums.  A band's rows add up one after another, two rows at a time:
+    512 bands, so up to 1,040 roundings, and the joins'."""
+    torch = torch_cuda
+    rows, cols, gate_rows, chunk = 1_060_000, 2048, 400_000, 20_000
+    assert gate_rows % chunk == 0 and rows % chunk == 0
+    t, rnd = torch.bfloat16, gen(torch, 1)
+    o, x = (torch.empty(rows, cols, dtype=t, device="cuda").normal_(generator=torch.Generator(device="cuda")
+                                                                   .manual_seed(s)) for s in (2, 3))
+    d = {"o": o, "x": x, "post_w": 1 + 0.1 * rnd(cols), "post_b": None, "gate": rnd(3, cols), "pre_w": 1 + rnd(cols),
+         "pre_b": None}
+    y, h, st = torch.empty_like(o), torch.empty_like(o), torch.empty(rows, 4, device="cuda")
+    j = struct(hip, 1, 1, d, rows, cols, gate_rows)
+    ctx.call("seeai_block_join_fwd", j, y.data_ptr(), h.data_ptr(), st.data_ptr())
+    grads = {"dx": torch.empty_like(o), "do": x, "dpost_w": torch.empty(cols, device="cuda"), "dpost_b": None,
+             "dgate": torch.empty(3, cols, device="cuda"), "dpre_w": torch.empty(cols, device="cuda"), "dpre_b": None}
+    n = hip.lib().seeai_block_join_workspace(rows, cols, gate_rows)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    ctx.call("seeai_block_join_bwd", j, y.data_ptr(), st.data_ptr(), h.data_ptr(), None,
+             hip.BlockJoinGrads(*(hip.ptr(grads[k]) for k in NAMES)), ws.data_ptr(), n)
+    run = 1100 + DEPTH  # a band's rows, the fold
+    sums = lambda *s: torch.zeros(*s, cols, dtype=torch.float64, device="cuda")  # noqa: E731
+    pre, e_pre, S1, e1 = sums(), sums(), sums(3), sums(3)
+    w, w2, gate = d["post_w"].double(), d["pre_w"].double(), d["gate"].double()
+    for at in range(0, rows, chunk):
+        s, g = slice(at, at + chunk), at // gate_rows
+        sd, H = st[s].double(), h[s].double()
+        hat = y[s].double() * sd[:, 3:4]
+        pre += (H * hat).sum(0)
+        e_pre += (run + 3) * U * (H * hat).abs().sum(0)
+        up = H * w2
+        T, e = back64(torch, 1, up, U * up.abs(), hat, 3 * U * hat.abs(), sd[:, 3:4])
+        ohat = o[s].double() * sd[:, 1:2]
+        S1[g] += (T * ohat).sum(0)
+        e1[g] += (run + 3) * U * (T * ohat).abs().sum(0) + (e * ohat.abs()).sum(0)
+    within(torch, grads["dpre_w"], pre, e_pre)
+    within(torch, grads["dgate"], S1 * w, (e1 + 4 * U * S1.abs()) * w.abs())
+    within(torch, grads["dpost_w"], (S1 * gate).sum(0), ((e1 + 8 * U * S1.abs()) * gate.abs()).sum(0))
+    # (a band left out or counted twice would show)
+    assert float((e_pre / pre.abs()).max()) < 1e-3
