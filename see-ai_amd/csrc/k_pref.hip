@@ -692,59 +692,51 @@ PrefPairKernel(PrefArgs P, double* __restrict__ terms) {
   if (i + 1 == P.pairs) ClearRows(P, cut[2], P.N, kPairThreads);
 }
 
-// All pairs in one workgroup, and their loss: a launch less.  A wave takes every
-// sixteenth sequence, or several a share of one each where there are fewer.
+// All pairs in one workgroup, and their loss: a launch less.  A wave takes a sequence,
+// or several a share of one each where there are fewer.
 constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / kWave;
-constexpr size_t kOnePairs = 256, kOneRows = 2048;
+constexpr size_t kOnePairs = kOneWaves / 2, kOneRows = 2048;
 __global__ void __launch_bounds__(kOneThreads)
 PrefOneKernel(PrefArgs P, float* __restrict__ loss) {
-  __shared__ double2 red[2 * kOnePairs];  // a sequence's sum and count; a share's, below sixteen sequences
+  __shared__ double2 red[kOneWaves];  // a wave's sum and count
   __shared__ float slope[2 * kOnePairs];
-  __shared__ double terms[kOneWaves];
   const int wave = Uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int seqs = static_cast<int>(2 * P.pairs);
   // Sequences' shares: 8, 4, 2 or 1 waves to each.
   int shares = 1;
   while (2 * shares * seqs <= kOneWaves) shares *= 2;
-  const int share = wave % shares, threads = shares * kWave;
-  for (int q = wave / shares; q < seqs; q += kOneWaves / shares) {
-    const double2 v = Sequence(P, StartOf(P, q), StartOf(P, q + 1), share * kWave + lane, threads);
-    if (lane == 0) red[q * shares + share] = v;
-  }
+  const int q = wave / shares, first = wave % shares * kWave + lane, threads = shares * kWave;
+  const size_t from = q < seqs ? StartOf(P, q) : 0, to = q < seqs ? StartOf(P, q + 1) : 0;
+  const double2 sum = Sequence(P, from, to, first, threads);
+  if (lane == 0) red[wave] = sum;
   __syncthreads();
-  double term = 0.0;
-  if (threadIdx.x < P.pairs) {
-    const int i = threadIdx.x;
-    double2 v[2];
+  if (wave == 0) {
+    double term = 0.0;
+    if (lane < static_cast<int>(P.pairs)) {
+      double2 v[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      v[k] = make_double2(0.0, 0.0);
-      for (int h = 0; h < shares; ++h) {
-        v[k].x += red[(2 * i + k) * shares + h].x;
-        v[k].y += red[(2 * i + k) * shares + h].y;
+      for (int k = 0; k < 2; ++k) {
+        v[k] = make_double2(0.0, 0.0);
+        for (int h = 0; h < shares; ++h) {
+          v[k].x += red[(2 * lane + k) * shares + h].x;
+          v[k].y += red[(2 * lane + k) * shares + h].y;
+        }
+        v[k].y = P.average ? fmax(v[k].y, 1.0) : 1.0;
       }
-      v[k].y = P.average ? fmax(v[k].y, 1.0) : 1.0;
+      const Pair pair(P, v[0].x / v[0].y, v[1].x / v[1].y);
+      term = pair.term;
+      if (P.margin) P.margin[lane] = static_cast<float>(pair.margin);
+      slope[2 * lane] = static_cast<float>(pair.d / v[0].y);
+      slope[2 * lane + 1] = static_cast<float>(-pair.d / v[1].y);
     }
-    const Pair pair(P, v[0].x / v[0].y, v[1].x / v[1].y);
-    term = pair.term;
-    if (P.margin) P.margin[i] = static_cast<float>(pair.margin);
-    slope[2 * i] = static_cast<float>(pair.d / v[0].y);
-    slope[2 * i + 1] = static_cast<float>(-pair.d / v[1].y);
-  }
-  term = WaveSumD(term);
-  if (lane == 0) terms[wave] = term;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kOneWaves; ++w) term += terms[w];
-    *loss = static_cast<float>(P.scale * term);
+    term = WaveSumD(term);
+    if (lane == 0) *loss = static_cast<float>(P.scale * term);
   }
   if (!P.dlogp) return;
-  for (int q = wave / shares; q < seqs; q += kOneWaves / shares) {
-    const size_t from = StartOf(P, q), to = StartOf(P, q + 1);
-    const float d = slope[q];
+  __syncthreads();
+  const float d = q < seqs ? slope[q] : 0.0f;
 #pragma unroll 8
-    for (size_t r = from + share * kWave + lane; r < to; r += threads) P.dlogp[r] = P.labels[r] < 0 ? 0.0f : d;
-  }
+  for (size_t r = from + first; r < to; r += threads) P.dlogp[r] = P.labels[r] < 0 ? 0.0f : d;
   ClearRows(P, 0, StartOf(P, 0), kOneThreads);
   ClearRows(P, StartOf(P, seqs), P.N, kOneThreads);
 }
@@ -836,8 +828,11 @@ hipError_t LaunchTokenLogpBwd(int bf16, const void* z, size_t ld, const int32_t*
 
 hipError_t LaunchPrefLoss(const PrefArgs& a, float* loss, void* ws, hipStream_t s) {
   double* terms = static_cast<double*>(ws);
-  // One launch while one CU's loads keep up (us, one against two kernels: 4 pairs of
-  // 701 rows 6.6 and 5.8 + 2.2, 8 of 8192 12.0 and 7.2 + 1.8, 32 of 16384 20 and 6.5 + 2).
+  // One launch where a wave has one sequence at most, and few rows (us, one launch
+  // against two: 4 pairs of 701 rows 5.4 and 7.2, 8 of 2048 5.6 and 7.5, 8 of 8192 6.8 and
+  // 7.8; with 32 pairs, sequences in turn, 12 and 7.2, with 256 80 and 7.5).  How long each
+  // answer is the device knows: one of 8 pairs with nearly all rows takes 12 against 7.4 of
+  // 2048, 21 against 8.1 of 4096.
   if (a.pairs && a.pairs <= kOnePairs && a.N <= kOneRows) {
     hipLaunchKernelGGL(PrefOneKernel, dim3(1), dim3(kOneThreads), 0, s, a, loss);
     return hipGetLastError();
