@@ -674,15 +674,18 @@ hipError_t RunBwd(const JoinArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Past 256 columns the forward holds 16 elements a lane: fewer waves meet in a
+// Past 512 columns the forward holds 16 elements a lane: fewer waves meet in a
 // row's sums and share its vectors' loads (8 a lane and 16, bf16, us: layer norms
 // 2000 x 8192 35 and 28, 4000 x 4095 34 and 33, 8000 x 2048 26 both; 32768 x 128,
-// half the lanes without columns, 7.8 and 9.9).
+// half the lanes without columns, 7.8 and 9.9).  From 257 to 512 columns a wave has a
+// row of 8 a lane: as two rows of 16 a lane each gathers its own gate (root mean
+// square, one gate, 16000 x 512: bf16 14 and 25, f32 22 and 25; without a gate 32000 x
+// 512 bf16 23 both, f32 41 and 45, f32 layer norms 52 and 51).
 template <class T, bool kOff>
 hipError_t Forward(const JoinArgs& a, hipStream_t s) {
   if (a.cols <= 128) return RunFwd<T, 16, 8, kOff>(a, s);
   if (a.cols <= 256) return RunFwd<T, 32, 8, kOff>(a, s);
-  if (a.cols <= 512) return RunFwd<T, 32, 16, kOff>(a, s);
+  if (a.cols <= 512) return RunFwd<T, 64, 8, kOff>(a, s);
   if (a.cols <= 1024) return RunFwd<T, 64, 16, kOff>(a, s);
   if (a.cols <= 2048) return RunFwd<T, 128, 16, kOff>(a, s);
   if (a.cols <= 4096) return RunFwd<T, 256, 16, kOff>(a, s);
