@@ -54,7 +54,14 @@ struct Soft {
   __device__ __forceinline__ Soft(const Lse& others, float zl) : m(others.m), rest(static_cast<float>(others.s)) {
     const float own = ExpNeg(zl - others.Base());
     s = static_cast<float>(others.s + static_cast<double>(own));
-    logp = ((zl - m) - logf(s)) - static_cast<float>(others.s - static_cast<double>(s - own)) * __builtin_amdgcn_rcpf(s);
+    // log s from 2^k f, f within 1 / sqrt 2 and sqrt 2, so that f32's logarithm is of
+    // a number near 1; the sum is rounded once.
+    int k = __builtin_amdgcn_frexp_expf(s);
+    float f = __builtin_amdgcn_frexp_mantf(s);
+    if (f < 0.70710678f) f += f, --k;
+    const float left = static_cast<float>(others.s - static_cast<double>(s - own)) * __builtin_amdgcn_rcpf(s);
+    const double log_s = fma(static_cast<double>(k), 0.6931471805599453, static_cast<double>(logf(f) + left));
+    logp = static_cast<float>((static_cast<double>(zl) - static_cast<double>(m)) - log_s);
   }
 };
 

@@ -119,6 +119,27 @@ def test_wide_rows_add_up_in_64_bits(ctx, torch_cuda, bf16):
         within(torch, logp, want, U * ((p * (6 * d + 30)).sum(1) + picked + 4 * log_s.abs() + 2 * want.abs() + 2))
 
 
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_log_probabilities_are_rounded_once(hip, ctx, torch_cuda, bf16):
+    """Equal logits but the label's, so that the others' sum is a whole number: what is
+    left is a logarithm of at most 0.35, good to 4 u of itself, and the result's own
+    rounding."""
+    torch = torch_cuda
+    t, _ = types(torch, bf16)
+    N = 64
+    for V in range(300, 40000, 1237):
+        below = torch.linspace(0.0, 16.0, N, device="cuda").to(t)
+        z = torch.zeros(N, V, dtype=t, device="cuda")
+        labels = torch.randint(0, V, (N,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+        z[torch.arange(N), labels] = -below
+        labels, zeros = labels.to(torch.int32), torch.zeros(N, device="cuda")
+        want = -below.double() - torch.log(V - 1 + torch.exp(-below.double()))
+        logp, _ = token_logp(ctx, torch, z, V, labels, V)
+        within(torch, logp, want, U * (want.abs() + 2))
+        _, again = policy_loss(hip, ctx, torch, z, V, labels, zeros, None, zeros, None, V, 0.0, 1.0)
+        within(torch, again, want, U * (want.abs() + 2))
+
+
 # --- far margins ----------------------------------------------------------------------------------
 
 def test_pairs_of_far_margins_keep_their_gradient(hip, ctx, torch_cuda):
