@@ -12,7 +12,7 @@ import math
 import pytest
 
 from tests.test_gpu_block import U, Guarded, ctx, gen, types, within  # noqa: F401
-from tests.test_gpu_join import DEPTH, NAMES, back64, struct
+from tests.test_gpu_join import DEPTH, NAMES, back64, backward, forward, inputs, struct
 from tests.test_gpu_pref import (policy64, policy_loss, pref_loss, softmax64, token_inputs, token_logp,
                                  token_logp_bwd)
 
@@ -241,7 +241,24 @@ def test_the_kl_term_of_a_token_that_the_policy_rules_out(hip, ctx, torch_cuda, 
         assert torch.isfinite(out[others]).all() and (side == 0 or torch.isfinite(out[3]).all())
 
 
-# --- the joins' column sums -----------------------------------------------------------------------
+# --- the joins ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_block_join_of_one_gate_for_more_rows_than_there_are(hip, ctx, torch_cuda, bf16):
+    """The bits of a gate for exactly these rows."""
+    torch = torch_cuda
+    t, _ = types(torch, bf16)
+    for rows, cols in ((5, 96), (300, 257), (300, 512), (2100, 130)):
+        d = inputs(torch, 0, 1, 1, 1, rows, cols, rows, t, 0)
+        dh, dy = gen(torch, 1)(rows, cols).to(t), gen(torch, 2)(rows, cols).to(t)
+        y, h, st = forward(hip, ctx, torch, 0, bf16, d, rows, cols, rows)
+        want = backward(hip, ctx, torch, 0, bf16, d, rows, y, st, dh, dy)
+        for gate_rows in (rows + 1, 2 ** 31, 2 ** 61):
+            got = forward(hip, ctx, torch, 0, bf16, d, rows, cols, gate_rows)
+            assert all(torch.equal(a, b) for a, b in zip(got, (y, h, st)))
+            got = backward(hip, ctx, torch, 0, bf16, d, gate_rows, y, st, dh, dy)
+            assert all(torch.equal(got[k], want[k]) for k in NAMES)
+
 
 def test_block_join_column_sums_past_32_bit_offsets(hip, ctx, torch_cuda):
     """Over 2^32 bytes and 2^31 elements, the last gate's rows few: the vectors' gradients
