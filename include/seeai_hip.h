@@ -451,8 +451,9 @@ typedef struct seeai_grad_tensor {
 } seeai_grad_tensor;
 typedef struct seeai_grad_group seeai_grad_group;
 /* Checks the tensors (device pointers, none sharing memory with another: status
- * 2) and keeps their table, and the norm's partial sums, on the device.  Not
- * while the stream is captured. */
+ * 2) and keeps their table, and the norm's partial sums, on the device.  A group is
+ * bound to these addresses; making one allocates, copies and, when it goes, waits.
+ * Not while the stream is captured. */
 int seeai_grad_group_create(seeai_ctx* ctx, const seeai_grad_tensor* tensors, uint64_t count,
                             seeai_grad_group** out);
 /* Waits for the device; the context outlives its groups. */

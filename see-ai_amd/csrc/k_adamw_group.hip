@@ -27,7 +27,7 @@
 // takes eight neighbours (a block is 16 lanes), a workgroup 2048 elements;
 // which tensor they lie in comes from a binary search of the device table.
 // 34.6 M parameters in five tensors, bf16 gradients and copy, on MI355X: 32-bit
-// moments 186 us (28 bytes each, 5.2 TB/s; a copy runs 5.1), 8-bit 113 to 131
+// moments 185 us (28 bytes each, 5.2 TB/s; a copy runs 5.1), 8-bit 113 to 131
 // (16 1/8 bytes; the hashes and the coding are not hidden entirely); 96 tensors
 // of 0.6 M together 6.9, a launch's length.
 #include "common.h"

@@ -376,13 +376,18 @@ Plan PlanOf(size_t rows, size_t cols, size_t gate_rows) {
 
 // bands' sums: [bands][4][cols]: dw', db', S1 and S0 (or dw and db where a
 // band's gates are whole), or the gradients themselves where there is one band.
-// A row's loads go out while the row before it is reduced (kAhead).
+// A row's loads go out while the row before it is reduced (kAhead; not with 16
+// elements a lane).  128 registers a lane, four waves a SIMD, are enough for bf16 rows
+// on dwords of up to 8192 columns (one instance spills 12 bytes).  Root mean squares in f32 up to
+// 256 columns and f32 layer norms spill 20 to 144 bytes a lane, some layer norms of bf16
+// rows off dwords 28 to 60, and 16 elements a lane up to 324: such reloads wait behind
+// the next row's loads.
 template <class T, int kTPR, int kE, bool kOff, bool kRms>
 __global__ void __launch_bounds__(BwdThreads(kTPR), 4)
 JoinBwdKernel(JoinArgs a, Plan plan) {
   using R = Row<T, kTPR, kE, kOff>;
   constexpr int kThreads = BwdThreads(kTPR), kRows = kThreads / kTPR;
-  constexpr bool kAhead = kE == 8;  // (with 16 the registers are full)
+  constexpr bool kAhead = kE == 8;
   __shared__ float lds[64];
   // Element e of thread t at ((e / 4) kTPR + t) 4 + e % 4: w', and gate w.
   __shared__ float wpre[kTPR * kE], wpost[kTPR * kE];

@@ -16,11 +16,16 @@
 // Bound by HBM: the logits read once (twice where a gradient needs a sum over
 // other rows first) and the gradient written once.  A row whose label is
 // negative is not judged: it is not read, and its gradient is zero.
-// Everything between is f32; sums along a row past its groups of 16 bytes, sums
-// over rows and the pairs' terms are f64.
+// A row's label stands apart from its other logits: where it is nearly sure, its
+// log-probability and its gradient are as small as the others' share of the sum and
+// come from that share, not from differences of numbers near 1.  Setting it apart
+// costs rows of one wave 3 to 5 % (16384 x 1000 bf16 log-probabilities 11.6 and 12.2
+// us), large ones nothing or 1 %.
+// Everything between is f32; sums along a row past its groups of 16 bytes, a
+// log-probability before its one rounding, sums over rows and the pairs' terms are f64.
 // 8192 x 32000 bf16 with 70 % of the rows judged, on MI355X: log-probabilities 66
-// us (5.5 TB/s; a copy runs 5.1), their backward 147 (6.0, part of the logits from
-// the last cache), the policy loss with its gradient 161 (5.5, VALU issue 69 %
+// us (5.6 TB/s; a copy runs 5.1), their backward 146 (6.1, part of the logits from
+// the last cache), the policy loss with its gradient 163 (5.5, VALU issue 70 %
 // busy).
 #include <type_traits>
 
@@ -756,8 +761,9 @@ unsigned Groups(size_t rows, int per) {
 }
 
 // Gradients that the last cache (256 MB) cannot hold beside the logits for the
-// product that reads them are stored past it: 8192 x 32000 bf16 paired loss 220 us
-// against 258, policy loss 164 against 174; 16384 x 1000 f32 23 both.
+// product that reads them are stored past it: 8192 x 32000 bf16 paired loss 242 us
+// against 261, policy loss 165 against 169, 2000 x 128000 paired 289 against 321; 2000 x
+// 16000 (64 MB) 43 against 42.
 bool GoesPast(size_t N, size_t ld, size_t size) { return N * ld * size > size_t{128} << 20; }
 
 // The 16-byte groups that a row of C may lie on.
